@@ -19,6 +19,8 @@ from .types import (  # noqa: F401
 from .api import (cast, dequantize, requantize, matmul, linear, gemm_operands,  # noqa: F401
                   attach_gemm_operands, AmaxHistory, cast_matmul)
 from . import bridges  # noqa: F401
+from .norm_rope import qk_norm_rope, qk_norm_rope_write  # noqa: F401
+from .kvcache import QuantizedKVCache, cache_attention  # noqa: F401
 from .autograd import cast_ste, cast_ste_clipped  # noqa: F401
 from .plugin import install, uninstall  # noqa: F401
 

@@ -64,7 +64,37 @@ PROTOTYPES = {
     "brc_gemm_bf16": ([_p, _p, _i, _i, _i, _p, _i, _p], _i),
     "brc_dequant_transposed": ([_p, _i64, _i64, _i, _i, _i, _i, _i, _p, _p, _p, _i, _p], _i),
     "brc_transpose_u8": ([_p, _i64, _i64, _p, _p], _i),
+    "brc_qk_norm_rope": ([_p, _p, _p, _p], _i),
+    "brc_qk_norm_rope_bwd_workspace": ([_i], _i64),
+    "brc_qk_norm_rope_bwd": ([_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p],
+                             _i),
+    "brc_qk_norm_rope_write": ([_p, _p, _i64, _i64, _p, _p, _p, _i, _p], _i),
+    "brc_kv_write": ([_p, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _p], _i),
+    "brc_kv_read": ([_p, _p, _i64, _i, _p, _i, _i64, _p, _p, _i, _p], _i),
+    "brc_kv_attention_workspace": ([_p, _i, _i, _i], _i64),
+    "brc_kv_attention": ([_p, _p, _i, _i, _i, _i, _p, _i64, _i, _p, _p, _p, _i64, ctypes.c_float,
+                          _p, _p, _p, _i64, _p], _i),
 }
+
+
+class NormRope(ctypes.Structure):
+    """``brc_norm_rope``."""
+
+    _fields_ = ([(n, _p) for n in ("q", "k")] +
+                [(n, _i64) for n in ("q_token", "q_head", "k_token", "k_head")] +
+                [(n, _p) for n in ("wq", "wk", "cos", "sin", "positions")] +
+                [(n, _i64) for n in ("tokens", "table_rows")] +
+                [(n, ctypes.c_int32) for n in ("hq", "hk", "d", "rot", "dtype", "w_dtype",
+                                               "index64", "interleaved")] +
+                [("eps", ctypes.c_float)])
+
+
+class KvCache(ctypes.Structure):
+    """``brc_kv_cache``."""
+
+    _fields_ = ([(n, _p) for n in ("k_data", "k_scale", "v_data", "v_scale")] +
+                [("num_pages", _i64)] +
+                [(n, ctypes.c_int32) for n in ("heads", "page_size", "head_dim", "kind", "fmt")])
 
 # status codes (include/breccia_b200.h)
 BRC_OK = 0

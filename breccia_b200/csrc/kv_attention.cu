@@ -1,0 +1,98 @@
+// Entry points of the attention over a quantised paged cache: argument checks,
+// the split of the query rows, the workspace.
+#include "kv_attention.cuh"
+
+using namespace brc;
+using namespace brc::kvatt;
+
+namespace {
+
+// Rows of one sequence and cache head: 16 or 32 to a warp (32 need twice the
+// accumulators, and do not fit at d = 256), up to four row warps to a block.
+struct Split {
+  int mt, row_warps, row_blocks, rows_per_block;
+};
+Split split_rows(int rows, int d) {
+  Split s;
+  s.mt = rows <= 16 || d == 256 ? 1 : 2;
+  const int tile = 16 * s.mt;
+  s.row_warps = rows <= tile ? 1 : rows <= 2 * tile ? 2 : 4;
+  s.rows_per_block = tile * s.row_warps;
+  s.row_blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
+  return s;
+}
+
+int blocks_of(int mt) { return sm_count() * (mt == 1 ? 3 : 2); }
+
+int check(const brc_kv_cache* c, int batch, int draft, int hq) {
+  if (const int rc = kv::check_cache(c)) return rc;
+  if (batch < 0 || draft < 0 || hq <= 0 || hq % c->heads) return BRC_ERR_SHAPE;
+  // rows, items and positions are counted in 32 bits
+  if ((int64_t)draft * hq > (1 << 24) || (int64_t)batch * c->heads > (1 << 24) ||
+      (int64_t)batch * draft * hq > 0x40000000)
+    return BRC_ERR_RANGE;
+  return BRC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t brc_kv_attention_workspace(const brc_kv_cache* c, int batch, int draft, int hq) {
+  if (check(c, batch, draft, hq) != BRC_OK) return 0;
+  const Split s = split_rows(draft * (hq / c->heads), c->head_dim);
+  return 2 * (int64_t)blocks_of(s.mt) * s.rows_per_block * (c->head_dim + 2) * 4;
+}
+
+int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batch, int draft,
+                     int hq, const int32_t* table, int64_t table_stride, int table_pages,
+                     const int32_t* context, const int32_t* drafts, const uint8_t* tree,
+                     int64_t tree_stride, float scale, void* out, float* lse, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  if (const int rc = check(c, batch, draft, hq)) return rc;
+  if (q_dtype != BRC_DTYPE_BF16 && q_dtype != BRC_DTYPE_F16) return BRC_ERR_DTYPE;
+  if (table_pages < 0 || table_stride < 0 || tree_stride < 0) return BRC_ERR_SHAPE;
+  if (batch == 0 || draft == 0) return BRC_OK;
+  if (!q || !context || !out || !workspace || (!table && table_pages)) return BRC_ERR_NULL;
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) return BRC_ERR_ALIGN;
+  if ((int64_t)table_pages * c->page_size > 0x7FFFFFF0) return BRC_ERR_RANGE;
+  const int group = hq / c->heads, rows = draft * group;
+  const Split s = split_rows(rows, c->head_dim);
+  const int blocks = blocks_of(s.mt);
+  if (workspace_bytes < brc_kv_attention_workspace(c, batch, draft, hq)) return BRC_ERR_SHAPE;
+  Args a{};
+  a.c = *c;
+  a.q = q;
+  a.q_f16 = q_dtype == BRC_DTYPE_F16;
+  a.batch = batch;
+  a.draft = draft;
+  a.hq = hq;
+  a.group = group;
+  a.rows = rows;
+  a.table = table;
+  a.table_stride = table_stride;
+  a.table_pages = table_pages;
+  for (a.page_shift = 4; (1 << a.page_shift) < c->page_size; ++a.page_shift) {}
+  a.context = context;
+  a.drafts = drafts;
+  a.tree = tree;
+  a.tree_stride = tree_stride;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.lse = lse;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + 2 * (int64_t)blocks * s.rows_per_block * c->head_dim;
+  a.row_warps = s.row_warps;
+  a.row_blocks = s.row_blocks;
+  a.rows_per_block = s.rows_per_block;
+  a.min_share = 2 * (kWarps / s.row_warps);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (c->kind == BRC_STE_NVFP4) return attend_nvfp4(a, s.mt, blocks, st);
+  if (c->kind == BRC_STE_MXFP8)
+    return c->fmt == BRC_FP8_E4M3 ? attend_mx_e4m3(a, s.mt, blocks, st)
+                                  : attend_mx_e5m2(a, s.mt, blocks, st);
+  return c->fmt == BRC_FP8_E4M3 ? attend_block_e4m3(a, s.mt, blocks, st)
+                                : attend_block_e5m2(a, s.mt, blocks, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,205 @@
+// Quantised key/value cache: rows written as they are produced, and read back.
+//
+// Both are streams: a row (one token, one head) is read once and written once,
+// and HBM bounds them at long prompts. A row lies on d / 8 lanes, eight
+// elements to a lane: a warp's loads and stores of elements are then 512
+// contiguous bytes, and the block amax of a scale is a few shuffles. Every
+// lane keeps the loads of several rows in flight.
+#include "kv_codec.cuh"
+#include "launch.h"
+
+namespace brc {
+namespace kv {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRows = 4;  // rows in flight per lane
+
+__device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
+  return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
+}
+
+struct WriteArgs {
+  brc_kv_cache c;
+  const void* x[2];  // keys, values
+  int64_t token[2], head[2];
+  const void* slots;
+  int slots64;
+  int64_t rows;  // tokens * heads
+};
+
+// blockIdx.y: 0 keys, 1 values.
+template <int DT, int KIND, int FMT, int LPR>
+__global__ void __launch_bounds__(kThreads) k_write(WriteArgs a) {
+  constexpr int G = 32 / LPR;
+  const int lane = threadIdx.x & 31, part = lane % LPR;
+  const int side = blockIdx.y;
+  const void* x = side ? a.x[1] : a.x[0];
+  const int64_t ts = side ? a.token[1] : a.token[0], hs = side ? a.head[1] : a.head[0];
+  uint8_t* data = side ? a.c.v_data : a.c.k_data;
+  void* scale = side ? a.c.v_scale : a.c.k_scale;
+  const int64_t slots = a.c.num_pages * a.c.page_size;
+  const int64_t first =
+      ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
+  float f[kRows][8];
+  int64_t row[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int64_t r = first + u * G;
+    row[u] = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+    if (r < a.rows) {
+      const int64_t t = r / a.c.heads;
+      const int h = (int)(r - t * a.c.heads);
+      load8<DT>(x, t * ts + h * hs + part * 8, f[u]);
+      const int64_t slot = load_index(a.slots, t, a.slots64);
+      if (slot >= 0 && slot < slots) row[u] = row_of(a.c, slot, h);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u)
+    encode_row<KIND, FMT, LPR>(f[u], part, row[u] >= 0, row[u], data, scale);
+}
+
+struct ReadArgs {
+  brc_kv_cache c;
+  const int32_t* table;
+  const int32_t* lengths;
+  int64_t table_stride, length, rows;  // rows: batch * length * heads
+  int table_pages;
+  void* out[2];
+};
+
+template <int DT, int KIND, int FMT, int LPR>
+__global__ void __launch_bounds__(kThreads) k_read(ReadArgs a) {
+  constexpr int G = 32 / LPR;
+  const int lane = threadIdx.x & 31, part = lane % LPR;
+  const int side = blockIdx.y;
+  const uint8_t* data = side ? a.c.v_data : a.c.k_data;
+  const void* scale = side ? a.c.v_scale : a.c.k_scale;
+  void* out = side ? a.out[1] : a.out[0];
+  const int64_t first =
+      ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
+  float f[kRows][8];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int64_t r = first + u * G;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+    if (r < a.rows) {
+      const int64_t bt = r / a.c.heads;
+      const int h = (int)(r - bt * a.c.heads);
+      const int64_t b = bt / a.length, t = bt - b * a.length;
+      const int64_t p = t / a.c.page_size;
+      if (t < a.lengths[b] && p < a.table_pages) {
+        const int64_t page = a.table[b * a.table_stride + p];
+        if (page >= 0 && page < a.c.num_pages)
+          decode_row<KIND, FMT, LPR>(
+              data, scale,
+              (page * a.c.heads + h) * a.c.page_size + (t - p * a.c.page_size), part, f[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int64_t r = first + u * G;
+    if (r < a.rows) store8<DT>(out, r * (LPR * 8) + part * 8, f[u]);
+  }
+}
+
+template <template <int, int, int, int> class Launch, int DT, int KIND, int FMT, class Args>
+int by_dim(int d, const Args& a, dim3 grid, cudaStream_t st) {
+  switch (d) {
+    case 64: Launch<DT, KIND, FMT, 8>::run(a, grid, st); break;
+    case 128: Launch<DT, KIND, FMT, 16>::run(a, grid, st); break;
+    default: Launch<DT, KIND, FMT, 32>::run(a, grid, st); break;
+  }
+  return check_launch();
+}
+template <template <int, int, int, int> class Launch, int DT, class Args>
+int by_kind(const Args& a, dim3 grid, cudaStream_t st) {
+  const int d = a.c.head_dim;
+  const bool e4 = a.c.fmt == BRC_FP8_E4M3;
+  if (a.c.kind == BRC_STE_BLOCK_FP8)
+    return e4 ? by_dim<Launch, DT, BRC_STE_BLOCK_FP8, BRC_FP8_E4M3>(d, a, grid, st)
+              : by_dim<Launch, DT, BRC_STE_BLOCK_FP8, BRC_FP8_E5M2>(d, a, grid, st);
+  if (a.c.kind == BRC_STE_MXFP8)
+    return e4 ? by_dim<Launch, DT, BRC_STE_MXFP8, BRC_FP8_E4M3>(d, a, grid, st)
+              : by_dim<Launch, DT, BRC_STE_MXFP8, BRC_FP8_E5M2>(d, a, grid, st);
+  return by_dim<Launch, DT, BRC_STE_NVFP4, BRC_FP8_E4M3>(d, a, grid, st);
+}
+template <template <int, int, int, int> class Launch, class Args>
+int by_dtype(int dt, const Args& a, dim3 grid, cudaStream_t st) {
+  switch (dt) {
+    case BRC_DTYPE_F32: return by_kind<Launch, BRC_DTYPE_F32>(a, grid, st);
+    case BRC_DTYPE_BF16: return by_kind<Launch, BRC_DTYPE_BF16>(a, grid, st);
+    default: return by_kind<Launch, BRC_DTYPE_F16>(a, grid, st);
+  }
+}
+template <int DT, int KIND, int FMT, int LPR>
+struct LaunchWrite {
+  static void run(const WriteArgs& a, dim3 grid, cudaStream_t st) {
+    k_write<DT, KIND, FMT, LPR><<<grid, kThreads, 0, st>>>(a);
+  }
+};
+template <int DT, int KIND, int FMT, int LPR>
+struct LaunchRead {
+  static void run(const ReadArgs& a, dim3 grid, cudaStream_t st) {
+    k_read<DT, KIND, FMT, LPR><<<grid, kThreads, 0, st>>>(a);
+  }
+};
+
+// Blocks for `rows` rows of d elements, or 0 past the grid's limit.
+int64_t blocks_for(int64_t rows, int d) {
+  const int per = (kThreads / 32) * kRows * (32 / (d / 8));
+  const int64_t n = (rows + per - 1) / per;
+  return n > 0x7FFFFFFF ? 0 : n;
+}
+
+bool bad_stride(int64_t s, int dtype) { return s % (dtype == BRC_DTYPE_F32 ? 4 : 8) != 0; }
+
+}  // namespace
+}  // namespace kv
+}  // namespace brc
+
+using namespace brc;
+using namespace brc::kv;
+
+extern "C" {
+
+int brc_kv_write(const brc_kv_cache* c, const void* k, const void* v, int dtype, int64_t tokens,
+                 int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                 const void* slots, int slots64, void* stream) {
+  if (const int rc = check_cache(c)) return rc;
+  if (tokens < 0) return BRC_ERR_SHAPE;
+  if (dtype < BRC_DTYPE_F32 || dtype > BRC_DTYPE_F16) return BRC_ERR_DTYPE;
+  if (tokens == 0) return BRC_OK;
+  if (!k || !v || !slots) return BRC_ERR_NULL;
+  if (((uintptr_t)k | (uintptr_t)v) & 15) return BRC_ERR_ALIGN;
+  if (bad_stride(k_token, dtype) || bad_stride(k_head, dtype) || bad_stride(v_token, dtype) ||
+      bad_stride(v_head, dtype))
+    return BRC_ERR_ALIGN;
+  WriteArgs a{*c, {k, v}, {k_token, v_token}, {k_head, v_head}, slots, slots64, tokens * c->heads};
+  const int64_t n = blocks_for(a.rows, c->head_dim);
+  if (n == 0) return BRC_ERR_RANGE;
+  return by_dtype<LaunchWrite>(dtype, a, dim3((unsigned)n, 2), (cudaStream_t)stream);
+}
+
+int brc_kv_read(const brc_kv_cache* c, const int32_t* table, int64_t table_stride,
+                int table_pages, const int32_t* lengths, int batch, int64_t length, void* k_out,
+                void* v_out, int out_dtype, void* stream) {
+  if (const int rc = check_cache(c)) return rc;
+  if (batch < 0 || length < 0 || table_pages < 0 || table_stride < 0) return BRC_ERR_SHAPE;
+  if (out_dtype < BRC_DTYPE_F32 || out_dtype > BRC_DTYPE_F16) return BRC_ERR_DTYPE;
+  if (batch == 0 || length == 0) return BRC_OK;
+  if ((!table && table_pages) || !lengths || !k_out || !v_out) return BRC_ERR_NULL;
+  if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return BRC_ERR_ALIGN;
+  ReadArgs a{*c, table, lengths, table_stride, length, (int64_t)batch * length * c->heads,
+             table_pages, {k_out, v_out}};
+  const int64_t n = blocks_for(a.rows, c->head_dim);
+  if (n == 0) return BRC_ERR_RANGE;
+  return by_dtype<LaunchRead>(out_dtype, a, dim3((unsigned)n, 2), (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -387,6 +387,106 @@ int brc_gemm_status(int reset);
  * bit per role that left its wait without the barrier completing (3 = both). */
 int brc_selftest_wait_timeout(int limit_us, int* roles_out, void* stream);
 
+/* ======================================================= attention block
+ * Extensions (no counterpart in the reference): the operators around a
+ * key/value cache held in the reference's recipes. Token-level indexes
+ * (positions, slots, page table, lengths) live on the device; an index out of
+ * its range is never followed (each function says what it gives instead). */
+
+/* Norm of every query and key head and position rotation, one pass. For a
+ * head x of d elements: r = (mean(x^2) + eps)^-1/2, z = x r w, and the first
+ * `rot` elements of z are rotated by the token's angles, pairs (i, i + rot/2)
+ * or, interleaved, (2i, 2i + 1): (a cos - b sin, b cos + a sin). float32
+ * arithmetic, one rounding into the outputs.
+ * q is (tokens, hq, d) with token and head strides in elements (last axis
+ * contiguous), k likewise with hk heads (either count may be 0); q_out
+ * (tokens, hq, d) and k_out (tokens, hk, d) contiguous, of the inputs' dtype.
+ * wq, wk: d weights of w_dtype. cos, sin: (table_rows, rot / 2) float32.
+ * positions: tokens int32, or int64 with index64 = 1; a token whose position
+ * is outside the table gives NaN.
+ * d % 16 == 0, d <= 256, rot % 16 == 0, 16 <= rot <= d; pointers and strides
+ * 16-byte aligned. */
+typedef struct {
+  const void* q;
+  const void* k;
+  int64_t q_token, q_head, k_token, k_head; /* strides in elements */
+  const void* wq;
+  const void* wk;
+  const float* cos;
+  const float* sin;
+  const void* positions;
+  int64_t tokens, table_rows;
+  int32_t hq, hk, d, rot;
+  int32_t dtype, w_dtype, index64, interleaved;
+  float eps;
+} brc_norm_rope;
+int brc_qk_norm_rope(const brc_norm_rope* a, void* q_out, void* k_out, void* stream);
+/* Its gradients: gq, gk (strides as q, k: gq_token ...) are the gradients of
+ * the outputs, of the inputs' dtype; dq, dk contiguous like q_out, k_out; dwq,
+ * dwk: d gradients of w_dtype, summed in float32 in a fixed order (the result
+ * does not change between runs). workspace: brc_qk_norm_rope_bwd_workspace(d)
+ * bytes, 16-byte aligned. */
+int64_t brc_qk_norm_rope_bwd_workspace(int d);
+int brc_qk_norm_rope_bwd(const brc_norm_rope* a, const void* gq, const void* gk, int64_t gq_token,
+                         int64_t gq_head, int64_t gk_token, int64_t gk_head, void* dq, void* dk,
+                         void* dwq, void* dwk, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/* A paged key/value cache. Codes: (num_pages, heads, page_size, row bytes),
+ * d bytes per row (FP8) or d / 2 (NVFP4, element 2i in the low nibble of byte
+ * i). Scales: (num_pages, heads, page_size, n): BRC_STE_BLOCK_FP8 one float32
+ * (block = head_dim), BRC_STE_MXFP8 d / 32 E8M0 bytes, BRC_STE_NVFP4 d / 16
+ * E4M3 bytes. Codes and scales are the casts' of the same rows, bit for bit.
+ * head_dim 64, 128 or 256; page_size a power of two >= 16; 16-byte aligned. */
+typedef struct {
+  uint8_t* k_data;
+  void* k_scale;
+  uint8_t* v_data;
+  void* v_scale;
+  int64_t num_pages;
+  int32_t heads, page_size, head_dim, kind, fmt;
+} brc_kv_cache;
+/* Quantise keys and values (tokens, heads, head_dim; strides in elements) into
+ * the rows slots[token] = page * page_size + place in page (int32, or int64
+ * with slots64). A slot outside the cache is not written (-1: padding). Two
+ * tokens of one call with the same slot leave either's row. */
+int brc_kv_write(const brc_kv_cache* c, const void* k, const void* v, int dtype, int64_t tokens,
+                 int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                 const void* slots, int slots64, void* stream);
+/* brc_qk_norm_rope of q and k (hk == heads, d == head_dim), k rounded to its
+ * dtype and written into the cache with v, in one launch: q_out, and the cache
+ * as brc_qk_norm_rope then brc_kv_write leave it. dtype bf16 or f16. */
+int brc_qk_norm_rope_write(const brc_norm_rope* a, const void* v, int64_t v_token, int64_t v_head,
+                           void* q_out, const brc_kv_cache* c, const void* slots, int slots64,
+                           void* stream);
+/* Keys and values of `batch` sequences as dense (batch, length, heads,
+ * head_dim) tensors of out_dtype: decode(code) * scale in float32, one
+ * rounding. Token t of sequence b lies in page table[b * table_stride + t /
+ * page_size]; tokens from lengths[b] on, past the table's `table_pages`
+ * columns, or in a page outside the cache read as zero. */
+int brc_kv_read(const brc_kv_cache* c, const int32_t* table, int64_t table_stride,
+                int table_pages, const int32_t* lengths, int batch, int64_t length, void* k_out,
+                void* v_out, int out_dtype, void* stream);
+/* Attention of the newest `draft` tokens of every sequence over the cache:
+ * sequence b holds context[b] tokens, then its drafted tokens (their rows
+ * already written). q is (batch, draft, hq, head_dim) contiguous bf16 or f16,
+ * hq % heads == 0, query head i reading cache head i / (hq / heads).
+ * drafts[b] (NULL: draft) of the drafted tokens exist; rows past them are not
+ * computed. Query i sees the whole context and drafted token j where
+ * tree[b * tree_stride + i * draft + j] is non-zero (NULL: j <= i).
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j     (q's dtype, as q)
+ *   lse_i = log(sum_j exp(scale q_i . k_j))          (optional, float32 (batch, draft, hq))
+ * A row that sees nothing gives out 0 and lse -inf. What lies in places that
+ * a row does not see (NaN included) does not reach it. Tokens past the
+ * table's columns or in a page outside the cache are not seen.
+ * workspace: brc_kv_attention_workspace(...) bytes, 16-byte aligned. */
+int64_t brc_kv_attention_workspace(const brc_kv_cache* c, int batch, int draft, int hq);
+int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batch, int draft,
+                     int hq, const int32_t* table, int64_t table_stride, int table_pages,
+                     const int32_t* context, const int32_t* drafts, const uint8_t* tree,
+                     int64_t tree_stride, float scale, void* out, float* lse, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 /* ======================================================= diagnostics
  * Writes, for each i, the float32 quotient x[i] / s[i] as the cast kernels
  * compute it (correctly rounded reciprocal refined by one FMA residual step)
