@@ -7,22 +7,23 @@ using namespace brc::kvatt;
 
 namespace {
 
-// Rows of one sequence and cache head: 16 or 32 to a warp (32 need twice the
-// accumulators, and do not fit at d = 256), up to four row warps to a block.
+// Rows of one sequence and cache head: tiles of 8 to a product's columns, up to
+// four tiles to a warp (their accumulators take d / 4 registers each: two at d =
+// 256), then up to four row warps to a block.
 struct Split {
-  int mt, row_warps, row_blocks, rows_per_block;
+  int nt, row_warps, row_blocks, rows_per_block;
 };
 Split split_rows(int rows, int d) {
   Split s;
-  s.mt = rows <= 16 || d == 256 ? 1 : 2;
-  const int tile = 16 * s.mt;
+  s.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : most_tiles(d);
+  const int tile = 8 * s.nt;
   s.row_warps = rows <= tile ? 1 : rows <= 2 * tile ? 2 : 4;
   s.rows_per_block = tile * s.row_warps;
   s.row_blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
   return s;
 }
 
-int blocks_of(int mt) { return sm_count() * (mt == 1 ? 3 : 2); }
+int blocks_of(int d, int nt) { return sm_count() * blocks_per_sm(d, nt); }
 
 int check(const brc_kv_cache* c, int batch, int draft, int hq) {
   if (const int rc = kv::check_cache(c)) return rc;
@@ -41,7 +42,7 @@ extern "C" {
 int64_t brc_kv_attention_workspace(const brc_kv_cache* c, int batch, int draft, int hq) {
   if (check(c, batch, draft, hq) != BRC_OK) return 0;
   const Split s = split_rows(draft * (hq / c->heads), c->head_dim);
-  return 2 * (int64_t)blocks_of(s.mt) * s.rows_per_block * (c->head_dim + 2) * 4;
+  return 2 * (int64_t)blocks_of(c->head_dim, s.nt) * s.rows_per_block * (c->head_dim + 2) * 4;
 }
 
 int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batch, int draft,
@@ -58,7 +59,7 @@ int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batc
   if ((int64_t)table_pages * c->page_size > 0x7FFFFFF0) return BRC_ERR_RANGE;
   const int group = hq / c->heads, rows = draft * group;
   const Split s = split_rows(rows, c->head_dim);
-  const int blocks = blocks_of(s.mt);
+  const int blocks = blocks_of(c->head_dim, s.nt);
   if (workspace_bytes < brc_kv_attention_workspace(c, batch, draft, hq)) return BRC_ERR_SHAPE;
   Args a{};
   a.c = *c;
@@ -87,12 +88,12 @@ int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batc
   a.rows_per_block = s.rows_per_block;
   a.min_share = 2 * (kWarps / s.row_warps);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (c->kind == BRC_STE_NVFP4) return attend_nvfp4(a, s.mt, blocks, st);
+  if (c->kind == BRC_STE_NVFP4) return attend_nvfp4(a, s.nt, blocks, st);
   if (c->kind == BRC_STE_MXFP8)
-    return c->fmt == BRC_FP8_E4M3 ? attend_mx_e4m3(a, s.mt, blocks, st)
-                                  : attend_mx_e5m2(a, s.mt, blocks, st);
-  return c->fmt == BRC_FP8_E4M3 ? attend_block_e4m3(a, s.mt, blocks, st)
-                                : attend_block_e5m2(a, s.mt, blocks, st);
+    return c->fmt == BRC_FP8_E4M3 ? attend_mx_e4m3(a, s.nt, blocks, st)
+                                  : attend_mx_e5m2(a, s.nt, blocks, st);
+  return c->fmt == BRC_FP8_E4M3 ? attend_block_e4m3(a, s.nt, blocks, st)
+                                : attend_block_e5m2(a, s.nt, blocks, st);
 }
 
 }  // extern "C"

@@ -7,15 +7,18 @@
 // every key and value, so the codes are read once for all of them: HBM bounds
 // single tokens and small trees. One pass with a running maximum and sum.
 //
-// Layout. A warp takes 16 tokens at a time straight from global memory into
-// the operand fragments of m16n8k16: which head elements stand at which place
-// of a fragment is free as long as both operands agree, so a lane's fragment
-// words are 16 contiguous bytes of a row, with no shared memory and no
-// shuffles between load and product.
-//   keys   (B of Q K^T): lane (r, c) holds token r, bytes 64 i + 16 c .. + 15
-//   values (B of P V):   lane (r, c) holds tokens 2c, 2c+1, 2c+8, 2c+9, bytes
-//                        16 r .. + 15; pairs of tokens are byte permutes
-// The score fragment is the probability fragment (A of P V) as it stands.
+// Layout. A warp takes 16 tokens at a time as the rows of m16n8k16 products, with
+// 8 query rows to a product's columns: S^T = K Q^T and O^T = V^T P^T, so a group
+// of 8 query heads or fewer wastes nothing and holds half the accumulators of
+// the other orientation. Which head elements stand at which place of a fragment
+// is free as long as both operands agree, so a lane's words are contiguous bytes
+// of a row, read whole:
+//   keys    (A of K Q^T):   lane (r, c) reads tokens r, r + 8, bytes 64 i + 16 c .. + 15
+//   values  (A of V^T P^T): lane (r, c) reads tokens 2c, 2c+1, 2c+8, 2c+9, bytes
+//                           16 r .. + 15; pairs of tokens are byte permutes
+// The scores' fragment becomes the probabilities' by two 8 x 8 transposes.
+// Codes come through a ring of 16-token stages of each warp's own (asynchronous
+// copies, no block barrier).
 //
 // Numbers. FP8 and FP4 codes are exact in f16. Queries are scaled per row by a
 // power of two into f16 (elements below 2^-21 of the row's largest lose bits).
@@ -138,142 +141,94 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^-n as f16 bits for n >= 0 (0 below the subnormals); n < 0 stands for infinity.
-__device__ __forceinline__ uint32_t half_pow2_neg(int n) {
-  if (n < 0) return 0x7C00u;
-  return n < 15 ? (uint32_t)(15 - n) << 10 : n < 25 ? 1u << (24 - n) : 0u;
-}
 // E8M0 byte to float32 (255 as the casts read it: infinity).
 __device__ __forceinline__ float e8m0_value(uint32_t e) {
   return e == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
 }
-template <int N>
-__device__ __forceinline__ void ldg_words(const void* p, uint32_t* w) {
-  if constexpr (N >= 4) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 v = ldg16(static_cast<const char*>(p) + 16 * i);
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (N == 2) {
-    const uint2 v = __ldg(static_cast<const uint2*>(p));
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = __ldg(static_cast<const uint32_t*>(p));
-  }
+// 2^(e - ref) of two E8M0 bytes as an f16 pair: subnormals and zero below
+// 2^-14, infinity for 255 (which never is the reference).
+__device__ __forceinline__ uint32_t half2_pow2(int e0, int e1, int ref) {
+  auto f = [&](int e) {
+    const int x = e == 255 ? 255 : max(e - ref + 127, 0);
+    return __uint_as_float((uint32_t)x << 23);
+  };
+  return half2_of(f(e0), f(e1));
 }
 
+// One step in shared memory: 16 rows of key codes, 16 of value codes, their
+// scales. A row's 16-byte pieces are permuted by its number so that the
+// operand reads below touch every bank once (64-byte rows: the value reads
+// twice).
 template <int KIND, int D>
 struct Shape {
   static constexpr bool kFp4 = KIND == BRC_STE_NVFP4;
   static constexpr int kRowBytes = kv::row_bytes(KIND, D);
+  static constexpr int kPieces = kRowBytes / 16;
   static constexpr int kScales = kv::row_scales(KIND, D);
+  static constexpr int kScaleBytes = kScales * (KIND == BRC_STE_BLOCK_FP8 ? 4 : 1);
   static constexpr int kKeyWords = kRowBytes / 16;    // per lane and token
   static constexpr int kValWords = kRowBytes / 32;    // per lane and token
+  static constexpr int kKeyRead = kKeyWords < 4 ? kKeyWords : 4;  // words to a read
+  static constexpr int kValRead = kValWords < 4 ? kValWords : 4;
   static constexpr int kSteps = D / 16;               // products along the head
-  static constexpr int kTiles = D / 8;                // output tiles of 8 elements
-  static constexpr int kKeyChunk = kKeyWords < 4 ? kKeyWords : 4;  // words loaded together
-  static constexpr int kValChunk = kValWords < 4 ? kValWords : 4;
-  static constexpr int kKeyScaleWords = KIND == BRC_STE_MXFP8 ? (D + 127) / 128 : 1;
-  // head element of output tile j, place n
-  __device__ static constexpr int elem(int j, int n) {
-    return !kFp4 && D == 256 ? 128 * (j / 16) + 16 * n + j % 16 : n * (D / 8) + j;
+  static constexpr int kTiles = D / 16;               // output tiles of 16 elements
+  static constexpr int kTileBytes = 16 * kRowBytes;
+  static constexpr int kKeyScales = 2 * kTileBytes;
+  static constexpr int kValScales = kKeyScales + 16 * kScaleBytes;
+  static constexpr int kStageBytes = kValScales + 16 * kScaleBytes;
+  __device__ static constexpr int key_piece(int t, int p) {
+    return kPieces >= 8 ? p ^ ((t & 1) << 2) : p;
+  }
+  __device__ static constexpr int val_piece(int t, int p) {
+    return kPieces >= 8 ? p ^ (t & 6) : kPieces == 4 ? p ^ (t & 2) : p;
+  }
+  // head element of a lane's output i (two to a tile), r = lane / 4
+  __device__ static constexpr int elem(int i, int r) {
+    return !kFp4 && D == 256 ? 128 * (i / 16) + 16 * r + i % 16 : r * (D / 8) + i;
   }
 };
 
-// One lane's codes and scales of a 16-token step.
-template <int KIND, int D>
-struct Keys {
-  using S = Shape<KIND, D>;
-  uint32_t w[2][S::kKeyWords];  // tokens r, r + 8
-  uint32_t s[2][2];             // block: the float scales of tokens 2c, 2c+1 (+ 8); else the
-                                // scale bytes of tokens r, r + 8
-};
-template <int KIND, int D>
-struct Vals {
-  using S = Shape<KIND, D>;
-  uint32_t w[4][S::kValWords];  // tokens 2c, 2c+1, 2c+8, 2c+9
-  uint32_t s[4][2];             // block: [0..3][0] float scales; else scale bytes per token
-};
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
+// Start the copy of the 16 rows from `row` on into a stage (a warp's own).
 template <int KIND, int D>
-__device__ __forceinline__ void load_keys(const brc_kv_cache& c, int64_t row, int lane,
-                                          Keys<KIND, D>& k) {
+__device__ __forceinline__ void copy_step(const brc_kv_cache& c, int64_t row, int lane,
+                                          uint32_t stage) {
   using S = Shape<KIND, D>;
-  const int r = lane >> 2, q = lane & 3;
+  const uint8_t* k = c.k_data + row * S::kRowBytes + lane * 16;
+  const uint8_t* v = c.v_data + row * S::kRowBytes + lane * 16;
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const uint8_t* p = c.k_data + (row + r + 8 * n) * S::kRowBytes + q * (4 * S::kKeyChunk);
-#pragma unroll
-    for (int i = 0; i < S::kKeyWords / S::kKeyChunk; ++i)
-      ldg_words<S::kKeyChunk>(p + 64 * i, &k.w[n][i * S::kKeyChunk]);
-    if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(
-          static_cast<const float*>(c.k_scale) + row + 8 * n + 2 * q));
-      k.s[n][0] = v.x;
-      k.s[n][1] = v.y;
-    } else if constexpr (KIND == BRC_STE_MXFP8) {
-      const uint8_t* sp = static_cast<const uint8_t*>(c.k_scale) + (row + r + 8 * n) * S::kScales;
-      if constexpr (D == 64) k.s[n][0] = __ldg(reinterpret_cast<const uint16_t*>(sp));
-      else ldg_words<D / 128>(sp, k.s[n]);
-    } else {
-      const uint8_t* sp = static_cast<const uint8_t*>(c.k_scale) + (row + r + 8 * n) * S::kScales;
-      if constexpr (D == 64) {
-        k.s[n][0] = __ldg(sp + q);
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 128; ++i)
-          k.s[n][i] = __ldg(reinterpret_cast<const uint16_t*>(sp + 8 * i + 2 * q));
-      }
-    }
+  for (int i = 0; i < S::kPieces / 2; ++i) {
+    const int id = lane + 32 * i, t = id / S::kPieces, p = id % S::kPieces;
+    cp16(stage + (t * S::kPieces + S::key_piece(t, p)) * 16, k + 512 * i);
+    cp16(stage + S::kTileBytes + (t * S::kPieces + S::val_piece(t, p)) * 16, v + 512 * i);
+  }
+  const int i = lane & 15;
+  if (i < S::kScaleBytes) {
+    const void* base = lane < 16 ? c.k_scale : c.v_scale;
+    cp16(stage + (lane < 16 ? S::kKeyScales : S::kValScales) + i * 16,
+         static_cast<const uint8_t*>(base) + row * S::kScaleBytes + i * 16);
   }
 }
 
-template <int KIND, int D>
-__device__ __forceinline__ void load_vals(const brc_kv_cache& c, int64_t row, int lane,
-                                          Vals<KIND, D>& v) {
-  using S = Shape<KIND, D>;
-  const int r = lane >> 2, q = lane & 3;
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t at = row + 2 * q + (t & 1) + 8 * (t >> 1);
-    const uint8_t* p = c.v_data + at * S::kRowBytes + r * (4 * S::kValChunk);
-#pragma unroll
-    for (int i = 0; i < S::kValWords / S::kValChunk; ++i)
-      ldg_words<S::kValChunk>(p + 128 * i, &v.w[t][i * S::kValChunk]);
-    if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-      v.s[t][0] = __ldg(static_cast<const uint32_t*>(c.v_scale) + at);
-    } else {
-      const uint8_t* sp = static_cast<const uint8_t*>(c.v_scale) + at * S::kScales;
-      if constexpr (KIND == BRC_STE_MXFP8) {  // the whole row's bytes: its largest is needed
-        if constexpr (D == 64) v.s[t][0] = __ldg(reinterpret_cast<const uint16_t*>(sp));
-        else ldg_words<D / 128>(sp, v.s[t]);
-      } else if constexpr (D == 256) {
-        v.s[t][0] = __ldg(reinterpret_cast<const uint16_t*>(sp + 2 * r));
-      } else {
-        v.s[t][0] = __ldg(sp + (D == 128 ? r : r >> 1));
-      }
-    }
-  }
-}
-
-// Largest byte of a scale row below 255 (255 stands for infinity and never
-// becomes the reference).
-template <int D>
-__device__ __forceinline__ uint32_t top_byte(const uint32_t* s) {
-  uint32_t m;
-  if constexpr (D == 64) {
-    m = s[0];  // two bytes
-  } else if constexpr (D == 128) {
-    m = s[0];
+template <int N>
+__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
   } else {
-    // 255 must not hide a smaller byte in the same place: taken out first
-    const uint32_t a = s[0] & ~__vcmpeq4(s[0], 0xFFFFFFFFu), b = s[1] & ~__vcmpeq4(s[1], 0xFFFFFFFFu);
-    m = __vmaxu4(a, b);
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
-  m &= ~__vcmpeq4(m, 0xFFFFFFFFu);
-  if constexpr (D != 64) m = __vmaxu4(m, m >> 16);
-  return max(m & 0xFFu, (m >> 8) & 0xFFu);
 }
 
 // True where a code word or a scale holds something that is not finite.
@@ -285,22 +240,24 @@ __device__ __forceinline__ bool odd_codes(uint32_t w) {
   else return (((w & 0x7C7C7C7Cu) + 0x04040404u) & 0x80808080u) != 0;
 }
 
-template <int KIND, int FMT, int D, int MT>
+template <int KIND, int FMT, int D, int NT>
 struct Warp {
   using S = Shape<KIND, D>;
-  float o[MT][S::kTiles][4];
-  float m[MT][2], l[MT][2];  // shift and sum of rows r, r + 8
-  int e;                     // value scales are relative to 2^e
+  float o[NT][S::kTiles][4];  // [elements 2j, 2j + 1][rows 2c, 2c + 1]
+  float m[NT][2], l[NT][2];   // shift and (the lane's part of the) sum of rows 2c, 2c + 1
+  int e;                      // value scales are relative to 2^e
+  int ke;                     // MXFP8: key scales are relative to this E8M0 byte
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < NT; ++i) {
 #pragma unroll
       for (int j = 0; j < S::kTiles; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
       m[i][0] = m[i][1] = -INFINITY;
       l[i][0] = l[i][1] = 0.f;
     }
     e = -1000;
+    ke = 0;
   }
   // Raise the reference of the value scales (a power of two) to 2^to, at least 2^-100.
   __device__ __forceinline__ void raise(int to) {
@@ -308,7 +265,7 @@ struct Warp {
     if (to <= e) return;
     const float f = e < -900 ? 1.f : __uint_as_float((uint32_t)max(127 + e - to, 0) << 23);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < S::kTiles; ++j)
 #pragma unroll
@@ -332,263 +289,372 @@ __device__ __forceinline__ float value_at(const brc_kv_cache& c, int64_t row, in
   }
 }
 
-template <int KIND, int FMT, int D, int MT>
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+
+template <int KIND, int FMT, int D, int NT>
 struct Step {
   using S = Shape<KIND, D>;
-  using W = Warp<KIND, FMT, D, MT>;
+  using W = Warp<KIND, FMT, D, NT>;
 
-  // s[mt][n][x]: scores of 16 tokens, not yet scaled by row.
-  __device__ static __forceinline__ void scores(const Keys<KIND, D>& k, const uint4* q, int lane,
-                                                float (&s)[MT][2][4]) {
+  // s[nt][2 h + x]: score of token r + 8 h and row 2c + x, in units of the rows'
+  // factors. Rows of the stage from `dead` on are past the end (their scales are
+  // not to be looked at).
+  __device__ static __forceinline__ void scores(W& w, const uint8_t* st, const uint4* q, int lane,
+                                                int dead, float (&s)[NT][4]) {
+    const int r = lane >> 2, c = lane & 3;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
-    uint32_t top[2];
+    for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    constexpr int kReads = S::kKeyWords / S::kKeyRead;
+    uint32_t f[2][kReads];  // scales of a read's codes
     if constexpr (KIND == BRC_STE_MXFP8) {
-      top[0] = top_byte<D>(k.s[0]);
-      top[1] = top_byte<D>(k.s[1]);
-    }
-#pragma unroll
-    for (int w = 0; w < S::kKeyWords; ++w) {
-      uint32_t b[2][S::kFp4 ? 4 : 2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t x = k.w[n][w];
-        if constexpr (S::kFp4) {
-          // 8 codes of one 16-element block; its E4M3 scale is exact in f16
-          uint32_t sc;
-          if constexpr (D == 64) sc = k.s[n][0] & 0xFFu;
-          else sc = (k.s[n][w / 4] >> (8 * ((w % 4) / 2))) & 0xFFu;
-          const uint32_t f = fp8x2_to_f16x2<BRC_FP8_E4M3>(sc | (sc << 8));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) b[n][i] = hmul2(kv::e2m1x2_to_f16x2(x >> (8 * i)), f);
-        } else {
-          b[n][0] = fp8x2_to_f16x2<FMT>(x);
-          b[n][1] = fp8x2_to_f16x2<FMT>(x >> 16);
-          if constexpr (KIND == BRC_STE_MXFP8) {
-            // chunk w / 4 holds elements 64 (w / 4) + 16 c ..: block 2 (w / 4) + c / 2
-            const uint32_t e =
-                (k.s[n][w / 8] >> (16 * ((w / 4) % 2) + 8 * ((lane & 3) >> 1))) & 0xFFu;
-            const uint32_t h = half_pow2_neg(e == 255 ? -1 : (int)top[n] - (int)e);
-            b[n][0] = hmul2(b[n][0], h | (h << 16));
-            b[n][1] = hmul2(b[n][1], h | (h << 16));
-          }
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < (S::kFp4 ? 2 : 1); ++g) {
-        const int ks = S::kFp4 ? 2 * w + g : w;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const uint4 a = q[(i * S::kSteps + ks) * 32 + lane];
-#pragma unroll
-          for (int n = 0; n < 2; ++n) mma(s[i][n], a, b[n][2 * g], b[n][2 * g + 1]);
-        }
-      }
-    }
-    // the token's own factor
-    float f[2][2];
-    if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        f[n][0] = __uint_as_float(k.s[n][0]);
-        f[n][1] = __uint_as_float(k.s[n][1]);
-      }
-    } else if constexpr (KIND == BRC_STE_MXFP8) {
+      int e[2][kReads], top = 0;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          f[n][i] = e8m0_value(__shfl_sync(0xFFFFFFFFu, top[n], (2 * (lane & 3) + i) * 4));
+        for (int i = 0; i < kReads; ++i) {
+          // read i holds elements 64 i + 16 c ..: block 2 i + c / 2
+          e[n][i] = r + 8 * n < dead
+                        ? st[S::kKeyScales + (r + 8 * n) * S::kScales + 2 * i + (c >> 1)] : 0;
+          if (e[n][i] != 255) top = max(top, e[n][i]);
+        }
+      if (__any_sync(0xFFFFFFFFu, top > w.ke)) w.ke = max(w.ke, (int)__reduce_max_sync(0xFFFFFFFFu, top));
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) f[n][i] = half2_pow2(e[n][i], e[n][i], w.ke);
     }
-    if constexpr (KIND != BRC_STE_NVFP4) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < kReads; ++i) {
+      uint32_t x[2][S::kKeyRead];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 2; ++n) {
+        const int t = r + 8 * n;
+        const uint8_t* p;
+        if constexpr (S::kKeyRead == 4)
+          p = st + (t * S::kPieces + S::key_piece(t, 4 * i + c)) * 16;
+        else p = st + t * S::kRowBytes + c * 8;
+        lds_words<S::kKeyRead>(p, x[n]);
+        if constexpr (S::kFp4) {
+          // a read is one or two 16-element blocks with their scales
+          const uint8_t* sp = st + S::kKeyScales + t * S::kScales;
+          if constexpr (D == 64) f[n][i] = sp[c];
+          else f[n][i] = *reinterpret_cast<const uint16_t*>(sp + 8 * i + 2 * c);
+        }
+      }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[i][n][x] *= f[n][x & 1];
+      for (int y = 0; y < S::kKeyRead; ++y) {
+        constexpr int kPer = S::kFp4 ? 2 : 1;  // products to a word
+        uint4 a[kPer];
+        if constexpr (S::kFp4) {
+          const uint32_t g0 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(f[0][i], 0, y < 2 ? 0x0000 : 0x0011));
+          const uint32_t g1 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(f[1][i], 0, y < 2 ? 0x0000 : 0x0011));
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            a[z].x = hmul2(kv::e2m1x2_to_f16x2(x[0][y] >> (16 * z)), g0);
+            a[z].y = hmul2(kv::e2m1x2_to_f16x2(x[1][y] >> (16 * z)), g1);
+            a[z].z = hmul2(kv::e2m1x2_to_f16x2(x[0][y] >> (16 * z + 8)), g0);
+            a[z].w = hmul2(kv::e2m1x2_to_f16x2(x[1][y] >> (16 * z + 8)), g1);
+          }
+        } else {
+          a[0].x = fp8x2_to_f16x2<FMT>(x[0][y]);
+          a[0].y = fp8x2_to_f16x2<FMT>(x[1][y]);
+          a[0].z = fp8x2_to_f16x2<FMT>(x[0][y] >> 16);
+          a[0].w = fp8x2_to_f16x2<FMT>(x[1][y] >> 16);
+          if constexpr (KIND == BRC_STE_MXFP8) {
+            a[0].x = hmul2(a[0].x, f[0][i]);
+            a[0].y = hmul2(a[0].y, f[1][i]);
+            a[0].z = hmul2(a[0].z, f[0][i]);
+            a[0].w = hmul2(a[0].w, f[1][i]);
+          }
+        }
+        const int ks = kPer * (S::kKeyRead * i + y);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 b = q[(n * (S::kSteps / 2) + ks / 2) * 32 + lane];
+          if constexpr (S::kFp4) {
+            mma(s[n], a[0], b.x, b.y);
+            mma(s[n], a[1], b.z, b.w);
+          } else {
+            if (ks & 1) mma(s[n], a[0], b.z, b.w);
+            else mma(s[n], a[0], b.x, b.y);
+          }
+        }
+      }
+    }
+    if constexpr (KIND == BRC_STE_BLOCK_FP8) {  // the token's own factor
+      const float g0 = *reinterpret_cast<const float*>(st + S::kKeyScales + r * 4);
+      const float g1 = *reinterpret_cast<const float*>(st + S::kKeyScales + (r + 8) * 4);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n][0] *= g0;
+        s[n][1] *= g0;
+        s[n][2] *= g1;
+        s[n][3] *= g1;
+      }
     }
   }
 
   // Running maximum and sum; s becomes the probabilities relative to the shift.
-  __device__ static __forceinline__ void softmax(W& w, float (&s)[MT][2][4]) {
+  __device__ static __forceinline__ void softmax(W& w, float (&s)[NT][4]) {
     bool grow = false;
-    float top[MT][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[i][h] = fmaxf(fmaxf(s[i][0][2 * h], s[i][0][2 * h + 1]),
-                          fmaxf(s[i][1][2 * h], s[i][1][2 * h + 1]));
-        grow |= top[i][h] > w.m[i][h] + kGrow;
-      }
+      for (int x = 0; x < 2; ++x) grow |= fmaxf(s[n][x], s[n][2 + x]) > w.m[n][x] + kGrow;
     if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float t = top[i][h];
-          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
-          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
-          const float m = fmaxf(w.m[i][h], t);
-          const float f = m == w.m[i][h] ? 1.f : ex2(w.m[i][h] - m);
-          w.m[i][h] = m;
-          w.l[i][h] *= f;
+        for (int x = 0; x < 2; ++x) {
+          float t = fmaxf(s[n][x], s[n][2 + x]);
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
+          const float m = fmaxf(w.m[n][x], t);
+          const float f = m == w.m[n][x] ? 1.f : ex2(w.m[n][x] - m);
+          w.m[n][x] = m;
+          w.l[n][x] *= f;
 #pragma unroll
           for (int j = 0; j < S::kTiles; ++j) {
-            w.o[i][j][2 * h] *= f;
-            w.o[i][j][2 * h + 1] *= f;
+            w.o[n][j][x] *= f;
+            w.o[n][j][2 + x] *= f;
           }
         }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float m = w.m[i][h] == -INFINITY ? 0.f : w.m[i][h];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int x = 2 * h; x < 2 * h + 2; ++x) {
-            s[i][n][x] = ex2(s[i][n][x] - m);
-            w.l[i][h] += s[i][n][x];
-          }
+      for (int x = 0; x < 2; ++x) {
+        const float m = w.m[n][x] == -INFINITY ? 0.f : w.m[n][x];
+        s[n][x] = ex2(s[n][x] - m);
+        s[n][2 + x] = ex2(s[n][2 + x] - m);
+        w.l[n][x] += s[n][x] + s[n][2 + x];
       }
   }
 
-  // o += p v. Probabilities carry a factor 2^6 (at most 2^8 before it), so that
-  // f16 keeps those down to 2^-30 of the largest.
-  __device__ static __forceinline__ void values(W& w, const Vals<KIND, D>& v, int lane,
-                                                const float (&p)[MT][2][4]) {
-    float f[4] = {64.f, 64.f, 64.f, 64.f};
+  // o += v^T p. Probabilities carry a factor 2^6 (at most 2^8 before it), so that
+  // f16 keeps those down to 2^-30 of the largest. TWO: a second product with
+  // what the rounding to f16 left (f16 outputs of few rows: its 2^-11 would
+  // show beside the output's own).
+  template <bool TWO>
+  __device__ static __forceinline__ void values(W& w, const uint8_t* st, int lane, int dead,
+                                                const float (&p)[NT][4]) {
+    const int r = lane >> 2, c = lane & 3;
+    auto token = [&](int t) { return 2 * c + (t & 1) + 8 * (t >> 1); };
+    float f[2] = {64.f, 64.f};  // of tokens r, r + 8
+    constexpr int kReads = S::kValWords / S::kValRead;
     uint32_t h[2][2];  // [token pair][half of the lane's elements]: f16 pair of value factors
     if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (v.s[t][0] < 0x7F800000u) top = max(top, v.s[t][0]);
+      const uint32_t* sp = reinterpret_cast<const uint32_t*>(st + S::kValScales);
+      const uint32_t s0 = r < dead ? sp[r] : 0u, s1 = r + 8 < dead ? sp[r + 8] : 0u;
+      const uint32_t top = max(s0 < 0x7F800000u ? s0 : 0u, s1 < 0x7F800000u ? s1 : 0u);
       if (__any_sync(0xFFFFFFFFu, (int)(top >> 23) - 127 > w.e))
         w.raise((int)(__reduce_max_sync(0xFFFFFFFFu, top) >> 23) - 127);
-      const float r = __uint_as_float((uint32_t)(127 - w.e + 6) << 23);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) f[t] = __uint_as_float(v.s[t][0]) * r;
+      const float g = __uint_as_float((uint32_t)(127 - w.e + 6) << 23);
+      f[0] = __uint_as_float(s0) * g;
+      f[1] = __uint_as_float(s1) * g;
     } else if constexpr (KIND == BRC_STE_MXFP8) {
-      uint32_t top = 0;
+      int e[4][2], top = 0;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) top = max(top, top_byte<D>(v.s[t]));
-      if (__any_sync(0xFFFFFFFFu, (int)top - 127 > w.e))
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) {
+          const int blk = D == 64 ? r >> 2 : 4 * i + (r >> 1);
+          e[t][i] = token(t) < dead ? st[S::kValScales + token(t) * S::kScales + blk] : 0;
+          if (e[t][i] != 255) top = max(top, e[t][i]);
+        }
+      if (__any_sync(0xFFFFFFFFu, top - 127 > w.e))
         w.raise((int)__reduce_max_sync(0xFFFFFFFFu, top) - 127);
 #pragma unroll
-      for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
-        const int r = lane >> 2, blk = D == 64 ? r >> 2 : 4 * i + (r >> 1);
+      for (int i = 0; i < kReads; ++i)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          uint32_t x[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t e = (v.s[2 * t + u][i] >> (8 * (blk % 4))) & 0xFFu;
-            x[u] = half_pow2_neg(e == 255 ? -1 : w.e + 127 - (int)e);
-          }
-          h[t][i] = x[0] | (x[1] << 16);
-        }
-      }
+        for (int t = 0; t < 2; ++t) h[t][i] = half2_pow2(e[2 * t][i], e[2 * t + 1][i], w.e + 127);
     } else {
       if (w.e < -900) w.e = 0;
 #pragma unroll
-      for (int i = 0; i < (D == 256 ? 2 : 1); ++i)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          h[t][i] = fp8x2_to_f16x2<BRC_FP8_E4M3>(((v.s[2 * t][0] >> (8 * i)) & 0xFFu) |
-                                                 (((v.s[2 * t + 1][0] >> (8 * i)) & 0xFFu) << 8));
-    }
-    uint4 a[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      a[i].x = half2_of(p[i][0][0] * f[0], p[i][0][1] * f[1]);
-      a[i].y = half2_of(p[i][0][2] * f[0], p[i][0][3] * f[1]);
-      a[i].z = half2_of(p[i][1][0] * f[2], p[i][1][1] * f[3]);
-      a[i].w = half2_of(p[i][1][2] * f[2], p[i][1][3] * f[3]);
-    }
-#pragma unroll
-    for (int x = 0; x < S::kValWords; ++x) {
-      constexpr int kPer = S::kFp4 ? 8 : 4;  // output tiles per word
-      uint32_t b[2][kPer];
-#pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const uint32_t u = v.w[2 * t][x], y = v.w[2 * t + 1][x];
-        if constexpr (S::kFp4) {
-          const uint32_t lo = (u & 0x0F0F0F0Fu) | ((y & 0x0F0F0F0Fu) << 4);
-          const uint32_t hi = ((u >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u);
-          const uint32_t s = h[t][D == 256 ? x / 2 : 0];
+        uint32_t g[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            b[t][2 * i] = hmul2(kv::e2m1x2_to_f16x2(lo >> (8 * i)), s);
-            b[t][2 * i + 1] = hmul2(kv::e2m1x2_to_f16x2(hi >> (8 * i)), s);
-          }
-        } else {
-          const uint32_t lo = __byte_perm(u, y, 0x5140), hi = __byte_perm(u, y, 0x7362);
-          b[t][0] = fp8x2_to_f16x2<FMT>(lo);
-          b[t][1] = fp8x2_to_f16x2<FMT>(lo >> 16);
-          b[t][2] = fp8x2_to_f16x2<FMT>(hi);
-          b[t][3] = fp8x2_to_f16x2<FMT>(hi >> 16);
-          if constexpr (KIND == BRC_STE_MXFP8) {
+        for (int u = 0; u < 2; ++u) {
+          const uint8_t* sp = st + S::kValScales + token(2 * t + u) * S::kScales;
+          if constexpr (D == 256) g[u] = *reinterpret_cast<const uint16_t*>(sp + 2 * r);
+          else g[u] = sp[D == 128 ? r : r >> 1];
+          if (token(2 * t + u) >= dead) g[u] = 0;
+        }
+        h[t][0] = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(g[0], g[1], 0x0040));
+        if constexpr (D == 256)
+          h[t][1] = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(g[0], g[1], 0x0051));
+      }
+    }
+    uint32_t b[NT][2], b2[NT][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) b[t][i] = hmul2(b[t][i], h[t][D == 256 ? x / 4 : 0]);
-          }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float x = p[n][2 * u] * f[u], y = p[n][2 * u + 1] * f[u];
+        const uint32_t hi = half2_of(x, y);
+        b[n][u] = transpose8(hi);
+        if constexpr (TWO) {
+          const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+          b2[n][u] = transpose8(half2_of(x - g.x, y - g.y));
         }
       }
 #pragma unroll
-      for (int j = 0; j < kPer; ++j)
+    for (int i = 0; i < kReads; ++i) {
+      uint32_t x[4][S::kValRead];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) mma(w.o[i][kPer * x + j], a[i], b[0][j], b[1][j]);
+      for (int t = 0; t < 4; ++t) {
+        const int tk = token(t);
+        const uint8_t* base = st + S::kTileBytes;
+        const uint8_t* q;
+        if constexpr (S::kValRead == 4)
+          q = base + (tk * S::kPieces + S::val_piece(tk, 8 * i + r)) * 16;
+        else if constexpr (S::kValRead == 2)
+          q = base + (tk * S::kPieces + S::val_piece(tk, r >> 1)) * 16 + (r & 1) * 8;
+        else q = base + tk * S::kRowBytes + r * 4;
+        lds_words<S::kValRead>(q, x[t]);
+      }
+      if (dead < 16) {  // rows past the end hold anything
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int y = 0; y < S::kValRead; ++y)
+            if (token(t) >= dead) x[t][y] = 0;
+      }
+#pragma unroll
+      for (int y = 0; y < S::kValRead; ++y) {
+        constexpr int kPer = S::kFp4 ? 8 : 4;  // elements to a word
+        uint32_t a[2][kPer];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t u = x[2 * t][y], v = x[2 * t + 1][y];
+          if constexpr (S::kFp4) {
+            const uint32_t lo = (u & 0x0F0F0F0Fu) | ((v & 0x0F0F0F0Fu) << 4);
+            const uint32_t hi = ((u >> 4) & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u);
+            const uint32_t g = h[t][D == 256 ? y / 2 : 0];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              a[t][2 * z] = hmul2(kv::e2m1x2_to_f16x2(lo >> (8 * z)), g);
+              a[t][2 * z + 1] = hmul2(kv::e2m1x2_to_f16x2(hi >> (8 * z)), g);
+            }
+          } else {
+            const uint32_t lo = __byte_perm(u, v, 0x5140), hi = __byte_perm(u, v, 0x7362);
+            a[t][0] = fp8x2_to_f16x2<FMT>(lo);
+            a[t][1] = fp8x2_to_f16x2<FMT>(lo >> 16);
+            a[t][2] = fp8x2_to_f16x2<FMT>(hi);
+            a[t][3] = fp8x2_to_f16x2<FMT>(hi >> 16);
+            if constexpr (KIND == BRC_STE_MXFP8) {
+#pragma unroll
+              for (int z = 0; z < 4; ++z) a[t][z] = hmul2(a[t][z], h[t][i]);
+            }
+          }
+        }
+#pragma unroll
+        for (int z = 0; z < kPer / 2; ++z) {
+          const uint4 av = make_uint4(a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1]);
+          const int j = kPer / 2 * (S::kValRead * i + y) + z;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma(w.o[n][j], av, b[n][0], b[n][1]);
+            if constexpr (TWO) mma(w.o[n][j], av, b2[n][0], b2[n][1]);
+          }
+        }
+      }
     }
+  }
+
+  // Does any value of the step's live rows stand for something not finite?
+  __device__ static __forceinline__ bool odd_values(const uint8_t* st, int lane, int dead) {
+    bool odd = false;
+    // lane: row lane / 2, half of its bytes
+    const int t = lane >> 1;
+    if (t < dead) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(st + S::kTileBytes + t * S::kRowBytes) +
+                          (lane & 1) * (S::kRowBytes / 8);
+      for (int i = 0; i < S::kRowBytes / 8; ++i) odd |= odd_codes<KIND, FMT>(p[i]);
+      const uint8_t* sp = st + S::kValScales + t * S::kScaleBytes;
+      if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+        odd |= (*reinterpret_cast<const uint32_t*>(sp) & 0x7F800000u) == 0x7F800000u;
+      } else {
+        for (int i = 0; i < S::kScales; ++i)
+          odd |= KIND == BRC_STE_NVFP4 ? (sp[i] & 0x7F) == 0x7F : sp[i] == 255;
+      }
+    }
+    return __any_sync(0xFFFFFFFFu, odd);
   }
 
   // The same for a step whose values are not all finite: token by token, only
   // where the row sees the token, so that what it does not see cannot reach it.
   __device__ static __forceinline__ void values_checked(W& w, const brc_kv_cache& c, int64_t row,
-                                                        int lane, const float (&p)[MT][2][4],
+                                                        int lane, const float (&p)[NT][4],
                                                         uint32_t seen) {
     if (w.e < -900) w.e = 0;
-    const float r = 64.f * exp2f((float)-w.e);
+    const float f = 64.f * exp2f((float)-w.e);
     for (int t = 0; t < 16; ++t) {
-      const int n = t >> 3, x = t & 1, src = (lane & ~3) | ((t & 7) >> 1);
-      float pr[MT][2];
+      const int half = t >> 3, src = (t & 7) * 4 + (lane & 3);
+      float pr[NT][2];
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float lo = n ? p[i][1][2 * h] : p[i][0][2 * h];
-          const float hi = n ? p[i][1][2 * h + 1] : p[i][0][2 * h + 1];
-          pr[i][h] = __shfl_sync(0xFFFFFFFFu, x ? hi : lo, src);
-        }
-      const uint32_t sees = __shfl_sync(0xFFFFFFFFu, seen, src);
+        for (int x = 0; x < 2; ++x)
+          pr[n][x] = __shfl_sync(0xFFFFFFFFu, half ? p[n][2 + x] : p[n][x], src) * f;
+      const uint32_t sees = __shfl_sync(0xFFFFFFFFu, seen, src) >> (2 * half);
 #pragma unroll
       for (int j = 0; j < S::kTiles; ++j)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float v = value_at<KIND, FMT, D>(c, row + t, S::elem(j, 2 * (lane & 3) + u));
+          const float v = value_at<KIND, FMT, D>(c, row + t, S::elem(2 * j + u, lane >> 2));
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if ((sees >> (((i * 2 + h) * 2 + n) * 2 + x)) & 1u) w.o[i][j][2 * h + u] += pr[i][h] * r * v;
+            for (int x = 0; x < 2; ++x)
+              if ((sees >> (4 * n + x)) & 1u) w.o[n][j][2 * u + x] += pr[n][x] * v;
         }
     }
   }
 };
 
-template <int KIND, int FMT, int D, int MT>
-__global__ void __launch_bounds__(kThreads) k_attend(Args a) {
+// Blocks that an SM is to hold, as many as the accumulators' registers allow.
+constexpr __host__ __device__ int blocks_per_sm(int d, int nt) {
+  return d * nt <= 128 ? 4 : d * nt <= 256 ? 3 : 2;
+}
+// Stages of a warp's ring: what fits beside the queries in the block's part of
+// shared memory, at most 6.
+constexpr __host__ __device__ int stage_bytes(int kind, int d) {
+  return 2 * 16 * (kv::row_bytes(kind, d) + kv::row_scales(kind, d) * (kind == BRC_STE_BLOCK_FP8 ? 4 : 1));
+}
+// Row warps of a block: more than one only with the largest row tile.
+constexpr __host__ __device__ int most_tiles(int d) { return d == 256 ? 2 : 4; }
+constexpr __host__ __device__ int query_bytes(int d, int nt) {
+  return (nt == most_tiles(d) ? kWarps : 1) * 8 * nt * d * 2;
+}
+constexpr __host__ __device__ int stages(int kind, int d, int nt) {
+  const int room = (227 * 1024) / blocks_per_sm(d, nt) - 2048 - query_bytes(d, nt);
+  const int n = room / (kWarps * stage_bytes(kind, d));
+  return n > 6 ? 6 : n;
+}
+constexpr __host__ __device__ int ring_bytes(int kind, int d, int nt) {
+  const int r = kWarps * stages(kind, d, nt) * stage_bytes(kind, d);
+  const int o = kWarps * 8 * nt * (d + 4) * 4;  // the warps' outputs
+  return r > o ? r : o;
+}
+
+template <int KIND, int FMT, int D, int NT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args a) {
   using S = Shape<KIND, D>;
-  using St = Step<KIND, FMT, D, MT>;
+  using St = Step<KIND, FMT, D, NT>;
+  constexpr int kStages = stages(KIND, D, NT);
+  constexpr bool kTwo = NT <= 2;
   extern __shared__ __align__(16) uint8_t smem[];
-  // queries as operand fragments, and (later) the warps' outputs
-  uint4* const sq = reinterpret_cast<uint4*>(smem);
+  // the warps' stages (later: their outputs), then the queries as operand fragments
+  uint8_t* const rings = smem;
   float* const so = reinterpret_cast<float*>(smem);
-  __shared__ float s_m[kWarps][16 * MT], s_l[kWarps][16 * MT], s_rowf[kWarps * 16 * MT];
+  uint4* const sq = reinterpret_cast<uint4*>(smem + ring_bytes(KIND, D, NT));
+  __shared__ float s_m[kWarps][8 * NT], s_l[kWarps][8 * NT], s_rowf[kWarps * 8 * NT];
   __shared__ Place s_place;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -643,43 +709,41 @@ __global__ void __launch_bounds__(kThreads) k_attend(Args a) {
         const float up = __uint_as_float((uint32_t)(127 + 7 - k) << 23);
         if (part == 0) s_rowf[rr] = a.scale_log2 * __uint_as_float((uint32_t)(127 + k - 7) << 23);
         uint32_t* const dst = reinterpret_cast<uint32_t*>(sq);
-        const int mt = rr >> 4, r16 = rr & 15;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = d0 + 2 * i;  // pair d, d + 1
           int ks, c, j;
           if constexpr (S::kFp4) {
-            constexpr int kLane = 8 * S::kKeyChunk;  // elements of a lane's chunk
+            constexpr int kLane = 8 * S::kKeyRead;  // elements of a lane's chunk
             const int in = d % (4 * kLane);
             c = in / kLane;
-            ks = (d / (4 * kLane)) * (2 * S::kKeyChunk) + (in % kLane) / 4;
+            ks = (d / (4 * kLane)) * (2 * S::kKeyRead) + (in % kLane) / 4;
             j = d % 4;
           } else {
             c = (d % 64) / 16;
             ks = (d / 64) * 4 + (d % 16) / 4;
             j = d % 4;
           }
-          const int reg = (j >> 1) * 2 + (r16 >> 3);
-          dst[((mt * S::kSteps + ks) * 32 + (r16 & 7) * 4 + c) * 4 + reg] =
+          dst[(((rr >> 3) * (S::kSteps / 2) + ks / 2) * 32 + (rr & 7) * 4 + c) * 4 + (ks & 1) * 2 + (j >> 1)] =
               half2_of(f[2 * i] * up, f[2 * i + 1] * up);
         }
       }
     }
     __syncthreads();
 
-    Warp<KIND, FMT, D, MT> w;
+    Warp<KIND, FMT, D, NT> w;
     w.clear();
-    const uint4* const q = sq + (int64_t)rw * MT * S::kSteps * 32;
-    float rowf[MT][2];
-    int node[MT][2];
+    const uint4* const q = sq + rw * NT * (S::kSteps / 2) * 32;
+    float rowf[NT][2];
+    int node[NT][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int rr = (rw * MT + i) * 16 + (lane >> 2) + 8 * h;
-        rowf[i][h] = s_rowf[rr];
+      for (int x = 0; x < 2; ++x) {
+        const int rr = (rw * NT + n) * 8 + 2 * (lane & 3) + x;
+        rowf[n][x] = s_rowf[rr];
         const int row = row0 + rr;
-        node[i][h] = row < a.rows ? row / a.group : a.draft;
+        node[n][x] = row < a.rows ? row / a.group : a.draft;
       }
 
     const int32_t* const table = a.table + b * a.table_stride;
@@ -691,105 +755,102 @@ __global__ void __launch_bounds__(kThreads) k_attend(Args a) {
       if (page < 0 || page >= a.c.num_pages) return -1;
       return (page * a.c.heads + head) * a.c.page_size + (t & page_mask);
     };
-    Keys<KIND, D> k;
-    Vals<KIND, D> v;
-    int s = s_begin + tw;
-    int64_t row = s < s_end ? row_at(s) : -1;
-    if (row >= 0) {
-      load_keys<KIND, D>(a.c, row, lane, k);
-      load_vals<KIND, D>(a.c, row, lane, v);
-    }
-    while (s < s_end) {
-      const int sn = s + token_warps;
-      const int64_t row_n = sn < s_end ? row_at(sn) : -1;
-      if (row >= 0) {
-        float p[MT][2][4];
-        St::scores(k, q, lane, p);
-        if (row_n >= 0) load_keys<KIND, D>(a.c, row_n, lane, k);
+    // the warp's own ring of stages
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rings) + warp * (kStages * S::kStageBytes);
+    const uint8_t* const ring_p = rings + warp * (kStages * S::kStageBytes);
+    uint32_t there = 0;  // bit i: the step i places behind the newest has a page
+    int s = s_begin + tw, ahead = s, slot_in = 0, slot_out = 0;
+    auto fetch = [&]() {
+      const int64_t row = ahead < s_end ? row_at(ahead) : -1;
+      if (row >= 0) copy_step<KIND, D>(a.c, row, lane, ring + slot_in * S::kStageBytes);
+      cp_commit();
+      there = there << 1 | (row >= 0 ? 1u : 0u);
+      ahead += token_warps;
+      slot_in = slot_in + 1 == kStages ? 0 : slot_in + 1;
+    };
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) p[i][n][y] *= rowf[i][y >> 1];
+    for (int i = 0; i < kStages - 1; ++i) fetch();
+    for (; s < s_end; s += token_warps) {
+      cp_wait<kStages - 2>();
+      __syncwarp();  // every lane's pieces are there, and the oldest stage is read
+      fetch();
+      if (there >> (kStages - 1) & 1u) {
+        const uint8_t* const st = ring_p + slot_out * S::kStageBytes;
         const int t0 = s << 4;
+        const int dead = min(seq.total - t0, 16);  // live rows
+        float p[NT][4];
+        St::scores(w, st, q, lane, dead, p);
+        const float kf = KIND == BRC_STE_MXFP8 ? e8m0_value(w.ke) : 1.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float f = KIND == BRC_STE_MXFP8 ? rowf[n][x] * kf : rowf[n][x];
+            p[n][x] *= f;
+            p[n][2 + x] *= f;
+          }
         uint32_t seen = 0;
         bool checked = false;
         if (t0 + 16 > seq.context) {  // drafted tokens, or past the end
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  const int t = t0 + n * 8 + 2 * (lane & 3) + y, j = t - seq.context;
-                  bool see = t < seq.total && node[i][h] < seq.drafts;
-                  if (see && j >= 0)
-                    see = a.tree ? a.tree[b * a.tree_stride + (int64_t)node[i][h] * a.draft + j] != 0
-                                 : j <= node[i][h];
-                  if (see) seen |= 1u << (((i * 2 + h) * 2 + n) * 2 + y);
-                  else p[i][n][2 * h + y] = -INFINITY;
-                }
-          // values past the end count as zero; a drafted value that is not
-          // finite must not meet a probability of zero in the product
-          bool odd = false;
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const bool live = t0 + 2 * (lane & 3) + (t & 1) + 8 * (t >> 1) < seq.total;
-#pragma unroll
-            for (int y = 0; y < S::kValWords; ++y) {
-              if (!live) v.w[t][y] = 0;
-              odd |= odd_codes<KIND, FMT>(v.w[t][y]);
-            }
-            if (!live) v.s[t][0] = v.s[t][1] = 0;
-            if constexpr (KIND == BRC_STE_BLOCK_FP8) odd |= (v.s[t][0] & 0x7F800000u) == 0x7F800000u;
-            else if constexpr (KIND == BRC_STE_NVFP4)
-              odd |= (v.s[t][0] & 0x7Fu) == 0x7Fu || (D == 256 && (v.s[t][0] & 0x7F00u) == 0x7F00u);
-            else
-              odd |= __vcmpeq4(v.s[t][0], 0xFFFFFFFFu) != 0 ||
-                     (D == 256 && __vcmpeq4(v.s[t][1], 0xFFFFFFFFu) != 0);
-          }
-          checked = __any_sync(0xFFFFFFFFu, odd);
+              for (int x = 0; x < 2; ++x) {
+                const int t = t0 + (lane >> 2) + 8 * h, j = t - seq.context;
+                bool see = t < seq.total && node[n][x] < seq.drafts;
+                if (see && j >= 0)
+                  see = a.tree ? a.tree[b * a.tree_stride + (int64_t)node[n][x] * a.draft + j] != 0
+                               : j <= node[n][x];
+                if (see) seen |= 1u << (4 * n + 2 * h + x);
+                else p[n][2 * h + x] = -INFINITY;
+              }
+          // a drafted value that is not finite must not meet a probability of
+          // zero in the product
+          checked = St::odd_values(st, lane, dead);
         }
         St::softmax(w, p);
-        if (checked) St::values_checked(w, a.c, row, lane, p, seen);
-        else St::values(w, v, lane, p);
-      } else if (row_n >= 0) {
-        load_keys<KIND, D>(a.c, row_n, lane, k);
+        if (checked) {
+          St::values_checked(w, a.c, row_at(s), lane, p, seen);
+        } else if constexpr (kTwo) {
+          if (a.q_f16) St::template values<true>(w, st, lane, dead, p);
+          else St::template values<false>(w, st, lane, dead, p);
+        } else {
+          St::template values<false>(w, st, lane, dead, p);
+        }
       }
-      if (row_n >= 0) load_vals<KIND, D>(a.c, row_n, lane, v);
-      row = row_n;
-      s = sn;
+      slot_out = slot_out + 1 == kStages ? 0 : slot_out + 1;
     }
+    cp_wait<0>();
 
     // ---- join the warps that share rows
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float l = w.l[i][h];
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-        if ((lane & 3) == 0) {
-          const int rr = i * 16 + (lane >> 2) + 8 * h;
-          s_m[warp][rr] = w.m[i][h];
-          s_l[warp][rr] = l;
+      for (int x = 0; x < 2; ++x) {
+        float l = w.l[n][x];
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 4);
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 8);
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
+        if (lane < 4) {
+          s_m[warp][8 * n + 2 * lane + x] = w.m[n][x];
+          s_l[warp][8 * n + 2 * lane + x] = l;
         }
       }
-    __syncthreads();  // the query fragments are no longer read
+    __syncthreads();  // the stages are no longer read
     const float scale_o = w.e < -900 ? 1.f : exp2f((float)(w.e - 6));
     constexpr int kPitch = D + 4;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < S::kTiles; ++j)
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int rr = i * 16 + (lane >> 2) + 8 * (y >> 1);
-          so[(warp * 16 * MT + rr) * kPitch + S::elem(j, 2 * (lane & 3) + (y & 1))] =
-              w.o[i][j][y] * scale_o;
+        for (int j = 0; j < S::kTiles; j += 2) {
+          const int rr = 8 * n + 2 * (lane & 3) + x;
+          *reinterpret_cast<float4*>(so + (warp * 8 * NT + rr) * kPitch + S::elem(2 * j, lane >> 2)) =
+              make_float4(w.o[n][j][x] * scale_o, w.o[n][j][2 + x] * scale_o,
+                          w.o[n][j + 1][x] * scale_o, w.o[n][j + 1][2 + x] * scale_o);
         }
     __syncthreads();
     const bool whole = s_begin == 0 && s_end == seq.steps;
@@ -798,7 +859,7 @@ __global__ void __launch_bounds__(kThreads) k_attend(Args a) {
       const int rr = at / (D / 4), d = (at - rr * (D / 4)) * 4;
       const int row = row0 + rr;
       if (row >= a.rows) continue;
-      const int w0 = rr / (16 * MT), r = rr - w0 * 16 * MT;  // row warp, row in its tile
+      const int w0 = rr / (8 * NT), r = rr - w0 * 8 * NT;  // row warp, row in its tile
       float m = -INFINITY;
       for (int t = 0; t < token_warps; ++t) m = fmaxf(m, s_m[t * row_warps + w0][r]);
       float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -806,7 +867,7 @@ __global__ void __launch_bounds__(kThreads) k_attend(Args a) {
         const int wi = t * row_warps + w0;
         const float f = m == -INFINITY ? 1.f : ex2(s_m[wi][r] - m);
         l += s_l[wi][r] * f;
-        const float4 y = *reinterpret_cast<const float4*>(so + (wi * 16 * MT + r) * kPitch + d);
+        const float4 y = *reinterpret_cast<const float4*>(so + (wi * 8 * NT + r) * kPitch + d);
         o[0] += y.x * f;
         o[1] += y.y * f;
         o[2] += y.z * f;
@@ -923,20 +984,14 @@ __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
 }
 
 // ------------------------------------------------------------------ host
-constexpr int smem_bytes(int d, int mt) {
-  const int q = kWarps * 16 * mt * d * 2;              // query fragments, most row warps
-  const int o = kWarps * 16 * mt * (d + 4) * 4;        // the warps' outputs
-  return q > o ? q : o;
-}
-constexpr int kBlocksPerSm = 4;  // at most; what fits is asked of the driver
-
-template <int KIND, int FMT, int D, int MT>
+template <int KIND, int FMT, int D, int NT>
 int launch(Args a, int blocks, cudaStream_t st) {
-  constexpr int bytes = smem_bytes(D, MT);
+  constexpr int bytes = ring_bytes(KIND, D, NT) + query_bytes(D, NT);
+  static_assert(stages(KIND, D, NT) >= 2, "a ring needs two stages");
   if (const int rc = check_cuda(cudaFuncSetAttribute(
-          k_attend<KIND, FMT, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)))
+          k_attend<KIND, FMT, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)))
     return rc;
-  k_attend<KIND, FMT, D, MT><<<blocks, kThreads, bytes, st>>>(a);
+  k_attend<KIND, FMT, D, NT><<<blocks, kThreads, bytes, st>>>(a);
   if (const int rc = check_launch()) return rc;
   const int64_t warps = (int64_t)a.batch * a.c.heads * a.row_blocks * a.rows_per_block;
   k_join<D><<<(unsigned)((warps + kWarps - 1) / kWarps), kThreads, 0, st>>>(a, blocks);
@@ -944,21 +999,24 @@ int launch(Args a, int blocks, cudaStream_t st) {
 }
 
 template <int KIND, int FMT>
-int by_shape(const Args& a, int mt, int blocks, cudaStream_t st) {
+int by_shape(const Args& a, int nt, int blocks, cudaStream_t st) {
   switch (a.c.head_dim) {
-    case 64: return mt == 1 ? launch<KIND, FMT, 64, 1>(a, blocks, st)
-                            : launch<KIND, FMT, 64, 2>(a, blocks, st);
-    case 128: return mt == 1 ? launch<KIND, FMT, 128, 1>(a, blocks, st)
-                             : launch<KIND, FMT, 128, 2>(a, blocks, st);
-    default: return launch<KIND, FMT, 256, 1>(a, blocks, st);
+    case 64: return nt == 1 ? launch<KIND, FMT, 64, 1>(a, blocks, st)
+                  : nt == 2 ? launch<KIND, FMT, 64, 2>(a, blocks, st)
+                            : launch<KIND, FMT, 64, 4>(a, blocks, st);
+    case 128: return nt == 1 ? launch<KIND, FMT, 128, 1>(a, blocks, st)
+                   : nt == 2 ? launch<KIND, FMT, 128, 2>(a, blocks, st)
+                             : launch<KIND, FMT, 128, 4>(a, blocks, st);
+    default: return nt == 1 ? launch<KIND, FMT, 256, 1>(a, blocks, st)
+                            : launch<KIND, FMT, 256, 2>(a, blocks, st);
   }
 }
 
-int attend_block_e4m3(const Args& a, int mt, int blocks, cudaStream_t st);
-int attend_block_e5m2(const Args& a, int mt, int blocks, cudaStream_t st);
-int attend_mx_e4m3(const Args& a, int mt, int blocks, cudaStream_t st);
-int attend_mx_e5m2(const Args& a, int mt, int blocks, cudaStream_t st);
-int attend_nvfp4(const Args& a, int mt, int blocks, cudaStream_t st);
+int attend_block_e4m3(const Args& a, int nt, int blocks, cudaStream_t st);
+int attend_block_e5m2(const Args& a, int nt, int blocks, cudaStream_t st);
+int attend_mx_e4m3(const Args& a, int nt, int blocks, cudaStream_t st);
+int attend_mx_e5m2(const Args& a, int nt, int blocks, cudaStream_t st);
+int attend_nvfp4(const Args& a, int nt, int blocks, cudaStream_t st);
 
 }  // namespace kvatt
 }  // namespace brc

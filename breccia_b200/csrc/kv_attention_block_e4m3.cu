@@ -3,8 +3,8 @@
 
 namespace brc {
 namespace kvatt {
-int attend_block_e4m3(const Args& a, int mt, int blocks, cudaStream_t st) {
-  return by_shape<BRC_STE_BLOCK_FP8, BRC_FP8_E4M3>(a, mt, blocks, st);
+int attend_block_e4m3(const Args& a, int nt, int blocks, cudaStream_t st) {
+  return by_shape<BRC_STE_BLOCK_FP8, BRC_FP8_E4M3>(a, nt, blocks, st);
 }
 }  // namespace kvatt
 }  // namespace brc

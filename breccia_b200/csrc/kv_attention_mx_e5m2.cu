@@ -3,8 +3,8 @@
 
 namespace brc {
 namespace kvatt {
-int attend_mx_e5m2(const Args& a, int mt, int blocks, cudaStream_t st) {
-  return by_shape<BRC_STE_MXFP8, BRC_FP8_E5M2>(a, mt, blocks, st);
+int attend_mx_e5m2(const Args& a, int nt, int blocks, cudaStream_t st) {
+  return by_shape<BRC_STE_MXFP8, BRC_FP8_E5M2>(a, nt, blocks, st);
 }
 }  // namespace kvatt
 }  // namespace brc

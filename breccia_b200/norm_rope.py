@@ -10,104 +10,117 @@ Arithmetic is float32 with one rounding into the result.
 
 from __future__ import annotations
 
-import ctypes
+from ctypes import addressof
 from typing import Tuple
 
 import torch
 
 from . import _lib
-from .api import _IN_DT, _require_cuda
-from .kvcache import QuantizedKVCache, _call, _heads, _index, _no_grad
+from .api import _IN_DT
+from .kvcache import QuantizedKVCache, _call, _heads, _index, _like, _no_grad, _on
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_write"]
 
 
-def _vector(w, what, d, dev):
-    _require_cuda(w, what)
-    if w.dtype not in _IN_DT:
-        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {w.dtype}")
-    if tuple(w.shape) != (d,):
-        raise ValueError(f"{what} must have shape ({d},), got {tuple(w.shape)}")
-    if w.device != dev:
-        raise ValueError(f"{what} is on {w.device}, expected {dev}")
-    w = w.contiguous()
-    return w.clone() if w.data_ptr() % 16 else w
-
-
-def _angles(t, what, dev):
-    _require_cuda(t, what)
-    if t.dtype != torch.float32:
-        raise TypeError(f"{what} must be float32, got {t.dtype}")
-    if t.ndim != 2 or t.shape[0] == 0:
-        raise ValueError(f"{what} must be (positions, rotated / 2), got {tuple(t.shape)}")
-    if t.device != dev:
-        raise ValueError(f"{what} is on {t.device}, expected {dev}")
+def _plain(t):
+    """Contiguous and 16-byte aligned."""
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
-def _arguments(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+def _arguments(q, k, wq, wk, cos, sin, positions, eps, interleaved):
     """The C ABI's argument record, and what it points to (kept alive by the
     caller until the launch)."""
     q = _heads(q, "q")
     dev = q.device
     k = _heads(k, "k", dev)
     tokens, hq, d = q.shape
-    if k.shape[0] != tokens or k.shape[2] != d or k.dtype != q.dtype:
-        raise ValueError(f"q and k differ: {tuple(q.shape)} {q.dtype}, {tuple(k.shape)} {k.dtype}")
+    k_tokens, hk, k_d = k.shape
+    dtype = q.dtype
+    if k_tokens != tokens or k_d != d or k.dtype is not dtype:
+        raise ValueError(f"q and k differ: {tuple(q.shape)} {dtype}, {tuple(k.shape)} {k.dtype}")
     if d % 16 or not 16 <= d <= 256:
         raise ValueError(f"head_dim must be a multiple of 16 up to 256, got {d}")
-    wq, wk = _vector(q_weight, "q_weight", d, dev), _vector(k_weight, "k_weight", d, dev)
-    if wq.dtype != wk.dtype:
+    for w, what in ((wq, "q_weight"), (wk, "k_weight")):
+        _on(w, what, dev)
+        if w.dtype not in _IN_DT:
+            raise TypeError(f"{what} must be float32, bfloat16 or float16, got {w.dtype}")
+        if w.shape != (d,):
+            raise ValueError(f"{what} must have shape ({d},), got {tuple(w.shape)}")
+    if wq.dtype is not wk.dtype:
         raise TypeError(f"q_weight and k_weight differ: {wq.dtype}, {wk.dtype}")
-    cos, sin = _angles(cos, "cos", dev), _angles(sin, "sin", dev)
-    rot = 2 * cos.shape[1]
-    if cos.shape != sin.shape:
-        raise ValueError(f"cos and sin differ: {tuple(cos.shape)}, {tuple(sin.shape)}")
+    for t, what in ((cos, "cos"), (sin, "sin")):
+        _on(t, what, dev)
+        if t.dtype is not torch.float32:
+            raise TypeError(f"{what} must be float32, got {t.dtype}")
+    rows = cos.shape
+    if rows != sin.shape:
+        raise ValueError(f"cos and sin differ: {tuple(rows)}, {tuple(sin.shape)}")
+    if len(rows) != 2 or rows[0] == 0:
+        raise ValueError(f"cos must be (positions, rotated / 2), got {tuple(rows)}")
+    rot = 2 * rows[1]
     if rot % 16 or not 16 <= rot <= d:
         raise ValueError(f"the rotated width must be a multiple of 16 up to head_dim={d}, got {rot}")
+    wq, wk, cos, sin = _plain(wq), _plain(wk), _plain(cos), _plain(sin)
     positions, is64 = _index(positions, "positions", tokens, dev)
-    a = _lib.NormRope(q.data_ptr(), k.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
-                      k.stride(1), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                      positions.data_ptr(), tokens, cos.shape[0], hq, k.shape[1], d, rot,
-                      _IN_DT[q.dtype], _IN_DT[wq.dtype], is64, int(bool(interleaved)), eps)
-    return a, (q, k, wq, wk, cos, sin, positions)
+    qs, ks = q.stride(), k.stride()
+    a = _lib.NormRope(q.data_ptr(), k.data_ptr(), qs[0], qs[1], ks[0], ks[1], wq.data_ptr(),
+                      wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), tokens,
+                      rows[0], hq, hk, d, rot, _IN_DT[dtype], _IN_DT[wq.dtype], is64,
+                      1 if interleaved else 0, eps)
+    return a, q, k, (wq, wk, cos, sin, positions)
 
 
-def _forward(a, keep):
-    q, k = keep[0], keep[1]
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=q.device)
-    _call(q.device, "brc_qk_norm_rope", ctypes.addressof(a), q_out.data_ptr(), k_out.data_ptr())
+def _forward(a, q, k):
+    q_out, k_out = _like(q), _like(k)
+    _call(q.get_device(), "brc_qk_norm_rope", addressof(a), q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
+
+
+def _shaped(t, like):
+    return t if t.ndim == like.ndim else t.view(like.shape)
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        a, keep = _arguments(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-        ctx.save_for_backward(*keep)
-        ctx.shapes = q.shape, k.shape
-        ctx.eps, ctx.interleaved = eps, interleaved
-        q_out, k_out = _forward(a, keep)
-        return q_out.view(q.shape), k_out.view(k.shape)
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved):
+        a, q3, k3, rest = _arguments(q, k, wq, wk, cos, sin, positions, eps, interleaved)
+        ctx.save_for_backward(q3, k3, *rest)
+        ctx.record, ctx.shapes = a, (q.shape, k.shape)
+        q_out, k_out = _forward(a, q3, k3)
+        return _shaped(q_out, q), _shaped(k_out, k)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        a, keep = _arguments(q, k, wq, wk, cos, sin, positions, ctx.eps, ctx.interleaved)
-        gq, gk = _heads(gq.to(q.dtype), "gradient"), _heads(gk.to(k.dtype), "gradient")
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=q.device)
-        dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
-        nbytes = _lib.lib().brc_qk_norm_rope_bwd_workspace(q.shape[2])
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _call(q.device, "brc_qk_norm_rope_bwd", ctypes.addressof(a), gq.data_ptr(), gk.data_ptr(),
-              gq.stride(0), gq.stride(1), gk.stride(0), gk.stride(1), dq.data_ptr(), dk.data_ptr(),
-              dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), nbytes)
-        return (dq.view(ctx.shapes[0]), dk.view(ctx.shapes[1]), dwq, dwk, None, None, None, None,
-                None)
+        # under create_graph the result is marked as not differentiable again;
+        # without it there is nothing to mark (and the mark costs 5 us)
+        return _backward_once(ctx, gq, gk) if torch.is_grad_enabled() else _backward(ctx, gq, gk)
+
+
+def _backward(ctx, gq, gk):
+    q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+    # what was saved may have been moved meanwhile (saved-tensor hooks)
+    a = _lib.NormRope.from_buffer_copy(ctx.record)
+    a.q, a.k, a.wq, a.wk = q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr()
+    a.cos, a.sin, a.positions = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+    a.q_token, a.q_head, _ = q.stride()
+    a.k_token, a.k_head, _ = k.stride()
+    gq, gk = _heads(gq, "gradient"), _heads(gk, "gradient")
+    dq, dk, dwq, dwk = _like(q), _like(k), _like(wq), _like(wk)
+    nbytes = _lib.lib().brc_qk_norm_rope_bwd_workspace(a.d)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    gqs, gks = gq.stride(), gk.stride()
+    _call(q.get_device(), "brc_qk_norm_rope_bwd", addressof(a), gq.data_ptr(), gk.data_ptr(),
+          gqs[0], gqs[1], gks[0], gks[1], dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
+          dwk.data_ptr(), ws.data_ptr(), nbytes)
+    if len(ctx.shapes[0]) != 3:
+        dq = dq.view(ctx.shapes[0])
+    if len(ctx.shapes[1]) != 3:
+        dk = dk.view(ctx.shapes[1])
+    return dq, dk, dwq, dwk, None, None, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -125,9 +138,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or
                                     k_weight.requires_grad):
         return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    a, keep = _arguments(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    q_out, k_out = _forward(a, keep)
-    return q_out.view(q.shape), k_out.view(k.shape)
+    a, q3, k3, _rest = _arguments(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    q_out, k_out = _forward(a, q3, k3)
+    return _shaped(q_out, q), _shaped(k_out, k)
 
 
 def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
@@ -141,19 +154,17 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
     if not isinstance(cache, QuantizedKVCache):
         raise TypeError(f"cache must be a QuantizedKVCache, got {type(cache).__name__}")
     _no_grad("qk_norm_rope_write", q, k, v, q_weight, k_weight)
-    a, keep = _arguments(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    q2, k2 = keep[0], keep[1]
-    if q2.dtype == torch.float32:
+    a, q3, k3, _rest = _arguments(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if q3.dtype is torch.float32:
         raise TypeError("qk_norm_rope_write takes bfloat16 or float16")
-    if k2.device != cache.device:
-        raise ValueError(f"k is on {k2.device}, expected {cache.device}")
-    cache._rows(k2, "k")
-    v2 = cache._rows(v, "v")
-    if v2.shape[0] != k2.shape[0] or v2.dtype != k2.dtype:
-        raise ValueError(f"k and v differ: {tuple(k2.shape)} {k2.dtype}, "
-                         f"{tuple(v2.shape)} {v2.dtype}")
-    slots, is64 = _index(slots, "slots", k2.shape[0], cache.device)
-    q_out = torch.empty(q2.shape, dtype=q2.dtype, device=q2.device)
-    _call(q2.device, "brc_qk_norm_rope_write", ctypes.addressof(a), v2.data_ptr(), v2.stride(0),
-          v2.stride(1), q_out.data_ptr(), cache._desc, slots.data_ptr(), is64)
-    return q_out.view(q.shape)
+    cache._rows(k3, "k")
+    v3 = cache._rows(v, "v")
+    if v3.shape != k3.shape or v3.dtype is not k3.dtype:
+        raise ValueError(f"k and v differ: {tuple(k3.shape)} {k3.dtype}, "
+                         f"{tuple(v3.shape)} {v3.dtype}")
+    slots, is64 = _index(slots, "slots", k3.shape[0], cache.device)
+    q_out = _like(q3)
+    vs = v3.stride()
+    _call(cache._device_index, "brc_qk_norm_rope_write", addressof(a), v3.data_ptr(), vs[0], vs[1],
+          q_out.data_ptr(), cache._desc, slots.data_ptr(), is64)
+    return _shaped(q_out, q)
