@@ -29,6 +29,7 @@ int check(const brc_kv_cache* c, int batch, int draft, int hq) {
   if (const int rc = kv::check_cache(c)) return rc;
   if (batch < 0 || draft < 0 || hq <= 0 || hq % c->heads) return BRC_ERR_SHAPE;
   // rows, items and positions are counted in 32 bits
+  if ((int64_t)c->heads * c->page_size > 0x40000000) return BRC_ERR_RANGE;
   if ((int64_t)draft * hq > (1 << 24) || (int64_t)batch * c->heads > (1 << 24) ||
       (int64_t)batch * draft * hq > 0x40000000)
     return BRC_ERR_RANGE;
@@ -74,6 +75,8 @@ int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batc
   a.table_stride = table_stride;
   a.table_pages = table_pages;
   for (a.page_shift = 4; (1 << a.page_shift) < c->page_size; ++a.page_shift) {}
+  a.step_shift = subtiles(c->head_dim) == 2 ? 5 : 4;
+  a.page_rows = (uint32_t)c->heads * c->page_size;
   a.context = context;
   a.drafts = drafts;
   a.tree = tree;

@@ -52,7 +52,8 @@ struct Args {
   int q_f16, batch, draft, hq, group, rows;  // rows = draft * group
   const int32_t* table;
   int64_t table_stride;
-  int table_pages, page_shift;
+  int table_pages, page_shift, step_shift;  // 2^step_shift tokens to a step
+  uint32_t page_rows;                       // rows from one page to the next: heads * page_size
   const int32_t* context;
   const int32_t* drafts;
   const uint8_t* tree;
@@ -67,7 +68,7 @@ struct Args {
 
 struct Seq {
   int context, drafts, total;  // tokens
-  int steps;                   // of 16 tokens, at least one
+  int steps;                   // at least one
 };
 __device__ __forceinline__ Seq load_seq(const Args& a, int b) {
   Seq s;
@@ -76,7 +77,7 @@ __device__ __forceinline__ Seq load_seq(const Args& a, int b) {
   s.drafts = a.drafts ? min(max(a.drafts[b], 0), a.draft) : a.draft;
   s.context = (int)min((int64_t)ctx, cap);
   s.total = (int)min((int64_t)ctx + s.drafts, cap);
-  s.steps = max((int)(((int64_t)s.total + 15) >> 4), 1);
+  s.steps = max((int)(((int64_t)s.total + (1 << a.step_shift) - 1) >> a.step_shift), 1);
   return s;
 }
 
@@ -101,8 +102,11 @@ __device__ __forceinline__ void locate(const Args& a, int per_seq, int blocks, i
     const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
     if (lane >= o) incl += v;
   }
+  const int64_t items = (int64_t)a.batch * per_seq;
   p.total = __shfl_sync(0xFFFFFFFFu, incl, 31) * per_seq;
-  p.share = max((p.total + blocks - 1) / blocks, (int64_t)a.min_share);
+  // small parts cost more to join than they save: at least min_share steps, or an item
+  p.share = max((p.total + blocks - 1) / blocks,
+                min((int64_t)a.min_share, (p.total + items - 1) / items));
   const int64_t x = block * p.share;
   const bool holds = want >= 0 ? (want >= b0 && want < b1)
                                : (x >= (incl - mine) * per_seq && x < incl * per_seq);
@@ -141,6 +145,24 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The four codes of a word as two f16 pairs (both halves named to the compiler
+// as 16-bit registers: no shift for the upper one).
+template <int FMT>
+__device__ __forceinline__ void fp8x4_to_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == BRC_FP8_E4M3)
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e5m2x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e5m2x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// The eight E2M1 codes of a word as four f16 pairs.
+__device__ __forceinline__ void e2m1x8_to_f16x8(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
 // E8M0 byte to float32 (255 as the casts read it: infinity).
 __device__ __forceinline__ float e8m0_value(uint32_t e) {
   return e == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
@@ -155,7 +177,11 @@ __device__ __forceinline__ uint32_t half2_pow2(int e0, int e1, int ref) {
   return half2_of(f(e0), f(e1));
 }
 
-// One step in shared memory: 16 rows of key codes, 16 of value codes, their
+// A step is two 16-token tiles: two independent chains of products, one set of
+// votes and waits for both. Heads of 256 take one, or a ring would not fit.
+constexpr __host__ __device__ int subtiles(int d) { return d == 256 ? 1 : 2; }
+
+// One step in shared memory: rows of key codes, rows of value codes, their
 // scales. A row's 16-byte pieces are permuted by its number so that the
 // operand reads below touch every bank once (64-byte rows: the value reads
 // twice).
@@ -172,10 +198,13 @@ struct Shape {
   static constexpr int kValRead = kValWords < 4 ? kValWords : 4;
   static constexpr int kSteps = D / 16;               // products along the head
   static constexpr int kTiles = D / 16;               // output tiles of 16 elements
-  static constexpr int kTileBytes = 16 * kRowBytes;
+  static constexpr int kSub = subtiles(D);
+  static constexpr int kRows = 16 * kSub;             // tokens of a step
+  static constexpr uint32_t kAll = kSub == 2 ? 0xFFFFFFFFu : 0xFFFFu;
+  static constexpr int kTileBytes = kRows * kRowBytes;
   static constexpr int kKeyScales = 2 * kTileBytes;
-  static constexpr int kValScales = kKeyScales + 16 * kScaleBytes;
-  static constexpr int kStageBytes = kValScales + 16 * kScaleBytes;
+  static constexpr int kValScales = kKeyScales + kRows * kScaleBytes;
+  static constexpr int kStageBytes = kValScales + kRows * kScaleBytes;
   __device__ static constexpr int key_piece(int t, int p) {
     return kPieces >= 8 ? p ^ ((t & 1) << 2) : p;
   }
@@ -197,23 +226,24 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Start the copy of the 16 rows from `row` on into a stage (a warp's own).
+// Start the copy of the 16 rows from `row` on into tile `sub` of a stage (a warp's own).
 template <int KIND, int D>
-__device__ __forceinline__ void copy_step(const brc_kv_cache& c, int64_t row, int lane,
-                                          uint32_t stage) {
+__device__ __forceinline__ void copy_tile(const brc_kv_cache& c, int64_t row, int lane,
+                                          uint32_t stage, int sub) {
   using S = Shape<KIND, D>;
   const uint8_t* k = c.k_data + row * S::kRowBytes + lane * 16;
   const uint8_t* v = c.v_data + row * S::kRowBytes + lane * 16;
+  const uint32_t at = stage + sub * 16 * S::kRowBytes;
 #pragma unroll
   for (int i = 0; i < S::kPieces / 2; ++i) {
     const int id = lane + 32 * i, t = id / S::kPieces, p = id % S::kPieces;
-    cp16(stage + (t * S::kPieces + S::key_piece(t, p)) * 16, k + 512 * i);
-    cp16(stage + S::kTileBytes + (t * S::kPieces + S::val_piece(t, p)) * 16, v + 512 * i);
+    cp16(at + (t * S::kPieces + S::key_piece(t, p)) * 16, k + 512 * i);
+    cp16(at + S::kTileBytes + (t * S::kPieces + S::val_piece(t, p)) * 16, v + 512 * i);
   }
   const int i = lane & 15;
   if (i < S::kScaleBytes) {
     const void* base = lane < 16 ? c.k_scale : c.v_scale;
-    cp16(stage + (lane < 16 ? S::kKeyScales : S::kValScales) + i * 16,
+    cp16(stage + (lane < 16 ? S::kKeyScales : S::kValScales) + (sub * S::kScaleBytes + i) * 16,
          static_cast<const uint8_t*>(base) + row * S::kScaleBytes + i * 16);
   }
 }
@@ -299,118 +329,141 @@ template <int KIND, int FMT, int D, int NT>
 struct Step {
   using S = Shape<KIND, D>;
   using W = Warp<KIND, FMT, D, NT>;
+  static constexpr int kSub = S::kSub;
 
-  // s[nt][2 h + x]: score of token r + 8 h and row 2c + x, in units of the rows'
-  // factors. Rows of the stage from `dead` on are past the end (their scales are
-  // not to be looked at).
+  // s[u][nt][2 h + x]: score of token 16 u + r + 8 h and row 2c + x, in units of
+  // the rows' factors. `live`: the rows of the stage that hold a token (the
+  // others' scales are not to be looked at).
   __device__ static __forceinline__ void scores(W& w, const uint8_t* st, const uint4* q, int lane,
-                                                int dead, float (&s)[NT][4]) {
+                                                uint32_t live, float (&s)[kSub][NT][4]) {
     const int r = lane >> 2, c = lane & 3;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) s[u][i][0] = s[u][i][1] = s[u][i][2] = s[u][i][3] = 0.f;
     constexpr int kReads = S::kKeyWords / S::kKeyRead;
-    uint32_t f[2][kReads];  // scales of a read's codes
+    uint32_t f[kSub][2][kReads];  // scales of a read's codes
     if constexpr (KIND == BRC_STE_MXFP8) {
-      int e[2][kReads], top = 0;
+      int e[kSub][2][kReads], top = 0;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int i = 0; i < kReads; ++i) {
-          // read i holds elements 64 i + 16 c ..: block 2 i + c / 2
-          e[n][i] = r + 8 * n < dead
-                        ? st[S::kKeyScales + (r + 8 * n) * S::kScales + 2 * i + (c >> 1)] : 0;
-          if (e[n][i] != 255) top = max(top, e[n][i]);
-        }
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < kReads; ++i) {
+            // read i holds elements 64 i + 16 c ..: block 2 i + c / 2
+            const int t = 16 * u + 8 * n + r;
+            e[u][n][i] = st[S::kKeyScales + t * S::kScales + 2 * i + (c >> 1)];
+            if (live != S::kAll && !((live >> t) & 1u)) e[u][n][i] = 0;
+            if (e[u][n][i] != 255) top = max(top, e[u][n][i]);
+          }
       if (__any_sync(0xFFFFFFFFu, top > w.ke)) w.ke = max(w.ke, (int)__reduce_max_sync(0xFFFFFFFFu, top));
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int i = 0; i < kReads; ++i) f[n][i] = half2_pow2(e[n][i], e[n][i], w.ke);
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < kReads; ++i) f[u][n][i] = half2_pow2(e[u][n][i], e[u][n][i], w.ke);
     }
 #pragma unroll
     for (int i = 0; i < kReads; ++i) {
-      uint32_t x[2][S::kKeyRead];
+      uint32_t x[kSub][2][S::kKeyRead];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int t = r + 8 * n;
-        const uint8_t* p;
-        if constexpr (S::kKeyRead == 4)
-          p = st + (t * S::kPieces + S::key_piece(t, 4 * i + c)) * 16;
-        else p = st + t * S::kRowBytes + c * 8;
-        lds_words<S::kKeyRead>(p, x[n]);
-        if constexpr (S::kFp4) {
-          // a read is one or two 16-element blocks with their scales
-          const uint8_t* sp = st + S::kKeyScales + t * S::kScales;
-          if constexpr (D == 64) f[n][i] = sp[c];
-          else f[n][i] = *reinterpret_cast<const uint16_t*>(sp + 8 * i + 2 * c);
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int t = 16 * u + 8 * n + r;
+          const uint8_t* p;
+          if constexpr (S::kKeyRead == 4)
+            p = st + (t * S::kPieces + S::key_piece(t, 4 * i + c)) * 16;
+          else p = st + t * S::kRowBytes + c * 8;
+          lds_words<S::kKeyRead>(p, x[u][n]);
+          if constexpr (S::kFp4) {
+            // a read is one or two 16-element blocks with their scales
+            const uint8_t* sp = st + S::kKeyScales + t * S::kScales;
+            if constexpr (D == 64) f[u][n][i] = sp[c];
+            else f[u][n][i] = *reinterpret_cast<const uint16_t*>(sp + 8 * i + 2 * c);
+          }
         }
-      }
 #pragma unroll
       for (int y = 0; y < S::kKeyRead; ++y) {
         constexpr int kPer = S::kFp4 ? 2 : 1;  // products to a word
-        uint4 a[kPer];
-        if constexpr (S::kFp4) {
-          const uint32_t g0 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(f[0][i], 0, y < 2 ? 0x0000 : 0x0011));
-          const uint32_t g1 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(f[1][i], 0, y < 2 ? 0x0000 : 0x0011));
+        uint4 a[kSub][kPer];
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            a[z].x = hmul2(kv::e2m1x2_to_f16x2(x[0][y] >> (16 * z)), g0);
-            a[z].y = hmul2(kv::e2m1x2_to_f16x2(x[1][y] >> (16 * z)), g1);
-            a[z].z = hmul2(kv::e2m1x2_to_f16x2(x[0][y] >> (16 * z + 8)), g0);
-            a[z].w = hmul2(kv::e2m1x2_to_f16x2(x[1][y] >> (16 * z + 8)), g1);
-          }
-        } else {
-          a[0].x = fp8x2_to_f16x2<FMT>(x[0][y]);
-          a[0].y = fp8x2_to_f16x2<FMT>(x[1][y]);
-          a[0].z = fp8x2_to_f16x2<FMT>(x[0][y] >> 16);
-          a[0].w = fp8x2_to_f16x2<FMT>(x[1][y] >> 16);
-          if constexpr (KIND == BRC_STE_MXFP8) {
-            a[0].x = hmul2(a[0].x, f[0][i]);
-            a[0].y = hmul2(a[0].y, f[1][i]);
-            a[0].z = hmul2(a[0].z, f[0][i]);
-            a[0].w = hmul2(a[0].w, f[1][i]);
+        for (int u = 0; u < kSub; ++u) {
+          if constexpr (S::kFp4) {
+            const uint32_t sel = y < 2 ? 0x0000 : 0x0011;
+            const uint32_t g0 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(f[u][0][i], 0, sel));
+            const uint32_t g1 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(f[u][1][i], 0, sel));
+            uint32_t h0[4], h1[4];
+            e2m1x8_to_f16x8(x[u][0][y], h0);
+            e2m1x8_to_f16x8(x[u][1][y], h1);
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+              a[u][z] = make_uint4(hmul2(h0[2 * z], g0), hmul2(h1[2 * z], g1),
+                                   hmul2(h0[2 * z + 1], g0), hmul2(h1[2 * z + 1], g1));
+          } else {
+            fp8x4_to_f16x4<FMT>(x[u][0][y], a[u][0].x, a[u][0].z);
+            fp8x4_to_f16x4<FMT>(x[u][1][y], a[u][0].y, a[u][0].w);
+            if constexpr (KIND == BRC_STE_MXFP8) {
+              a[u][0].x = hmul2(a[u][0].x, f[u][0][i]);
+              a[u][0].y = hmul2(a[u][0].y, f[u][1][i]);
+              a[u][0].z = hmul2(a[u][0].z, f[u][0][i]);
+              a[u][0].w = hmul2(a[u][0].w, f[u][1][i]);
+            }
           }
         }
         const int ks = kPer * (S::kKeyRead * i + y);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint4 b = q[(n * (S::kSteps / 2) + ks / 2) * 32 + lane];
-          if constexpr (S::kFp4) {
-            mma(s[n], a[0], b.x, b.y);
-            mma(s[n], a[1], b.z, b.w);
-          } else {
-            if (ks & 1) mma(s[n], a[0], b.z, b.w);
-            else mma(s[n], a[0], b.x, b.y);
+#pragma unroll
+          for (int u = 0; u < kSub; ++u) {
+            if constexpr (S::kFp4) {
+              mma(s[u][n], a[u][0], b.x, b.y);
+              mma(s[u][n], a[u][1], b.z, b.w);
+            } else {
+              if (ks & 1) mma(s[u][n], a[u][0], b.z, b.w);
+              else mma(s[u][n], a[u][0], b.x, b.y);
+            }
           }
         }
       }
     }
     if constexpr (KIND == BRC_STE_BLOCK_FP8) {  // the token's own factor
-      const float g0 = *reinterpret_cast<const float*>(st + S::kKeyScales + r * 4);
-      const float g1 = *reinterpret_cast<const float*>(st + S::kKeyScales + (r + 8) * 4);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        s[n][0] *= g0;
-        s[n][1] *= g0;
-        s[n][2] *= g1;
-        s[n][3] *= g1;
+      for (int u = 0; u < kSub; ++u) {
+        const float* g = reinterpret_cast<const float*>(st + S::kKeyScales) + 16 * u + r;
+        const float g0 = g[0], g1 = g[8];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          s[u][n][0] *= g0;
+          s[u][n][1] *= g0;
+          s[u][n][2] *= g1;
+          s[u][n][3] *= g1;
+        }
       }
     }
   }
 
   // Running maximum and sum; s becomes the probabilities relative to the shift.
-  __device__ static __forceinline__ void softmax(W& w, float (&s)[NT][4]) {
+  __device__ static __forceinline__ void softmax(W& w, float (&s)[kSub][NT][4]) {
     bool grow = false;
+    float top[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) grow |= fmaxf(s[n][x], s[n][2 + x]) > w.m[n][x] + kGrow;
+      for (int x = 0; x < 2; ++x) {
+        top[n][x] = fmaxf(s[0][n][x], s[0][n][2 + x]);
+        if constexpr (kSub == 2) top[n][x] = fmaxf(top[n][x], fmaxf(s[kSub - 1][n][x], s[kSub - 1][n][2 + x]));
+        grow |= top[n][x] > w.m[n][x] + kGrow;
+      }
     if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float t = fmaxf(s[n][x], s[n][2 + x]);
+          float t = top[n][x];
           t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 4));
           t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
           t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
@@ -430,9 +483,12 @@ struct Step {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float m = w.m[n][x] == -INFINITY ? 0.f : w.m[n][x];
-        s[n][x] = ex2(s[n][x] - m);
-        s[n][2 + x] = ex2(s[n][2 + x] - m);
-        w.l[n][x] += s[n][x] + s[n][2 + x];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+          s[u][n][x] = ex2(s[u][n][x] - m);
+          s[u][n][2 + x] = ex2(s[u][n][2 + x] - m);
+          w.l[n][x] += s[u][n][x] + s[u][n][2 + x];
+        }
       }
   }
 
@@ -441,141 +497,171 @@ struct Step {
   // what the rounding to f16 left (f16 outputs of few rows: its 2^-11 would
   // show beside the output's own).
   template <bool TWO>
-  __device__ static __forceinline__ void values(W& w, const uint8_t* st, int lane, int dead,
-                                                const float (&p)[NT][4]) {
+  __device__ static __forceinline__ void values(W& w, const uint8_t* st, int lane, uint32_t live,
+                                                const float (&p)[kSub][NT][4]) {
     const int r = lane >> 2, c = lane & 3;
-    auto token = [&](int t) { return 2 * c + (t & 1) + 8 * (t >> 1); };
-    float f[2] = {64.f, 64.f};  // of tokens r, r + 8
+    auto token = [&](int u, int t) { return 16 * u + 2 * c + (t & 1) + 8 * (t >> 1); };
+    const bool all = live == S::kAll;
     constexpr int kReads = S::kValWords / S::kValRead;
-    uint32_t h[2][2];  // [token pair][half of the lane's elements]: f16 pair of value factors
+    float f[kSub][2];        // factor of tokens r, r + 8
+    uint32_t h[kSub][2][2];  // [token pair][half of the lane's elements]: f16 pair of value factors
     if constexpr (KIND == BRC_STE_BLOCK_FP8) {
       const uint32_t* sp = reinterpret_cast<const uint32_t*>(st + S::kValScales);
-      const uint32_t s0 = r < dead ? sp[r] : 0u, s1 = r + 8 < dead ? sp[r + 8] : 0u;
-      const uint32_t top = max(s0 < 0x7F800000u ? s0 : 0u, s1 < 0x7F800000u ? s1 : 0u);
+      uint32_t sv[kSub][2], top = 0;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int t = 16 * u + 8 * n + r;
+          sv[u][n] = sp[t];
+          if (!all && !((live >> t) & 1u)) sv[u][n] = 0;
+          if (sv[u][n] < 0x7F800000u) top = max(top, sv[u][n]);
+        }
       if (__any_sync(0xFFFFFFFFu, (int)(top >> 23) - 127 > w.e))
         w.raise((int)(__reduce_max_sync(0xFFFFFFFFu, top) >> 23) - 127);
       const float g = __uint_as_float((uint32_t)(127 - w.e + 6) << 23);
-      f[0] = __uint_as_float(s0) * g;
-      f[1] = __uint_as_float(s1) * g;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) f[u][n] = __uint_as_float(sv[u][n]) * g;
     } else if constexpr (KIND == BRC_STE_MXFP8) {
-      int e[4][2], top = 0;
+      int e[kSub][4][2], top = 0;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < kReads; ++i) {
-          const int blk = D == 64 ? r >> 2 : 4 * i + (r >> 1);
-          e[t][i] = token(t) < dead ? st[S::kValScales + token(t) * S::kScales + blk] : 0;
-          if (e[t][i] != 255) top = max(top, e[t][i]);
-        }
-      if (__any_sync(0xFFFFFFFFu, top - 127 > w.e))
-        w.raise((int)__reduce_max_sync(0xFFFFFFFFu, top) - 127);
-#pragma unroll
-      for (int i = 0; i < kReads; ++i)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) h[t][i] = half2_pow2(e[2 * t][i], e[2 * t + 1][i], w.e + 127);
-    } else {
-      if (w.e < -900) w.e = 0;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        uint32_t g[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint8_t* sp = st + S::kValScales + token(2 * t + u) * S::kScales;
-          if constexpr (D == 256) g[u] = *reinterpret_cast<const uint16_t*>(sp + 2 * r);
-          else g[u] = sp[D == 128 ? r : r >> 1];
-          if (token(2 * t + u) >= dead) g[u] = 0;
-        }
-        h[t][0] = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(g[0], g[1], 0x0040));
-        if constexpr (D == 256)
-          h[t][1] = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(g[0], g[1], 0x0051));
-      }
-    }
-    uint32_t b[NT][2], b2[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float x = p[n][2 * u] * f[u], y = p[n][2 * u + 1] * f[u];
-        const uint32_t hi = half2_of(x, y);
-        b[n][u] = transpose8(hi);
-        if constexpr (TWO) {
-          const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-          b2[n][u] = transpose8(half2_of(x - g.x, y - g.y));
-        }
-      }
-#pragma unroll
-    for (int i = 0; i < kReads; ++i) {
-      uint32_t x[4][S::kValRead];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int tk = token(t);
-        const uint8_t* base = st + S::kTileBytes;
-        const uint8_t* q;
-        if constexpr (S::kValRead == 4)
-          q = base + (tk * S::kPieces + S::val_piece(tk, 8 * i + r)) * 16;
-        else if constexpr (S::kValRead == 2)
-          q = base + (tk * S::kPieces + S::val_piece(tk, r >> 1)) * 16 + (r & 1) * 8;
-        else q = base + tk * S::kRowBytes + r * 4;
-        lds_words<S::kValRead>(q, x[t]);
-      }
-      if (dead < 16) {  // rows past the end hold anything
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int y = 0; y < S::kValRead; ++y)
-            if (token(t) >= dead) x[t][y] = 0;
-      }
+          for (int i = 0; i < kReads; ++i) {
+            const int blk = D == 64 ? r >> 2 : 4 * i + (r >> 1);
+            e[u][t][i] = st[S::kValScales + token(u, t) * S::kScales + blk];
+            if (!all && !((live >> token(u, t)) & 1u)) e[u][t][i] = 0;
+            if (e[u][t][i] != 255) top = max(top, e[u][t][i]);
+          }
+      if (__any_sync(0xFFFFFFFFu, top - 127 > w.e))
+        w.raise((int)__reduce_max_sync(0xFFFFFFFFu, top) - 127);
 #pragma unroll
-      for (int y = 0; y < S::kValRead; ++y) {
-        constexpr int kPer = S::kFp4 ? 8 : 4;  // elements to a word
-        uint32_t a[2][kPer];
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint32_t u = x[2 * t][y], v = x[2 * t + 1][y];
-          if constexpr (S::kFp4) {
-            const uint32_t lo = (u & 0x0F0F0F0Fu) | ((v & 0x0F0F0F0Fu) << 4);
-            const uint32_t hi = ((u >> 4) & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u);
-            const uint32_t g = h[t][D == 256 ? y / 2 : 0];
+          f[u][t] = 64.f;
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              a[t][2 * z] = hmul2(kv::e2m1x2_to_f16x2(lo >> (8 * z)), g);
-              a[t][2 * z + 1] = hmul2(kv::e2m1x2_to_f16x2(hi >> (8 * z)), g);
-            }
-          } else {
-            const uint32_t lo = __byte_perm(u, v, 0x5140), hi = __byte_perm(u, v, 0x7362);
-            a[t][0] = fp8x2_to_f16x2<FMT>(lo);
-            a[t][1] = fp8x2_to_f16x2<FMT>(lo >> 16);
-            a[t][2] = fp8x2_to_f16x2<FMT>(hi);
-            a[t][3] = fp8x2_to_f16x2<FMT>(hi >> 16);
-            if constexpr (KIND == BRC_STE_MXFP8) {
+          for (int i = 0; i < kReads; ++i)
+            h[u][t][i] = half2_pow2(e[u][2 * t][i], e[u][2 * t + 1][i], w.e + 127);
+        }
+    } else {
+      if (w.e < -900) w.e = 0;
 #pragma unroll
-              for (int z = 0; z < 4; ++z) a[t][z] = hmul2(a[t][z], h[t][i]);
-            }
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f[u][t] = 64.f;
+          uint32_t g[2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int tk = token(u, 2 * t + y);
+            const uint8_t* sp = st + S::kValScales + tk * S::kScales;
+            if constexpr (D == 256) g[y] = *reinterpret_cast<const uint16_t*>(sp + 2 * r);
+            else g[y] = sp[D == 128 ? r : r >> 1];
+            if (!all && !((live >> tk) & 1u)) g[y] = 0;
+          }
+          h[u][t][0] = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(g[0], g[1], 0x0040));
+          if constexpr (D == 256)
+            h[u][t][1] = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(g[0], g[1], 0x0051));
+        }
+    }
+    uint32_t b[kSub][NT][2], b2[kSub][NT][2];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float v0 = p[u][n][2 * y] * f[u][y], v1 = p[u][n][2 * y + 1] * f[u][y];
+          const uint32_t hi = half2_of(v0, v1);
+          b[u][n][y] = transpose8(hi);
+          if constexpr (TWO) {
+            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            b2[u][n][y] = transpose8(half2_of(v0 - g.x, v1 - g.y));
           }
         }
 #pragma unroll
-        for (int z = 0; z < kPer / 2; ++z) {
-          const uint4 av = make_uint4(a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1]);
-          const int j = kPer / 2 * (S::kValRead * i + y) + z;
+    for (int i = 0; i < kReads; ++i) {
+      uint32_t x[kSub][4][S::kValRead];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma(w.o[n][j], av, b[n][0], b[n][1]);
-            if constexpr (TWO) mma(w.o[n][j], av, b2[n][0], b2[n][1]);
-          }
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int tk = token(u, t);
+          const uint8_t* base = st + S::kTileBytes;
+          const uint8_t* q;
+          if constexpr (S::kValRead == 4)
+            q = base + (tk * S::kPieces + S::val_piece(tk, 8 * i + r)) * 16;
+          else if constexpr (S::kValRead == 2)
+            q = base + (tk * S::kPieces + S::val_piece(tk, r >> 1)) * 16 + (r & 1) * 8;
+          else q = base + tk * S::kRowBytes + r * 4;
+          lds_words<S::kValRead>(q, x[u][t]);
         }
+      if (!all) {  // rows without a token hold anything
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int y = 0; y < S::kValRead; ++y)
+              if (!((live >> token(u, t)) & 1u)) x[u][t][y] = 0;
       }
+#pragma unroll
+      for (int y = 0; y < S::kValRead; ++y)
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+          constexpr int kPer = S::kFp4 ? 8 : 4;  // elements to a word
+          uint32_t a[2][kPer];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t v0 = x[u][2 * t][y], v1 = x[u][2 * t + 1][y];
+            if constexpr (S::kFp4) {
+              uint32_t lo[4], hi[4];
+              e2m1x8_to_f16x8((v0 & 0x0F0F0F0Fu) | ((v1 & 0x0F0F0F0Fu) << 4), lo);
+              e2m1x8_to_f16x8(((v0 >> 4) & 0x0F0F0F0Fu) | (v1 & 0xF0F0F0F0u), hi);
+              const uint32_t g = h[u][t][D == 256 ? y / 2 : 0];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                a[t][2 * z] = hmul2(lo[z], g);
+                a[t][2 * z + 1] = hmul2(hi[z], g);
+              }
+            } else {
+              fp8x4_to_f16x4<FMT>(__byte_perm(v0, v1, 0x5140), a[t][0], a[t][1]);
+              fp8x4_to_f16x4<FMT>(__byte_perm(v0, v1, 0x7362), a[t][2], a[t][3]);
+              if constexpr (KIND == BRC_STE_MXFP8) {
+#pragma unroll
+                for (int z = 0; z < 4; ++z) a[t][z] = hmul2(a[t][z], h[u][t][i]);
+              }
+            }
+          }
+#pragma unroll
+          for (int z = 0; z < kPer / 2; ++z) {
+            const uint4 av = make_uint4(a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1]);
+            const int j = kPer / 2 * (S::kValRead * i + y) + z;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma(w.o[n][j], av, b[u][n][0], b[u][n][1]);
+              if constexpr (TWO) mma(w.o[n][j], av, b2[u][n][0], b2[u][n][1]);
+            }
+          }
+        }
     }
   }
 
   // Does any value of the step's live rows stand for something not finite?
-  __device__ static __forceinline__ bool odd_values(const uint8_t* st, int lane, int dead) {
+  __device__ static __forceinline__ bool odd_values(const uint8_t* st, int lane, uint32_t live) {
     bool odd = false;
-    // lane: row lane / 2, half of its bytes
-    const int t = lane >> 1;
-    if (t < dead) {
+    constexpr int kLanes = 32 / S::kRows;  // to a row
+    const int t = lane / kLanes;
+    if ((live >> t) & 1u) {
+      constexpr int kWords = S::kRowBytes / 4 / kLanes;
       const uint32_t* p = reinterpret_cast<const uint32_t*>(st + S::kTileBytes + t * S::kRowBytes) +
-                          (lane & 1) * (S::kRowBytes / 8);
-      for (int i = 0; i < S::kRowBytes / 8; ++i) odd |= odd_codes<KIND, FMT>(p[i]);
+                          (lane % kLanes) * kWords;
+      for (int i = 0; i < kWords; ++i) odd |= odd_codes<KIND, FMT>(p[i]);
       const uint8_t* sp = st + S::kValScales + t * S::kScaleBytes;
       if constexpr (KIND == BRC_STE_BLOCK_FP8) {
         odd |= (*reinterpret_cast<const uint32_t*>(sp) & 0x7F800000u) == 0x7F800000u;
@@ -589,43 +675,49 @@ struct Step {
 
   // The same for a step whose values are not all finite: token by token, only
   // where the row sees the token, so that what it does not see cannot reach it.
-  __device__ static __forceinline__ void values_checked(W& w, const brc_kv_cache& c, int64_t row,
-                                                        int lane, const float (&p)[NT][4],
-                                                        uint32_t seen) {
+  // row[u]: the first cache row of tile u; seen: bits (u, n, h, x) as s.
+  __device__ static __forceinline__ void values_checked(W& w, const brc_kv_cache& c,
+                                                        const int64_t (&row)[kSub], int lane,
+                                                        const float (&p)[kSub][NT][4],
+                                                        uint32_t live, uint32_t seen) {
     if (w.e < -900) w.e = 0;
     const float f = 64.f * exp2f((float)-w.e);
-    for (int t = 0; t < 16; ++t) {
-      const int half = t >> 3, src = (t & 7) * 4 + (lane & 3);
-      float pr[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int u = 0; u < kSub; ++u)
+      for (int t = 0; t < 16; ++t) {
+        if (!((live >> (16 * u + t)) & 1u)) continue;
+        const int half = t >> 3, src = (t & 7) * 4 + (lane & 3);
+        float pr[NT][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          pr[n][x] = __shfl_sync(0xFFFFFFFFu, half ? p[n][2 + x] : p[n][x], src) * f;
-      const uint32_t sees = __shfl_sync(0xFFFFFFFFu, seen, src) >> (2 * half);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < S::kTiles; ++j)
+          for (int x = 0; x < 2; ++x)
+            pr[n][x] = __shfl_sync(0xFFFFFFFFu, half ? p[u][n][2 + x] : p[u][n][x], src) * f;
+        const uint32_t sees = __shfl_sync(0xFFFFFFFFu, seen, src) >> (4 * NT * u + 2 * half);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float v = value_at<KIND, FMT, D>(c, row + t, S::elem(2 * j + u, lane >> 2));
+        for (int j = 0; j < S::kTiles; ++j)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int y = 0; y < 2; ++y) {
+            const float v = value_at<KIND, FMT, D>(c, row[u] + t, S::elem(2 * j + y, lane >> 2));
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              if ((sees >> (4 * n + x)) & 1u) w.o[n][j][2 * u + x] += pr[n][x] * v;
-        }
-    }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                if ((sees >> (4 * n + x)) & 1u) w.o[n][j][2 * y + x] += pr[n][x] * v;
+          }
+      }
   }
 };
 
 // Blocks that an SM is to hold, as many as the accumulators' registers allow.
 constexpr __host__ __device__ int blocks_per_sm(int d, int nt) {
-  return d * nt <= 128 ? 4 : d * nt <= 256 ? 3 : 2;
+  return d * nt <= 64 ? 4 : d * nt <= 256 ? 3 : 2;
 }
 // Stages of a warp's ring: what fits beside the queries in the block's part of
 // shared memory, at most 6.
 constexpr __host__ __device__ int stage_bytes(int kind, int d) {
-  return 2 * 16 * (kv::row_bytes(kind, d) + kv::row_scales(kind, d) * (kind == BRC_STE_BLOCK_FP8 ? 4 : 1));
+  return 2 * 16 * subtiles(d) *
+         (kv::row_bytes(kind, d) + kv::row_scales(kind, d) * (kind == BRC_STE_BLOCK_FP8 ? 4 : 1));
 }
 // Row warps of a block: more than one only with the largest row tile.
 constexpr __host__ __device__ int most_tiles(int d) { return d == 256 ? 2 : 4; }
@@ -649,6 +741,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
   using St = Step<KIND, FMT, D, NT>;
   constexpr int kStages = stages(KIND, D, NT);
   constexpr bool kTwo = NT <= 2;
+  constexpr int kSub = S::kSub;
   extern __shared__ __align__(16) uint8_t smem[];
   // the warps' stages (later: their outputs), then the queries as operand fragments
   uint8_t* const rings = smem;
@@ -683,6 +776,50 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
     const int s_begin = (int)(x - item_start);
     const int s_end = (int)min((int64_t)seq.steps, end - item_start);
     const int row0 = rb * rows_per_block;
+
+    // ---- the first stages are on their way while the queries are laid out
+    const int32_t* const table = a.table + b * a.table_stride;
+    const int page_mask = a.c.page_size - 1;
+    const uint32_t head_row = (uint32_t)head * a.c.page_size;
+    // First cache row of the 16-token tile at token t, or -1.
+    auto row_at = [&](int64_t t) -> int64_t {
+      if (t >= seq.total) return -1;
+      const int64_t page = __ldg(table + (t >> a.page_shift));
+      if (page < 0 || page >= a.c.num_pages) return -1;
+      return page * a.page_rows + head_row + (uint32_t)(t & page_mask);
+    };
+    // the warp's own ring of stages
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rings) + warp * (kStages * S::kStageBytes);
+    const uint8_t* const ring_p = rings + warp * (kStages * S::kStageBytes);
+    uint32_t there = 0;  // kSub bits to a step, the newest lowest: its tiles that have a page
+    int s = s_begin + tw, ahead = s, slot_in = 0, slot_out = 0;
+    auto fetch = [&]() {
+      uint32_t bits = 0;
+      if (ahead < s_end) {
+        const int64_t t = (int64_t)ahead * S::kRows;
+        const uint32_t to = ring + slot_in * S::kStageBytes;
+        const int64_t row = row_at(t);
+        if (row >= 0) {
+          copy_tile<KIND, D>(a.c, row, lane, to, 0);
+          bits = 1;
+        }
+        if constexpr (kSub == 2) {
+          // pages of 32 tokens and more hold the step whole
+          const int64_t row1 = a.page_shift > 4 ? (row >= 0 && t + 16 < seq.total ? row + 16 : -1)
+                                                : row_at(t + 16);
+          if (row1 >= 0) {
+            copy_tile<KIND, D>(a.c, row1, lane, to, 1);
+            bits |= 2;
+          }
+        }
+      }
+      cp_commit();
+      there = there << kSub | bits;
+      ahead += token_warps;
+      slot_in = slot_in + 1 == kStages ? 0 : slot_in + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch();
 
     // ---- queries: scaled per row by a power of two into f16 fragments
     {
@@ -746,78 +883,66 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
         node[n][x] = row < a.rows ? row / a.group : a.draft;
       }
 
-    const int32_t* const table = a.table + b * a.table_stride;
-    const int page_mask = a.c.page_size - 1;
-    auto row_at = [&](int s) -> int64_t {  // first cache row of a step, or -1
-      const int64_t t = (int64_t)s << 4;
-      if (t >= seq.total) return -1;
-      const int64_t page = __ldg(table + (t >> a.page_shift));
-      if (page < 0 || page >= a.c.num_pages) return -1;
-      return (page * a.c.heads + head) * a.c.page_size + (t & page_mask);
-    };
-    // the warp's own ring of stages
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rings) + warp * (kStages * S::kStageBytes);
-    const uint8_t* const ring_p = rings + warp * (kStages * S::kStageBytes);
-    uint32_t there = 0;  // bit i: the step i places behind the newest has a page
-    int s = s_begin + tw, ahead = s, slot_in = 0, slot_out = 0;
-    auto fetch = [&]() {
-      const int64_t row = ahead < s_end ? row_at(ahead) : -1;
-      if (row >= 0) copy_step<KIND, D>(a.c, row, lane, ring + slot_in * S::kStageBytes);
-      cp_commit();
-      there = there << 1 | (row >= 0 ? 1u : 0u);
-      ahead += token_warps;
-      slot_in = slot_in + 1 == kStages ? 0 : slot_in + 1;
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch();
     for (; s < s_end; s += token_warps) {
       cp_wait<kStages - 2>();
       __syncwarp();  // every lane's pieces are there, and the oldest stage is read
       fetch();
-      if (there >> (kStages - 1) & 1u) {
+      const uint32_t bits = there >> ((kStages - 1) * kSub) & ((1u << kSub) - 1);
+      if (bits) {
         const uint8_t* const st = ring_p + slot_out * S::kStageBytes;
-        const int t0 = s << 4;
-        const int dead = min(seq.total - t0, 16);  // live rows
-        float p[NT][4];
-        St::scores(w, st, q, lane, dead, p);
+        const int64_t t0 = (int64_t)s * S::kRows;
+        uint32_t live = S::kAll;
+        if (t0 + S::kRows > seq.total) live >>= S::kRows - (int)(seq.total - t0);
+        if (kSub == 2 && bits != 3) live &= bits == 1 ? 0xFFFFu : 0xFFFF0000u;
+        float p[kSub][NT][4];
+        St::scores(w, st, q, lane, live, p);
         const float kf = KIND == BRC_STE_MXFP8 ? e8m0_value(w.ke) : 1.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float f = KIND == BRC_STE_MXFP8 ? rowf[n][x] * kf : rowf[n][x];
-            p[n][x] *= f;
-            p[n][2 + x] *= f;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+              p[u][n][x] *= f;
+              p[u][n][2 + x] *= f;
+            }
           }
         uint32_t seen = 0;
         bool checked = false;
-        if (t0 + 16 > seq.context) {  // drafted tokens, or past the end
+        if (t0 + S::kRows > seq.context || live != S::kAll) {  // drafted tokens, or none
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int u = 0; u < kSub; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int t = t0 + (lane >> 2) + 8 * h, j = t - seq.context;
-                bool see = t < seq.total && node[n][x] < seq.drafts;
-                if (see && j >= 0)
-                  see = a.tree ? a.tree[b * a.tree_stride + (int64_t)node[n][x] * a.draft + j] != 0
-                               : j <= node[n][x];
-                if (see) seen |= 1u << (4 * n + 2 * h + x);
-                else p[n][2 * h + x] = -INFINITY;
-              }
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  const int at = 16 * u + 8 * h + (lane >> 2);
+                  const int64_t j = t0 + at - seq.context;
+                  bool see = ((live >> at) & 1u) && node[n][x] < seq.drafts;
+                  if (see && j >= 0)
+                    see = a.tree ? a.tree[b * a.tree_stride + (int64_t)node[n][x] * a.draft + j] != 0
+                                 : j <= node[n][x];
+                  if (see) seen |= 1u << (4 * (NT * u + n) + 2 * h + x);
+                  else p[u][n][2 * h + x] = -INFINITY;
+                }
           // a drafted value that is not finite must not meet a probability of
           // zero in the product
-          checked = St::odd_values(st, lane, dead);
+          checked = St::odd_values(st, lane, live);
         }
         St::softmax(w, p);
         if (checked) {
-          St::values_checked(w, a.c, row_at(s), lane, p, seen);
+          int64_t rows[kSub];
+#pragma unroll
+          for (int u = 0; u < kSub; ++u) rows[u] = row_at(t0 + 16 * u);
+          St::values_checked(w, a.c, rows, lane, p, live, seen);
         } else if constexpr (kTwo) {
-          if (a.q_f16) St::template values<true>(w, st, lane, dead, p);
-          else St::template values<false>(w, st, lane, dead, p);
+          if (a.q_f16) St::template values<true>(w, st, lane, live, p);
+          else St::template values<false>(w, st, lane, live, p);
         } else {
-          St::template values<false>(w, st, lane, dead, p);
+          St::template values<false>(w, st, lane, live, p);
         }
       }
       slot_out = slot_out + 1 == kStages ? 0 : slot_out + 1;
@@ -904,6 +1029,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
     }
     __syncthreads();
     x = item_start + s_end;
+    if (x >= end) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (s_end == seq.steps && item + 1 == per_seq) {
       seq_start += (int64_t)per_seq * seq.steps;
       ++b;
@@ -929,6 +1055,7 @@ __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
   Place p;
   locate(a, per_seq, blocks, 0, b, p);
   const Seq seq = load_seq(a, b);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
   const int64_t start = p.before * per_seq + (int64_t)(head * a.row_blocks + rb) * seq.steps;
   const int64_t c0 = start / p.share, c1 = (start + seq.steps - 1) / p.share;
   if (c0 == c1) return;
@@ -994,8 +1121,17 @@ int launch(Args a, int blocks, cudaStream_t st) {
   k_attend<KIND, FMT, D, NT><<<blocks, kThreads, bytes, st>>>(a);
   if (const int rc = check_launch()) return rc;
   const int64_t warps = (int64_t)a.batch * a.c.heads * a.row_blocks * a.rows_per_block;
-  k_join<D><<<(unsigned)((warps + kWarps - 1) / kWarps), kThreads, 0, st>>>(a, blocks);
-  return check_launch();
+  // the join's blocks start, and find their places, while the last parts are written
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((warps + kWarps - 1) / kWarps));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, k_join<D>, a, blocks));
 }
 
 template <int KIND, int FMT>
