@@ -28,11 +28,22 @@ __host__ __device__ constexpr int row_scales(int kind, int d) {
   return kind == BRC_STE_BLOCK_FP8 ? 1 : kind == BRC_STE_MXFP8 ? d / 32 : d / 16;
 }
 
-// Row index of (slot, head) in the (page, head, token) order of the cache.
+// Row index of (slot, head) in the (page, head, token) order of the cache; the
+// page size is a power of two.
 __device__ __forceinline__ int64_t row_of(const brc_kv_cache& c, int64_t slot, int head) {
-  const int64_t page = slot / c.page_size;
-  return (page * c.heads + head) * c.page_size + (slot - page * c.page_size);
+  const int shift = 31 - __clz(c.page_size);
+  return (((slot >> shift) * c.heads + head) << shift) + (slot & (c.page_size - 1));
 }
+
+// n / d for 32-bit n and a d fixed at launch, by one multiplication.
+struct Divide {
+  uint32_t d;
+  uint64_t m;  // ceil(2^64 / d); d = 1: unused
+  explicit Divide(uint32_t by) : d(by), m(by > 1 ? ~0ull / by + 1 : 0) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    return d == 1 ? n : (uint32_t)__umul64hi(n, m);
+  }
+};
 
 // A byte of two E2M1 codes (low nibble first) to an f16 pair, exactly.
 __device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {

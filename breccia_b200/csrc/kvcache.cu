@@ -25,7 +25,8 @@ struct WriteArgs {
   int64_t token[2], head[2];
   const void* slots;
   int slots64;
-  int64_t rows;  // tokens * heads
+  uint32_t rows;  // tokens * heads
+  Divide heads;
 };
 
 // blockIdx.y: 0 keys, 1 values.
@@ -39,22 +40,21 @@ __global__ void __launch_bounds__(kThreads) k_write(WriteArgs a) {
   uint8_t* data = side ? a.c.v_data : a.c.k_data;
   void* scale = side ? a.c.v_scale : a.c.k_scale;
   const int64_t slots = a.c.num_pages * a.c.page_size;
-  const int64_t first =
-      ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
+  const uint32_t first =
+      (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
   float f[kRows][8];
   int64_t row[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int64_t r = first + u * G;
+    const uint32_t r = first + u * G;
     row[u] = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
     if (r < a.rows) {
-      const int64_t t = r / a.c.heads;
-      const int h = (int)(r - t * a.c.heads);
+      const uint32_t t = a.heads(r), h = r - t * a.heads.d;
       load8<DT>(x, t * ts + h * hs + part * 8, f[u]);
       const int64_t slot = load_index(a.slots, t, a.slots64);
-      if (slot >= 0 && slot < slots) row[u] = row_of(a.c, slot, h);
+      if (slot >= 0 && slot < slots) row[u] = row_of(a.c, slot, (int)h);
     }
   }
 #pragma unroll
@@ -66,8 +66,10 @@ struct ReadArgs {
   brc_kv_cache c;
   const int32_t* table;
   const int32_t* lengths;
-  int64_t table_stride, length, rows;  // rows: batch * length * heads
+  int64_t table_stride;
+  uint32_t rows;  // batch * length * heads
   int table_pages;
+  Divide heads, length;
   void* out[2];
 };
 
@@ -79,32 +81,32 @@ __global__ void __launch_bounds__(kThreads) k_read(ReadArgs a) {
   const uint8_t* data = side ? a.c.v_data : a.c.k_data;
   const void* scale = side ? a.c.v_scale : a.c.k_scale;
   void* out = side ? a.out[1] : a.out[0];
-  const int64_t first =
-      ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
+  const uint32_t first =
+      (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
+  const int shift = 31 - __clz(a.c.page_size);
   float f[kRows][8];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int64_t r = first + u * G;
+    const uint32_t r = first + u * G;
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
     if (r < a.rows) {
-      const int64_t bt = r / a.c.heads;
-      const int h = (int)(r - bt * a.c.heads);
-      const int64_t b = bt / a.length, t = bt - b * a.length;
-      const int64_t p = t / a.c.page_size;
-      if (t < a.lengths[b] && p < a.table_pages) {
+      const uint32_t bt = a.heads(r), h = r - bt * a.heads.d;
+      const uint32_t b = a.length(bt), t = bt - b * a.length.d;
+      const uint32_t p = t >> shift;
+      if ((int64_t)t < a.lengths[b] && p < (uint32_t)a.table_pages) {
         const int64_t page = a.table[b * a.table_stride + p];
         if (page >= 0 && page < a.c.num_pages)
           decode_row<KIND, FMT, LPR>(
-              data, scale,
-              (page * a.c.heads + h) * a.c.page_size + (t - p * a.c.page_size), part, f[u]);
+              data, scale, ((page * a.c.heads + h) << shift) + (t & (a.c.page_size - 1)), part,
+              f[u]);
       }
     }
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int64_t r = first + u * G;
-    if (r < a.rows) store8<DT>(out, r * (LPR * 8) + part * 8, f[u]);
+    const uint32_t r = first + u * G;
+    if (r < a.rows) store8<DT>(out, (int64_t)r * (LPR * 8) + part * 8, f[u]);
   }
 }
 
@@ -150,11 +152,10 @@ struct LaunchRead {
   }
 };
 
-// Blocks for `rows` rows of d elements, or 0 past the grid's limit.
+// Blocks for `rows` rows of d elements; 0 where 32 bits do not count the rows.
 int64_t blocks_for(int64_t rows, int d) {
   const int per = (kThreads / 32) * kRows * (32 / (d / 8));
-  const int64_t n = (rows + per - 1) / per;
-  return n > 0x7FFFFFFF ? 0 : n;
+  return rows > 0xFFFFFFFFll - per ? 0 : (rows + per - 1) / per;
 }
 
 bool bad_stride(int64_t s, int dtype) { return s % (dtype == BRC_DTYPE_F32 ? 4 : 8) != 0; }
@@ -180,9 +181,11 @@ int brc_kv_write(const brc_kv_cache* c, const void* k, const void* v, int dtype,
   if (bad_stride(k_token, dtype) || bad_stride(k_head, dtype) || bad_stride(v_token, dtype) ||
       bad_stride(v_head, dtype))
     return BRC_ERR_ALIGN;
-  WriteArgs a{*c, {k, v}, {k_token, v_token}, {k_head, v_head}, slots, slots64, tokens * c->heads};
-  const int64_t n = blocks_for(a.rows, c->head_dim);
+  if (tokens > 0xFFFFFFFFll) return BRC_ERR_RANGE;
+  const int64_t n = blocks_for(tokens * c->heads, c->head_dim);
   if (n == 0) return BRC_ERR_RANGE;
+  WriteArgs a{*c, {k, v}, {k_token, v_token}, {k_head, v_head}, slots, slots64,
+              (uint32_t)(tokens * c->heads), Divide((uint32_t)c->heads)};
   return by_dtype<LaunchWrite>(dtype, a, dim3((unsigned)n, 2), (cudaStream_t)stream);
 }
 
@@ -195,10 +198,12 @@ int brc_kv_read(const brc_kv_cache* c, const int32_t* table, int64_t table_strid
   if (batch == 0 || length == 0) return BRC_OK;
   if ((!table && table_pages) || !lengths || !k_out || !v_out) return BRC_ERR_NULL;
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return BRC_ERR_ALIGN;
-  ReadArgs a{*c, table, lengths, table_stride, length, (int64_t)batch * length * c->heads,
-             table_pages, {k_out, v_out}};
-  const int64_t n = blocks_for(a.rows, c->head_dim);
+  if (length > 0x7FFFFFFF || (int64_t)batch * length > 0xFFFFFFFFll) return BRC_ERR_RANGE;
+  const int64_t rows = (int64_t)batch * length * c->heads;
+  const int64_t n = blocks_for(rows, c->head_dim);
   if (n == 0) return BRC_ERR_RANGE;
+  ReadArgs a{*c, table, lengths, table_stride, (uint32_t)rows, table_pages,
+             Divide((uint32_t)c->heads), Divide((uint32_t)length), {k_out, v_out}};
   return by_dtype<LaunchRead>(out_dtype, a, dim3((unsigned)n, 2), (cudaStream_t)stream);
 }
 

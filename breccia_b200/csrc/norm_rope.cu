@@ -5,10 +5,12 @@
 //   gz = R^T gy,  gw = sum gz x r,  gx = r (gz w - x r mean(gz w x r))
 //
 // A stream: HBM bounds it at long prompts, launch latency at single tokens. A
-// head lies on LPR = 8, 16 or 32 lanes, eight elements to a lane, so its loads
-// and stores are contiguous, its sums are shuffles, and a rotated pair is two
-// lanes' (halves) or one lane's (interleaved) values. A warp takes several
-// heads of ONE token, so the token's cosines and sines are loaded once.
+// head lies on LPR = 8, 16 or 32 lanes, eight elements to a lane in two groups
+// of four that hold whole rotated pairs (halves: elements 4 p .. and rot / 2 +
+// 4 p ..; interleaved: 8 p .. 8 p + 7), so a lane turns its pairs by itself with
+// four cosines and sines, and a head's sums are shuffles. A warp takes several
+// heads of one token, all queries or all keys: the token's angles and the
+// weights are loaded once.
 #include "kv_codec.cuh"
 #include "launch.h"
 
@@ -21,8 +23,7 @@ constexpr int kWarps = kThreads / 32;
 struct FwdArgs {
   brc_norm_rope a;
   void* q_out;
-  void* k_out;
-  // fused write
+  // the write
   brc_kv_cache c;
   const void* v;
   int64_t v_token, v_head;
@@ -32,78 +33,6 @@ struct FwdArgs {
 
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
   return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
-}
-
-__device__ __forceinline__ void load_w(const void* w, int dtype, int e, float* f) {
-  if (dtype == BRC_DTYPE_F32) kv::load8<BRC_DTYPE_F32>(w, e, f);
-  else if (dtype == BRC_DTYPE_BF16) kv::load8<BRC_DTYPE_BF16>(w, e, f);
-  else kv::load8<BRC_DTYPE_F16>(w, e, f);
-}
-
-// The rotation's factors for one lane's eight elements: y_i = z_i c_i + o_i s_i
-// with o the pair's other element, s signed. Elements past `rot` get c = 1, s = 0.
-struct Turn {
-  float c[8], s[8];
-  int other;  // lane of the head that holds the other elements (halves)
-};
-
-__device__ __forceinline__ void load_turn(const brc_norm_rope& a, int64_t token, int part,
-                                          Turn& t) {
-  const int64_t pos = load_index(a.positions, token, a.index64);
-  const bool in = pos >= 0 && pos < a.table_rows;
-  const int half = a.rot >> 1, e = part * 8;
-  t.other = part;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    t.c[i] = 1.f;
-    t.s[i] = 0.f;
-  }
-  if (e < a.rot) {
-    const int64_t row = (in ? pos : 0) * half;
-    if (a.interleaved) {
-      const float4 c = *reinterpret_cast<const float4*>(a.cos + row + e / 2);
-      const float4 s = *reinterpret_cast<const float4*>(a.sin + row + e / 2);
-      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        t.c[2 * i] = t.c[2 * i + 1] = cc[i];
-        t.s[2 * i] = -ss[i];
-        t.s[2 * i + 1] = ss[i];
-      }
-    } else {
-      const bool low = e < half;
-      const int at = low ? e : e - half;
-      t.other = low ? part + half / 8 : part - half / 8;
-      kv::load8<BRC_DTYPE_F32>(a.cos, row + at, t.c);
-      kv::load8<BRC_DTYPE_F32>(a.sin, row + at, t.s);
-      if (low) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t.s[i] = -t.s[i];
-      }
-    }
-  }
-  if (!in) {  // outside the table: NaN, not a wrong angle
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t.c[i] = __uint_as_float(0x7FC00000u);
-  }
-}
-
-// R z (or, back, R^T z) of one lane's elements; every lane of the warp calls it.
-template <int LPR>
-__device__ __forceinline__ void turn8(const Turn& t, bool interleaved, bool back, float* z) {
-  float o[8];
-  if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = z[i ^ 1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xFFFFFFFFu, z[i], t.other, LPR);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float b = o[i] * t.s[i];  // R^T: the sines change sign
-    z[i] = z[i] * t.c[i] + (back ? -b : b);
-  }
 }
 
 template <int LPR>
@@ -121,7 +50,7 @@ __device__ __forceinline__ float square_sum(float* x, float& ss, float& eps) {
   auto sum = [&]() {
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += x[i] * x[i];
+    for (int i = 0; i < 8; ++i) v = __fmaf_rn(x[i], x[i], v);
     return sum_row<LPR>(v);
   };
   ss = sum();
@@ -136,195 +65,382 @@ __device__ __forceinline__ float square_sum(float* x, float& ss, float& eps) {
   return by;
 }
 
+// ------------------------------------------------------------------ pairs in a lane
+// First elements of lane `part`'s two groups of four.
+template <bool INTER>
+__device__ __forceinline__ void groups(int rot, int part, int& e0, int& e1) {
+  if (!INTER && part * 8 < rot) {
+    e0 = 4 * part;
+    e1 = (rot >> 1) + 4 * part;
+  } else {  // whole pairs, or elements that are not rotated
+    e0 = 8 * part;
+    e1 = e0 + 4;
+  }
+}
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, int64_t e, float* f) {
+  if constexpr (DT == BRC_DTYPE_F32) {
+    unpack<DT>(ldg16(static_cast<const char*>(p) + 4 * e), f);
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const char*>(p) + 2 * e));
+    if constexpr (DT == BRC_DTYPE_BF16) {
+      f[0] = __uint_as_float(v.x << 16);
+      f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+      f[2] = __uint_as_float(v.y << 16);
+      f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+    } else {
+      f16x2_to_f32(v.x, f[0], f[1]);
+      f16x2_to_f32(v.y, f[2], f[3]);
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store4(void* p, int64_t e, const float* f) {
+  if constexpr (DT == BRC_DTYPE_F32) {
+    stg16(static_cast<char*>(p) + 4 * e, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
+                                                    __float_as_uint(f[2]), __float_as_uint(f[3])));
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (DT == BRC_DTYPE_BF16) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint2*>(static_cast<char*>(p) + 2 * e) = make_uint2(w[0], w[1]);
+  }
+}
+__device__ __forceinline__ void load_w4(const void* w, int dtype, int e, float* f) {
+  if (dtype == BRC_DTYPE_F32) load4<BRC_DTYPE_F32>(w, e, f);
+  else if (dtype == BRC_DTYPE_BF16) load4<BRC_DTYPE_BF16>(w, e, f);
+  else load4<BRC_DTYPE_F16>(w, e, f);
+}
+// The four angles of lane `part`'s pairs; (1, 0) where nothing is rotated; a
+// NaN cosine for a position outside the table (not a wrong angle).
+__device__ __forceinline__ void load_angles(const brc_norm_rope& a, int64_t token, int part,
+                                            float* c, float* s) {
+  const int64_t pos = load_index(a.positions, token, a.index64);
+  const bool in = pos >= 0 && pos < a.table_rows;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+  }
+  if (part * 8 < a.rot) {
+    const int64_t at = (in ? pos : 0) * (a.rot >> 1) + 4 * part;
+    load4<BRC_DTYPE_F32>(a.cos, at, c);
+    load4<BRC_DTYPE_F32>(a.sin, at, s);
+  }
+  if (!in) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = __uint_as_float(0x7FC00000u);
+  }
+}
+// R z (BACK: R^T z) of the lane's eight elements.
+template <bool INTER, bool BACK>
+__device__ __forceinline__ void turn_pairs(const float* c, const float* s, float* z) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int x = INTER ? 2 * i : i, y = INTER ? 2 * i + 1 : i + 4;
+    const float u = z[x], v = z[y], t = BACK ? -s[i] : s[i];
+    z[x] = __fmaf_rn(u, c[i], -__fmul_rn(v, t));
+    z[y] = __fmaf_rn(v, c[i], __fmul_rn(u, t));
+  }
+}
+
+// ------------------------------------------------------------------ forward
+// One row, in place; every lane of the warp calls it. Each operation is named,
+// so that both kernels below round alike.
+template <int LPR, bool INTER>
+__device__ __forceinline__ void norm_turn(float* x, const float* w, const float* c, const float* s,
+                                          float inv_d, float eps) {
+  float ss;
+  square_sum<LPR>(x, ss, eps);
+  const float r = rsqrtf(__fmaf_rn(ss, inv_d, eps));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
+  turn_pairs<INTER, false>(c, s, x);
+}
+
 constexpr int kHeads = 4;  // heads in flight per lane
 
-// KIND < 0: norm and rotation only; else the write into a cache of that kind.
-template <int DT, int LPR, int KIND, int FMT>
-__global__ void __launch_bounds__(kThreads) k_fwd(FwdArgs g) {
+// blockIdx.y: a chunk of `iters` x kHeads x (32 / LPR) heads, the queries' first.
+template <int DT, int LPR, bool INTER>
+__global__ void __launch_bounds__(kThreads, 3) k_fwd(brc_norm_rope a, void* q_out, void* k_out,
+                                                  int q_chunks, int iters) {
   constexpr int G = 32 / LPR;
-  constexpr bool kWrite = KIND >= 0;
-  const brc_norm_rope& a = g.a;
-  const int lane = threadIdx.x & 31, part = lane % LPR, e = part * 8;
+  const int lane = threadIdx.x & 31, part = lane % LPR;
   const int64_t token = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (token >= a.tokens) return;
-  const int heads = a.hq + (kWrite ? 2 : 1) * a.hk;
-  const int h0 = blockIdx.y * (kHeads * G) + lane / LPR;
+  const bool is_q = (int)blockIdx.y < q_chunks;
+  const int heads = is_q ? a.hq : a.hk;
+  const int chunk = is_q ? blockIdx.y : blockIdx.y - q_chunks;
+  const int64_t hs = is_q ? a.q_head : a.k_head;
+  const void* const x = is_q ? a.q : a.k;
+  void* const out = is_q ? q_out : k_out;
+  const int64_t in0 = token * (is_q ? a.q_token : a.k_token);
+  const int64_t out0 = token * heads * a.d;
+  const bool on = part * 8 < a.d;
+  int e0, e1;
+  groups<INTER>(a.rot, part, e0, e1);
+  const float inv_d = 1.f / (float)a.d;
+  float w[8], c[4], s[4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 0.f;
+  int h0 = chunk * iters * (kHeads * G) + lane / LPR;
+  for (int it = 0; it < iters; ++it, h0 += kHeads * G) {
+    float f[kHeads][8];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * G;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+      if (on && h < heads) {
+        load4<DT>(x, in0 + h * hs + e0, f[u]);
+        load4<DT>(x, in0 + h * hs + e1, f[u] + 4);
+      }
+    }
+    if (it == 0) {
+      if (on) {
+        load_w4(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
+        load_w4(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
+      }
+      load_angles(a, token, part, c, s);
+    }
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * G;
+      norm_turn<LPR, INTER>(f[u], w, c, s, inv_d, a.eps);
+      if (on && h < heads) {
+        store4<DT>(out, out0 + h * a.d + e0, f[u]);
+        store4<DT>(out, out0 + h * a.d + e1, f[u] + 4);
+      }
+    }
+  }
+}
+
+// Norm, rotation and the write into a cache. blockIdx.y: a batch of heads of
+// queries, of keys or of values. The arithmetic is k_fwd's, operation by
+// operation; a key's scales are over elements in a row, so its groups of four
+// change lanes (as halves, after their rounding) before they are encoded.
+template <int DT, int LPR, bool INTER, int KIND, int FMT>
+__global__ void __launch_bounds__(kThreads) k_fwd_write(FwdArgs g, int q_chunks, int k_chunks) {
+  constexpr int G = 32 / LPR;
+  const brc_norm_rope& a = g.a;
+  const int lane = threadIdx.x & 31, part = lane % LPR;
+  const int64_t token = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (token >= a.tokens) return;
+  const bool is_q = (int)blockIdx.y < q_chunks, is_v = (int)blockIdx.y >= q_chunks + k_chunks;
+  const int heads = is_q ? a.hq : a.hk;
+  const int chunk = is_q ? blockIdx.y : blockIdx.y - q_chunks - (is_v ? k_chunks : 0);
+  const int h0 = chunk * (kHeads * G) + lane / LPR;
+  int64_t slot = load_index(g.slots, token, g.slots64);
+  if (slot >= g.c.num_pages * g.c.page_size) slot = -1;
   float f[kHeads][8];
+  if (is_v) {
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * G;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+      if (h < heads) kv::load8<DT>(g.v, token * g.v_token + h * g.v_head + part * 8, f[u]);
+    }
+  } else {
+    const int64_t hs = is_q ? a.q_head : a.k_head;
+    const void* const x = is_q ? a.q : a.k;
+    const int64_t in0 = token * (is_q ? a.q_token : a.k_token);
+    int e0, e1;
+    groups<INTER>(a.rot, part, e0, e1);
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * G;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+      if (h < heads) {
+        load4<DT>(x, in0 + h * hs + e0, f[u]);
+        load4<DT>(x, in0 + h * hs + e1, f[u] + 4);
+      }
+    }
+    float w[8], c[4], s[4];
+    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
+    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
+    load_angles(a, token, part, c, s);
+    const float inv_d = 1.f / (float)a.d;
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      norm_turn<LPR, INTER>(f[u], w, c, s, inv_d, a.eps);
+      const int h = h0 + u * G;
+      if (is_q) {
+        if (h < heads) {
+          store4<DT>(g.q_out, (token * heads + h) * a.d + e0, f[u]);
+          store4<DT>(g.q_out, (token * heads + h) * a.d + e1, f[u] + 4);
+        }
+      } else {
+        // the key as the separate call would have left it, in its own dtype
+        uint4 y = kv::pack8<DT>(f[u]);
+        if constexpr (!INTER) {
+          uint32_t z[4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // elements 8 part + 4 i ..
+            const int four = 2 * part + i, half = a.rot >> 3;
+            const bool turned = four < 2 * half;
+            const int from = turned ? (four < half ? four : four - half) : part;
+            const bool second = turned ? four >= half : i;
+            const uint32_t a0 = __shfl_sync(0xFFFFFFFFu, y.x, from, LPR);
+            const uint32_t a1 = __shfl_sync(0xFFFFFFFFu, y.y, from, LPR);
+            const uint32_t b0 = __shfl_sync(0xFFFFFFFFu, y.z, from, LPR);
+            const uint32_t b1 = __shfl_sync(0xFFFFFFFFu, y.w, from, LPR);
+            z[2 * i] = second ? b0 : a0;
+            z[2 * i + 1] = second ? b1 : a1;
+          }
+          y = make_uint4(z[0], z[1], z[2], z[3]);
+        }
+        unpack<DT>(y, f[u]);
+      }
+    }
+    if (is_q) return;
+  }
 #pragma unroll
   for (int u = 0; u < kHeads; ++u) {
     const int h = h0 + u * G;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
-    if (h < heads && e < a.d) {
-      if (h < a.hq) kv::load8<DT>(a.q, token * a.q_token + h * a.q_head + e, f[u]);
-      else if (h < a.hq + a.hk)
-        kv::load8<DT>(a.k, token * a.k_token + (h - a.hq) * a.k_head + e, f[u]);
-      else if constexpr (kWrite)
-        kv::load8<DT>(g.v, token * g.v_token + (h - a.hq - a.hk) * g.v_head + e, f[u]);
-    }
-  }
-  Turn t;
-  load_turn(a, token, part, t);
-  int64_t slot = -1;
-  if constexpr (kWrite) {
-    slot = load_index(g.slots, token, g.slots64);
-    if (slot >= g.c.num_pages * g.c.page_size) slot = -1;
-  }
-#pragma unroll
-  for (int u = 0; u < kHeads; ++u) {
-    const int h = h0 + u * G;
-    const bool on = h < heads && e < a.d, is_v = h >= a.hq + a.hk;
-    float ss, eps = a.eps, x[8], z[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = is_v ? 0.f : f[u][i];
-      z[i] = 0.f;
-    }
-    square_sum<LPR>(x, ss, eps);
-    const float r = rsqrtf(ss / (float)a.d + eps);
-    if (on && !is_v) {
-      load_w(h < a.hq ? a.wq : a.wk, a.w_dtype, e, z);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = x[i] * r * z[i];
-    }
-    turn8<LPR>(t, a.interleaved, false, z);
-    if (on && h < a.hq) kv::store8<DT>(g.q_out, (token * a.hq + h) * a.d + e, z);
-    if constexpr (!kWrite) {
-      if (on && h >= a.hq) kv::store8<DT>(g.k_out, (token * a.hk + h - a.hq) * a.d + e, z);
-    } else {
-      // the key as the separate call would have left it, in its own dtype
-      if (!is_v) unpack<DT>(kv::pack8<DT>(z), f[u]);
-      const bool keep = on && h >= a.hq && slot >= 0;
-      const int head = is_v ? h - a.hq - a.hk : h - a.hq;
-      kv::encode_row<KIND, FMT, LPR>(f[u], part, keep, keep ? kv::row_of(g.c, slot, head) : 0,
-                                     is_v ? g.c.v_data : g.c.k_data,
-                                     is_v ? g.c.v_scale : g.c.k_scale);
-    }
+    const bool keep = h < heads && slot >= 0;
+    kv::encode_row<KIND, FMT, LPR>(f[u], part, keep, keep ? kv::row_of(g.c, slot, h) : 0,
+                                   is_v ? g.c.v_data : g.c.k_data,
+                                   is_v ? g.c.v_scale : g.c.k_scale);
   }
 }
 
 // ------------------------------------------------------------------ backward
 struct BwdArgs {
   brc_norm_rope a;
-  const void* gq;
-  const void* gk;
-  int64_t gq_token, gq_head, gk_token, gk_head;
-  void* dq;
-  void* dk;
-  float* part;  // (blocks, 2, d) sums of the weight gradients
-  int64_t units;  // tokens * chunks
-  int chunks;
+  const void* g[2];  // gradients of the queries' and keys' outputs
+  int64_t g_token[2], g_head[2];
+  void* dx[2];
+  float* part;      // (blocks, d) sums of the weight gradients
+  int q_blocks;     // blocks that take queries; the rest take keys
+  int parts_shift;  // a token's heads go to 2^parts_shift warps
 };
 
 constexpr int kBwdHeads = 2;
-constexpr int kBwdBlocksMax = 148 * 4;
+constexpr int kBwdPerSm = 3;
 
 // Persistent: a lane sums the weight gradients of its eight elements over all
-// the heads that it takes, so that only one row per block is written.
-template <int DT, int LPR>
-__global__ void __launch_bounds__(kThreads) k_bwd(BwdArgs g) {
+// the heads that it takes, so that one row per block is written.
+template <int DT, int LPR, bool INTER>
+__global__ void __launch_bounds__(kThreads, kBwdPerSm) k_bwd(BwdArgs g) {
   constexpr int G = 32 / LPR;
   const brc_norm_rope& a = g.a;
-  const int lane = threadIdx.x & 31, part = lane % LPR, e = part * 8;
-  const int heads = a.hq + a.hk;
-  float dwq[8], dwk[8];
+  const int lane = threadIdx.x & 31, part = lane % LPR;
+  const bool is_q = (int)blockIdx.x < g.q_blocks;
+  const int side = is_q ? 0 : 1, heads = is_q ? a.hq : a.hk;
+  const int block = is_q ? blockIdx.x : blockIdx.x - g.q_blocks;
+  const int blocks = is_q ? g.q_blocks : gridDim.x - g.q_blocks;
+  const int64_t xt = is_q ? a.q_token : a.k_token, xh = is_q ? a.q_head : a.k_head;
+  const int64_t gt = is_q ? g.g_token[0] : g.g_token[1], gh = is_q ? g.g_head[0] : g.g_head[1];
+  const void* const px = is_q ? a.q : a.k;
+  const void* const pg = is_q ? g.g[0] : g.g[1];
+  void* const dx = is_q ? g.dx[0] : g.dx[1];
+  const bool on = part * 8 < a.d;
+  int e0, e1;
+  groups<INTER>(a.rot, part, e0, e1);
+  const float inv_d = 1.f / (float)a.d;
+  float w[8], dw[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dwq[i] = dwk[i] = 0.f;
-  float wq[8], wk[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) wq[i] = wk[i] = 0.f;
-  if (e < a.d) {
-    if (a.hq) load_w(a.wq, a.w_dtype, e, wq);
-    if (a.hk) load_w(a.wk, a.w_dtype, e, wk);
+  for (int i = 0; i < 8; ++i) w[i] = dw[i] = 0.f;
+  if (on) {
+    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
+    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
   }
-  const int64_t step = (int64_t)gridDim.x * kWarps;
-  for (int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); unit < g.units;
-       unit += step) {
-    const int64_t token = unit / g.chunks;
-    const int h0 = (int)(unit - token * g.chunks) * (kBwdHeads * G) + lane / LPR;
-    float x[kBwdHeads][8], gy[kBwdHeads][8];
+  const int n_parts = 1 << g.parts_shift;
+  const int per = (heads + n_parts - 1) >> g.parts_shift;  // heads of one warp
+  const int64_t units = a.tokens << g.parts_shift;
+  for (int64_t unit = (int64_t)block * kWarps + (threadIdx.x >> 5); unit < units;
+       unit += (int64_t)blocks * kWarps) {
+    const int64_t token = unit >> g.parts_shift;
+    const int first = (int)(unit & (n_parts - 1)) * per, last = min(first + per, heads);
+    float c[4], s[4];
+    load_angles(a, token, part, c, s);
+    for (int h0 = first; h0 < last; h0 += kBwdHeads * G) {
+      float x[kBwdHeads][8], gy[kBwdHeads][8];
 #pragma unroll
-    for (int u = 0; u < kBwdHeads; ++u) {
-      const int h = h0 + u * G;
+      for (int u = 0; u < kBwdHeads; ++u) {
+        const int h = h0 + u * G + lane / LPR;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][i] = gy[u][i] = 0.f;
-      if (h < heads && e < a.d) {
-        if (h < a.hq) {
-          kv::load8<DT>(a.q, token * a.q_token + h * a.q_head + e, x[u]);
-          kv::load8<DT>(g.gq, token * g.gq_token + h * g.gq_head + e, gy[u]);
-        } else {
-          kv::load8<DT>(a.k, token * a.k_token + (h - a.hq) * a.k_head + e, x[u]);
-          kv::load8<DT>(g.gk, token * g.gk_token + (h - a.hq) * g.gk_head + e, gy[u]);
+        for (int i = 0; i < 8; ++i) x[u][i] = gy[u][i] = 0.f;
+        if (on && h < last) {
+          load4<DT>(px, token * xt + h * xh + e0, x[u]);
+          load4<DT>(px, token * xt + h * xh + e1, x[u] + 4);
+          load4<DT>(pg, token * gt + h * gh + e0, gy[u]);
+          load4<DT>(pg, token * gt + h * gh + e1, gy[u] + 4);
         }
       }
-    }
-    Turn t;
-    load_turn(a, token, part, t);
 #pragma unroll
-    for (int u = 0; u < kBwdHeads; ++u) {
-      const int h = h0 + u * G;
-      const bool on = h < heads && e < a.d, is_q = h < a.hq;
-      turn8<LPR>(t, a.interleaved, true, gy[u]);
-      float ss, hx = 0.f, eps = a.eps;
-      const float by = square_sum<LPR>(x[u], ss, eps);
+      for (int u = 0; u < kBwdHeads; ++u) {
+        const int h = h0 + u * G + lane / LPR;
+        turn_pairs<INTER, true>(c, s, gy[u]);
+        float ss, hx = 0.f, eps = a.eps;
+        const float by = square_sum<LPR>(x[u], ss, eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) hx += gy[u][i] * (is_q ? wq[i] : wk[i]) * x[u][i];
-      hx = sum_row<LPR>(hx);
-      const float r = rsqrtf(ss / (float)a.d + eps);
-      const float m = hx * r / (float)a.d;  // mean(gz w x r)
-      float o[8];
+        for (int i = 0; i < 8; ++i) hx += gy[u][i] * w[i] * x[u][i];
+        hx = sum_row<LPR>(hx);
+        const float r = rsqrtf(ss * inv_d + eps);
+        const float m = hx * r * inv_d;  // mean(gz w x r)
+        if (on && h < last) {
+          float o[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float n = x[u][i] * r;
-        dwq[i] += on && is_q ? gy[u][i] * n : 0.f;
-        dwk[i] += on && !is_q ? gy[u][i] * n : 0.f;
-        o[i] = r * (gy[u][i] * (is_q ? wq[i] : wk[i]) - n * m) * by;
-      }
-      if (on) {
-        if (is_q) kv::store8<DT>(g.dq, (token * a.hq + h) * a.d + e, o);
-        else kv::store8<DT>(g.dk, (token * a.hk + h - a.hq) * a.d + e, o);
+          for (int i = 0; i < 8; ++i) {
+            const float n = x[u][i] * r;
+            dw[i] += gy[u][i] * n;
+            o[i] = r * (gy[u][i] * w[i] - n * m) * by;
+          }
+          store4<DT>(dx, (token * heads + h) * a.d + e0, o);
+          store4<DT>(dx, (token * heads + h) * a.d + e1, o + 4);
+        }
       }
     }
   }
   // lanes of the same elements: G per warp, kWarps warps
-  __shared__ float sm[kWarps * G][2][LPR * 8];
+  __shared__ float sm[kWarps * G][LPR * 8];
   const int mine = (threadIdx.x >> 5) * G + lane / LPR;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    sm[mine][0][e + i] = dwq[i];
-    sm[mine][1][e + i] = dwk[i];
+  for (int i = 0; i < 4; ++i) {
+    sm[mine][e0 + i] = dw[i];
+    sm[mine][e1 + i] = dw[4 + i];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * a.d; i += kThreads) {
-    const int side = i >= a.d, at = i - side * a.d;
-    float s = 0.f;
+  for (int i = threadIdx.x; i < a.d; i += kThreads) {
+    float t = 0.f;
 #pragma unroll
-    for (int j = 0; j < kWarps * G; ++j) s += sm[j][side][at];
-    g.part[(int64_t)blockIdx.x * 2 * a.d + i] = s;
+    for (int j = 0; j < kWarps * G; ++j) t += sm[j][i];
+    g.part[(int64_t)blockIdx.x * a.d + i] = t;
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Sums of the blocks' rows: 32 columns to a block, 16 row groups.
-__global__ void __launch_bounds__(512) k_bwd_weights(const float* part, int blocks, int d,
-                                                     int w_dtype, void* dwq, void* dwk) {
+// Sums of the blocks' rows: 32 columns to a block, 16 row groups, in order.
+__global__ void __launch_bounds__(512) k_bwd_weights(const float* part, int q_blocks, int blocks,
+                                                     int d, int w_dtype, void* dwq, void* dwk) {
   __shared__ float sm[16][33];
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), grp = threadIdx.x >> 5;
+  void* const out = blockIdx.y ? dwk : dwq;
+  const int first = blockIdx.y ? q_blocks : 0, last = blockIdx.y ? blocks : q_blocks;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float s = 0.f;
-  if (col < 2 * d)
-    for (int b = grp; b < blocks; b += 16) s += part[(int64_t)b * 2 * d + col];
+  if (col < d)
+    for (int b = first + grp; b < last; b += 16) s += part[(int64_t)b * d + col];
   sm[grp][threadIdx.x & 31] = s;
   __syncthreads();
-  if (grp == 0 && col < 2 * d) {
+  if (grp == 0 && col < d && out) {
 #pragma unroll
     for (int j = 1; j < 16; ++j) s += sm[j][threadIdx.x];
-    void* out = col < d ? dwq : dwk;
-    const int at = col < d ? col : col - d;
-    if (out) {
-      if (w_dtype == BRC_DTYPE_F32) static_cast<float*>(out)[at] = s;
-      else if (w_dtype == BRC_DTYPE_BF16)
-        static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(s);
-      else static_cast<__half*>(out)[at] = __float2half_rn(s);
-    }
+    if (w_dtype == BRC_DTYPE_F32) static_cast<float*>(out)[col] = s;
+    else if (w_dtype == BRC_DTYPE_BF16)
+      static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(s);
+    else static_cast<__half*>(out)[col] = __float2half_rn(s);
   }
 }
 
@@ -355,38 +471,71 @@ int check(const brc_norm_rope* a) {
 
 int lanes_per_row(int d) { return d <= 64 ? 8 : d <= 128 ? 16 : 32; }
 
-template <int DT, int KIND, int FMT>
-int launch_fwd(const FwdArgs& g, cudaStream_t st) {
-  const int lpr = lanes_per_row(g.a.d), per = kHeads * (32 / lpr);
-  const int heads = g.a.hq + (KIND >= 0 ? 2 : 1) * g.a.hk;
-  const int64_t bx = (g.a.tokens + kWarps - 1) / kWarps;
-  const int64_t by = (heads + per - 1) / per;
-  if (bx > 0x7FFFFFFF || by > 65535) return BRC_ERR_RANGE;
-  const dim3 grid((unsigned)bx, (unsigned)by);
-  if (lpr == 8) k_fwd<DT, 8, KIND, FMT><<<grid, kThreads, 0, st>>>(g);
-  else if (lpr == 16) k_fwd<DT, 16, KIND, FMT><<<grid, kThreads, 0, st>>>(g);
-  else k_fwd<DT, 32, KIND, FMT><<<grid, kThreads, 0, st>>>(g);
+template <int DT, int LPR>
+int launch_fwd(const brc_norm_rope& a, void* q_out, void* k_out, cudaStream_t st) {
+  const int64_t bx = (a.tokens + kWarps - 1) / kWarps;
+  // one batch of heads to a warp while that leaves SMs free, then two (the
+  // token's angles and the weights are loaded half as often)
+  const int per1 = kHeads * (32 / LPR);
+  const int64_t blocks1 = bx * ((a.hq + per1 - 1) / per1 + (a.hk + per1 - 1) / per1);
+  const int iters = blocks1 > 8 * sm_count() ? 2 : 1, per = per1 * iters;
+  const int q_chunks = (a.hq + per - 1) / per, chunks = q_chunks + (a.hk + per - 1) / per;
+  if (bx > 0x7FFFFFFF || chunks > 65535) return BRC_ERR_RANGE;
+  const dim3 grid((unsigned)bx, (unsigned)chunks);
+  if (a.interleaved) k_fwd<DT, LPR, true><<<grid, kThreads, 0, st>>>(a, q_out, k_out, q_chunks, iters);
+  else k_fwd<DT, LPR, false><<<grid, kThreads, 0, st>>>(a, q_out, k_out, q_chunks, iters);
   return check_launch();
+}
+template <int DT>
+int launch_fwd_any(const brc_norm_rope& a, void* q_out, void* k_out, cudaStream_t st) {
+  const int lpr = lanes_per_row(a.d);
+  return lpr == 8    ? launch_fwd<DT, 8>(a, q_out, k_out, st)
+         : lpr == 16 ? launch_fwd<DT, 16>(a, q_out, k_out, st)
+                     : launch_fwd<DT, 32>(a, q_out, k_out, st);
+}
+
+template <int DT, int LPR, int KIND, int FMT>
+int launch_fwd_write(const FwdArgs& g, cudaStream_t st) {
+  const int per = kHeads * (32 / LPR);
+  const int64_t bx = (g.a.tokens + kWarps - 1) / kWarps;
+  const int q_chunks = (g.a.hq + per - 1) / per, k_chunks = (g.a.hk + per - 1) / per;
+  if (bx > 0x7FFFFFFF || q_chunks + 2 * k_chunks > 65535) return BRC_ERR_RANGE;
+  const dim3 grid((unsigned)bx, (unsigned)(q_chunks + 2 * k_chunks));
+  if (g.a.interleaved)
+    k_fwd_write<DT, LPR, true, KIND, FMT><<<grid, kThreads, 0, st>>>(g, q_chunks, k_chunks);
+  else k_fwd_write<DT, LPR, false, KIND, FMT><<<grid, kThreads, 0, st>>>(g, q_chunks, k_chunks);
+  return check_launch();
+}
+template <int DT, int KIND, int FMT>
+int launch_write_dim(const FwdArgs& g, cudaStream_t st) {
+  return g.a.d == 64    ? launch_fwd_write<DT, 8, KIND, FMT>(g, st)
+         : g.a.d == 128 ? launch_fwd_write<DT, 16, KIND, FMT>(g, st)
+                        : launch_fwd_write<DT, 32, KIND, FMT>(g, st);
 }
 
 template <int DT>
 int launch_write(const FwdArgs& g, cudaStream_t st) {
   const bool e4 = g.c.fmt == BRC_FP8_E4M3;
   if (g.c.kind == BRC_STE_BLOCK_FP8)
-    return e4 ? launch_fwd<DT, BRC_STE_BLOCK_FP8, BRC_FP8_E4M3>(g, st)
-              : launch_fwd<DT, BRC_STE_BLOCK_FP8, BRC_FP8_E5M2>(g, st);
+    return e4 ? launch_write_dim<DT, BRC_STE_BLOCK_FP8, BRC_FP8_E4M3>(g, st)
+              : launch_write_dim<DT, BRC_STE_BLOCK_FP8, BRC_FP8_E5M2>(g, st);
   if (g.c.kind == BRC_STE_MXFP8)
-    return e4 ? launch_fwd<DT, BRC_STE_MXFP8, BRC_FP8_E4M3>(g, st)
-              : launch_fwd<DT, BRC_STE_MXFP8, BRC_FP8_E5M2>(g, st);
-  return launch_fwd<DT, BRC_STE_NVFP4, BRC_FP8_E4M3>(g, st);
+    return e4 ? launch_write_dim<DT, BRC_STE_MXFP8, BRC_FP8_E4M3>(g, st)
+              : launch_write_dim<DT, BRC_STE_MXFP8, BRC_FP8_E5M2>(g, st);
+  return launch_write_dim<DT, BRC_STE_NVFP4, BRC_FP8_E4M3>(g, st);
 }
 
-template <int DT>
+template <int DT, int LPR>
 void launch_bwd(const BwdArgs& g, int blocks, cudaStream_t st) {
+  if (g.a.interleaved) k_bwd<DT, LPR, true><<<blocks, kThreads, 0, st>>>(g);
+  else k_bwd<DT, LPR, false><<<blocks, kThreads, 0, st>>>(g);
+}
+template <int DT>
+void launch_bwd_any(const BwdArgs& g, int blocks, cudaStream_t st) {
   const int lpr = lanes_per_row(g.a.d);
-  if (lpr == 8) k_bwd<DT, 8><<<blocks, kThreads, 0, st>>>(g);
-  else if (lpr == 16) k_bwd<DT, 16><<<blocks, kThreads, 0, st>>>(g);
-  else k_bwd<DT, 32><<<blocks, kThreads, 0, st>>>(g);
+  if (lpr == 8) launch_bwd<DT, 8>(g, blocks, st);
+  else if (lpr == 16) launch_bwd<DT, 16>(g, blocks, st);
+  else launch_bwd<DT, 32>(g, blocks, st);
 }
 
 }  // namespace
@@ -401,14 +550,10 @@ int brc_qk_norm_rope(const brc_norm_rope* a, void* q_out, void* k_out, void* str
   if (a->tokens == 0 || a->hq + a->hk == 0) return BRC_OK;
   if ((a->hq && !q_out) || (a->hk && !k_out)) return BRC_ERR_NULL;
   if (((uintptr_t)q_out | (uintptr_t)k_out) & 15) return BRC_ERR_ALIGN;
-  FwdArgs g{};
-  g.a = *a;
-  g.q_out = q_out;
-  g.k_out = k_out;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (a->dtype == BRC_DTYPE_F32) return launch_fwd<BRC_DTYPE_F32, -1, 0>(g, st);
-  if (a->dtype == BRC_DTYPE_BF16) return launch_fwd<BRC_DTYPE_BF16, -1, 0>(g, st);
-  return launch_fwd<BRC_DTYPE_F16, -1, 0>(g, st);
+  if (a->dtype == BRC_DTYPE_F32) return launch_fwd_any<BRC_DTYPE_F32>(*a, q_out, k_out, st);
+  if (a->dtype == BRC_DTYPE_BF16) return launch_fwd_any<BRC_DTYPE_BF16>(*a, q_out, k_out, st);
+  return launch_fwd_any<BRC_DTYPE_F16>(*a, q_out, k_out, st);
 }
 
 int brc_qk_norm_rope_write(const brc_norm_rope* a, const void* v, int64_t v_token, int64_t v_head,
@@ -437,7 +582,7 @@ int brc_qk_norm_rope_write(const brc_norm_rope* a, const void* v, int64_t v_toke
 }
 
 int64_t brc_qk_norm_rope_bwd_workspace(int d) {
-  return d < 16 || d > 256 ? 0 : (int64_t)kBwdBlocksMax * 2 * d * 4;
+  return d < 16 || d > 256 ? 0 : (int64_t)sm_count() * kBwdPerSm * d * 4;
 }
 
 int brc_qk_norm_rope_bwd(const brc_norm_rope* a, const void* gq, const void* gk, int64_t gq_token,
@@ -448,7 +593,7 @@ int brc_qk_norm_rope_bwd(const brc_norm_rope* a, const void* gq, const void* gk,
   if ((a->hq && !dwq) || (a->hk && !dwk) || !workspace) return BRC_ERR_NULL;
   if (workspace_bytes < brc_qk_norm_rope_bwd_workspace(a->d)) return BRC_ERR_SHAPE;
   const cudaStream_t st = (cudaStream_t)stream;
-  int blocks = 0;
+  int blocks = 0, q_blocks = 0;
   if (a->tokens > 0 && a->hq + a->hk > 0) {
     if ((a->hq && (!gq || !dq)) || (a->hk && (!gk || !dk))) return BRC_ERR_NULL;
     if (((uintptr_t)gq | (uintptr_t)gk | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)workspace) & 15)
@@ -456,20 +601,48 @@ int brc_qk_norm_rope_bwd(const brc_norm_rope* a, const void* gq, const void* gk,
     if (bad_stride(gq_token, a->dtype) || bad_stride(gq_head, a->dtype) ||
         bad_stride(gk_token, a->dtype) || bad_stride(gk_head, a->dtype))
       return BRC_ERR_ALIGN;
-    const int per = kBwdHeads * (32 / lanes_per_row(a->d));
-    BwdArgs g{*a, gq, gk, gq_token, gq_head, gk_token, gk_head, dq, dk,
-              static_cast<float*>(workspace), 0, (a->hq + a->hk + per - 1) / per};
-    g.units = a->tokens * g.chunks;
-    const int64_t want = (g.units + kWarps - 1) / kWarps;
-    blocks = (int)(want < kBwdBlocksMax ? want : kBwdBlocksMax);
-    if (a->dtype == BRC_DTYPE_F32) launch_bwd<BRC_DTYPE_F32>(g, blocks, st);
-    else if (a->dtype == BRC_DTYPE_BF16) launch_bwd<BRC_DTYPE_BF16>(g, blocks, st);
-    else launch_bwd<BRC_DTYPE_F16>(g, blocks, st);
+    BwdArgs g{};
+    g.a = *a;
+    g.g[0] = gq;
+    g.g[1] = gk;
+    g.g_token[0] = gq_token;
+    g.g_token[1] = gk_token;
+    g.g_head[0] = gq_head;
+    g.g_head[1] = gk_head;
+    g.dx[0] = dq;
+    g.dx[1] = dk;
+    g.part = static_cast<float*>(workspace);
+    // enough warps for every SM, none with less than a batch of heads
+    const int most = sm_count() * kBwdPerSm, per = kBwdHeads * (32 / lanes_per_row(a->d));
+    const int heads = a->hq > a->hk ? a->hq : a->hk;
+    while (g.parts_shift < 4 && (a->tokens << g.parts_shift) < 8 * (int64_t)most * kWarps &&
+           (heads >> g.parts_shift) > per)
+      ++g.parts_shift;
+    const int64_t want = ((a->tokens << g.parts_shift) + kWarps - 1) / kWarps;  // of one side
+    // the SMs are shared out by the number of heads
+    int q_share = a->hk ? (int)((int64_t)most * a->hq / (a->hq + a->hk)) : most;
+    if (a->hq && q_share < 1) q_share = 1;
+    if (a->hk && q_share > most - 1) q_share = most - 1;
+    q_blocks = a->hq ? (int)(want < q_share ? want : q_share) : 0;
+    const int k_share = most - q_share;
+    blocks = q_blocks + (a->hk ? (int)(want < k_share ? want : k_share) : 0);
+    g.q_blocks = q_blocks;
+    if (a->dtype == BRC_DTYPE_F32) launch_bwd_any<BRC_DTYPE_F32>(g, blocks, st);
+    else if (a->dtype == BRC_DTYPE_BF16) launch_bwd_any<BRC_DTYPE_BF16>(g, blocks, st);
+    else launch_bwd_any<BRC_DTYPE_F16>(g, blocks, st);
     if (const int rc = check_launch()) return rc;
   }
-  k_bwd_weights<<<(2 * a->d + 31) / 32, 512, 0, st>>>(static_cast<const float*>(workspace), blocks,
-                                                      a->d, a->w_dtype, dwq, dwk);
-  return check_launch();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((a->d + 31) / 32, 2);
+  cfg.blockDim = dim3(512);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, k_bwd_weights, static_cast<const float*>(workspace),
+                                       q_blocks, blocks, a->d, a->w_dtype, dwq, dwk));
 }
 
 }  // extern "C"

@@ -425,7 +425,7 @@ int brc_qk_norm_rope(const brc_norm_rope* a, void* q_out, void* k_out, void* str
  * the outputs, of the inputs' dtype; dq, dk contiguous like q_out, k_out; dwq,
  * dwk: d gradients of w_dtype, summed in float32 in a fixed order (the result
  * does not change between runs). workspace: brc_qk_norm_rope_bwd_workspace(d)
- * bytes, 16-byte aligned. */
+ * bytes (for the current device), 16-byte aligned. */
 int64_t brc_qk_norm_rope_bwd_workspace(int d);
 int brc_qk_norm_rope_bwd(const brc_norm_rope* a, const void* gq, const void* gk, int64_t gq_token,
                          int64_t gq_head, int64_t gk_token, int64_t gk_head, void* dq, void* dk,
