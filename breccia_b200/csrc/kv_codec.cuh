@@ -81,6 +81,25 @@ __device__ __forceinline__ void load8(const void* p, int64_t e, float* f) {
     unpack<DT>(ldg16(static_cast<const char*>(p) + 2 * e), f);
   }
 }
+// The same as they lie in memory: rows in flight wait in this form.
+template <int DT>
+struct Raw8 {
+  uint4 v;
+};
+template <>
+struct Raw8<BRC_DTYPE_F32> {
+  uint4 v, w;
+};
+template <int DT>
+__device__ __forceinline__ void load_raw8(const void* p, int64_t e, Raw8<DT>& r) {
+  r.v = ldg16(static_cast<const char*>(p) + (DT == BRC_DTYPE_F32 ? 4 : 2) * e);
+  if constexpr (DT == BRC_DTYPE_F32) r.w = ldg16(static_cast<const char*>(p) + 4 * e + 16);
+}
+template <int DT>
+__device__ __forceinline__ void expand8(const Raw8<DT>& r, float* f) {
+  unpack<DT>(r.v, f);
+  if constexpr (DT == BRC_DTYPE_F32) unpack<DT>(r.w, f + 4);
+}
 template <int DT>
 __device__ __forceinline__ void store8(void* p, int64_t e, const float* f) {
   if constexpr (DT == BRC_DTYPE_F32) {
@@ -171,29 +190,43 @@ __device__ __forceinline__ void encode_row(const float* f, int part, bool on, in
   }
 }
 
-// Eight decoded elements of a row: decode(code) * scale in float32.
-template <int KIND, int FMT, int LPR>
-__device__ __forceinline__ void decode_row(const uint8_t* data, const void* scale, int64_t row,
-                                           int part, float* f) {
+// One lane's eight codes of a row and their scale (zeros decode to zeros).
+template <int KIND>
+struct RowCodes {
+  uint32_t w[KIND == BRC_STE_NVFP4 ? 1 : 2];
+  uint32_t s;
+};
+template <int KIND, int LPR>
+__device__ __forceinline__ void load_codes(const uint8_t* data, const void* scale, int64_t row,
+                                           int part, RowCodes<KIND>& c) {
+  if constexpr (KIND == BRC_STE_NVFP4) {
+    c.w[0] = __ldg(reinterpret_cast<const uint32_t*>(data + row * (LPR * 4)) + part);
+    c.s = __ldg(static_cast<const uint8_t*>(scale) + row * (LPR / 2) + part / 2);
+  } else {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(data + row * (LPR * 8)) + part);
+    c.w[0] = w.x;
+    c.w[1] = w.y;
+    if constexpr (KIND == BRC_STE_BLOCK_FP8) c.s = __ldg(static_cast<const uint32_t*>(scale) + row);
+    else c.s = __ldg(static_cast<const uint8_t*>(scale) + row * (LPR / 4) + part / 4);
+  }
+}
+// decode(code) * scale in float32.
+template <int KIND, int FMT>
+__device__ __forceinline__ void decode_codes(const RowCodes<KIND>& c, float* f) {
   float s;
   if constexpr (KIND == BRC_STE_NVFP4) {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(data + row * (LPR * 4))[part];
-    s = dec_e4m3(static_cast<const uint8_t*>(scale)[row * (LPR / 2) + part / 2]);
+    s = dec_e4m3(c.s);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      f16x2_to_f32(e2m1x2_to_f16x2(w >> (8 * i)), f[2 * i], f[2 * i + 1]);
+      f16x2_to_f32(e2m1x2_to_f16x2(c.w[0] >> (8 * i)), f[2 * i], f[2 * i + 1]);
   } else {
-    const uint2 w = reinterpret_cast<const uint2*>(data + row * (LPR * 8))[part];
-    if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-      s = static_cast<const float*>(scale)[row];
-    } else {
-      const uint32_t e = static_cast<const uint8_t*>(scale)[row * (LPR / 4) + part / 4];
-      s = e == 255 ? __uint_as_float(0x7F800000u) : pow2i((int)e - 127);
+    if constexpr (KIND == BRC_STE_BLOCK_FP8) s = __uint_as_float(c.s);
+    else s = c.s == 255 ? __uint_as_float(0x7F800000u) : pow2i((int)c.s - 127);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f16x2_to_f32(fp8x2_to_f16x2<FMT>(c.w[i]), f[4 * i], f[4 * i + 1]);
+      f16x2_to_f32(fp8x2_to_f16x2<FMT>(c.w[i] >> 16), f[4 * i + 2], f[4 * i + 3]);
     }
-    f16x2_to_f32(fp8x2_to_f16x2<FMT>(w.x), f[0], f[1]);
-    f16x2_to_f32(fp8x2_to_f16x2<FMT>(w.x >> 16), f[2], f[3]);
-    f16x2_to_f32(fp8x2_to_f16x2<FMT>(w.y), f[4], f[5]);
-    f16x2_to_f32(fp8x2_to_f16x2<FMT>(w.y >> 16), f[6], f[7]);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], s);

@@ -13,7 +13,8 @@ namespace kv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 4;  // rows in flight per lane
+constexpr int kRows = 4;  // rows in flight per lane, as they lie in memory
+constexpr int kReadRows = 8;
 
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
   return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
@@ -31,7 +32,7 @@ struct WriteArgs {
 
 // blockIdx.y: 0 keys, 1 values.
 template <int DT, int KIND, int FMT, int LPR>
-__global__ void __launch_bounds__(kThreads) k_write(WriteArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) k_write(WriteArgs a) {
   constexpr int G = 32 / LPR;
   const int lane = threadIdx.x & 31, part = lane % LPR;
   const int side = blockIdx.y;
@@ -42,24 +43,26 @@ __global__ void __launch_bounds__(kThreads) k_write(WriteArgs a) {
   const int64_t slots = a.c.num_pages * a.c.page_size;
   const uint32_t first =
       (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
-  float f[kRows][8];
+  Raw8<DT> f[kRows];
   int64_t row[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const uint32_t r = first + u * G;
     row[u] = -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+    f[u] = Raw8<DT>{};
     if (r < a.rows) {
       const uint32_t t = a.heads(r), h = r - t * a.heads.d;
-      load8<DT>(x, t * ts + h * hs + part * 8, f[u]);
+      load_raw8<DT>(x, t * ts + h * hs + part * 8, f[u]);
       const int64_t slot = load_index(a.slots, t, a.slots64);
       if (slot >= 0 && slot < slots) row[u] = row_of(a.c, slot, (int)h);
     }
   }
 #pragma unroll
-  for (int u = 0; u < kRows; ++u)
-    encode_row<KIND, FMT, LPR>(f[u], part, row[u] >= 0, row[u], data, scale);
+  for (int u = 0; u < kRows; ++u) {
+    float y[8];
+    expand8<DT>(f[u], y);
+    encode_row<KIND, FMT, LPR>(y, part, row[u] >= 0, row[u], data, scale);
+  }
 }
 
 struct ReadArgs {
@@ -82,14 +85,13 @@ __global__ void __launch_bounds__(kThreads) k_read(ReadArgs a) {
   const void* scale = side ? a.c.v_scale : a.c.k_scale;
   void* out = side ? a.out[1] : a.out[0];
   const uint32_t first =
-      (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
+      (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kReadRows * G) + lane / LPR;
   const int shift = 31 - __clz(a.c.page_size);
-  float f[kRows][8];
+  RowCodes<KIND> w[kReadRows];
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
+  for (int u = 0; u < kReadRows; ++u) {
     const uint32_t r = first + u * G;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+    w[u] = RowCodes<KIND>{};
     if (r < a.rows) {
       const uint32_t bt = a.heads(r), h = r - bt * a.heads.d;
       const uint32_t b = a.length(bt), t = bt - b * a.length.d;
@@ -97,16 +99,20 @@ __global__ void __launch_bounds__(kThreads) k_read(ReadArgs a) {
       if ((int64_t)t < a.lengths[b] && p < (uint32_t)a.table_pages) {
         const int64_t page = a.table[b * a.table_stride + p];
         if (page >= 0 && page < a.c.num_pages)
-          decode_row<KIND, FMT, LPR>(
-              data, scale, ((page * a.c.heads + h) << shift) + (t & (a.c.page_size - 1)), part,
-              f[u]);
+          load_codes<KIND, LPR>(data, scale,
+                                ((page * a.c.heads + h) << shift) + (t & (a.c.page_size - 1)),
+                                part, w[u]);
       }
     }
   }
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
+  for (int u = 0; u < kReadRows; ++u) {
     const uint32_t r = first + u * G;
-    if (r < a.rows) store8<DT>(out, (int64_t)r * (LPR * 8) + part * 8, f[u]);
+    if (r < a.rows) {
+      float f[8];
+      decode_codes<KIND, FMT>(w[u], f);
+      store8<DT>(out, (int64_t)r * (LPR * 8) + part * 8, f);
+    }
   }
 }
 
@@ -153,8 +159,8 @@ struct LaunchRead {
 };
 
 // Blocks for `rows` rows of d elements; 0 where 32 bits do not count the rows.
-int64_t blocks_for(int64_t rows, int d) {
-  const int per = (kThreads / 32) * kRows * (32 / (d / 8));
+int64_t blocks_for(int64_t rows, int d, int in_flight) {
+  const int per = (kThreads / 32) * in_flight * (32 / (d / 8));
   return rows > 0xFFFFFFFFll - per ? 0 : (rows + per - 1) / per;
 }
 
@@ -182,7 +188,7 @@ int brc_kv_write(const brc_kv_cache* c, const void* k, const void* v, int dtype,
       bad_stride(v_head, dtype))
     return BRC_ERR_ALIGN;
   if (tokens > 0xFFFFFFFFll) return BRC_ERR_RANGE;
-  const int64_t n = blocks_for(tokens * c->heads, c->head_dim);
+  const int64_t n = blocks_for(tokens * c->heads, c->head_dim, kRows);
   if (n == 0) return BRC_ERR_RANGE;
   WriteArgs a{*c, {k, v}, {k_token, v_token}, {k_head, v_head}, slots, slots64,
               (uint32_t)(tokens * c->heads), Divide((uint32_t)c->heads)};
@@ -200,7 +206,7 @@ int brc_kv_read(const brc_kv_cache* c, const int32_t* table, int64_t table_strid
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return BRC_ERR_ALIGN;
   if (length > 0x7FFFFFFF || (int64_t)batch * length > 0xFFFFFFFFll) return BRC_ERR_RANGE;
   const int64_t rows = (int64_t)batch * length * c->heads;
-  const int64_t n = blocks_for(rows, c->head_dim);
+  const int64_t n = blocks_for(rows, c->head_dim, kReadRows);
   if (n == 0) return BRC_ERR_RANGE;
   ReadArgs a{*c, table, lengths, table_stride, (uint32_t)rows, table_pages,
              Divide((uint32_t)c->heads), Divide((uint32_t)length), {k_out, v_out}};

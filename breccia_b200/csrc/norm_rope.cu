@@ -77,22 +77,40 @@ __device__ __forceinline__ void groups(int rot, int part, int& e0, int& e1) {
     e1 = e0 + 4;
   }
 }
+// Four elements as they lie in memory (rows in flight wait in this form: half
+// the registers of their float32 values).
+template <int DT>
+struct Raw {
+  uint2 v;
+};
+template <>
+struct Raw<BRC_DTYPE_F32> {
+  uint4 v;
+};
+template <int DT>
+__device__ __forceinline__ void load_raw(const void* p, int64_t e, Raw<DT>& r) {
+  if constexpr (DT == BRC_DTYPE_F32) r.v = ldg16(static_cast<const char*>(p) + 4 * e);
+  else r.v = __ldg(reinterpret_cast<const uint2*>(static_cast<const char*>(p) + 2 * e));
+}
+template <int DT>
+__device__ __forceinline__ void expand(const Raw<DT>& r, float* f) {
+  if constexpr (DT == BRC_DTYPE_F32) {
+    unpack<DT>(r.v, f);
+  } else if constexpr (DT == BRC_DTYPE_BF16) {
+    f[0] = __uint_as_float(r.v.x << 16);
+    f[1] = __uint_as_float(r.v.x & 0xFFFF0000u);
+    f[2] = __uint_as_float(r.v.y << 16);
+    f[3] = __uint_as_float(r.v.y & 0xFFFF0000u);
+  } else {
+    f16x2_to_f32(r.v.x, f[0], f[1]);
+    f16x2_to_f32(r.v.y, f[2], f[3]);
+  }
+}
 template <int DT>
 __device__ __forceinline__ void load4(const void* p, int64_t e, float* f) {
-  if constexpr (DT == BRC_DTYPE_F32) {
-    unpack<DT>(ldg16(static_cast<const char*>(p) + 4 * e), f);
-  } else {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const char*>(p) + 2 * e));
-    if constexpr (DT == BRC_DTYPE_BF16) {
-      f[0] = __uint_as_float(v.x << 16);
-      f[1] = __uint_as_float(v.x & 0xFFFF0000u);
-      f[2] = __uint_as_float(v.y << 16);
-      f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-    } else {
-      f16x2_to_f32(v.x, f[0], f[1]);
-      f16x2_to_f32(v.y, f[2], f[3]);
-    }
-  }
+  Raw<DT> r;
+  load_raw<DT>(p, e, r);
+  expand<DT>(r, f);
 }
 template <int DT>
 __device__ __forceinline__ void store4(void* p, int64_t e, const float* f) {
@@ -166,13 +184,15 @@ __device__ __forceinline__ void norm_turn(float* x, const float* w, const float*
   turn_pairs<INTER, false>(c, s, x);
 }
 
-constexpr int kHeads = 4;  // heads in flight per lane
+// heads in flight per lane (a float32 element takes twice the registers)
+constexpr __host__ __device__ int heads_in_flight(int dt) { return dt == BRC_DTYPE_F32 ? 2 : 4; }
+constexpr int kHeads = 4;
 
-// blockIdx.y: a chunk of `iters` x kHeads x (32 / LPR) heads, the queries' first.
+// blockIdx.y: a chunk of `iters` batches of heads, the queries' first.
 template <int DT, int LPR, bool INTER>
-__global__ void __launch_bounds__(kThreads, 3) k_fwd(brc_norm_rope a, void* q_out, void* k_out,
+__global__ void __launch_bounds__(kThreads, 4) k_fwd(brc_norm_rope a, void* q_out, void* k_out,
                                                   int q_chunks, int iters) {
-  constexpr int G = 32 / LPR;
+  constexpr int G = 32 / LPR, kHeads = heads_in_flight(DT);
   const int lane = threadIdx.x & 31, part = lane % LPR;
   const int64_t token = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (token >= a.tokens) return;
@@ -193,15 +213,14 @@ __global__ void __launch_bounds__(kThreads, 3) k_fwd(brc_norm_rope a, void* q_ou
   for (int i = 0; i < 8; ++i) w[i] = 0.f;
   int h0 = chunk * iters * (kHeads * G) + lane / LPR;
   for (int it = 0; it < iters; ++it, h0 += kHeads * G) {
-    float f[kHeads][8];
+    Raw<DT> ra[kHeads], rb[kHeads];
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       const int h = h0 + u * G;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+      ra[u] = rb[u] = Raw<DT>{};
       if (on && h < heads) {
-        load4<DT>(x, in0 + h * hs + e0, f[u]);
-        load4<DT>(x, in0 + h * hs + e1, f[u] + 4);
+        load_raw<DT>(x, in0 + h * hs + e0, ra[u]);
+        load_raw<DT>(x, in0 + h * hs + e1, rb[u]);
       }
     }
     if (it == 0) {
@@ -214,10 +233,13 @@ __global__ void __launch_bounds__(kThreads, 3) k_fwd(brc_norm_rope a, void* q_ou
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       const int h = h0 + u * G;
-      norm_turn<LPR, INTER>(f[u], w, c, s, inv_d, a.eps);
+      float f[8];
+      expand<DT>(ra[u], f);
+      expand<DT>(rb[u], f + 4);
+      norm_turn<LPR, INTER>(f, w, c, s, inv_d, a.eps);
       if (on && h < heads) {
-        store4<DT>(out, out0 + h * a.d + e0, f[u]);
-        store4<DT>(out, out0 + h * a.d + e1, f[u] + 4);
+        store4<DT>(out, out0 + h * a.d + e0, f);
+        store4<DT>(out, out0 + h * a.d + e1, f + 4);
       }
     }
   }
@@ -365,27 +387,31 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) k_bwd(BwdArgs g) {
     float c[4], s[4];
     load_angles(a, token, part, c, s);
     for (int h0 = first; h0 < last; h0 += kBwdHeads * G) {
-      float x[kBwdHeads][8], gy[kBwdHeads][8];
+      Raw<DT> xa[kBwdHeads], xb[kBwdHeads], ga[kBwdHeads], gb[kBwdHeads];
 #pragma unroll
       for (int u = 0; u < kBwdHeads; ++u) {
         const int h = h0 + u * G + lane / LPR;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[u][i] = gy[u][i] = 0.f;
+        xa[u] = xb[u] = ga[u] = gb[u] = Raw<DT>{};
         if (on && h < last) {
-          load4<DT>(px, token * xt + h * xh + e0, x[u]);
-          load4<DT>(px, token * xt + h * xh + e1, x[u] + 4);
-          load4<DT>(pg, token * gt + h * gh + e0, gy[u]);
-          load4<DT>(pg, token * gt + h * gh + e1, gy[u] + 4);
+          load_raw<DT>(px, token * xt + h * xh + e0, xa[u]);
+          load_raw<DT>(px, token * xt + h * xh + e1, xb[u]);
+          load_raw<DT>(pg, token * gt + h * gh + e0, ga[u]);
+          load_raw<DT>(pg, token * gt + h * gh + e1, gb[u]);
         }
       }
 #pragma unroll
       for (int u = 0; u < kBwdHeads; ++u) {
         const int h = h0 + u * G + lane / LPR;
-        turn_pairs<INTER, true>(c, s, gy[u]);
+        float x[8], gy[8];
+        expand<DT>(xa[u], x);
+        expand<DT>(xb[u], x + 4);
+        expand<DT>(ga[u], gy);
+        expand<DT>(gb[u], gy + 4);
+        turn_pairs<INTER, true>(c, s, gy);
         float ss, hx = 0.f, eps = a.eps;
-        const float by = square_sum<LPR>(x[u], ss, eps);
+        const float by = square_sum<LPR>(x, ss, eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hx += gy[u][i] * w[i] * x[u][i];
+        for (int i = 0; i < 8; ++i) hx += gy[i] * w[i] * x[i];
         hx = sum_row<LPR>(hx);
         const float r = rsqrtf(ss * inv_d + eps);
         const float m = hx * r * inv_d;  // mean(gz w x r)
@@ -393,9 +419,9 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) k_bwd(BwdArgs g) {
           float o[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float n = x[u][i] * r;
-            dw[i] += gy[u][i] * n;
-            o[i] = r * (gy[u][i] * w[i] - n * m) * by;
+            const float n = x[i] * r;
+            dw[i] += gy[i] * n;
+            o[i] = r * (gy[i] * w[i] - n * m) * by;
           }
           store4<DT>(dx, (token * heads + h) * a.d + e0, o);
           store4<DT>(dx, (token * heads + h) * a.d + e1, o + 4);
@@ -476,7 +502,7 @@ int launch_fwd(const brc_norm_rope& a, void* q_out, void* k_out, cudaStream_t st
   const int64_t bx = (a.tokens + kWarps - 1) / kWarps;
   // one batch of heads to a warp while that leaves SMs free, then two (the
   // token's angles and the weights are loaded half as often)
-  const int per1 = kHeads * (32 / LPR);
+  const int per1 = heads_in_flight(DT) * (32 / LPR);
   const int64_t blocks1 = bx * ((a.hq + per1 - 1) / per1 + (a.hk + per1 - 1) / per1);
   const int iters = blocks1 > 8 * sm_count() ? 2 : 1, per = per1 * iters;
   const int q_chunks = (a.hq + per - 1) / per, chunks = q_chunks + (a.hk + per - 1) / per;
