@@ -833,8 +833,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
         if (row < a.rows && node < seq.drafts) {
           const int64_t at =
               (((int64_t)b * a.draft + node) * a.hq + head * a.group + (row - node * a.group)) * D + d0;
-          if (a.q_f16) kv::load8<BRC_DTYPE_F16>(a.q, at, f);
-          else kv::load8<BRC_DTYPE_BF16>(a.q, at, f);
+          const uint4 v = ldg16(static_cast<const uint16_t*>(a.q) + at);
+          if (a.q_f16) unpack<BRC_DTYPE_F16>(v, f);
+          else unpack<BRC_DTYPE_BF16>(v, f);
         }
         float top = 0.f;
 #pragma unroll

@@ -70,18 +70,8 @@ __device__ __forceinline__ uint4 pack8(const float* f) {  // 8 values, one round
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 8 consecutive elements of a row from / to global memory.
-template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t e, float* f) {
-  if constexpr (DT == BRC_DTYPE_F32) {
-    const char* s = static_cast<const char*>(p) + 4 * e;
-    unpack<DT>(ldg16(s), f);
-    unpack<DT>(ldg16(s + 16), f + 4);
-  } else {
-    unpack<DT>(ldg16(static_cast<const char*>(p) + 2 * e), f);
-  }
-}
-// The same as they lie in memory: rows in flight wait in this form.
+// 8 consecutive elements of a row as they lie in memory: rows in flight wait in
+// this form (half the registers of their float32 values, for half types).
 template <int DT>
 struct Raw8 {
   uint4 v;
@@ -113,80 +103,86 @@ __device__ __forceinline__ void store8(void* p, int64_t e, const float* f) {
   }
 }
 
-// Encode one row of LPR * 8 elements, eight to a lane (`part` = lane's place in
+// Encode one row of LPR * 16 elements, sixteen to a lane (`part` = lane's place in
 // the row), into row `row` of a cache side. Every lane of the warp calls it;
 // lanes with `on` false only take part in the shuffles.
 template <int KIND, int FMT, int LPR>
 __device__ __forceinline__ void encode_row(const float* f, int part, bool on, int64_t row,
                                            uint8_t* data, void* scale) {
-  constexpr int kBlockLanes = KIND == BRC_STE_BLOCK_FP8 ? LPR : KIND == BRC_STE_MXFP8 ? 4 : 2;
-  float am = fabsf(f[0]);
+  constexpr int kBlockLanes = KIND == BRC_STE_BLOCK_FP8 ? LPR : KIND == BRC_STE_MXFP8 ? 2 : 1;
+  float am = fmax_nan(fabsf(f[0]), fabsf(f[1]));
 #pragma unroll
-  for (int i = 1; i < 8; ++i) am = fmax_nan(am, fabsf(f[i]));
+  for (int i = 2; i < 16; ++i) am = fmax_nan(am, fabsf(f[i]));
 #pragma unroll
   for (int o = 1; o < kBlockLanes; o <<= 1)
     am = fmax_nan(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
   am = fmax_nan(am, 1e-10f);
+  if (!on) return;
   constexpr float kMax = FMT == BRC_FP8_E4M3 ? 448.f : 57344.f;
   constexpr float kRcp = FMT == BRC_FP8_E4M3 ? kRcp448 : kRcp57344;
-  const bool first = on && part % kBlockLanes == 0;
-  uint32_t w[2];
+  const bool first = part % kBlockLanes == 0;
+  uint32_t w[4];
   if constexpr (KIND == BRC_STE_BLOCK_FP8) {
     const float s = div_const(am, kMax, kRcp);
     if (first) static_cast<float*>(scale)[row] = canon_nan(s);
     if (isfinite(s)) {
       const float r = __frcp_rn(s);
-      w[0] = enc4_div<enc4p_fp8<FMT>>(f, s, r);
-      w[1] = enc4_div<enc4p_fp8<FMT>>(f + 4, s, r);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = enc4_div<enc4p_fp8<FMT>>(f + 4 * j, s, r);
     } else {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 4; ++j) {
         w[j] = 0;
         for (int i = 0; i < 4; ++i) w[j] |= enc1_fp8<FMT>(div_ieee(f[4 * j + i], s)) << (8 * i);
       }
     }
   } else if constexpr (KIND == BRC_STE_MXFP8) {
     const uint32_t e = e8m0_code(div_const(am, kMax, kRcp), g_thr);
-    if (first) static_cast<uint8_t*>(scale)[row * (LPR / 4) + part / 4] = (uint8_t)e;
+    if (first) static_cast<uint8_t*>(scale)[row * (LPR / 2) + part / 2] = (uint8_t)e;
     if (isfinite(am)) {
       const float r = pow2i(127 - (int)e);  // exact reciprocal of the scale
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        w[j] = enc4_fp8<FMT>(__fmul_rn(f[4 * j], r), __fmul_rn(f[4 * j + 1], r),
-                             __fmul_rn(f[4 * j + 2], r), __fmul_rn(f[4 * j + 3], r));
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = __fmul2_rn(make_float2(f[4 * j], f[4 * j + 1]), make_float2(r, r));
+        const float2 b = __fmul2_rn(make_float2(f[4 * j + 2], f[4 * j + 3]), make_float2(r, r));
+        w[j] = enc4p_fp8<FMT>(a.x, a.y, b.x, b.y);
+      }
     } else {
       const float s = pow2i((int)e - 127);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 4; ++j) {
         w[j] = 0;
         for (int i = 0; i < 4; ++i) w[j] |= enc1_fp8<FMT>(div_ieee(f[4 * j + i], s)) << (8 * i);
       }
     }
   } else {
     const uint32_t sc = enc1_e4m3(div_const(am, 6.f, kRcp6));
-    if (first) static_cast<uint8_t*>(scale)[row * (LPR / 2) + part / 2] = (uint8_t)sc;
+    static_cast<uint8_t*>(scale)[row * LPR + part] = (uint8_t)sc;
     float s = dec_e4m3(sc);
     if (!(s > 0.f)) s = 0x1p-9f;
     if (isfinite(am)) {
       const float r = __frcp_rn(s);
-      w[0] = enc4_div<enc4p_e2m1>(f, s, r);
-      w[1] = enc4_div<enc4p_e2m1>(f + 4, s, r);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = enc4_div<enc4p_e2m1>(f + 4 * j, s, r);
     } else {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 4; ++j) {
         w[j] = 0;
         for (int i = 0; i < 4; ++i) w[j] |= enc1_e2m1(div_ieee(f[4 * j + i], s)) << (8 * i);
       }
     }
   }
-  if (!on) return;
   if constexpr (KIND == BRC_STE_NVFP4) {
     // bytes (c0 c1 c2 c3) to nibble pairs: element 2i in the low half
-    const uint32_t a = w[0] | (w[0] >> 4), b = w[1] | (w[1] >> 4);
-    reinterpret_cast<uint32_t*>(data + row * (LPR * 4))[part] =
-        __byte_perm(a, b, 0x6420);
+    uint32_t n[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t a = w[2 * j] | (w[2 * j] >> 4), b = w[2 * j + 1] | (w[2 * j + 1] >> 4);
+      n[j] = __byte_perm(a, b, 0x6420);
+    }
+    reinterpret_cast<uint2*>(data + row * (LPR * 8))[part] = make_uint2(n[0], n[1]);
   } else {
-    reinterpret_cast<uint2*>(data + row * (LPR * 8))[part] = make_uint2(w[0], w[1]);
+    stg16(data + row * (LPR * 16) + part * 16, make_uint4(w[0], w[1], w[2], w[3]));
   }
 }
 

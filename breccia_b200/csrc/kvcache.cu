@@ -1,10 +1,12 @@
 // Quantised key/value cache: rows written as they are produced, and read back.
 //
-// Both are streams: a row (one token, one head) is read once and written once,
-// and HBM bounds them at long prompts. A row lies on d / 8 lanes, eight
-// elements to a lane: a warp's loads and stores of elements are then 512
-// contiguous bytes, and the block amax of a scale is a few shuffles. Every
-// lane keeps the loads of several rows in flight.
+// Both are streams: a row (one token, one head) is read once and written once;
+// HBM bounds the read at long prompts, the encoders' integer arithmetic the
+// write. To write, a row lies on d / 16 lanes, sixteen elements to a lane, so
+// that a scale's block is one or two lanes (block FP8: the row) and what a row
+// costs beside its elements is shared by twice as many. To read, it lies on d /
+// 8: the 16-byte stores of a warp are then 512 contiguous bytes. Every lane has
+// several rows in flight.
 #include "kv_codec.cuh"
 #include "launch.h"
 
@@ -13,8 +15,8 @@ namespace kv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 4;  // rows in flight per lane, as they lie in memory
-constexpr int kReadRows = 8;
+constexpr int kReadRows = 8;  // rows in flight per lane, as they lie in memory
+constexpr __host__ __device__ int write_rows(int dt) { return dt == BRC_DTYPE_F32 ? 1 : 2; }
 
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
   return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
@@ -33,7 +35,7 @@ struct WriteArgs {
 // blockIdx.y: 0 keys, 1 values.
 template <int DT, int KIND, int FMT, int LPR>
 __global__ void __launch_bounds__(kThreads, 4) k_write(WriteArgs a) {
-  constexpr int G = 32 / LPR;
+  constexpr int G = 32 / LPR, kRows = write_rows(DT);
   const int lane = threadIdx.x & 31, part = lane % LPR;
   const int side = blockIdx.y;
   const void* x = side ? a.x[1] : a.x[0];
@@ -43,25 +45,28 @@ __global__ void __launch_bounds__(kThreads, 4) k_write(WriteArgs a) {
   const int64_t slots = a.c.num_pages * a.c.page_size;
   const uint32_t first =
       (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (kRows * G) + lane / LPR;
-  Raw8<DT> f[kRows];
+  Raw8<DT> lo[kRows], hi[kRows];
   int64_t row[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const uint32_t r = first + u * G;
     row[u] = -1;
-    f[u] = Raw8<DT>{};
+    lo[u] = hi[u] = Raw8<DT>{};
     if (r < a.rows) {
       const uint32_t t = a.heads(r), h = r - t * a.heads.d;
-      load_raw8<DT>(x, t * ts + h * hs + part * 8, f[u]);
+      const int64_t at = t * ts + h * hs + part * 16;
+      load_raw8<DT>(x, at, lo[u]);
+      load_raw8<DT>(x, at + 8, hi[u]);
       const int64_t slot = load_index(a.slots, t, a.slots64);
       if (slot >= 0 && slot < slots) row[u] = row_of(a.c, slot, (int)h);
     }
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    float y[8];
-    expand8<DT>(f[u], y);
-    encode_row<KIND, FMT, LPR>(y, part, row[u] >= 0, row[u], data, scale);
+    float f[16];
+    expand8<DT>(lo[u], f);
+    expand8<DT>(hi[u], f + 8);
+    encode_row<KIND, FMT, LPR>(f, part, row[u] >= 0, row[u], data, scale);
   }
 }
 
@@ -116,12 +121,13 @@ __global__ void __launch_bounds__(kThreads) k_read(ReadArgs a) {
   }
 }
 
+// Launch gets the head dimension.
 template <template <int, int, int, int> class Launch, int DT, int KIND, int FMT, class Args>
 int by_dim(int d, const Args& a, dim3 grid, cudaStream_t st) {
   switch (d) {
-    case 64: Launch<DT, KIND, FMT, 8>::run(a, grid, st); break;
-    case 128: Launch<DT, KIND, FMT, 16>::run(a, grid, st); break;
-    default: Launch<DT, KIND, FMT, 32>::run(a, grid, st); break;
+    case 64: Launch<DT, KIND, FMT, 64>::run(a, grid, st); break;
+    case 128: Launch<DT, KIND, FMT, 128>::run(a, grid, st); break;
+    default: Launch<DT, KIND, FMT, 256>::run(a, grid, st); break;
   }
   return check_launch();
 }
@@ -145,22 +151,22 @@ int by_dtype(int dt, const Args& a, dim3 grid, cudaStream_t st) {
     default: return by_kind<Launch, BRC_DTYPE_F16>(a, grid, st);
   }
 }
-template <int DT, int KIND, int FMT, int LPR>
+template <int DT, int KIND, int FMT, int D>
 struct LaunchWrite {
   static void run(const WriteArgs& a, dim3 grid, cudaStream_t st) {
-    k_write<DT, KIND, FMT, LPR><<<grid, kThreads, 0, st>>>(a);
+    k_write<DT, KIND, FMT, D / 16><<<grid, kThreads, 0, st>>>(a);
   }
 };
-template <int DT, int KIND, int FMT, int LPR>
+template <int DT, int KIND, int FMT, int D>
 struct LaunchRead {
   static void run(const ReadArgs& a, dim3 grid, cudaStream_t st) {
-    k_read<DT, KIND, FMT, LPR><<<grid, kThreads, 0, st>>>(a);
+    k_read<DT, KIND, FMT, D / 8><<<grid, kThreads, 0, st>>>(a);
   }
 };
 
-// Blocks for `rows` rows of d elements; 0 where 32 bits do not count the rows.
-int64_t blocks_for(int64_t rows, int d, int in_flight) {
-  const int per = (kThreads / 32) * in_flight * (32 / (d / 8));
+// Blocks for `rows` rows, `per_warp` to a warp; 0 where 32 bits do not count them.
+int64_t blocks_for(int64_t rows, int per_warp) {
+  const int per = (kThreads / 32) * per_warp;
   return rows > 0xFFFFFFFFll - per ? 0 : (rows + per - 1) / per;
 }
 
@@ -188,7 +194,7 @@ int brc_kv_write(const brc_kv_cache* c, const void* k, const void* v, int dtype,
       bad_stride(v_head, dtype))
     return BRC_ERR_ALIGN;
   if (tokens > 0xFFFFFFFFll) return BRC_ERR_RANGE;
-  const int64_t n = blocks_for(tokens * c->heads, c->head_dim, kRows);
+  const int64_t n = blocks_for(tokens * c->heads, write_rows(dtype) * (32 / (c->head_dim / 16)));
   if (n == 0) return BRC_ERR_RANGE;
   WriteArgs a{*c, {k, v}, {k_token, v_token}, {k_head, v_head}, slots, slots64,
               (uint32_t)(tokens * c->heads), Divide((uint32_t)c->heads)};
@@ -206,7 +212,7 @@ int brc_kv_read(const brc_kv_cache* c, const int32_t* table, int64_t table_strid
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return BRC_ERR_ALIGN;
   if (length > 0x7FFFFFFF || (int64_t)batch * length > 0xFFFFFFFFll) return BRC_ERR_RANGE;
   const int64_t rows = (int64_t)batch * length * c->heads;
-  const int64_t n = blocks_for(rows, c->head_dim, kReadRows);
+  const int64_t n = blocks_for(rows, kReadRows * (32 / (c->head_dim / 8)));
   if (n == 0) return BRC_ERR_RANGE;
   ReadArgs a{*c, table, lengths, table_stride, (uint32_t)rows, table_pages,
              Divide((uint32_t)c->heads), Divide((uint32_t)length), {k_out, v_out}};

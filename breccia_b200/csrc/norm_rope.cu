@@ -5,12 +5,14 @@
 //   gz = R^T gy,  gw = sum gz x r,  gx = r (gz w - x r mean(gz w x r))
 //
 // A stream: HBM bounds it at long prompts, launch latency at single tokens. A
-// head lies on LPR = 8, 16 or 32 lanes, eight elements to a lane in two groups
-// of four that hold whole rotated pairs (halves: elements 4 p .. and rot / 2 +
-// 4 p ..; interleaved: 8 p .. 8 p + 7), so a lane turns its pairs by itself with
-// four cosines and sines, and a head's sums are shuffles. A warp takes several
-// heads of one token, all queries or all keys: the token's angles and the
-// weights are loaded once.
+// head lies on LPR = d / 16 lanes (rounded up to 4, 8 or 16), sixteen elements to a
+// lane in two groups of eight that hold whole rotated pairs (halves: elements 8 p
+// .. and rot / 2 + 8 p ..; interleaved: 16 p .. 16 p + 15), so a lane turns its
+// pairs by itself with eight cosines and sines, and a head's sums are shuffles.
+// Eight elements to a lane took 1.6 times the instructions per element and were
+// bound by them. A warp takes several heads of one token, all queries or all
+// keys: the token's angles and the weights are loaded once. Arithmetic is in
+// packed pairs.
 #include "kv_codec.cuh"
 #include "launch.h"
 
@@ -42,16 +44,18 @@ __device__ __forceinline__ float sum_row(float v) {
   return v;
 }
 
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
 // Sum of squares of a row; where it passes float32's range the row is taken
 // 2^-64 times (x r does not change when eps goes with 2^-128). Every lane of
-// the warp calls it. Returns what the row's reciprocal root comes out scaled by.
+// the warp calls it. Returns what the row was multiplied by.
 template <int LPR>
-__device__ __forceinline__ float square_sum(float* x, float& ss, float& eps) {
+__device__ __forceinline__ float square_sum(float2* x, float& ss, float& eps) {
   auto sum = [&]() {
-    float v = 0.f;
+    float2 v = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v = __fmaf_rn(x[i], x[i], v);
-    return sum_row<LPR>(v);
+    for (int i = 0; i < 8; ++i) v = __ffma2_rn(x[i], x[i], v);
+    return sum_row<LPR>(__fadd_rn(v.x, v.y));
   };
   ss = sum();
   float by = 1.f;
@@ -59,139 +63,116 @@ __device__ __forceinline__ float square_sum(float* x, float& ss, float& eps) {
     by = isinf(ss) ? 0x1p-64f : 1.f;
     eps *= by * by;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= by;
+    for (int i = 0; i < 8; ++i) x[i] = __fmul2_rn(x[i], splat(by));
     ss = sum();
   }
   return by;
 }
 
-// ------------------------------------------------------------------ pairs in a lane
-// First elements of lane `part`'s two groups of four.
+// First elements of lane `part`'s two groups of eight.
 template <bool INTER>
 __device__ __forceinline__ void groups(int rot, int part, int& e0, int& e1) {
-  if (!INTER && part * 8 < rot) {
-    e0 = 4 * part;
-    e1 = (rot >> 1) + 4 * part;
-  } else {  // whole pairs, or elements that are not rotated
+  if (!INTER && part * 16 < rot) {
     e0 = 8 * part;
-    e1 = e0 + 4;
-  }
-}
-// Four elements as they lie in memory (rows in flight wait in this form: half
-// the registers of their float32 values).
-template <int DT>
-struct Raw {
-  uint2 v;
-};
-template <>
-struct Raw<BRC_DTYPE_F32> {
-  uint4 v;
-};
-template <int DT>
-__device__ __forceinline__ void load_raw(const void* p, int64_t e, Raw<DT>& r) {
-  if constexpr (DT == BRC_DTYPE_F32) r.v = ldg16(static_cast<const char*>(p) + 4 * e);
-  else r.v = __ldg(reinterpret_cast<const uint2*>(static_cast<const char*>(p) + 2 * e));
-}
-template <int DT>
-__device__ __forceinline__ void expand(const Raw<DT>& r, float* f) {
-  if constexpr (DT == BRC_DTYPE_F32) {
-    unpack<DT>(r.v, f);
-  } else if constexpr (DT == BRC_DTYPE_BF16) {
-    f[0] = __uint_as_float(r.v.x << 16);
-    f[1] = __uint_as_float(r.v.x & 0xFFFF0000u);
-    f[2] = __uint_as_float(r.v.y << 16);
-    f[3] = __uint_as_float(r.v.y & 0xFFFF0000u);
-  } else {
-    f16x2_to_f32(r.v.x, f[0], f[1]);
-    f16x2_to_f32(r.v.y, f[2], f[3]);
+    e1 = (rot >> 1) + 8 * part;
+  } else {  // whole pairs, or elements that are not rotated
+    e0 = 16 * part;
+    e1 = e0 + 8;
   }
 }
 template <int DT>
-__device__ __forceinline__ void load4(const void* p, int64_t e, float* f) {
-  Raw<DT> r;
-  load_raw<DT>(p, e, r);
+__device__ __forceinline__ void expand(const kv::Raw8<DT>& r, float2* f) {
+  float g[8];
+  kv::expand8<DT>(r, g);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(g[2 * i], g[2 * i + 1]);
+}
+template <int DT>
+__device__ __forceinline__ void store(void* p, int64_t e, const float2* f) {
+  float g[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    g[2 * i] = f[i].x;
+    g[2 * i + 1] = f[i].y;
+  }
+  kv::store8<DT>(p, e, g);
+}
+template <int DT>
+__device__ __forceinline__ void load_w_as(const void* w, int e, float2* f) {
+  kv::Raw8<DT> r;
+  kv::load_raw8<DT>(w, e, r);
   expand<DT>(r, f);
 }
-template <int DT>
-__device__ __forceinline__ void store4(void* p, int64_t e, const float* f) {
-  if constexpr (DT == BRC_DTYPE_F32) {
-    stg16(static_cast<char*>(p) + 4 * e, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
-                                                    __float_as_uint(f[2]), __float_as_uint(f[3])));
-  } else {
-    uint32_t w[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (DT == BRC_DTYPE_BF16) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&b);
-      } else {
-        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    *reinterpret_cast<uint2*>(static_cast<char*>(p) + 2 * e) = make_uint2(w[0], w[1]);
-  }
+__device__ __forceinline__ void load_w(const void* w, int dtype, int e, float2* f) {
+  if (dtype == BRC_DTYPE_F32) load_w_as<BRC_DTYPE_F32>(w, e, f);
+  else if (dtype == BRC_DTYPE_BF16) load_w_as<BRC_DTYPE_BF16>(w, e, f);
+  else load_w_as<BRC_DTYPE_F16>(w, e, f);
 }
-__device__ __forceinline__ void load_w4(const void* w, int dtype, int e, float* f) {
-  if (dtype == BRC_DTYPE_F32) load4<BRC_DTYPE_F32>(w, e, f);
-  else if (dtype == BRC_DTYPE_BF16) load4<BRC_DTYPE_BF16>(w, e, f);
-  else load4<BRC_DTYPE_F16>(w, e, f);
-}
-// The four angles of lane `part`'s pairs; (1, 0) where nothing is rotated; a
+// The eight angles of lane `part`'s pairs; (1, 0) where nothing is rotated; a
 // NaN cosine for a position outside the table (not a wrong angle).
 __device__ __forceinline__ void load_angles(const brc_norm_rope& a, int64_t token, int part,
-                                            float* c, float* s) {
+                                            float2* c, float2* s) {
   const int64_t pos = load_index(a.positions, token, a.index64);
   const bool in = pos >= 0 && pos < a.table_rows;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
+    c[i] = splat(1.f);
+    s[i] = splat(0.f);
   }
-  if (part * 8 < a.rot) {
-    const int64_t at = (in ? pos : 0) * (a.rot >> 1) + 4 * part;
-    load4<BRC_DTYPE_F32>(a.cos, at, c);
-    load4<BRC_DTYPE_F32>(a.sin, at, s);
+  if (part * 16 < a.rot) {
+    const int64_t at = (in ? pos : 0) * (a.rot >> 1) + 8 * part;
+    kv::Raw8<BRC_DTYPE_F32> r;
+    kv::load_raw8<BRC_DTYPE_F32>(a.cos, at, r);
+    expand<BRC_DTYPE_F32>(r, c);
+    kv::load_raw8<BRC_DTYPE_F32>(a.sin, at, r);
+    expand<BRC_DTYPE_F32>(r, s);
   }
   if (!in) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = __uint_as_float(0x7FC00000u);
+    for (int i = 0; i < 4; ++i) c[i] = splat(__uint_as_float(0x7FC00000u));
   }
 }
-// R z (BACK: R^T z) of the lane's eight elements.
+// R z (BACK: R^T z) of the lane's sixteen elements. Each operation is named, so
+// that every kernel rounds alike.
 template <bool INTER, bool BACK>
-__device__ __forceinline__ void turn_pairs(const float* c, const float* s, float* z) {
+__device__ __forceinline__ void turn_pairs(const float2* c, const float2* s, float2* z) {
+  if constexpr (INTER) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int x = INTER ? 2 * i : i, y = INTER ? 2 * i + 1 : i + 4;
-    const float u = z[x], v = z[y], t = BACK ? -s[i] : s[i];
-    z[x] = __fmaf_rn(u, c[i], -__fmul_rn(v, t));
-    z[y] = __fmaf_rn(v, c[i], __fmul_rn(u, t));
+    for (int i = 0; i < 8; ++i) {
+      const float ci = i & 1 ? c[i / 2].y : c[i / 2].x, si = i & 1 ? s[i / 2].y : s[i / 2].x;
+      const float t = BACK ? -si : si;
+      z[i] = __ffma2_rn(z[i], splat(ci), __fmul2_rn(make_float2(z[i].y, z[i].x), make_float2(-t, t)));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 u = z[i], v = z[i + 4], n = make_float2(-s[i].x, -s[i].y);
+      z[i] = __ffma2_rn(u, c[i], __fmul2_rn(v, BACK ? s[i] : n));
+      z[i + 4] = __ffma2_rn(v, c[i], __fmul2_rn(u, BACK ? n : s[i]));
+    }
   }
 }
 
 // ------------------------------------------------------------------ forward
-// One row, in place; every lane of the warp calls it. Each operation is named,
-// so that both kernels below round alike.
+// One row, in place; every lane of the warp calls it.
 template <int LPR, bool INTER>
-__device__ __forceinline__ void norm_turn(float* x, const float* w, const float* c, const float* s,
-                                          float inv_d, float eps) {
+__device__ __forceinline__ void norm_turn(float2* x, const float2* w, const float2* c,
+                                          const float2* s, float inv_d, float eps) {
   float ss;
   square_sum<LPR>(x, ss, eps);
   const float r = rsqrtf(__fmaf_rn(ss, inv_d, eps));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
+  for (int i = 0; i < 8; ++i) x[i] = __fmul2_rn(__fmul2_rn(x[i], splat(r)), w[i]);
   turn_pairs<INTER, false>(c, s, x);
 }
 
-// heads in flight per lane (a float32 element takes twice the registers)
-constexpr __host__ __device__ int heads_in_flight(int dt) { return dt == BRC_DTYPE_F32 ? 2 : 4; }
-constexpr int kHeads = 4;
+// Heads in flight per lane (a float32 element takes twice the registers).
+constexpr __host__ __device__ int heads_in_flight(int dt) { return dt == BRC_DTYPE_F32 ? 1 : 2; }
 
 // blockIdx.y: a chunk of `iters` batches of heads, the queries' first.
 template <int DT, int LPR, bool INTER>
-__global__ void __launch_bounds__(kThreads, 4) k_fwd(brc_norm_rope a, void* q_out, void* k_out,
-                                                  int q_chunks, int iters) {
+__global__ void __launch_bounds__(kThreads, 3) k_fwd(brc_norm_rope a, void* q_out, void* k_out,
+                                                     int q_chunks, int iters) {
   constexpr int G = 32 / LPR, kHeads = heads_in_flight(DT);
   const int lane = threadIdx.x & 31, part = lane % LPR;
   const int64_t token = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -204,42 +185,42 @@ __global__ void __launch_bounds__(kThreads, 4) k_fwd(brc_norm_rope a, void* q_ou
   void* const out = is_q ? q_out : k_out;
   const int64_t in0 = token * (is_q ? a.q_token : a.k_token);
   const int64_t out0 = token * heads * a.d;
-  const bool on = part * 8 < a.d;
+  const bool on = part * 16 < a.d;
   int e0, e1;
   groups<INTER>(a.rot, part, e0, e1);
   const float inv_d = 1.f / (float)a.d;
-  float w[8], c[4], s[4];
+  float2 w[8], c[4], s[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = 0.f;
+  for (int i = 0; i < 8; ++i) w[i] = splat(0.f);
   int h0 = chunk * iters * (kHeads * G) + lane / LPR;
   for (int it = 0; it < iters; ++it, h0 += kHeads * G) {
-    Raw<DT> ra[kHeads], rb[kHeads];
+    kv::Raw8<DT> ra[kHeads], rb[kHeads];
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       const int h = h0 + u * G;
-      ra[u] = rb[u] = Raw<DT>{};
+      ra[u] = rb[u] = kv::Raw8<DT>{};
       if (on && h < heads) {
-        load_raw<DT>(x, in0 + h * hs + e0, ra[u]);
-        load_raw<DT>(x, in0 + h * hs + e1, rb[u]);
+        kv::load_raw8<DT>(x, in0 + h * hs + e0, ra[u]);
+        kv::load_raw8<DT>(x, in0 + h * hs + e1, rb[u]);
       }
     }
     if (it == 0) {
       if (on) {
-        load_w4(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
-        load_w4(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
+        load_w(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
+        load_w(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
       }
       load_angles(a, token, part, c, s);
     }
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       const int h = h0 + u * G;
-      float f[8];
+      float2 f[8];
       expand<DT>(ra[u], f);
       expand<DT>(rb[u], f + 4);
       norm_turn<LPR, INTER>(f, w, c, s, inv_d, a.eps);
       if (on && h < heads) {
-        store4<DT>(out, out0 + h * a.d + e0, f);
-        store4<DT>(out, out0 + h * a.d + e1, f + 4);
+        store<DT>(out, out0 + h * a.d + e0, f);
+        store<DT>(out, out0 + h * a.d + e1, f + 4);
       }
     }
   }
@@ -247,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_fwd(brc_norm_rope a, void* q_ou
 
 // Norm, rotation and the write into a cache. blockIdx.y: a batch of heads of
 // queries, of keys or of values. The arithmetic is k_fwd's, operation by
-// operation; a key's scales are over elements in a row, so its groups of four
+// operation; a key's scales are over elements in a row, so its groups of eight
 // change lanes (as halves, after their rounding) before they are encoded.
 template <int DT, int LPR, bool INTER, int KIND, int FMT>
 __global__ void __launch_bounds__(kThreads) k_fwd_write(FwdArgs g, int q_chunks, int k_chunks) {
@@ -259,81 +240,76 @@ __global__ void __launch_bounds__(kThreads) k_fwd_write(FwdArgs g, int q_chunks,
   const bool is_q = (int)blockIdx.y < q_chunks, is_v = (int)blockIdx.y >= q_chunks + k_chunks;
   const int heads = is_q ? a.hq : a.hk;
   const int chunk = is_q ? blockIdx.y : blockIdx.y - q_chunks - (is_v ? k_chunks : 0);
-  const int h0 = chunk * (kHeads * G) + lane / LPR;
-  int64_t slot = load_index(g.slots, token, g.slots64);
+  const int h = chunk * G + lane / LPR;
+  const bool on = h < heads;
+  int64_t slot = -1;
+  if (!is_q) slot = load_index(g.slots, token, g.slots64);
   if (slot >= g.c.num_pages * g.c.page_size) slot = -1;
-  float f[kHeads][8];
+  kv::Raw8<DT> ra{}, rb{};
+  float y[16];
   if (is_v) {
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int h = h0 + u * G;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
-      if (h < heads) kv::load8<DT>(g.v, token * g.v_token + h * g.v_head + part * 8, f[u]);
+    if (on) {
+      kv::load_raw8<DT>(g.v, token * g.v_token + h * g.v_head + part * 16, ra);
+      kv::load_raw8<DT>(g.v, token * g.v_token + h * g.v_head + part * 16 + 8, rb);
     }
   } else {
-    const int64_t hs = is_q ? a.q_head : a.k_head;
-    const void* const x = is_q ? a.q : a.k;
-    const int64_t in0 = token * (is_q ? a.q_token : a.k_token);
+    const int64_t at = is_q ? token * a.q_token + h * a.q_head : token * a.k_token + h * a.k_head;
     int e0, e1;
     groups<INTER>(a.rot, part, e0, e1);
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int h = h0 + u * G;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
-      if (h < heads) {
-        load4<DT>(x, in0 + h * hs + e0, f[u]);
-        load4<DT>(x, in0 + h * hs + e1, f[u] + 4);
-      }
+    if (on) {
+      kv::load_raw8<DT>(is_q ? a.q : a.k, at + e0, ra);
+      kv::load_raw8<DT>(is_q ? a.q : a.k, at + e1, rb);
     }
-    float w[8], c[4], s[4];
-    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
-    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
+    float2 w[8], c[4], s[4], f[8];
+    load_w(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
+    load_w(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
     load_angles(a, token, part, c, s);
-    const float inv_d = 1.f / (float)a.d;
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      norm_turn<LPR, INTER>(f[u], w, c, s, inv_d, a.eps);
-      const int h = h0 + u * G;
-      if (is_q) {
-        if (h < heads) {
-          store4<DT>(g.q_out, (token * heads + h) * a.d + e0, f[u]);
-          store4<DT>(g.q_out, (token * heads + h) * a.d + e1, f[u] + 4);
-        }
-      } else {
-        // the key as the separate call would have left it, in its own dtype
-        uint4 y = kv::pack8<DT>(f[u]);
-        if constexpr (!INTER) {
-          uint32_t z[4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {  // elements 8 part + 4 i ..
-            const int four = 2 * part + i, half = a.rot >> 3;
-            const bool turned = four < 2 * half;
-            const int from = turned ? (four < half ? four : four - half) : part;
-            const bool second = turned ? four >= half : i;
-            const uint32_t a0 = __shfl_sync(0xFFFFFFFFu, y.x, from, LPR);
-            const uint32_t a1 = __shfl_sync(0xFFFFFFFFu, y.y, from, LPR);
-            const uint32_t b0 = __shfl_sync(0xFFFFFFFFu, y.z, from, LPR);
-            const uint32_t b1 = __shfl_sync(0xFFFFFFFFu, y.w, from, LPR);
-            z[2 * i] = second ? b0 : a0;
-            z[2 * i + 1] = second ? b1 : a1;
-          }
-          y = make_uint4(z[0], z[1], z[2], z[3]);
-        }
-        unpack<DT>(y, f[u]);
+    expand<DT>(ra, f);
+    expand<DT>(rb, f + 4);
+    norm_turn<LPR, INTER>(f, w, c, s, 1.f / (float)a.d, a.eps);
+    if (is_q) {
+      if (on) {
+        store<DT>(g.q_out, (token * heads + h) * a.d + e0, f);
+        store<DT>(g.q_out, (token * heads + h) * a.d + e1, f + 4);
       }
+      return;
     }
-    if (is_q) return;
-  }
+    // the key as the separate call would have left it, in its own dtype
 #pragma unroll
-  for (int u = 0; u < kHeads; ++u) {
-    const int h = h0 + u * G;
-    const bool keep = h < heads && slot >= 0;
-    kv::encode_row<KIND, FMT, LPR>(f[u], part, keep, keep ? kv::row_of(g.c, slot, h) : 0,
-                                   is_v ? g.c.v_data : g.c.k_data,
-                                   is_v ? g.c.v_scale : g.c.k_scale);
+    for (int i = 0; i < 8; ++i) {
+      y[2 * i] = f[i].x;
+      y[2 * i + 1] = f[i].y;
+    }
+    ra.v = kv::pack8<DT>(y);
+    rb.v = kv::pack8<DT>(y + 8);
+    if constexpr (!INTER) {
+      uint4 z[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // elements 16 part + 8 i ..
+        const int eight = 2 * part + i, half = a.rot >> 4;
+        const bool turned = eight < 2 * half;
+        const int from = turned ? (eight < half ? eight : eight - half) : part;
+        const bool second = turned ? eight >= half : i;
+        auto take = [&](uint32_t u, uint32_t v) {
+          u = __shfl_sync(0xFFFFFFFFu, u, from, LPR);
+          v = __shfl_sync(0xFFFFFFFFu, v, from, LPR);
+          return second ? v : u;
+        };
+        z[i].x = take(ra.v.x, rb.v.x);
+        z[i].y = take(ra.v.y, rb.v.y);
+        z[i].z = take(ra.v.z, rb.v.z);
+        z[i].w = take(ra.v.w, rb.v.w);
+      }
+      ra.v = z[0];
+      rb.v = z[1];
+    }
   }
+  kv::expand8<DT>(ra, y);
+  kv::expand8<DT>(rb, y + 8);
+  const bool keep = on && slot >= 0;
+  kv::encode_row<KIND, FMT, LPR>(y, part, keep, keep ? kv::row_of(g.c, slot, h) : 0,
+                                 is_v ? g.c.v_data : g.c.k_data,
+                                 is_v ? g.c.v_scale : g.c.k_scale);
 }
 
 // ------------------------------------------------------------------ backward
@@ -347,18 +323,18 @@ struct BwdArgs {
   int parts_shift;  // a token's heads go to 2^parts_shift warps
 };
 
-constexpr int kBwdHeads = 2;
-constexpr int kBwdPerSm = 3;
+constexpr int kBwdPerSm = 2;
 
-// Persistent: a lane sums the weight gradients of its eight elements over all
-// the heads that it takes, so that one row per block is written.
+// Persistent: a lane sums the weight gradients of its sixteen elements over all
+// the heads that it takes, so that one row per block is written. The next head's
+// rows are on their way while one is worked on.
 template <int DT, int LPR, bool INTER>
 __global__ void __launch_bounds__(kThreads, kBwdPerSm) k_bwd(BwdArgs g) {
   constexpr int G = 32 / LPR;
   const brc_norm_rope& a = g.a;
   const int lane = threadIdx.x & 31, part = lane % LPR;
   const bool is_q = (int)blockIdx.x < g.q_blocks;
-  const int side = is_q ? 0 : 1, heads = is_q ? a.hq : a.hk;
+  const int heads = is_q ? a.hq : a.hk;
   const int block = is_q ? blockIdx.x : blockIdx.x - g.q_blocks;
   const int blocks = is_q ? g.q_blocks : gridDim.x - g.q_blocks;
   const int64_t xt = is_q ? a.q_token : a.k_token, xh = is_q ? a.q_head : a.k_head;
@@ -366,76 +342,101 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) k_bwd(BwdArgs g) {
   const void* const px = is_q ? a.q : a.k;
   const void* const pg = is_q ? g.g[0] : g.g[1];
   void* const dx = is_q ? g.dx[0] : g.dx[1];
-  const bool on = part * 8 < a.d;
+  const bool on = part * 16 < a.d;
   int e0, e1;
   groups<INTER>(a.rot, part, e0, e1);
   const float inv_d = 1.f / (float)a.d;
-  float w[8], dw[8];
+  // the weights wait in shared memory: sixteen registers that the rows in flight need
+  __shared__ __align__(16) float sw[LPR * 16];
+  if (threadIdx.x < LPR * 2) {
+    float2 v[4] = {splat(0.f), splat(0.f), splat(0.f), splat(0.f)};
+    if ((int)threadIdx.x * 8 < a.d) load_w(is_q ? a.wq : a.wk, a.w_dtype, threadIdx.x * 8, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = dw[i] = 0.f;
-  if (on) {
-    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
-    load_w4(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(&sw[threadIdx.x * 8 + 2 * i]) = v[i];
   }
+  __syncthreads();
+  float2 dw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dw[i] = splat(0.f);
   const int n_parts = 1 << g.parts_shift;
   const int per = (heads + n_parts - 1) >> g.parts_shift;  // heads of one warp
-  const int64_t units = a.tokens << g.parts_shift;
-  for (int64_t unit = (int64_t)block * kWarps + (threadIdx.x >> 5); unit < units;
-       unit += (int64_t)blocks * kWarps) {
-    const int64_t token = unit >> g.parts_shift;
-    const int first = (int)(unit & (n_parts - 1)) * per, last = min(first + per, heads);
-    float c[4], s[4];
+  const int64_t units = a.tokens << g.parts_shift, step = (int64_t)blocks * kWarps;
+  struct Rows {
+    kv::Raw8<DT> x0, x1, g0, g1;
+  };
+  auto fetch = [&](int64_t token, int h, int last, Rows& r) {
+    r = Rows{};
+    if (on && h < last) {
+      kv::load_raw8<DT>(px, token * xt + h * xh + e0, r.x0);
+      kv::load_raw8<DT>(px, token * xt + h * xh + e1, r.x1);
+      kv::load_raw8<DT>(pg, token * gt + h * gh + e0, r.g0);
+      kv::load_raw8<DT>(pg, token * gt + h * gh + e1, r.g1);
+    }
+  };
+  int64_t unit = (int64_t)block * kWarps + (threadIdx.x >> 5);
+  if (unit < units) {
+    int64_t token = unit >> g.parts_shift;
+    int first = (int)(unit & (n_parts - 1)) * per, last = min(first + per, heads), h0 = first;
+    Rows next;
+    fetch(token, h0 + lane / LPR, last, next);
+    float2 c[4], s[4];
     load_angles(a, token, part, c, s);
-    for (int h0 = first; h0 < last; h0 += kBwdHeads * G) {
-      Raw<DT> xa[kBwdHeads], xb[kBwdHeads], ga[kBwdHeads], gb[kBwdHeads];
-#pragma unroll
-      for (int u = 0; u < kBwdHeads; ++u) {
-        const int h = h0 + u * G + lane / LPR;
-        xa[u] = xb[u] = ga[u] = gb[u] = Raw<DT>{};
-        if (on && h < last) {
-          load_raw<DT>(px, token * xt + h * xh + e0, xa[u]);
-          load_raw<DT>(px, token * xt + h * xh + e1, xb[u]);
-          load_raw<DT>(pg, token * gt + h * gh + e0, ga[u]);
-          load_raw<DT>(pg, token * gt + h * gh + e1, gb[u]);
-        }
+    while (true) {
+      const Rows now = next;
+      const int64_t t = token;
+      const int h = h0 + lane / LPR;
+      const bool mine = on && h < last;
+      // the next batch: of this token, or of the warp's next unit
+      h0 += G;
+      const bool turn = h0 >= last;
+      if (turn) {
+        unit += step;
+        token = unit >> g.parts_shift;
+        first = (int)(unit & (n_parts - 1)) * per;
+        last = min(first + per, heads);
+        h0 = first;
       }
+      if (unit < units) fetch(token, h0 + lane / LPR, last, next);
+      float2 x[8], y[8];
+      expand<DT>(now.x0, x);
+      expand<DT>(now.x1, x + 4);
+      expand<DT>(now.g0, y);
+      expand<DT>(now.g1, y + 4);
+      turn_pairs<INTER, true>(c, s, y);
+      float ss, eps = a.eps;
+      const float by = square_sum<LPR>(x, ss, eps);
+      float2 hx2 = splat(0.f), gw[8];
 #pragma unroll
-      for (int u = 0; u < kBwdHeads; ++u) {
-        const int h = h0 + u * G + lane / LPR;
-        float x[8], gy[8];
-        expand<DT>(xa[u], x);
-        expand<DT>(xb[u], x + 4);
-        expand<DT>(ga[u], gy);
-        expand<DT>(gb[u], gy + 4);
-        turn_pairs<INTER, true>(c, s, gy);
-        float ss, hx = 0.f, eps = a.eps;
-        const float by = square_sum<LPR>(x, ss, eps);
+      for (int i = 0; i < 8; ++i) {
+        gw[i] = __fmul2_rn(y[i], *reinterpret_cast<const float2*>(&sw[(i < 4 ? e0 : e1 - 8) + 2 * i]));
+        hx2 = __ffma2_rn(gw[i], x[i], hx2);
+      }
+      const float hx = sum_row<LPR>(hx2.x + hx2.y);
+      const float r = rsqrtf(__fmaf_rn(ss, inv_d, eps));
+      const float m = -(hx * r * inv_d);  // -mean(gz w x r)
+      if (mine) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hx += gy[i] * w[i] * x[i];
-        hx = sum_row<LPR>(hx);
-        const float r = rsqrtf(ss * inv_d + eps);
-        const float m = hx * r * inv_d;  // mean(gz w x r)
-        if (on && h < last) {
-          float o[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float n = x[i] * r;
-            dw[i] += gy[i] * n;
-            o[i] = r * (gy[i] * w[i] - n * m) * by;
-          }
-          store4<DT>(dx, (token * heads + h) * a.d + e0, o);
-          store4<DT>(dx, (token * heads + h) * a.d + e1, o + 4);
+        for (int i = 0; i < 8; ++i) {
+          const float2 n = __fmul2_rn(x[i], splat(r));
+          dw[i] = __ffma2_rn(y[i], n, dw[i]);
+          gw[i] = __fmul2_rn(__ffma2_rn(n, splat(m), gw[i]), splat(r * by));
         }
+        store<DT>(dx, (t * heads + h) * a.d + e0, gw);
+        store<DT>(dx, (t * heads + h) * a.d + e1, gw + 4);
+      }
+      if (turn) {
+        if (unit >= units) break;
+        load_angles(a, token, part, c, s);
       }
     }
   }
   // lanes of the same elements: G per warp, kWarps warps
-  __shared__ float sm[kWarps * G][LPR * 8];
+  __shared__ float sm[kWarps * G][LPR * 16];
   const int mine = (threadIdx.x >> 5) * G + lane / LPR;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    sm[mine][e0 + i] = dw[i];
-    sm[mine][e1 + i] = dw[4 + i];
+    *reinterpret_cast<float2*>(&sm[mine][e0 + 2 * i]) = dw[i];
+    *reinterpret_cast<float2*>(&sm[mine][e1 + 2 * i]) = dw[4 + i];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.d; i += kThreads) {
@@ -495,7 +496,7 @@ int check(const brc_norm_rope* a) {
   return BRC_OK;
 }
 
-int lanes_per_row(int d) { return d <= 64 ? 8 : d <= 128 ? 16 : 32; }
+int lanes_per_row(int d) { return d <= 64 ? 4 : d <= 128 ? 8 : 16; }
 
 template <int DT, int LPR>
 int launch_fwd(const brc_norm_rope& a, void* q_out, void* k_out, cudaStream_t st) {
@@ -515,14 +516,14 @@ int launch_fwd(const brc_norm_rope& a, void* q_out, void* k_out, cudaStream_t st
 template <int DT>
 int launch_fwd_any(const brc_norm_rope& a, void* q_out, void* k_out, cudaStream_t st) {
   const int lpr = lanes_per_row(a.d);
-  return lpr == 8    ? launch_fwd<DT, 8>(a, q_out, k_out, st)
-         : lpr == 16 ? launch_fwd<DT, 16>(a, q_out, k_out, st)
-                     : launch_fwd<DT, 32>(a, q_out, k_out, st);
+  return lpr == 4   ? launch_fwd<DT, 4>(a, q_out, k_out, st)
+         : lpr == 8 ? launch_fwd<DT, 8>(a, q_out, k_out, st)
+                    : launch_fwd<DT, 16>(a, q_out, k_out, st);
 }
 
 template <int DT, int LPR, int KIND, int FMT>
 int launch_fwd_write(const FwdArgs& g, cudaStream_t st) {
-  const int per = kHeads * (32 / LPR);
+  const int per = 32 / LPR;
   const int64_t bx = (g.a.tokens + kWarps - 1) / kWarps;
   const int q_chunks = (g.a.hq + per - 1) / per, k_chunks = (g.a.hk + per - 1) / per;
   if (bx > 0x7FFFFFFF || q_chunks + 2 * k_chunks > 65535) return BRC_ERR_RANGE;
@@ -534,9 +535,9 @@ int launch_fwd_write(const FwdArgs& g, cudaStream_t st) {
 }
 template <int DT, int KIND, int FMT>
 int launch_write_dim(const FwdArgs& g, cudaStream_t st) {
-  return g.a.d == 64    ? launch_fwd_write<DT, 8, KIND, FMT>(g, st)
-         : g.a.d == 128 ? launch_fwd_write<DT, 16, KIND, FMT>(g, st)
-                        : launch_fwd_write<DT, 32, KIND, FMT>(g, st);
+  return g.a.d == 64    ? launch_fwd_write<DT, 4, KIND, FMT>(g, st)
+         : g.a.d == 128 ? launch_fwd_write<DT, 8, KIND, FMT>(g, st)
+                        : launch_fwd_write<DT, 16, KIND, FMT>(g, st);
 }
 
 template <int DT>
@@ -559,9 +560,9 @@ void launch_bwd(const BwdArgs& g, int blocks, cudaStream_t st) {
 template <int DT>
 void launch_bwd_any(const BwdArgs& g, int blocks, cudaStream_t st) {
   const int lpr = lanes_per_row(g.a.d);
-  if (lpr == 8) launch_bwd<DT, 8>(g, blocks, st);
-  else if (lpr == 16) launch_bwd<DT, 16>(g, blocks, st);
-  else launch_bwd<DT, 32>(g, blocks, st);
+  if (lpr == 4) launch_bwd<DT, 4>(g, blocks, st);
+  else if (lpr == 8) launch_bwd<DT, 8>(g, blocks, st);
+  else launch_bwd<DT, 16>(g, blocks, st);
 }
 
 }  // namespace
@@ -639,7 +640,7 @@ int brc_qk_norm_rope_bwd(const brc_norm_rope* a, const void* gq, const void* gk,
     g.dx[1] = dk;
     g.part = static_cast<float*>(workspace);
     // enough warps for every SM, none with less than a batch of heads
-    const int most = sm_count() * kBwdPerSm, per = kBwdHeads * (32 / lanes_per_row(a->d));
+    const int most = sm_count() * kBwdPerSm, per = 2 * (32 / lanes_per_row(a->d));
     const int heads = a->hq > a->hk ? a->hq : a->hk;
     while (g.parts_shift < 4 && (a->tokens << g.parts_shift) < 8 * (int64_t)most * kWarps &&
            (heads >> g.parts_shift) > per)
