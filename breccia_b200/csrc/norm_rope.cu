@@ -166,62 +166,209 @@ __device__ __forceinline__ void norm_turn(float2* x, const float2* w, const floa
   turn_pairs<INTER, false>(c, s, x);
 }
 
-// Heads in flight per lane (a float32 element takes twice the registers).
-constexpr __host__ __device__ int heads_in_flight(int dt) { return dt == BRC_DTYPE_F32 ? 1 : 2; }
+// ------------------------------------------------------------------ units of a token
+// The persistent kernels' work: unit p of a token is a run of its query heads (p
+// < q_parts) or key heads. A warp takes every `stride`th unit, in order.
+struct Units {
+  int64_t tokens;
+  int q_parts, parts;   // units of a token
+  int q_per, k_per;     // heads of a unit
+  int step_p;           // stride % parts
+  int64_t step_token;   // stride / parts
+};
+struct Unit {
+  int64_t token;
+  int p;
+  __device__ __forceinline__ void next(const Units& u) {
+    p += u.step_p;
+    token += u.step_token;
+    if (p >= u.parts) {
+      p -= u.parts;
+      ++token;
+    }
+  }
+};
 
-// blockIdx.y: a chunk of `iters` batches of heads, the queries' first.
+// A warp's angles: cosines and sines of two tokens, one in use and one on its
+// way (asynchronous copies), so that a new token does not wait for them.
+constexpr int kAngles = 128;  // at most d / 2 pairs, padded with (1, 0)
+struct Angles {
+  float* buf;  // [2][cosines, sines][kAngles]
+  int at;
+  __device__ __forceinline__ void init(float* b, int rot, int lane) {
+    buf = b;
+    at = 0;
+    for (int i = (rot >> 1) + lane; i < kAngles; i += 32) {
+      buf[i] = buf[2 * kAngles + i] = 1.f;
+      buf[kAngles + i] = buf[3 * kAngles + i] = 0.f;
+    }
+  }
+  // Start loading a token's angles into the buffer that is not in use. A
+  // position outside the table gives NaN cosines (not a wrong angle).
+  __device__ __forceinline__ void fetch(const brc_norm_rope& a, int64_t token, int lane) {
+    float* const to = buf + (at ^ 1) * 2 * kAngles;
+    const int64_t pos = load_index(a.positions, token, a.index64);
+    const int half = a.rot >> 1;
+    if (pos >= 0 && pos < a.table_rows) {
+      for (int i = lane * 4; i < half; i += 128) {
+        cp16(to + i, a.cos + pos * half + i);
+        cp16(to + kAngles + i, a.sin + pos * half + i);
+      }
+    } else {
+      for (int i = lane; i < kAngles; i += 32) to[i] = __uint_as_float(0x7FC00000u);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // The angles last fetched are the ones in use from here on.
+  __device__ __forceinline__ void turn(int rot, int lane) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    // the other buffer's padding may hold a NaN token's: restore it
+    at ^= 1;
+    float* const other = buf + (at ^ 1) * 2 * kAngles;
+    for (int i = (rot >> 1) + lane; i < kAngles; i += 32) other[i] = 1.f;
+    __syncwarp();
+  }
+  __device__ __forceinline__ const float* cosines() const { return buf + at * 2 * kAngles; }
+  static __device__ __forceinline__ void cp16(float* dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(dst)),
+                 "l"(src)
+                 : "memory");
+  }
+};
+// Eight floats of shared memory as four pairs.
+__device__ __forceinline__ void lds8(const float* p, float2* f) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  f[0] = make_float2(a.x, a.y);
+  f[1] = make_float2(a.z, a.w);
+  f[2] = make_float2(b.x, b.y);
+  f[3] = make_float2(b.z, b.w);
+}
+// Both weights as float32 in shared memory, zeros past d: sw[side][LPR * 16].
+template <int LPR>
+__device__ __forceinline__ void load_weights(const brc_norm_rope& a, float* sw) {
+  for (int i = threadIdx.x; i < LPR * 4; i += blockDim.x) {
+    const int side = i / (LPR * 2), e = (i % (LPR * 2)) * 8;
+    float2 v[4] = {splat(0.f), splat(0.f), splat(0.f), splat(0.f)};
+    if (e < a.d && (side ? a.hk : a.hq)) load_w(side ? a.wk : a.wq, a.w_dtype, e, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(sw + side * LPR * 16 + e + 2 * j) = v[j];
+  }
+}
+
+#ifndef FPS
+#define FPS 5
+#endif
+constexpr int kFwdPerSm = FPS;
+
+// The next rows are on their way while these are worked on.
 template <int DT, int LPR, bool INTER>
-__global__ void __launch_bounds__(kThreads, 3) k_fwd(brc_norm_rope a, void* q_out, void* k_out,
-                                                     int q_chunks, int iters) {
-  constexpr int G = 32 / LPR, kHeads = heads_in_flight(DT);
-  const int lane = threadIdx.x & 31, part = lane % LPR;
-  const int64_t token = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (token >= a.tokens) return;
-  const bool is_q = (int)blockIdx.y < q_chunks;
-  const int heads = is_q ? a.hq : a.hk;
-  const int chunk = is_q ? blockIdx.y : blockIdx.y - q_chunks;
-  const int64_t hs = is_q ? a.q_head : a.k_head;
-  const void* const x = is_q ? a.q : a.k;
-  void* const out = is_q ? q_out : k_out;
-  const int64_t in0 = token * (is_q ? a.q_token : a.k_token);
-  const int64_t out0 = token * heads * a.d;
+__global__ void __launch_bounds__(kThreads, kFwdPerSm) k_fwd(brc_norm_rope a, Units us, void* q_out,
+                                                             void* k_out) {
+  constexpr int G = 32 / LPR;
+  __shared__ __align__(16) float sw[2 * LPR * 16];
+  __shared__ __align__(16) float sa[kWarps][4 * kAngles];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LPR;
   const bool on = part * 16 < a.d;
   int e0, e1;
   groups<INTER>(a.rot, part, e0, e1);
+  Unit u;
+  {
+    const int64_t first = (int64_t)blockIdx.x * kWarps + warp;
+    u.token = first / us.parts;
+    u.p = (int)(first - u.token * us.parts);
+  }
+  Angles an;
+  an.init(sa[warp], a.rot, lane);
+  kv::Raw8<DT> r0{}, r1{};
+  constexpr int kB = DT == BRC_DTYPE_F32 ? 4 : 2;
+  // the row that comes next: where it lies, where it goes, heads left to the warp
+  // (this lane's is there when more than lane / LPR are left)
+  const char* px = nullptr;
+  char* po = nullptr;
+  int64_t step_x = 0;
+  int left = 0;
+  bool is_q = true;
+  const int mine = on ? lane / LPR : 0x7FFFFFFF;
+  const int off = (e1 - e0) * kB;
+  auto begin = [&]() {
+    is_q = u.p < us.q_parts;
+    const int per = is_q ? us.q_per : us.k_per, heads = is_q ? a.hq : a.hk;
+    const int first = (is_q ? u.p : u.p - us.q_parts) * per;
+    left = min(per, heads - first);
+    const int64_t hs = is_q ? a.q_head : a.k_head;
+    const int h = first + lane / LPR;
+    px = static_cast<const char*>(is_q ? a.q : a.k) +
+         (u.token * (is_q ? a.q_token : a.k_token) + h * hs + e0) * kB;
+    po = static_cast<char*>(is_q ? q_out : k_out) + ((u.token * heads + h) * a.d + e0) * kB;
+    step_x = G * hs * kB;
+  };
+  auto fetch = [&]() {
+    r0 = r1 = kv::Raw8<DT>{};
+    if (mine < left) {
+      kv::load_raw8<DT>(px, 0, r0);
+      kv::load_raw8<DT>(px + off, 0, r1);
+    }
+  };
+  const bool any = u.token < us.tokens;
+  if (any) {
+    begin();
+    fetch();
+    an.fetch(a, u.token, lane);
+  }
+  load_weights<LPR>(a, sw);
+  __syncthreads();
+  if (!any) return;
+  an.turn(a.rot, lane);
   const float inv_d = 1.f / (float)a.d;
-  float2 w[8], c[4], s[4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = splat(0.f);
-  int h0 = chunk * iters * (kHeads * G) + lane / LPR;
-  for (int it = 0; it < iters; ++it, h0 += kHeads * G) {
-    kv::Raw8<DT> ra[kHeads], rb[kHeads];
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int h = h0 + u * G;
-      ra[u] = rb[u] = kv::Raw8<DT>{};
-      if (on && h < heads) {
-        kv::load_raw8<DT>(x, in0 + h * hs + e0, ra[u]);
-        kv::load_raw8<DT>(x, in0 + h * hs + e1, rb[u]);
+  Unit nu = u;
+  nu.next(us);
+  if (nu.token < us.tokens && nu.token != u.token) an.fetch(a, nu.token, lane);
+  while (true) {
+    float2 f[8];
+    expand<DT>(r0, f);
+    expand<DT>(r1, f + 4);
+    const int64_t token = u.token;
+    const bool there = mine < left;
+    char* const out = po;
+    const float* const w = sw + (is_q ? 0 : LPR * 16);
+    left -= G;
+    const bool turn = left <= 0;
+    if (turn) {
+      u = nu;
+      if (u.token < us.tokens) {
+        begin();
+        fetch();
       }
+    } else {
+      px += step_x;
+      po += G * a.d * kB;
+      fetch();
     }
-    if (it == 0) {
-      if (on) {
-        load_w(is_q ? a.wq : a.wk, a.w_dtype, e0, w);
-        load_w(is_q ? a.wq : a.wk, a.w_dtype, e1, w + 4);
-      }
-      load_angles(a, token, part, c, s);
-    }
+    float ss, eps = a.eps;
+    square_sum<LPR>(f, ss, eps);
+    const float2 r = splat(rsqrtf(__fmaf_rn(ss, inv_d, eps)));
+    float2 t[4], c[4];
+    lds8(w + e0, t);
 #pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int h = h0 + u * G;
-      float2 f[8];
-      expand<DT>(ra[u], f);
-      expand<DT>(rb[u], f + 4);
-      norm_turn<LPR, INTER>(f, w, c, s, inv_d, a.eps);
-      if (on && h < heads) {
-        store<DT>(out, out0 + h * a.d + e0, f);
-        store<DT>(out, out0 + h * a.d + e1, f + 4);
-      }
+    for (int j = 0; j < 4; ++j) f[j] = __fmul2_rn(__fmul2_rn(f[j], r), t[j]);
+    lds8(w + e1, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[4 + j] = __fmul2_rn(__fmul2_rn(f[4 + j], r), t[j]);
+    const float* const cs = an.cosines() + 8 * part;
+    lds8(cs, c);
+    lds8(cs + kAngles, t);
+    turn_pairs<INTER, false>(c, t, f);
+    if (there) {
+      store<DT>(out, 0, f);
+      store<DT>(out + off, 0, f + 4);
+    }
+    if (turn) {
+      if (u.token >= us.tokens) break;
+      nu.next(us);
+      if (u.token != token) an.turn(a.rot, lane);
+      if (nu.token < us.tokens && nu.token != u.token) an.fetch(a, nu.token, lane);
     }
   }
 }
@@ -315,28 +462,36 @@ __global__ void __launch_bounds__(kThreads) k_fwd_write(FwdArgs g, int q_chunks,
 // ------------------------------------------------------------------ backward
 struct BwdArgs {
   brc_norm_rope a;
+  Units us;  // of one side each: q_parts == parts, or 0
   const void* g[2];  // gradients of the queries' and keys' outputs
   int64_t g_token[2], g_head[2];
   void* dx[2];
-  float* part;      // (blocks, d) sums of the weight gradients
-  int q_blocks;     // blocks that take queries; the rest take keys
-  int parts_shift;  // a token's heads go to 2^parts_shift warps
+  float* part;   // (blocks, d) sums of the weight gradients
+  int q_blocks;  // blocks that take queries; the rest take keys
+  Units ks;
 };
 
-constexpr int kBwdPerSm = 2;
+constexpr int kBwdThreads = 128;
+constexpr int kBwdWarps = kBwdThreads / 32;
+#ifndef BPS
+#define BPS 5
+#endif
+constexpr int kBwdPerSm = BPS;
 
-// Persistent: a lane sums the weight gradients of its sixteen elements over all
-// the heads that it takes, so that one row per block is written. The next head's
-// rows are on their way while one is worked on.
+// A lane sums the weight gradients of its sixteen elements over all the heads
+// that it takes (a block takes one side), so that one row per block is written.
 template <int DT, int LPR, bool INTER>
-__global__ void __launch_bounds__(kThreads, kBwdPerSm) k_bwd(BwdArgs g) {
+__global__ void __launch_bounds__(kBwdThreads, kBwdPerSm) k_bwd(BwdArgs g) {
   constexpr int G = 32 / LPR;
   const brc_norm_rope& a = g.a;
-  const int lane = threadIdx.x & 31, part = lane % LPR;
+  __shared__ __align__(16) float sw[2 * LPR * 16];
+  __shared__ __align__(16) float sa[kBwdWarps][4 * kAngles];
+  __shared__ __align__(16) float sm[kBwdWarps * G][LPR * 16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LPR;
   const bool is_q = (int)blockIdx.x < g.q_blocks;
   const int heads = is_q ? a.hq : a.hk;
   const int block = is_q ? blockIdx.x : blockIdx.x - g.q_blocks;
-  const int blocks = is_q ? g.q_blocks : gridDim.x - g.q_blocks;
+  const Units& us = is_q ? g.us : g.ks;
   const int64_t xt = is_q ? a.q_token : a.k_token, xh = is_q ? a.q_head : a.k_head;
   const int64_t gt = is_q ? g.g_token[0] : g.g_token[1], gh = is_q ? g.g_head[0] : g.g_head[1];
   const void* const px = is_q ? a.q : a.k;
@@ -345,104 +500,126 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) k_bwd(BwdArgs g) {
   const bool on = part * 16 < a.d;
   int e0, e1;
   groups<INTER>(a.rot, part, e0, e1);
-  const float inv_d = 1.f / (float)a.d;
-  // the weights wait in shared memory: sixteen registers that the rows in flight need
-  __shared__ __align__(16) float sw[LPR * 16];
-  if (threadIdx.x < LPR * 2) {
-    float2 v[4] = {splat(0.f), splat(0.f), splat(0.f), splat(0.f)};
-    if ((int)threadIdx.x * 8 < a.d) load_w(is_q ? a.wq : a.wk, a.w_dtype, threadIdx.x * 8, v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(&sw[threadIdx.x * 8 + 2 * i]) = v[i];
+  Unit u;
+  {
+    const int64_t first = (int64_t)block * kBwdWarps + warp;
+    u.token = first / us.parts;
+    u.p = (int)(first - u.token * us.parts);
   }
-  __syncthreads();
+  Angles an;
+  an.init(sa[warp], a.rot, lane);
+  kv::Raw8<DT> nx0{}, nx1{}, ng0{}, ng1{};
+  constexpr int kB = DT == BRC_DTYPE_F32 ? 4 : 2;
+  // as in k_fwd
+  const char *qx = nullptr, *qg = nullptr;
+  char* po = nullptr;
+  int left = 0;
+  const int mine = on ? lane / LPR : 0x7FFFFFFF;
+  const int off = (e1 - e0) * kB;
+  auto begin = [&]() {
+    const int first = u.p * us.q_per, h = first + lane / LPR;
+    left = min(us.q_per, heads - first);
+    qx = static_cast<const char*>(px) + (u.token * xt + h * xh + e0) * kB;
+    qg = static_cast<const char*>(pg) + (u.token * gt + h * gh + e0) * kB;
+    po = static_cast<char*>(dx) + ((u.token * heads + h) * a.d + e0) * kB;
+  };
+  auto fetch = [&]() {
+    nx0 = nx1 = ng0 = ng1 = kv::Raw8<DT>{};
+    if (mine < left) {
+      kv::load_raw8<DT>(qx, 0, nx0);
+      kv::load_raw8<DT>(qx + off, 0, nx1);
+      kv::load_raw8<DT>(qg, 0, ng0);
+      kv::load_raw8<DT>(qg + off, 0, ng1);
+    }
+  };
+  const bool any = u.token < us.tokens;
+  if (any) {
+    begin();
+    fetch();
+    an.fetch(a, u.token, lane);
+  }
+  load_weights<LPR>(a, sw);
   float2 dw[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[i] = splat(0.f);
-  const int n_parts = 1 << g.parts_shift;
-  const int per = (heads + n_parts - 1) >> g.parts_shift;  // heads of one warp
-  const int64_t units = a.tokens << g.parts_shift, step = (int64_t)blocks * kWarps;
-  struct Rows {
-    kv::Raw8<DT> x0, x1, g0, g1;
-  };
-  auto fetch = [&](int64_t token, int h, int last, Rows& r) {
-    r = Rows{};
-    if (on && h < last) {
-      kv::load_raw8<DT>(px, token * xt + h * xh + e0, r.x0);
-      kv::load_raw8<DT>(px, token * xt + h * xh + e1, r.x1);
-      kv::load_raw8<DT>(pg, token * gt + h * gh + e0, r.g0);
-      kv::load_raw8<DT>(pg, token * gt + h * gh + e1, r.g1);
-    }
-  };
-  int64_t unit = (int64_t)block * kWarps + (threadIdx.x >> 5);
-  if (unit < units) {
-    int64_t token = unit >> g.parts_shift;
-    int first = (int)(unit & (n_parts - 1)) * per, last = min(first + per, heads), h0 = first;
-    Rows next;
-    fetch(token, h0 + lane / LPR, last, next);
-    float2 c[4], s[4];
-    load_angles(a, token, part, c, s);
+  __syncthreads();
+  if (any) {
+    an.turn(a.rot, lane);
+    const float inv_d = 1.f / (float)a.d;
+    const float* const w = sw + (is_q ? 0 : LPR * 16);
+    Unit nu = u;
+    nu.next(us);
+    if (nu.token < us.tokens && nu.token != u.token) an.fetch(a, nu.token, lane);
     while (true) {
-      const Rows now = next;
-      const int64_t t = token;
-      const int h = h0 + lane / LPR;
-      const bool mine = on && h < last;
-      // the next batch: of this token, or of the warp's next unit
-      h0 += G;
-      const bool turn = h0 >= last;
-      if (turn) {
-        unit += step;
-        token = unit >> g.parts_shift;
-        first = (int)(unit & (n_parts - 1)) * per;
-        last = min(first + per, heads);
-        h0 = first;
-      }
-      if (unit < units) fetch(token, h0 + lane / LPR, last, next);
       float2 x[8], y[8];
-      expand<DT>(now.x0, x);
-      expand<DT>(now.x1, x + 4);
-      expand<DT>(now.g0, y);
-      expand<DT>(now.g1, y + 4);
-      turn_pairs<INTER, true>(c, s, y);
+      expand<DT>(nx0, x);
+      expand<DT>(nx1, x + 4);
+      expand<DT>(ng0, y);
+      expand<DT>(ng1, y + 4);
+      const int64_t token = u.token;
+      const bool there = mine < left;
+      char* const out = po;
+      left -= G;
+      const bool turn = left <= 0;
+      if (turn) {
+        u = nu;
+        if (u.token < us.tokens) {
+          begin();
+          fetch();
+        }
+      } else {
+        qx += G * xh * kB;
+        qg += G * gh * kB;
+        po += G * a.d * kB;
+        fetch();
+      }
+      {
+        const float* const cs = an.cosines() + 8 * part;
+        float2 c[4], s[4];
+        lds8(cs, c);
+        lds8(cs + kAngles, s);
+        turn_pairs<INTER, true>(c, s, y);
+      }
       float ss, eps = a.eps;
       const float by = square_sum<LPR>(x, ss, eps);
-      float2 hx2 = splat(0.f), gw[8];
+      float2 wt[8], hx2 = splat(0.f);
+      lds8(w + e0, wt);
+      lds8(w + e1, wt + 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        gw[i] = __fmul2_rn(y[i], *reinterpret_cast<const float2*>(&sw[(i < 4 ? e0 : e1 - 8) + 2 * i]));
-        hx2 = __ffma2_rn(gw[i], x[i], hx2);
-      }
-      const float hx = sum_row<LPR>(hx2.x + hx2.y);
+      for (int i = 0; i < 8; ++i) hx2 = __ffma2_rn(__fmul2_rn(y[i], wt[i]), x[i], hx2);
+      const float hx = sum_row<LPR>(__fadd_rn(hx2.x, hx2.y));
       const float r = rsqrtf(__fmaf_rn(ss, inv_d, eps));
       const float m = -(hx * r * inv_d);  // -mean(gz w x r)
-      if (mine) {
+      if (there) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float2 n = __fmul2_rn(x[i], splat(r));
           dw[i] = __ffma2_rn(y[i], n, dw[i]);
-          gw[i] = __fmul2_rn(__ffma2_rn(n, splat(m), gw[i]), splat(r * by));
+          x[i] = __fmul2_rn(__ffma2_rn(n, splat(m), __fmul2_rn(y[i], wt[i])), splat(r * by));
         }
-        store<DT>(dx, (t * heads + h) * a.d + e0, gw);
-        store<DT>(dx, (t * heads + h) * a.d + e1, gw + 4);
+        store<DT>(out, 0, x);
+        store<DT>(out + off, 0, x + 4);
       }
       if (turn) {
-        if (unit >= units) break;
-        load_angles(a, token, part, c, s);
+        if (u.token >= us.tokens) break;
+        nu.next(us);
+        if (u.token != token) an.turn(a.rot, lane);
+        if (nu.token < us.tokens && nu.token != u.token) an.fetch(a, nu.token, lane);
       }
     }
   }
-  // lanes of the same elements: G per warp, kWarps warps
-  __shared__ float sm[kWarps * G][LPR * 16];
-  const int mine = (threadIdx.x >> 5) * G + lane / LPR;
+  // lanes of the same elements: G per warp
+  const int row = warp * G + lane / LPR;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    *reinterpret_cast<float2*>(&sm[mine][e0 + 2 * i]) = dw[i];
-    *reinterpret_cast<float2*>(&sm[mine][e1 + 2 * i]) = dw[4 + i];
+    *reinterpret_cast<float2*>(&sm[row][e0 + 2 * i]) = dw[i];
+    *reinterpret_cast<float2*>(&sm[row][e1 + 2 * i]) = dw[4 + i];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.d; i += kThreads) {
+  for (int i = threadIdx.x; i < a.d; i += kBwdThreads) {
     float t = 0.f;
 #pragma unroll
-    for (int j = 0; j < kWarps * G; ++j) t += sm[j][i];
+    for (int j = 0; j < kBwdWarps * G; ++j) t += sm[j][i];
     g.part[(int64_t)blockIdx.x * a.d + i] = t;
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -498,19 +675,38 @@ int check(const brc_norm_rope* a) {
 
 int lanes_per_row(int d) { return d <= 64 ? 4 : d <= 128 ? 8 : 16; }
 
+// Split `heads` into runs of whole batches of `batch`: as few as give `want` units
+// over all tokens (a token's angles are then loaded once for many heads).
+int split_heads(int heads, int batch, int64_t tokens, int64_t want, int& per) {
+  if (!heads) {
+    per = 1;
+    return 0;
+  }
+  const int most = (heads + batch - 1) / batch;
+  int64_t parts = (want + tokens - 1) / tokens;
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
+  per = (int)((most + parts - 1) / parts) * batch;
+  return (heads + per - 1) / per;
+}
+void set_stride(Units& u, int64_t warps) {
+  u.step_p = (int)(warps % u.parts);
+  u.step_token = warps / u.parts;
+}
+
 template <int DT, int LPR>
 int launch_fwd(const brc_norm_rope& a, void* q_out, void* k_out, cudaStream_t st) {
-  const int64_t bx = (a.tokens + kWarps - 1) / kWarps;
-  // one batch of heads to a warp while that leaves SMs free, then two (the
-  // token's angles and the weights are loaded half as often)
-  const int per1 = heads_in_flight(DT) * (32 / LPR);
-  const int64_t blocks1 = bx * ((a.hq + per1 - 1) / per1 + (a.hk + per1 - 1) / per1);
-  const int iters = blocks1 > 8 * sm_count() ? 2 : 1, per = per1 * iters;
-  const int q_chunks = (a.hq + per - 1) / per, chunks = q_chunks + (a.hk + per - 1) / per;
-  if (bx > 0x7FFFFFFF || chunks > 65535) return BRC_ERR_RANGE;
-  const dim3 grid((unsigned)bx, (unsigned)chunks);
-  if (a.interleaved) k_fwd<DT, LPR, true><<<grid, kThreads, 0, st>>>(a, q_out, k_out, q_chunks, iters);
-  else k_fwd<DT, LPR, false><<<grid, kThreads, 0, st>>>(a, q_out, k_out, q_chunks, iters);
+  const int64_t most = (int64_t)sm_count() * kFwdPerSm;  // blocks
+  Units u{};
+  u.tokens = a.tokens;
+  const int batch = 32 / LPR;
+  u.q_parts = split_heads(a.hq, batch, a.tokens, 8 * most * kWarps, u.q_per);
+  u.parts = u.q_parts + split_heads(a.hk, batch, a.tokens, 8 * most * kWarps, u.k_per);
+  const int64_t want = (a.tokens * u.parts + kWarps - 1) / kWarps;
+  const int blocks = (int)(want < most ? want : most);
+  set_stride(u, (int64_t)blocks * kWarps);
+  if (a.interleaved) k_fwd<DT, LPR, true><<<blocks, kThreads, 0, st>>>(a, u, q_out, k_out);
+  else k_fwd<DT, LPR, false><<<blocks, kThreads, 0, st>>>(a, u, q_out, k_out);
   return check_launch();
 }
 template <int DT>
@@ -554,8 +750,8 @@ int launch_write(const FwdArgs& g, cudaStream_t st) {
 
 template <int DT, int LPR>
 void launch_bwd(const BwdArgs& g, int blocks, cudaStream_t st) {
-  if (g.a.interleaved) k_bwd<DT, LPR, true><<<blocks, kThreads, 0, st>>>(g);
-  else k_bwd<DT, LPR, false><<<blocks, kThreads, 0, st>>>(g);
+  if (g.a.interleaved) k_bwd<DT, LPR, true><<<blocks, kBwdThreads, 0, st>>>(g);
+  else k_bwd<DT, LPR, false><<<blocks, kBwdThreads, 0, st>>>(g);
 }
 template <int DT>
 void launch_bwd_any(const BwdArgs& g, int blocks, cudaStream_t st) {
@@ -639,20 +835,28 @@ int brc_qk_norm_rope_bwd(const brc_norm_rope* a, const void* gq, const void* gk,
     g.dx[0] = dq;
     g.dx[1] = dk;
     g.part = static_cast<float*>(workspace);
-    // enough warps for every SM, none with less than a batch of heads
-    const int most = sm_count() * kBwdPerSm, per = 2 * (32 / lanes_per_row(a->d));
-    const int heads = a->hq > a->hk ? a->hq : a->hk;
-    while (g.parts_shift < 4 && (a->tokens << g.parts_shift) < 8 * (int64_t)most * kWarps &&
-           (heads >> g.parts_shift) > per)
-      ++g.parts_shift;
-    const int64_t want = ((a->tokens << g.parts_shift) + kWarps - 1) / kWarps;  // of one side
-    // the SMs are shared out by the number of heads
+    // the SMs are shared out by the number of heads; enough units for every warp
+    const int most = sm_count() * kBwdPerSm, batch = 32 / lanes_per_row(a->d);
     int q_share = a->hk ? (int)((int64_t)most * a->hq / (a->hq + a->hk)) : most;
     if (a->hq && q_share < 1) q_share = 1;
     if (a->hk && q_share > most - 1) q_share = most - 1;
-    q_blocks = a->hq ? (int)(want < q_share ? want : q_share) : 0;
-    const int k_share = most - q_share;
-    blocks = q_blocks + (a->hk ? (int)(want < k_share ? want : k_share) : 0);
+    int k_blocks = 0;
+    for (int side = 0; side < 2; ++side) {
+      Units& u = side ? g.ks : g.us;
+      const int heads = side ? a->hk : a->hq, share = side ? most - q_share : q_share;
+      u.tokens = a->tokens;
+      if (!heads) {
+        u.parts = 1;
+        continue;
+      }
+      u.parts = u.q_parts =
+          split_heads(heads, batch, a->tokens, 8 * (int64_t)share * kBwdWarps, u.q_per);
+      const int64_t want = (a->tokens * u.parts + kBwdWarps - 1) / kBwdWarps;
+      const int n = (int)(want < share ? want : share);
+      (side ? k_blocks : q_blocks) = n;
+      set_stride(u, (int64_t)n * kBwdWarps);
+    }
+    blocks = q_blocks + k_blocks;
     g.q_blocks = q_blocks;
     if (a->dtype == BRC_DTYPE_F32) launch_bwd_any<BRC_DTYPE_F32>(g, blocks, st);
     else if (a->dtype == BRC_DTYPE_BF16) launch_bwd_any<BRC_DTYPE_BF16>(g, blocks, st);
