@@ -10,11 +10,22 @@ namespace {
 // Rows of one sequence and cache head: tiles of 8 to a product's columns, up to
 // four tiles to a warp (their accumulators take d / 4 registers each: two at d =
 // 256), then up to four row warps to a block.
+//
+// More rows than kTcRows go to the tensor-core kernel: 256 to a block.
 struct Split {
+  bool tc;
   int nt, row_warps, row_blocks, rows_per_block;
 };
-Split split_rows(int rows, int d) {
-  Split s;
+constexpr int kTcRows = 64;
+Split split_rows(int rows, const brc_kv_cache* c) {
+  const int d = c->head_dim;
+  Split s{};
+  s.tc = rows > kTcRows && (d == 128 || (d == 64 && c->kind != BRC_STE_NVFP4));
+  if (s.tc) {
+    s.rows_per_block = 256;
+    s.row_blocks = (rows + 255) / 256;
+    return s;
+  }
   s.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : most_tiles(d);
   const int tile = 8 * s.nt;
   s.row_warps = rows <= tile ? 1 : rows <= 2 * tile ? 2 : 4;
@@ -23,7 +34,7 @@ Split split_rows(int rows, int d) {
   return s;
 }
 
-int blocks_of(int d, int nt) { return sm_count() * blocks_per_sm(d, nt); }
+int blocks_of(int d, const Split& s) { return sm_count() * (s.tc ? 1 : blocks_per_sm(d, s.nt)); }
 
 int check(const brc_kv_cache* c, int batch, int draft, int hq) {
   if (const int rc = kv::check_cache(c)) return rc;
@@ -42,8 +53,8 @@ extern "C" {
 
 int64_t brc_kv_attention_workspace(const brc_kv_cache* c, int batch, int draft, int hq) {
   if (check(c, batch, draft, hq) != BRC_OK) return 0;
-  const Split s = split_rows(draft * (hq / c->heads), c->head_dim);
-  return 2 * (int64_t)blocks_of(c->head_dim, s.nt) * s.rows_per_block * (c->head_dim + 2) * 4;
+  const Split s = split_rows(draft * (hq / c->heads), c);
+  return 2 * (int64_t)blocks_of(c->head_dim, s) * s.rows_per_block * (c->head_dim + 2) * 4;
 }
 
 int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batch, int draft,
@@ -59,8 +70,8 @@ int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batc
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) return BRC_ERR_ALIGN;
   if ((int64_t)table_pages * c->page_size > 0x7FFFFFF0) return BRC_ERR_RANGE;
   const int group = hq / c->heads, rows = draft * group;
-  const Split s = split_rows(rows, c->head_dim);
-  const int blocks = blocks_of(c->head_dim, s.nt);
+  const Split s = split_rows(rows, c);
+  const int blocks = blocks_of(c->head_dim, s);
   if (workspace_bytes < brc_kv_attention_workspace(c, batch, draft, hq)) return BRC_ERR_SHAPE;
   Args a{};
   a.c = *c;
@@ -75,7 +86,7 @@ int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batc
   a.table_stride = table_stride;
   a.table_pages = table_pages;
   for (a.page_shift = 4; (1 << a.page_shift) < c->page_size; ++a.page_shift) {}
-  a.step_shift = subtiles(c->head_dim) == 2 ? 5 : 4;
+  a.step_shift = s.tc ? 7 : subtiles(c->head_dim) == 2 ? 5 : 4;
   a.page_rows = (uint32_t)c->heads * c->page_size;
   a.context = context;
   a.drafts = drafts;
@@ -89,8 +100,16 @@ int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batc
   a.row_warps = s.row_warps;
   a.row_blocks = s.row_blocks;
   a.rows_per_block = s.rows_per_block;
-  a.min_share = 2 * (kWarps / s.row_warps);
+  a.min_share = s.tc ? 2 : 2 * (kWarps / s.row_warps);
   const cudaStream_t st = (cudaStream_t)stream;
+  if (s.tc) {
+    if (c->kind == BRC_STE_NVFP4) return attend_tc_nvfp4(a, blocks, st);
+    if (c->kind == BRC_STE_MXFP8)
+      return c->fmt == BRC_FP8_E4M3 ? attend_tc_mx_e4m3(a, blocks, st)
+                                    : attend_tc_mx_e5m2(a, blocks, st);
+    return c->fmt == BRC_FP8_E4M3 ? attend_tc_block_e4m3(a, blocks, st)
+                                  : attend_tc_block_e5m2(a, blocks, st);
+  }
   if (c->kind == BRC_STE_NVFP4) return attend_nvfp4(a, s.nt, blocks, st);
   if (c->kind == BRC_STE_MXFP8)
     return c->fmt == BRC_FP8_E4M3 ? attend_mx_e4m3(a, s.nt, blocks, st)

@@ -1112,17 +1112,10 @@ __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
 }
 
 // ------------------------------------------------------------------ host
-template <int KIND, int FMT, int D, int NT>
-int launch(Args a, int blocks, cudaStream_t st) {
-  constexpr int bytes = ring_bytes(KIND, D, NT) + query_bytes(D, NT);
-  static_assert(stages(KIND, D, NT) >= 2, "a ring needs two stages");
-  if (const int rc = check_cuda(cudaFuncSetAttribute(
-          k_attend<KIND, FMT, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)))
-    return rc;
-  k_attend<KIND, FMT, D, NT><<<blocks, kThreads, bytes, st>>>(a);
-  if (const int rc = check_launch()) return rc;
+// The join's blocks start, and find their places, while the last parts are written.
+template <int D>
+int launch_join(const Args& a, int blocks, cudaStream_t st) {
   const int64_t warps = (int64_t)a.batch * a.c.heads * a.row_blocks * a.rows_per_block;
-  // the join's blocks start, and find their places, while the last parts are written
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((warps + kWarps - 1) / kWarps));
   cfg.blockDim = dim3(kThreads);
@@ -1133,6 +1126,18 @@ int launch(Args a, int blocks, cudaStream_t st) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, k_join<D>, a, blocks));
+}
+
+template <int KIND, int FMT, int D, int NT>
+int launch(const Args& a, int blocks, cudaStream_t st) {
+  constexpr int bytes = ring_bytes(KIND, D, NT) + query_bytes(D, NT);
+  static_assert(stages(KIND, D, NT) >= 2, "a ring needs two stages");
+  if (const int rc = check_cuda(cudaFuncSetAttribute(
+          k_attend<KIND, FMT, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)))
+    return rc;
+  k_attend<KIND, FMT, D, NT><<<blocks, kThreads, bytes, st>>>(a);
+  if (const int rc = check_launch()) return rc;
+  return launch_join<D>(a, blocks, st);
 }
 
 template <int KIND, int FMT>
@@ -1154,6 +1159,13 @@ int attend_block_e5m2(const Args& a, int nt, int blocks, cudaStream_t st);
 int attend_mx_e4m3(const Args& a, int nt, int blocks, cudaStream_t st);
 int attend_mx_e5m2(const Args& a, int nt, int blocks, cudaStream_t st);
 int attend_nvfp4(const Args& a, int nt, int blocks, cudaStream_t st);
+// The same with the tcgen05 kernel (kv_attention_tc.cuh): 256 rows to a block,
+// steps of 128 tokens; head_dim 128, or 64 with FP8 codes.
+int attend_tc_block_e4m3(const Args& a, int blocks, cudaStream_t st);
+int attend_tc_block_e5m2(const Args& a, int blocks, cudaStream_t st);
+int attend_tc_mx_e4m3(const Args& a, int blocks, cudaStream_t st);
+int attend_tc_mx_e5m2(const Args& a, int blocks, cudaStream_t st);
+int attend_tc_nvfp4(const Args& a, int blocks, cudaStream_t st);
 
 }  // namespace kvatt
 }  // namespace brc

@@ -1,0 +1,740 @@
+// Attention of many query rows (trees of drafted tokens, large groups) over the
+// quantised paged cache, on the 5th-generation tensor cores.
+//
+// The mathematics, the numbers and the split of the work are kv_attention.cuh's;
+// with more than kTcRows rows to a cache head the products bound it, not HBM.
+//
+// One block to an SM, 13 warps, two tiles of 128 query rows, tiles of 128 tokens:
+//   warps 0-7   softmax, a thread to a row: scores from TMEM, probabilities back
+//               into the same TMEM columns as f16 (the A operand of P V)
+//   warps 8-11  codes and scales from global memory, decoded to f16 in shared
+//               memory (128-byte swizzled rows; keys are K-major, values the same
+//               bytes read as MN-major); loads run one tile ahead in registers
+//   warp 12     issues tcgen05.mma: S = Q K^T and O += P V of each row tile in turn,
+//               so that one row tile's products run under the other's softmax
+// TMEM: two score tiles and two output tiles of 128 columns. The codes are decoded
+// once for 256 rows, where the register path decodes them for every 32.
+//
+// A row's shift follows its maximum only when it is 2^8 behind (as in the register
+// path); then the softmax threads rescale their row of O in TMEM.
+#pragma once
+
+#include "kv_attention.cuh"
+#include "sm100.cuh"
+
+#include <cstddef>
+
+namespace brc {
+uint32_t* gemm_status_ptr();  // gemm_sm100.cu: the sticky status word of bounded waits
+
+namespace kvtc {
+
+using namespace kvatt;
+using namespace sm100;
+
+constexpr int kTok = 128;
+constexpr int kSoftWarps = 8, kLoadWarps = 4;
+constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr int kBlockBytes = 128 * 128;  // 128 rows of 64 f16, swizzled
+constexpr int kMeta = 4;                // a tile's scales outlive its key stage
+
+struct alignas(16) Meta {
+  float sk[kTok], sv[kTok];  // block FP8
+  int ek, ev;                // MXFP8: E8M0 bytes that the tile is relative to; block FP8: ev
+  uint32_t live[4];          // token 4 i + k: bit i of word k
+  uint32_t all;              // every token is live
+};
+
+template <int D>
+struct alignas(128) Smem {
+  uint8_t q[2][D / 64][kBlockBytes];
+  uint8_t k[2][D / 64][kBlockBytes];
+  uint8_t v[2][D / 64][kBlockBytes];
+  Meta meta[kMeta];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+  Place place;
+  uint32_t tmem, abort;
+  uint32_t odd[4];  // (the loads are at most two items ahead) number of the item whose drafted values are not all finite
+};
+
+__device__ __forceinline__ void fence_proxy_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], f16 inputs.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// kind::f16 with f16 operands, float32 accumulator; b_mn: B is MN-major.
+constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// What every role walks through: the items of this block's share.
+struct Walk {
+  int64_t x, end, seq_start;
+  int b, per_seq;
+  // current item
+  Seq seq;
+  int item, head, row0, s_begin, s_end;
+  int64_t item_start;
+  __device__ __forceinline__ Walk(const Args& a, const Place& p)
+      : x((int64_t)blockIdx.x * p.share), end(min(x + p.share, p.total)),
+        per_seq(a.c.heads * a.row_blocks) {
+    b = p.b;
+    seq_start = p.before * per_seq;
+  }
+  __device__ __forceinline__ bool take(const Args& a) {
+    if (x >= end) return false;
+    seq = load_seq(a, b);
+    item = (int)((x - seq_start) / seq.steps);
+    item_start = seq_start + (int64_t)item * seq.steps;
+    head = item / a.row_blocks;
+    row0 = (item - head * a.row_blocks) * a.rows_per_block;
+    s_begin = (int)(x - item_start);
+    s_end = (int)min((int64_t)seq.steps, end - item_start);
+    return true;
+  }
+  __device__ __forceinline__ void next() {
+    x = item_start + s_end;
+    if (s_end == seq.steps && item + 1 == per_seq) {
+      seq_start += (int64_t)per_seq * seq.steps;
+      ++b;
+    }
+  }
+};
+
+// ------------------------------------------------------------------ loading
+// A warp decodes 32 of a tile's tokens: lane (t, c) reads token 8 g + t, piece 4 i
+// + c, for g < 4 and i < kHalves.
+template <int KIND, int FMT, int D>
+struct Loader {
+  using S = Shape<KIND, D>;
+  static constexpr int kHalves = S::kRowBytes / 64;
+  static_assert(kHalves >= 1, "rows of at least 64 bytes");
+  uint4 w[4][kHalves];
+  uint32_t s[4][kHalves];  // scale byte(s) of the piece
+  uint4 e;                 // MXFP8: the scale bytes of tokens 4 lane .. + 3 (top of the tile)
+
+  __device__ __forceinline__ void fetch(const uint8_t* data, const void* scale,
+                                        const int64_t (&row)[4], int64_t row4, int lane) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i) {
+        w[g][i] = make_uint4(0u, 0u, 0u, 0u);
+        s[g][i] = 0u;
+        if (row[g] >= 0) {
+          const int piece = 4 * i + (lane & 3);
+          w[g][i] = ldg16(data + row[g] * S::kRowBytes + piece * 16);
+          const uint8_t* sp = static_cast<const uint8_t*>(scale) + row[g] * S::kScales;
+          if constexpr (KIND == BRC_STE_MXFP8) s[g][i] = __ldg(sp + piece / 2);
+          else if constexpr (KIND == BRC_STE_NVFP4)
+            s[g][i] = __ldg(reinterpret_cast<const uint16_t*>(sp + 2 * piece));
+        }
+      }
+    if constexpr (KIND == BRC_STE_MXFP8) {
+      e = make_uint4(0u, 0u, 0u, 0u);
+      if (row4 >= 0) {
+        const uint8_t* sp = static_cast<const uint8_t*>(scale) + row4 * S::kScales;
+        if constexpr (D == 128) {
+          e = ldg16(sp);
+        } else {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp));
+          e.x = v.x;
+          e.y = v.y;
+        }
+      }
+    }
+  }
+  // Largest E8M0 byte of the tile's live tokens, below 255; every lane gets it.
+  __device__ __forceinline__ int top(int live4) const {
+    uint32_t m = 0;
+    const uint32_t v[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+    for (int i = 0; i < 4 * S::kScales; ++i) {
+      const uint32_t x = (v[i / 4] >> (8 * (i % 4))) & 0xFFu;
+      if (x != 255u && i / S::kScales < live4) m = max(m, x);
+    }
+    return (int)__reduce_max_sync(0xFFFFFFFFu, m);
+  }
+  // Decode into a stage. `first`: token of the warp's first row; rows from `dead`
+  // on hold anything and become zero. ODD: drafted tokens (from `drafted` on) that
+  // hold something not finite become zero too; returns whether there was one.
+  template <bool ODD>
+  __device__ __forceinline__ bool decode(uint8_t* stage, int first, int lane, int ref,
+                                         int dead, int drafted) {
+    bool any = false;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int t = first + 8 * g + (lane >> 2);
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i) {
+        const int piece = 4 * i + (lane & 3);
+        uint32_t x[4] = {w[g][i].x, w[g][i].y, w[g][i].z, w[g][i].w};
+        bool zero = t >= dead;
+        if constexpr (ODD) {
+          if (t >= drafted && !zero) {
+            bool odd = false;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) odd |= odd_codes<KIND, FMT>(x[y]);
+            if constexpr (KIND == BRC_STE_MXFP8) odd |= s[g][i] == 255u;
+            if constexpr (KIND == BRC_STE_NVFP4)
+              odd |= (s[g][i] & 0x7Fu) == 0x7Fu || (s[g][i] & 0x7F00u) == 0x7F00u;
+            any |= odd;
+            zero |= odd;
+          }
+        }
+        if (zero) x[0] = x[1] = x[2] = x[3] = s[g][i] = 0u;
+        uint32_t h[S::kFp4 ? 16 : 8];
+        if constexpr (S::kFp4) {
+          const uint32_t f0 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(s[g][i], 0, 0x0000));
+          const uint32_t f1 = fp8x2_to_f16x2<BRC_FP8_E4M3>(__byte_perm(s[g][i], 0, 0x0011));
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            uint32_t q[4];
+            e2m1x8_to_f16x8(x[y], q);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) h[4 * y + z] = hmul2(q[z], y < 2 ? f0 : f1);
+          }
+        } else {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) fp8x4_to_f16x4<FMT>(x[y], h[2 * y], h[2 * y + 1]);
+          if constexpr (KIND == BRC_STE_MXFP8) {
+            const uint32_t f = half2_pow2((int)s[g][i], (int)s[g][i], ref);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) h[y] = hmul2(h[y], f);
+          }
+        }
+        // a piece is kUnits 16-byte units of a 64-element block's row
+        constexpr int kUnits = S::kFp4 ? 4 : 2;
+        const int unit = piece * kUnits;
+        uint8_t* const dst = stage + (unit >> 3) * kBlockBytes + t * 128;
+#pragma unroll
+        for (int y = 0; y < kUnits; ++y)
+          *reinterpret_cast<uint4*>(dst + ((((unit & 7) + y) ^ (t & 7)) << 4)) =
+              make_uint4(h[4 * y], h[4 * y + 1], h[4 * y + 2], h[4 * y + 3]);
+      }
+    }
+    return any;
+  }
+};
+
+template <int KIND, int FMT, int D>
+__global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* status) {
+  using S = Shape<KIND, D>;
+  extern __shared__ uint8_t raw[];
+  Smem<D>& sm = *reinterpret_cast<Smem<D>*>(
+      raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u));  // swizzled tiles: 1024-byte aligned
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  volatile uint32_t* const abort = &sm.abort;
+
+  if (warp == kSoftWarps + kLoadWarps) {
+    tmem_alloc(&sm.tmem, 512);
+    tmem_relinquish();
+  }
+  if (warp == 0) {
+    Place p;
+    locate(a, a.c.heads * a.row_blocks, gridDim.x, blockIdx.x, -1, p);
+    if (lane == 0) {
+      sm.place = p;
+      sm.abort = 0;
+      sm.odd[0] = sm.odd[1] = sm.odd[2] = sm.odd[3] = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.k_full[i], kLoadWarps);
+        mbar_init(&sm.v_full[i], kLoadWarps);
+        mbar_init(&sm.k_empty[i], 1);
+        mbar_init(&sm.v_empty[i], 1);
+        mbar_init(&sm.q_full[i], 128);
+        mbar_init(&sm.s_full[i], 1);
+        mbar_init(&sm.p_full[i], 128);
+        mbar_init(&sm.o_full[i], 1);
+      }
+      mbar_init(&sm.drain, 1);
+      fence_mbar_init();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const uint32_t s_col[2] = {tmem, tmem + 128}, o_col[2] = {tmem + 256, tmem + 256 + D};
+  Walk walk(a, sm.place);
+
+  if (warp < kSoftWarps) {
+    // ================================================================ softmax
+    const int r = warp >> 2;  // row tile
+    const int mine = tid & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes, in bits 16 ..
+    const uint32_t sc = (r ? s_col[1] : s_col[0]) + lanes, oc = (r ? o_col[1] : o_col[0]) + lanes;
+    uint32_t tile = 0, number = 0;  // tiles and items so far
+    uint32_t s_phase = 0, o_phase = 0;
+    bool ok = true;
+    for (; ok && walk.take(a); walk.next()) {
+      ++number;
+      const Seq seq = walk.seq;
+      const int rows_left = a.rows - walk.row0;
+      const bool active = r == 0 || rows_left > 128;
+      const uint32_t tile0 = tile;
+      tile += walk.s_end - walk.s_begin;
+      if (!active) continue;
+      const int row = walk.row0 + r * 128 + mine, node = row / a.group;
+      const bool valid = row < a.rows && node < seq.drafts;
+      const int64_t at_row = ((int64_t)walk.b * a.draft + node) * a.hq + walk.head * a.group +
+                             (row - node * a.group);
+      // ---- this row of the queries, scaled by a power of two into f16
+      float rowf;
+      {
+        const uint16_t* const src = static_cast<const uint16_t*>(a.q) + at_row * D;
+        float top = 0.f;
+        if (valid) {
+#pragma unroll 4
+          for (int i = 0; i < D / 8; ++i) {
+            float f[8];
+            const uint4 v = ldg16(src + 8 * i);
+            if (a.q_f16) unpack<BRC_DTYPE_F16>(v, f);
+            else unpack<BRC_DTYPE_BF16>(v, f);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) top = fmaxf(top, fabsf(f[y]));
+          }
+        }
+        const int k = min(max((int)(__float_as_uint(top) >> 23) - 127, -119), 127);
+        // the factor of a score is not negative: its sign goes onto the query
+        const float up = copysignf(__uint_as_float((uint32_t)(127 + 7 - k) << 23), a.scale_log2);
+        rowf = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + k - 7) << 23);
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          uint4 y = make_uint4(0u, 0u, 0u, 0u);
+          if (valid) {
+            float f[8];
+            const uint4 v = ldg16(src + 8 * i);
+            if (a.q_f16) unpack<BRC_DTYPE_F16>(v, f);
+            else unpack<BRC_DTYPE_BF16>(v, f);
+            y = make_uint4(half2_of(f[0] * up, f[1] * up), half2_of(f[2] * up, f[3] * up),
+                           half2_of(f[4] * up, f[5] * up), half2_of(f[6] * up, f[7] * up));
+          }
+          *reinterpret_cast<uint4*>(sm.q[r][i / 8] + mine * 128 + (((i & 7) ^ (mine & 7)) << 4)) = y;
+        }
+        fence_proxy_smem();
+        mbar_arrive(&sm.q_full[r]);
+      }
+      float m = -INFINITY, l = 0.f;
+      int ev = -1000;
+      for (int j = walk.s_begin; j < walk.s_end; ++j) {
+        if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.s_full[r], s_phase, abort, status, 1u)))) break;
+        s_phase ^= 1u;
+        tc_fence_after();
+        const Meta& meta = sm.meta[(tile0 + (j - walk.s_begin)) % kMeta];
+        const int64_t t0 = (int64_t)j * kTok;
+        const float f = KIND == BRC_STE_MXFP8 ? rowf * e8m0_value(meta.ek) : rowf;
+        const bool masked = t0 + kTok > seq.context || !meta.all;
+        uint32_t vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            vis[c] = 0;
+            for (int i = 0; i < 32; ++i) {
+              const int t = 32 * c + i;
+              const int64_t n = t0 + t - seq.context;
+              bool see = valid && ((meta.live[t & 3] >> (t >> 2)) & 1u);
+              if (see && n >= 0)
+                see = a.tree ? a.tree[walk.b * a.tree_stride + (int64_t)node * a.draft + n] != 0
+                             : n <= node;
+              vis[c] |= (see ? 1u : 0u) << i;
+            }
+          }
+        }
+        __syncwarp();
+        // ---- the row's maximum
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          tmem_ld32(sc + 32 * c, x);
+          tmem_ld_wait();
+          reg_bind32(x);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[y] = __uint_as_float(x[i + y]);
+            if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+              const float4 g = *reinterpret_cast<const float4*>(&meta.sk[32 * c + i]);
+              v[0] *= g.x;
+              v[1] *= g.y;
+              v[2] *= g.z;
+              v[3] *= g.w;
+            }
+            if (masked) {
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                if (!((vis[c] >> (i + y)) & 1u)) v[y] = -INFINITY;
+            }
+            top = fmaxf(top, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+          }
+        }
+        top = top == -INFINITY ? top : top * f;
+        bool up_e = false;
+        if constexpr (KIND != BRC_STE_NVFP4) up_e = meta.ev > ev + 4;
+        if (__any_sync(0xFFFFFFFFu, top > m + kGrow || up_e)) {
+          const float nm = fmaxf(m, top);
+          float g = nm == m ? 1.f : ex2(m - nm);
+          m = nm;
+          l *= g;
+          if constexpr (KIND != BRC_STE_NVFP4) {
+            if (up_e) {
+              if (ev > -900) g *= __uint_as_float((uint32_t)max(127 + ev - meta.ev, 0) << 23);
+              ev = meta.ev;
+            }
+          }
+          if (j > walk.s_begin) {  // the products up to here are done: S came after them
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t x[16];
+              tmem_ld16(oc + 16 * c, x);
+              tmem_ld_wait16(x);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * g);
+              tmem_st16(oc + 16 * c, x);
+            }
+            tmem_st_wait();
+          }
+        }
+        // ---- probabilities, into the columns that their scores leave
+        const float shift = m == -INFINITY ? 0.f : m;
+        float vf = 64.f;
+        if constexpr (KIND == BRC_STE_BLOCK_FP8)
+          vf = __uint_as_float((uint32_t)(127 + 2 - ev) << 23);
+        else if constexpr (KIND == BRC_STE_MXFP8)
+          vf = __uint_as_float((uint32_t)max(127 + 2 + meta.ev - ev, 0) << 23);
+        const float2 f2 = make_float2(f, f), n2 = make_float2(-shift, -shift);
+        float2 l2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32], p[16];
+          tmem_ld32(sc + 32 * c, x);
+          tmem_ld_wait();
+          reg_bind32(x);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float2 u = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+            float2 v = make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+            if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+              const float4 g = *reinterpret_cast<const float4*>(&meta.sk[32 * c + i]);
+              u = __fmul2_rn(u, make_float2(g.x, g.y));
+              v = __fmul2_rn(v, make_float2(g.z, g.w));
+            }
+            u = __ffma2_rn(u, f2, n2);
+            v = __ffma2_rn(v, f2, n2);
+            if (masked) {
+              if (!((vis[c] >> i) & 1u)) u.x = -INFINITY;
+              if (!((vis[c] >> (i + 1)) & 1u)) u.y = -INFINITY;
+              if (!((vis[c] >> (i + 2)) & 1u)) v.x = -INFINITY;
+              if (!((vis[c] >> (i + 3)) & 1u)) v.y = -INFINITY;
+            }
+            u = make_float2(ex2(u.x), ex2(u.y));
+            v = make_float2(ex2(v.x), ex2(v.y));
+            l2 = __fadd2_rn(l2, __fadd2_rn(u, v));
+            u = __fmul2_rn(u, make_float2(vf, vf));
+            v = __fmul2_rn(v, make_float2(vf, vf));
+            if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+              const float4 g = *reinterpret_cast<const float4*>(&meta.sv[32 * c + i]);
+              u = __fmul2_rn(u, make_float2(g.x, g.y));
+              v = __fmul2_rn(v, make_float2(g.z, g.w));
+            }
+            p[i / 2] = half2_of(u.x, u.y);
+            p[i / 2 + 1] = half2_of(v.x, v.y);
+          }
+          tmem_st16(sc + 16 * c, p);
+        }
+        l += l2.x + l2.y;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sm.p_full[r]);
+      }
+      if (!ok) break;
+      // ---- the item's output
+      if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.o_full[r], o_phase, abort, status, 1u)))) break;
+      o_phase ^= 1u;
+      tc_fence_after();
+      const bool whole = walk.s_begin == 0 && walk.s_end == seq.steps;
+      const float so = KIND == BRC_STE_NVFP4 ? 0x1p-6f : ev < -900 ? 1.f : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : 0) - 2));
+      const bool none = !valid || l == 0.f;
+      const float mul = whole ? (none ? 0.f : so / l) : so;
+      const bool odd = sm.odd[number & 3u] == number && !none;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (walk.s_begin > 0 ? 0 : 1);
+      const int rr = r * 128 + mine;
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t x[16];
+        __syncwarp();
+        tmem_ld16(oc + 16 * c, x);
+        tmem_ld_wait16(x);
+        float o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = none ? 0.f : __uint_as_float(x[i]) * mul;
+        if (odd) {  // what was left out of the product, where this row sees it
+          const int32_t* const table = a.table + walk.b * a.table_stride;
+          for (int64_t t = max((int64_t)walk.s_begin * kTok, (int64_t)seq.context);
+               t < min((int64_t)walk.s_end * kTok, (int64_t)seq.total); ++t) {
+            const int64_t n = t - seq.context;
+            if (!(a.tree ? a.tree[walk.b * a.tree_stride + (int64_t)node * a.draft + n] != 0 : n <= node))
+              continue;
+            const int64_t page = table[t >> a.page_shift];
+            if (page < 0 || page >= a.c.num_pages) continue;
+            const int64_t src = page * a.page_rows + (int64_t)walk.head * a.c.page_size +
+                                (t & (a.c.page_size - 1));
+            for (int i = 0; i < 16; ++i) {
+              const float v = value_at<KIND, FMT, D>(a.c, src, 16 * c + i);
+              if (!isfinite(v)) o[i] += v;
+            }
+          }
+        }
+        if (row < a.rows) {
+          if (whole) {
+            uint32_t y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (a.q_f16) {
+                y[i] = half2_of(o[2 * i], o[2 * i + 1]);
+              } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+                y[i] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+            }
+            uint16_t* const dst = static_cast<uint16_t*>(a.out) + at_row * D + 16 * c;
+            stg16(dst, make_uint4(y[0], y[1], y[2], y[3]));
+            stg16(dst + 8, make_uint4(y[4], y[5], y[6], y[7]));
+          } else {
+            float* const dst = a.part_o + (slot * a.rows_per_block + rr) * D + 16 * c;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      }
+      if (row < a.rows) {
+        if (whole) {
+          if (a.lse) a.lse[at_row] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        } else {
+          float* const ml = a.part_ml + (slot * a.rows_per_block + rr) * 2;
+          ml[0] = valid ? m : -INFINITY;
+          ml[1] = valid ? l : 0.f;
+        }
+      }
+      tc_fence_before();  // O is read before the next item's products overwrite it
+    }
+  } else if (warp < kSoftWarps + kLoadWarps) {
+    // ================================================================ codes
+    const int lw = warp - kSoftWarps, first = 32 * lw;
+    uint32_t tile = 0, number = 0;
+    bool ok = true;
+    for (; ok && walk.take(a); walk.next()) {
+      ++number;
+      const Seq seq = walk.seq;
+      const int32_t* const table = a.table + walk.b * a.table_stride;
+      const int64_t head_row = (int64_t)walk.head * a.c.page_size;
+      auto row_at = [&](int64_t t) -> int64_t {
+        if (t >= seq.total) return -1;
+        const int64_t page = __ldg(table + (t >> a.page_shift));
+        if (page < 0 || page >= a.c.num_pages) return -1;
+        return page * a.page_rows + head_row + (t & (a.c.page_size - 1));
+      };
+      Loader<KIND, FMT, D> k, v;
+      int64_t row[4], row4;
+      auto rows_of_tile = [&](int j) {
+        const int64_t t0 = (int64_t)j * kTok;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) row[g] = row_at(t0 + first + 8 * g + (lane >> 2));
+        row4 = row_at(t0 + 4 * lane);
+      };
+      rows_of_tile(walk.s_begin);
+      k.fetch(a.c.k_data, a.c.k_scale, row, row4, lane);
+      for (int j = walk.s_begin; j < walk.s_end; ++j, ++tile) {
+        const uint32_t st = tile & 1u, use = (tile >> 1) & 1u;
+        const int64_t t0 = (int64_t)j * kTok;
+        const int dead = (int)min((int64_t)kTok, seq.total - t0);
+        const bool drafted = t0 + kTok > seq.context;
+        const int from = (int)max((int64_t)0, seq.context - t0);
+        const int live4 = row4 < 0 ? 0 : min(max(dead - 4 * lane, 0), 4);
+        v.fetch(a.c.v_data, a.c.v_scale, row, row4, lane);
+        int ek = 0, ev = 0;
+        float4 sk4 = make_float4(0.f, 0.f, 0.f, 0.f), sv4 = sk4;
+        if constexpr (KIND == BRC_STE_MXFP8) {
+          ek = k.top(live4);
+          ev = v.top(live4);
+        }
+        if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+          if (lw == 0 && row4 >= 0) {
+            sk4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.k_scale) + row4));
+            sv4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.v_scale) + row4));
+          }
+        }
+        if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.k_empty[st], use ^ 1u, abort, status, 1u)))) break;
+        if (lw == 0) {
+          Meta& meta = sm.meta[tile % kMeta];
+          if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+            float s4[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
+            uint32_t top = 0;
+            bool odd = false;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              if (y >= live4) s4[y] = 0.f;
+              const bool fine = isfinite(s4[y]);
+              if (!fine && 4 * lane + y >= from) {  // a drafted token
+                odd = true;
+                s4[y] = 0.f;
+              }
+              if (fine) top = max(top, __float_as_uint(s4[y]) & 0x7FFFFFFFu);
+            }
+            ev = max((int)(__reduce_max_sync(0xFFFFFFFFu, top) >> 23) - 127, -100);
+            if (__any_sync(0xFFFFFFFFu, odd) && lane == 0) sm.odd[number & 3u] = number;
+            *reinterpret_cast<float4*>(&meta.sk[4 * lane]) = sk4;
+            *reinterpret_cast<float4*>(&meta.sv[4 * lane]) = make_float4(s4[0], s4[1], s4[2], s4[3]);
+          }
+          uint32_t bal[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) bal[y] = __ballot_sync(0xFFFFFFFFu, y < live4);
+          if (lane == 0) {
+            meta.ek = ek;
+            meta.ev = KIND == BRC_STE_MXFP8 ? max(ev, 27) : ev;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) meta.live[y] = bal[y];
+            meta.all = (bal[0] & bal[1] & bal[2] & bal[3]) == 0xFFFFFFFFu;
+          }
+        }
+        k.template decode<false>(sm.k[st][0], first, lane, ek, dead, kTok);
+        fence_proxy_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.k_full[st]);
+        if (j + 1 < walk.s_end) {
+          rows_of_tile(j + 1);
+          k.fetch(a.c.k_data, a.c.k_scale, row, row4, lane);
+        }
+        if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.v_empty[st], use ^ 1u, abort, status, 1u)))) break;
+        const int vref = max(ev, 27);  // no lower than 2^-100
+        if (drafted) {
+          if (v.template decode<true>(sm.v[st][0], first, lane, vref, dead, from)) sm.odd[number & 3u] = number;
+        } else {
+          v.template decode<false>(sm.v[st][0], first, lane, vref, dead, kTok);
+        }
+        fence_proxy_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.v_full[st]);
+      }
+    }
+  } else {
+    // ================================================================ products
+    uint32_t tile = 0, q_phase = 0, p_phase[2] = {0, 0}, q_phase1 = 0;
+    bool ok = true;
+    constexpr uint32_t kIdS = idesc_f16(128, kTok, false), kIdO = idesc_f16(128, D, true);
+    const uint64_t hi_k = desc_sw128_hi();
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort, status, 1u));
+    };
+    auto scores = [&](int r, uint32_t st) {  // S_r = Q_r K^T
+      if (elect_lane()) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t off = (i / 4) * kBlockBytes + (i % 4) * 32;
+          mma_bf16(s_col[r], hi_k | desc_sw128_lo(smem_u32(sm.q[r][0]) + off),
+                   hi_k | desc_sw128_lo(smem_u32(sm.k[st][0]) + off), kIdS, i > 0);
+        }
+        tc_commit(&sm.s_full[r]);
+      }
+      __syncwarp();
+    };
+    for (; ok && walk.take(a); walk.next()) {
+      const int tiles = a.rows - walk.row0 > 128 ? 2 : 1;
+      const int n = walk.s_end - walk.s_begin;
+      for (int r = 0; ok && r < tiles; ++r) {
+        ok = wait(&sm.q_full[r], r ? q_phase1 : q_phase);
+        if (r) q_phase1 ^= 1u;
+        else q_phase ^= 1u;
+        if (ok && r == 0) ok = wait(&sm.k_full[tile & 1u], (tile >> 1) & 1u);
+        tc_fence_after();
+        if (ok) scores(r, tile & 1u);
+      }
+      if (ok && elect_lane()) tc_commit(&sm.k_empty[tile & 1u]);
+      __syncwarp();
+      for (int j = 0; ok && j < n; ++j, ++tile) {
+        const uint32_t st = tile & 1u, nx = (tile + 1) & 1u;
+        for (int r = 0; ok && r < tiles; ++r) {
+          ok = wait(&sm.p_full[r], p_phase[r]);
+          p_phase[r] ^= 1u;
+          if (ok && r == 0) ok = wait(&sm.v_full[st], (tile >> 1) & 1u);
+          tc_fence_after();
+          if (!ok) break;
+          if (elect_lane()) {
+#pragma unroll
+            for (int i = 0; i < kTok / 16; ++i)  // 16 tokens: 8 columns of P, 16 rows of V
+              mma_f16_ts(o_col[r], s_col[r] + 8 * i,
+                         smem_desc(smem_u32(sm.v[st][0]) + 2048 * i, kBlockBytes, 1024, 2), kIdO,
+                         j > 0 || i > 0);
+            if (j + 1 == n) tc_commit(&sm.o_full[r]);
+            if (r + 1 == tiles) tc_commit(&sm.v_empty[st]);
+          }
+          __syncwarp();
+          if (j + 1 < n) {
+            if (r == 0) ok = wait(&sm.k_full[nx], ((tile + 1) >> 1) & 1u);
+            tc_fence_after();
+            if (!ok) break;
+            scores(r, nx);
+            if (r + 1 == tiles) {
+              if (elect_lane()) tc_commit(&sm.k_empty[nx]);
+              __syncwarp();
+            }
+          }
+        }
+      }
+    }
+    // all products are done before TMEM is given back (after a timeout too)
+    if (elect_lane()) tc_commit(&sm.drain);
+    __syncwarp();
+    uint32_t none = 0;
+    mbar_wait(&sm.drain, 0u, &none, status, 1u);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftWarps + kLoadWarps) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+static_assert(sizeof(Meta) % 16 == 0 && offsetof(Meta, sv) % 16 == 0, "16-byte accesses");
+static_assert(offsetof(Smem<128>, meta) % 16 == 0 && offsetof(Smem<128>, k) % 1024 == 0 &&
+                  offsetof(Smem<128>, v) % 1024 == 0 && offsetof(Smem<64>, v) % 1024 == 0,
+              "swizzled tiles");
+
+template <int KIND, int FMT, int D>
+int launch_tc(const Args& a, int blocks, cudaStream_t st) {
+  constexpr int bytes = (int)sizeof(Smem<D>) + 1024;
+  if (const int rc = check_cuda(cudaFuncSetAttribute(
+          k_attend_tc<KIND, FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)))
+    return rc;
+  k_attend_tc<KIND, FMT, D><<<blocks, kTcThreads, bytes, st>>>(a, gemm_status_ptr());
+  if (const int rc = check_launch()) return rc;
+  return launch_join<D>(a, blocks, st);
+}
+
+}  // namespace kvtc
+}  // namespace brc
