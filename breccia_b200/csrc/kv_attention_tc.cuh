@@ -34,7 +34,11 @@ using namespace sm100;
 
 constexpr int kTok = 128;
 constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgroups: three warps idle
+// Registers of a thread after setmaxnreg, by warpgroup; 2 x softmax + loads +
+// products are no more than the 4 x 128 that the block was launched with.
+constexpr uint32_t kSoftRegs = 152, kLoadRegs = 136, kMmaRegs = 72;
+static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs <= 4 * 128, "registers of the launch");
 constexpr int kBlockBytes = 128 * 128;  // 128 rows of 64 f16, swizzled
 constexpr int kMeta = 4;                // a tile's scales outlive its key stage
 
@@ -280,6 +284,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
 
   if (warp < kSoftWarps) {
     // ================================================================ softmax
+    regs_inc<kSoftRegs>();
     const int r = warp >> 2;  // row tile
     const int mine = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes, in bits 16 ..
@@ -362,109 +367,152 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           }
         }
         __syncwarp();
-        // ---- the row's maximum
-        float top = -INFINITY;
+        const float2 f2 = make_float2(f, f);
+        // 32 scores in units of the row's factor; masked ones -inf
+        auto take = [&](const uint32_t (&x)[32], int c, float2 (&u)[16]) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          tmem_ld32(sc + 32 * c, x);
-          tmem_ld_wait();
-          reg_bind32(x);
+          for (int i = 0; i < 16; ++i)
+            u[i] = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+          if constexpr (KIND == BRC_STE_BLOCK_FP8) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float v[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) v[y] = __uint_as_float(x[i + y]);
-            if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-              const float4 g = *reinterpret_cast<const float4*>(&meta.sk[32 * c + i]);
-              v[0] *= g.x;
-              v[1] *= g.y;
-              v[2] *= g.z;
-              v[3] *= g.w;
+            for (int i = 0; i < 16; i += 2) {
+              const float4 g = *reinterpret_cast<const float4*>(&meta.sk[32 * c + 2 * i]);
+              u[i] = __fmul2_rn(u[i], make_float2(g.x, g.y));
+              u[i + 1] = __fmul2_rn(u[i + 1], make_float2(g.z, g.w));
             }
-            if (masked) {
+          }
+          if (masked) {
+            const uint32_t bits = vis[c];
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
-                if (!((vis[c] >> (i + y)) & 1u)) v[y] = -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+              if (!((bits >> (2 * i)) & 1u)) u[i].x = -INFINITY;
+              if (!((bits >> (2 * i + 1)) & 1u)) u[i].y = -INFINITY;
             }
-            top = fmaxf(top, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+          }
+        };
+        // O times g; the products up to here are done: S came after them
+        auto scale_o = [&](float g) {
+          if (j == walk.s_begin) return;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t x[16];
+            tmem_ld16(oc + 16 * c, x);
+            tmem_ld_wait16(x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * g);
+            tmem_st16(oc + 16 * c, x);
+          }
+        };
+        if constexpr (KIND != BRC_STE_NVFP4) {
+          if (meta.ev > ev + 4) {  // (the same for every row)
+            if (ev > -900) scale_o(__uint_as_float((uint32_t)max(127 + ev - meta.ev, 0) << 23));
+            ev = meta.ev;
           }
         }
-        top = top == -INFINITY ? top : top * f;
-        bool up_e = false;
-        if constexpr (KIND != BRC_STE_NVFP4) up_e = meta.ev > ev + 4;
-        if (__any_sync(0xFFFFFFFFu, top > m + kGrow || up_e)) {
-          const float nm = fmaxf(m, top);
-          float g = nm == m ? 1.f : ex2(m - nm);
-          m = nm;
-          l *= g;
-          if constexpr (KIND != BRC_STE_NVFP4) {
-            if (up_e) {
-              if (ev > -900) g *= __uint_as_float((uint32_t)max(127 + ev - meta.ev, 0) << 23);
-              ev = meta.ev;
-            }
-          }
-          if (j > walk.s_begin) {  // the products up to here are done: S came after them
+        if (j == walk.s_begin) {  // the first shift: the first tile's maximum
+          float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t x[16];
-              tmem_ld16(oc + 16 * c, x);
-              tmem_ld_wait16(x);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            float2 u[16];
+            tmem_ld32(sc + 32 * c, x);
+            tmem_ld_wait();
+            reg_bind32(x);
+            take(x, c, u);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * g);
-              tmem_st16(oc + 16 * c, x);
-            }
-            tmem_st_wait();
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(u[i].x, u[i].y));
           }
+          if (top != -INFINITY) m = top * f;
         }
-        // ---- probabilities, into the columns that their scores leave
-        const float shift = m == -INFINITY ? 0.f : m;
-        float vf = 64.f;
-        if constexpr (KIND == BRC_STE_BLOCK_FP8)
-          vf = __uint_as_float((uint32_t)(127 + 2 - ev) << 23);
-        else if constexpr (KIND == BRC_STE_MXFP8)
-          vf = __uint_as_float((uint32_t)max(127 + 2 + meta.ev - ev, 0) << 23);
-        const float2 f2 = make_float2(f, f), n2 = make_float2(-shift, -shift);
+        // Probabilities carry the factor 2^lift that the value scales ask for.
+        float lift = 6.f;
+        if constexpr (KIND == BRC_STE_BLOCK_FP8) lift = (float)(2 - ev);
+        else if constexpr (KIND == BRC_STE_MXFP8) lift = (float)(2 + meta.ev - ev);
+        float base = lift - (m == -INFINITY ? 0.f : m);
+        const float most = ex2(lift + kGrow);
         float2 l2 = make_float2(0.f, 0.f);
+        auto exps = [&](float2 (&u)[16]) {
+          float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32], p[16];
-          tmem_ld32(sc + 32 * c, x);
-          tmem_ld_wait();
-          reg_bind32(x);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float2 u = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-            float2 v = make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-            if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-              const float4 g = *reinterpret_cast<const float4*>(&meta.sk[32 * c + i]);
-              u = __fmul2_rn(u, make_float2(g.x, g.y));
-              v = __fmul2_rn(v, make_float2(g.z, g.w));
-            }
-            u = __ffma2_rn(u, f2, n2);
-            v = __ffma2_rn(v, f2, n2);
-            if (masked) {
-              if (!((vis[c] >> i) & 1u)) u.x = -INFINITY;
-              if (!((vis[c] >> (i + 1)) & 1u)) u.y = -INFINITY;
-              if (!((vis[c] >> (i + 2)) & 1u)) v.x = -INFINITY;
-              if (!((vis[c] >> (i + 3)) & 1u)) v.y = -INFINITY;
-            }
-            u = make_float2(ex2(u.x), ex2(u.y));
-            v = make_float2(ex2(v.x), ex2(v.y));
-            l2 = __fadd2_rn(l2, __fadd2_rn(u, v));
-            u = __fmul2_rn(u, make_float2(vf, vf));
-            v = __fmul2_rn(v, make_float2(vf, vf));
-            if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-              const float4 g = *reinterpret_cast<const float4*>(&meta.sv[32 * c + i]);
-              u = __fmul2_rn(u, make_float2(g.x, g.y));
-              v = __fmul2_rn(v, make_float2(g.z, g.w));
-            }
-            p[i / 2] = half2_of(u.x, u.y);
-            p[i / 2 + 1] = half2_of(v.x, v.y);
+          for (int i = 0; i < 16; ++i) {
+            u[i] = __ffma2_rn(u[i], f2, make_float2(base, base));
+            u[i] = make_float2(ex2(u[i].x), ex2(u[i].y));
+            t = __fadd2_rn(t, u[i]);
           }
+          return t;
+        };
+        // 32 scores to probabilities, into columns that their scores have left
+        auto work = [&](const uint32_t (&x)[32], int c) {
+          float2 u[16];
+          take(x, c, u);
+          float2 t = exps(u);
+          // a score far above the shift shows in the sum (which has no lower bound
+          // on a row that has seen nothing: its shift is 0)
+          const float all = t.x + t.y;
+          if (__any_sync(0xFFFFFFFFu, all > most || (m == -INFINITY && all > 0.f))) {
+            // the shift follows; sums, outputs and this tile's earlier columns with it
+            uint32_t y[32];
+            tmem_ld32(sc + 32 * c, y);
+            tmem_ld_wait();
+            reg_bind32(y);
+            take(y, c, u);
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(u[i].x, u[i].y));
+            top = top == -INFINITY ? top : top * f;
+            const float nm = fmaxf(m, top), g = nm == m || m == -INFINITY ? 1.f : ex2(m - nm);
+            m = nm;
+            base = lift - (m == -INFINITY ? 0.f : m);
+            l *= g;
+            l2 = __fmul2_rn(l2, make_float2(g, g));
+            scale_o(g);
+            tmem_st_wait();
+            const uint32_t gh = half2_of(g, g);
+#pragma unroll 1
+            for (int b = 0; b < c; ++b) {
+              uint32_t z[16];
+              tmem_ld16(sc + 16 * b, z);
+              tmem_ld_wait16(z);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) z[i] = hmul2(z[i], gh);
+              tmem_st16(sc + 16 * b, z);
+            }
+            t = exps(u);
+          }
+          l2 = __fadd2_rn(l2, t);
+          if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float4 g = *reinterpret_cast<const float4*>(&meta.sv[32 * c + 2 * i]);
+              u[i] = __fmul2_rn(u[i], make_float2(g.x, g.y));
+              u[i + 1] = __fmul2_rn(u[i + 1], make_float2(g.z, g.w));
+            }
+          }
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = half2_of(u[i].x, u[i].y);
           tmem_st16(sc + 16 * c, p);
+        };
+        {
+          uint32_t x0[32], x1[32];
+          tmem_ld32(sc, x0);
+          tmem_ld_wait();
+          reg_bind32(x0);
+          tmem_ld32(sc + 32, x1);
+          work(x0, 0);
+          tmem_ld_wait();
+          reg_bind32(x1);
+          tmem_ld32(sc + 64, x0);
+          work(x1, 1);
+          tmem_ld_wait();
+          reg_bind32(x0);
+          tmem_ld32(sc + 96, x1);
+          work(x0, 2);
+          tmem_ld_wait();
+          reg_bind32(x1);
+          work(x1, 3);
         }
-        l += l2.x + l2.y;
+        l += (l2.x + l2.y) * ex2(-lift);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&sm.p_full[r]);
@@ -543,6 +591,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     }
   } else if (warp < kSoftWarps + kLoadWarps) {
     // ================================================================ codes
+    regs_inc<kLoadRegs>();
     const int lw = warp - kSoftWarps, first = 32 * lw;
     uint32_t tile = 0, number = 0;
     bool ok = true;
@@ -642,6 +691,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     }
   } else {
     // ================================================================ products
+    regs_dec<kMmaRegs>();
+    if (warp == kSoftWarps + kLoadWarps) {
     uint32_t tile = 0, q_phase = 0, p_phase[2] = {0, 0}, q_phase1 = 0;
     bool ok = true;
     constexpr uint32_t kIdS = idesc_f16(128, kTok, false), kIdO = idesc_f16(128, D, true);
@@ -710,6 +761,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     __syncwarp();
     uint32_t none = 0;
     mbar_wait(&sm.drain, 0u, &none, status, 1u);
+    }
   }
   tc_fence_before();
   __syncthreads();
