@@ -38,19 +38,38 @@ _current_stream = torch._C._cuda_getCurrentRawStream
 _CONTIGUOUS = torch.contiguous_format
 
 
-def _call(index: int, name: str, *args) -> None:
-    """``_lib.call`` on device ``index``'s current stream, with it current."""
-    if index == _current_device():
-        _lib.call(name, *args, _current_stream(index))
-        return
-    with torch.cuda.device(index):
-        _lib.call(name, *args, _current_stream(index))
+class _Entry:
+    """A C entry point, called on a device's current stream with that device
+    current: ``entry(index, *arguments without the stream)``."""
+
+    __slots__ = ("name", "fn")
+
+    def __init__(self, name: str):
+        self.name, self.fn = name, None
+
+    def __call__(self, index: int, *args) -> None:
+        fn = self.fn
+        if fn is None:
+            fn = self.fn = getattr(_lib.lib(), self.name)
+        if index == _current_device():
+            if fn(*args, _current_stream(index)) == 0:
+                return
+        else:
+            with torch.cuda.device(index):
+                if fn(*args, _current_stream(index)) == 0:
+                    return
+        with torch.cuda.device(index):  # refused: once more, for its exception
+            _lib.call(self.name, *args, _current_stream(index))
+
+
+_kv_write, _kv_read, _kv_attention = (_Entry(n) for n in
+                                      ("brc_kv_write", "brc_kv_read", "brc_kv_attention"))
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
     """An uninitialised contiguous tensor like ``x`` (the cheapest allocation
     there is from Python)."""
-    return torch.empty_like(x, memory_format=_CONTIGUOUS, requires_grad=False)
+    return torch.empty_like(x, memory_format=_CONTIGUOUS)
 
 
 def _no_grad(what: str, *tensors) -> None:
@@ -258,8 +277,8 @@ class QuantizedKVCache:
                              f"{tuple(v.shape)} {v.dtype}")
         slots, is64 = _index(slots, "slots", k.shape[0], self.device)
         ks, vs = k.stride(), v.stride()
-        _call(self._device_index, "brc_kv_write", self._desc, k.data_ptr(), v.data_ptr(),
-              _IN_DT[k.dtype], k.shape[0], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), is64)
+        _kv_write(self._device_index, self._desc, k.data_ptr(), v.data_ptr(), _IN_DT[k.dtype],
+                  k.shape[0], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), is64)
 
     def read(self, page_table: torch.Tensor, lengths: torch.Tensor, max_length: int,
              out_dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -278,9 +297,9 @@ class QuantizedKVCache:
         shape = (batch, max_length, self.num_heads, self.head_dim)
         k = torch.empty(shape, dtype=out_dtype, device=self.device)
         v = _like(k)
-        _call(self._device_index, "brc_kv_read", self._desc, table.data_ptr(), table.stride(0),
-              table.shape[1], lengths.data_ptr(), batch, max_length, k.data_ptr(), v.data_ptr(),
-              _IN_DT[out_dtype])
+        _kv_read(self._device_index, self._desc, table.data_ptr(), table.stride(0), table.shape[1],
+                 lengths.data_ptr(), batch, max_length, k.data_ptr(), v.data_ptr(),
+                 _IN_DT[out_dtype])
         return k, v
 
 
@@ -341,10 +360,10 @@ def cache_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.
     lse = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
     if out.numel():
         nbytes, ws = cache._workspace(draft, hq)
-        _call(cache._device_index, "brc_kv_attention", cache._desc, q.data_ptr(), _IN_DT[q.dtype],
-              batch, draft, hq, table.data_ptr(), table.stride(0), table.shape[1],
-              context.data_ptr(), None if drafts is None else drafts.data_ptr(),
-              None if tree is None else tree.data_ptr(), tree_stride,
-              cache.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
-              None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes)
+        _kv_attention(cache._device_index, cache._desc, q.data_ptr(), _IN_DT[q.dtype], batch,
+                      draft, hq, table.data_ptr(), table.stride(0), table.shape[1],
+                      context.data_ptr(), None if drafts is None else drafts.data_ptr(),
+                      None if tree is None else tree.data_ptr(), tree_stride,
+                      cache.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                      None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out

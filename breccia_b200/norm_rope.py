@@ -17,15 +17,44 @@ import torch
 
 from . import _lib
 from .api import _IN_DT
-from .kvcache import QuantizedKVCache, _call, _heads, _index, _like, _no_grad, _on
+from .kvcache import QuantizedKVCache, _Entry, _heads, _index, _like, _no_grad, _on
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_write"]
+
+_norm_rope, _norm_rope_bwd, _norm_rope_write = (_Entry(n) for n in (
+    "brc_qk_norm_rope", "brc_qk_norm_rope_bwd", "brc_qk_norm_rope_write"))
 
 
 def _plain(t):
     """Contiguous and 16-byte aligned."""
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
+
+
+def _check_parameters(wq, wk, cos, sin, d, dev):
+    """The parameters' checks, message by message."""
+    for w, what in ((wq, "q_weight"), (wk, "k_weight")):
+        _on(w, what, dev)
+        if w.dtype not in _IN_DT:
+            raise TypeError(f"{what} must be float32, bfloat16 or float16, got {w.dtype}")
+        if w.shape != (d,):
+            raise ValueError(f"{what} must have shape ({d},), got {tuple(w.shape)}")
+    if wq.dtype is not wk.dtype:
+        raise TypeError(f"q_weight and k_weight differ: {wq.dtype}, {wk.dtype}")
+    for t, what in ((cos, "cos"), (sin, "sin")):
+        _on(t, what, dev)
+        if t.dtype is not torch.float32:
+            raise TypeError(f"{what} must be float32, got {t.dtype}")
+    if cos.shape != sin.shape:
+        raise ValueError(f"cos and sin differ: {tuple(cos.shape)}, {tuple(sin.shape)}")
+    if cos.ndim != 2 or cos.shape[0] == 0:
+        raise ValueError(f"cos must be (positions, rotated / 2), got {tuple(cos.shape)}")
+    rot = 2 * cos.shape[1]
+    if rot % 16 or not 16 <= rot <= d:
+        raise ValueError(f"the rotated width must be a multiple of 16 up to head_dim={d}, got {rot}")
+
+
+_F32 = torch.float32
 
 
 def _arguments(q, k, wq, wk, cos, sin, positions, eps, interleaved):
@@ -41,39 +70,32 @@ def _arguments(q, k, wq, wk, cos, sin, positions, eps, interleaved):
         raise ValueError(f"q and k differ: {tuple(q.shape)} {dtype}, {tuple(k.shape)} {k.dtype}")
     if d % 16 or not 16 <= d <= 256:
         raise ValueError(f"head_dim must be a multiple of 16 up to 256, got {d}")
-    for w, what in ((wq, "q_weight"), (wk, "k_weight")):
-        _on(w, what, dev)
-        if w.dtype not in _IN_DT:
-            raise TypeError(f"{what} must be float32, bfloat16 or float16, got {w.dtype}")
-        if w.shape != (d,):
-            raise ValueError(f"{what} must have shape ({d},), got {tuple(w.shape)}")
-    if wq.dtype is not wk.dtype:
-        raise TypeError(f"q_weight and k_weight differ: {wq.dtype}, {wk.dtype}")
-    for t, what in ((cos, "cos"), (sin, "sin")):
-        _on(t, what, dev)
-        if t.dtype is not torch.float32:
-            raise TypeError(f"{what} must be float32, got {t.dtype}")
-    rows = cos.shape
-    if rows != sin.shape:
-        raise ValueError(f"cos and sin differ: {tuple(rows)}, {tuple(sin.shape)}")
-    if len(rows) != 2 or rows[0] == 0:
-        raise ValueError(f"cos must be (positions, rotated / 2), got {tuple(rows)}")
-    rot = 2 * rows[1]
-    if rot % 16 or not 16 <= rot <= d:
-        raise ValueError(f"the rotated width must be a multiple of 16 up to head_dim={d}, got {rot}")
-    wq, wk, cos, sin = _plain(wq), _plain(wk), _plain(cos), _plain(sin)
+    try:  # all at once (a single token's call is bound by the host)
+        w_dtype, rows = wq.dtype, cos.shape
+        fine = (w_dtype is wk.dtype and w_dtype in _IN_DT and wq.shape == wk.shape == (d,) and
+                cos.dtype is _F32 and sin.dtype is _F32 and rows == sin.shape and
+                len(rows) == 2 and rows[0] > 0 and rows[1] % 8 == 0 and 0 < 2 * rows[1] <= d and
+                wq.device == wk.device == cos.device == sin.device == dev)
+    except AttributeError:
+        fine = False
+    if not fine:
+        _check_parameters(wq, wk, cos, sin, d, dev)
+    pwq, pwk, pc, ps = wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    if (pwq | pwk | pc | ps) % 16 or not (wq.is_contiguous() and wk.is_contiguous() and
+                                          cos.is_contiguous() and sin.is_contiguous()):
+        wq, wk, cos, sin = _plain(wq), _plain(wk), _plain(cos), _plain(sin)
+        pwq, pwk, pc, ps = wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr()
     positions, is64 = _index(positions, "positions", tokens, dev)
     qs, ks = q.stride(), k.stride()
-    a = _lib.NormRope(q.data_ptr(), k.data_ptr(), qs[0], qs[1], ks[0], ks[1], wq.data_ptr(),
-                      wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), tokens,
-                      rows[0], hq, hk, d, rot, _IN_DT[dtype], _IN_DT[wq.dtype], is64,
-                      1 if interleaved else 0, eps)
+    a = _lib.NormRope(q.data_ptr(), k.data_ptr(), qs[0], qs[1], ks[0], ks[1], pwq, pwk, pc, ps,
+                      positions.data_ptr(), tokens, rows[0], hq, hk, d, 2 * rows[1], _IN_DT[dtype],
+                      _IN_DT[w_dtype], is64, 1 if interleaved else 0, eps)
     return a, q, k, (wq, wk, cos, sin, positions)
 
 
 def _forward(a, q, k):
     q_out, k_out = _like(q), _like(k)
-    _call(q.get_device(), "brc_qk_norm_rope", addressof(a), q_out.data_ptr(), k_out.data_ptr())
+    _norm_rope(q.get_device(), addressof(a), q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -110,9 +132,9 @@ def _backward(ctx, gq, gk):
     nbytes = _lib.lib().brc_qk_norm_rope_bwd_workspace(a.d)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     gqs, gks = gq.stride(), gk.stride()
-    _call(q.get_device(), "brc_qk_norm_rope_bwd", addressof(a), gq.data_ptr(), gk.data_ptr(),
-          gqs[0], gqs[1], gks[0], gks[1], dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
-          dwk.data_ptr(), ws.data_ptr(), nbytes)
+    _norm_rope_bwd(q.get_device(), addressof(a), gq.data_ptr(), gk.data_ptr(), gqs[0], gqs[1],
+                   gks[0], gks[1], dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
+                   ws.data_ptr(), nbytes)
     if len(ctx.shapes[0]) != 3:
         dq = dq.view(ctx.shapes[0])
     if len(ctx.shapes[1]) != 3:
@@ -165,6 +187,6 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
     slots, is64 = _index(slots, "slots", k3.shape[0], cache.device)
     q_out = _like(q3)
     vs = v3.stride()
-    _call(cache._device_index, "brc_qk_norm_rope_write", addressof(a), v3.data_ptr(), vs[0], vs[1],
-          q_out.data_ptr(), cache._desc, slots.data_ptr(), is64)
+    _norm_rope_write(cache._device_index, addressof(a), v3.data_ptr(), vs[0], vs[1],
+                     q_out.data_ptr(), cache._desc, slots.data_ptr(), is64)
     return _shaped(q_out, q)
