@@ -34,7 +34,9 @@ Split split_rows(int rows, const brc_kv_cache* c) {
   return s;
 }
 
-int blocks_of(int d, const Split& s) { return sm_count() * (s.tc ? 1 : blocks_per_sm(d, s.nt)); }
+int blocks_of(const brc_kv_cache* c, const Split& s) {
+  return sm_count() * (s.tc ? 1 : blocks_per_sm(c->kind, c->head_dim, s.nt));
+}
 
 int check(const brc_kv_cache* c, int batch, int draft, int hq) {
   if (const int rc = kv::check_cache(c)) return rc;
@@ -54,7 +56,7 @@ extern "C" {
 int64_t brc_kv_attention_workspace(const brc_kv_cache* c, int batch, int draft, int hq) {
   if (check(c, batch, draft, hq) != BRC_OK) return 0;
   const Split s = split_rows(draft * (hq / c->heads), c);
-  return 2 * (int64_t)blocks_of(c->head_dim, s) * s.rows_per_block * (c->head_dim + 2) * 4;
+  return 2 * (int64_t)blocks_of(c, s) * s.rows_per_block * (c->head_dim + 2) * 4;
 }
 
 int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batch, int draft,
@@ -71,7 +73,7 @@ int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batc
   if ((int64_t)table_pages * c->page_size > 0x7FFFFFF0) return BRC_ERR_RANGE;
   const int group = hq / c->heads, rows = draft * group;
   const Split s = split_rows(rows, c);
-  const int blocks = blocks_of(c->head_dim, s);
+  const int blocks = blocks_of(c, s);
   if (workspace_bytes < brc_kv_attention_workspace(c, batch, draft, hq)) return BRC_ERR_SHAPE;
   Args a{};
   a.c = *c;

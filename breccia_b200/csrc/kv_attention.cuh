@@ -168,10 +168,12 @@ __device__ __forceinline__ float e8m0_value(uint32_t e) {
   return e == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
 }
 // 2^(e - ref) of two E8M0 bytes as an f16 pair: subnormals and zero below
-// 2^-14, infinity for 255 (which never is the reference).
+// 2^-14. INF: a byte of 255 (which never is the reference) gives infinity.
+template <bool INF>
 __device__ __forceinline__ uint32_t half2_pow2(int e0, int e1, int ref) {
   auto f = [&](int e) {
-    const int x = e == 255 ? 255 : max(e - ref + 127, 0);
+    int x = max(e - ref + 127, 0);
+    if constexpr (INF) x = e == 255 ? 255 : x;
     return __uint_as_float((uint32_t)x << 23);
   };
   return half2_of(f(e0), f(e1));
@@ -205,6 +207,22 @@ struct Shape {
   static constexpr int kKeyScales = 2 * kTileBytes;
   static constexpr int kValScales = kKeyScales + kRows * kScaleBytes;
   static constexpr int kStageBytes = kValScales + kRows * kScaleBytes;
+  // Where a lane reads: keys, read i of token r (others: constants further on);
+  // values, read i of token 2 c.
+  __device__ static __forceinline__ int key_offset(int lane, int i) {
+    const int r = lane >> 2, c = lane & 3;
+    if constexpr (kKeyRead < 4) return r * kRowBytes + c * 8;
+    else if constexpr (kPieces >= 8)
+      return r * kRowBytes + c * 16 + 64 * ((i & 1) ^ (r & 1)) + 128 * (i >> 1);
+    else return r * kRowBytes + c * 16 + 64 * i;
+  }
+  __device__ static __forceinline__ int val_offset(int lane, int i) {
+    const int r = lane >> 2, c = lane & 3;
+    if constexpr (kValRead == 4) return 2 * c * kRowBytes + ((r ^ (2 * c)) + 8 * i) * 16;
+    else if constexpr (kValRead == 2)
+      return 2 * c * kRowBytes + (((r >> 1) ^ ((2 * c) & 2)) * 16) + (r & 1) * 8;
+    else return 2 * c * kRowBytes + r * 4;
+  }
   __device__ static constexpr int key_piece(int t, int p) {
     return kPieces >= 8 ? p ^ ((t & 1) << 2) : p;
   }
@@ -325,6 +343,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return d;
 }
 
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
+
 template <int KIND, int FMT, int D, int NT>
 struct Step {
   using S = Shape<KIND, D>;
@@ -355,15 +378,31 @@ struct Step {
             const int t = 16 * u + 8 * n + r;
             e[u][n][i] = st[S::kKeyScales + t * S::kScales + 2 * i + (c >> 1)];
             if (live != S::kAll && !((live >> t) & 1u)) e[u][n][i] = 0;
-            if (e[u][n][i] != 255) top = max(top, e[u][n][i]);
+            top = max(top, e[u][n][i]);
           }
-      if (__any_sync(0xFFFFFFFFu, top > w.ke)) w.ke = max(w.ke, (int)__reduce_max_sync(0xFFFFFFFFu, top));
+      auto factors = [&](auto inf) {
 #pragma unroll
-      for (int u = 0; u < kSub; ++u)
+        for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int i = 0; i < kReads; ++i) f[u][n][i] = half2_pow2(e[u][n][i], e[u][n][i], w.ke);
+            for (int i = 0; i < kReads; ++i)
+              f[u][n][i] = half2_pow2<decltype(inf)::value>(e[u][n][i], e[u][n][i], w.ke);
+      };
+      if (__any_sync(0xFFFFFFFFu, top > w.ke)) {  // a larger scale, or 255
+        int t = 0;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < kReads; ++i)
+              if (e[u][n][i] != 255) t = max(t, e[u][n][i]);
+        w.ke = max(w.ke, (int)__reduce_max_sync(0xFFFFFFFFu, t));
+        factors(Bool<true>{});
+      } else {
+        factors(Bool<false>{});
+      }
     }
 #pragma unroll
     for (int i = 0; i < kReads; ++i) {
@@ -373,11 +412,8 @@ struct Step {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int t = 16 * u + 8 * n + r;
-          const uint8_t* p;
-          if constexpr (S::kKeyRead == 4)
-            p = st + (t * S::kPieces + S::key_piece(t, 4 * i + c)) * 16;
-          else p = st + t * S::kRowBytes + c * 8;
-          lds_words<S::kKeyRead>(p, x[u][n]);
+          lds_words<S::kKeyRead>(st + (S::key_offset(lane, i) + (16 * u + 8 * n) * S::kRowBytes),
+                                 x[u][n]);
           if constexpr (S::kFp4) {
             // a read is one or two 16-element blocks with their scales
             const uint8_t* sp = st + S::kKeyScales + t * S::kScales;
@@ -535,19 +571,34 @@ struct Step {
             const int blk = D == 64 ? r >> 2 : 4 * i + (r >> 1);
             e[u][t][i] = st[S::kValScales + token(u, t) * S::kScales + blk];
             if (!all && !((live >> token(u, t)) & 1u)) e[u][t][i] = 0;
-            if (e[u][t][i] != 255) top = max(top, e[u][t][i]);
+            top = max(top, e[u][t][i]);
           }
-      if (__any_sync(0xFFFFFFFFu, top - 127 > w.e))
-        w.raise((int)__reduce_max_sync(0xFFFFFFFFu, top) - 127);
+      auto factors = [&](auto inf) {
 #pragma unroll
-      for (int u = 0; u < kSub; ++u)
+        for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          f[u][t] = 64.f;
+          for (int t = 0; t < 2; ++t) {
+            f[u][t] = 64.f;
 #pragma unroll
-          for (int i = 0; i < kReads; ++i)
-            h[u][t][i] = half2_pow2(e[u][2 * t][i], e[u][2 * t + 1][i], w.e + 127);
-        }
+            for (int i = 0; i < kReads; ++i)
+              h[u][t][i] = half2_pow2<decltype(inf)::value>(e[u][2 * t][i], e[u][2 * t + 1][i],
+                                                            w.e + 127);
+          }
+      };
+      if (__any_sync(0xFFFFFFFFu, top - 127 > w.e)) {  // a larger scale, or 255
+        int m = 0;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < kReads; ++i)
+              if (e[u][t][i] != 255) m = max(m, e[u][t][i]);
+        w.raise((int)__reduce_max_sync(0xFFFFFFFFu, m) - 127);
+        factors(Bool<true>{});
+      } else {
+        factors(Bool<false>{});
+      }
     } else {
       if (w.e < -900) w.e = 0;
 #pragma unroll
@@ -591,14 +642,8 @@ struct Step {
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int tk = token(u, t);
-          const uint8_t* base = st + S::kTileBytes;
-          const uint8_t* q;
-          if constexpr (S::kValRead == 4)
-            q = base + (tk * S::kPieces + S::val_piece(tk, 8 * i + r)) * 16;
-          else if constexpr (S::kValRead == 2)
-            q = base + (tk * S::kPieces + S::val_piece(tk, r >> 1)) * 16 + (r & 1) * 8;
-          else q = base + tk * S::kRowBytes + r * 4;
+          const uint8_t* q = st + (S::kTileBytes + S::val_offset(lane, i) +
+                                   (16 * u + (t & 1) + 8 * (t >> 1)) * S::kRowBytes);
           lds_words<S::kValRead>(q, x[u][t]);
         }
       if (!all) {  // rows without a token hold anything
@@ -710,7 +755,8 @@ struct Step {
 };
 
 // Blocks that an SM is to hold, as many as the accumulators' registers allow.
-constexpr __host__ __device__ int blocks_per_sm(int d, int nt) {
+constexpr __host__ __device__ int blocks_per_sm(int kind, int d, int nt) {
+  if (kind == BRC_STE_NVFP4 && d * nt == 128) return 4;
   return d * nt <= 64 ? 4 : d * nt <= 256 ? 3 : 2;
 }
 // Stages of a warp's ring: what fits beside the queries in the block's part of
@@ -725,7 +771,7 @@ constexpr __host__ __device__ int query_bytes(int d, int nt) {
   return (nt == most_tiles(d) ? kWarps : 1) * 8 * nt * d * 2;
 }
 constexpr __host__ __device__ int stages(int kind, int d, int nt) {
-  const int room = (227 * 1024) / blocks_per_sm(d, nt) - 2048 - query_bytes(d, nt);
+  const int room = (227 * 1024) / blocks_per_sm(kind, d, nt) - 2048 - query_bytes(d, nt);
   const int n = room / (kWarps * stage_bytes(kind, d));
   return n > 6 ? 6 : n;
 }
@@ -736,7 +782,7 @@ constexpr __host__ __device__ int ring_bytes(int kind, int d, int nt) {
 }
 
 template <int KIND, int FMT, int D, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args a) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend(Args a) {
   using S = Shape<KIND, D>;
   using St = Step<KIND, FMT, D, NT>;
   constexpr int kStages = stages(KIND, D, NT);
@@ -782,11 +828,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
     const int page_mask = a.c.page_size - 1;
     const uint32_t head_row = (uint32_t)head * a.c.page_size;
     // First cache row of the 16-token tile at token t, or -1.
-    auto row_at = [&](int64_t t) -> int64_t {
+    auto row_at = [&](int t) -> int64_t {
       if (t >= seq.total) return -1;
-      const int64_t page = __ldg(table + (t >> a.page_shift));
+      const int page = __ldg(table + (t >> a.page_shift));
       if (page < 0 || page >= a.c.num_pages) return -1;
-      return page * a.page_rows + head_row + (uint32_t)(t & page_mask);
+      return (int64_t)((uint64_t)(uint32_t)page * a.page_rows) + (head_row + (t & page_mask));
     };
     // the warp's own ring of stages
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rings) + warp * (kStages * S::kStageBytes);
@@ -796,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
     auto fetch = [&]() {
       uint32_t bits = 0;
       if (ahead < s_end) {
-        const int64_t t = (int64_t)ahead * S::kRows;
+        const int t = ahead * S::kRows;  // (positions fit in 31 bits)
         const uint32_t to = ring + slot_in * S::kStageBytes;
         const int64_t row = row_at(t);
         if (row >= 0) {
@@ -891,9 +937,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
       const uint32_t bits = there >> ((kStages - 1) * kSub) & ((1u << kSub) - 1);
       if (bits) {
         const uint8_t* const st = ring_p + slot_out * S::kStageBytes;
-        const int64_t t0 = (int64_t)s * S::kRows;
+        const int t0 = s * S::kRows;
         uint32_t live = S::kAll;
-        if (t0 + S::kRows > seq.total) live >>= S::kRows - (int)(seq.total - t0);
+        if (t0 > seq.total - S::kRows) live >>= S::kRows - (seq.total - t0);
         if (kSub == 2 && bits != 3) live &= bits == 1 ? 0xFFFFu : 0xFFFF0000u;
         float p[kSub][NT][4];
         St::scores(w, st, q, lane, live, p);
@@ -911,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
           }
         uint32_t seen = 0;
         bool checked = false;
-        if (t0 + S::kRows > seq.context || live != S::kAll) {  // drafted tokens, or none
+        if (t0 > seq.context - S::kRows || live != S::kAll) {  // drafted tokens, or none
 #pragma unroll
           for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -921,7 +967,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) k_attend(Args 
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                   const int at = 16 * u + 8 * h + (lane >> 2);
-                  const int64_t j = t0 + at - seq.context;
+                  const int j = t0 - seq.context + at;
                   bool see = ((live >> at) & 1u) && node[n][x] < seq.drafts;
                   if (see && j >= 0)
                     see = a.tree ? a.tree[b * a.tree_stride + (int64_t)node[n][x] * a.draft + j] != 0

@@ -221,7 +221,7 @@ struct Loader {
 #pragma unroll
           for (int y = 0; y < 4; ++y) fp8x4_to_f16x4<FMT>(x[y], h[2 * y], h[2 * y + 1]);
           if constexpr (KIND == BRC_STE_MXFP8) {
-            const uint32_t f = half2_pow2((int)s[g][i], (int)s[g][i], ref);
+            const uint32_t f = half2_pow2<true>((int)s[g][i], (int)s[g][i], ref);
 #pragma unroll
             for (int y = 0; y < 8; ++y) h[y] = hmul2(h[y], f);
           }
