@@ -4,19 +4,23 @@
 // The mathematics, the numbers and the split of the work are kv_attention.cuh's;
 // with more than kTcRows rows to a cache head the products bound it, not HBM.
 //
-// One block to an SM, 13 warps, two tiles of 128 query rows, tiles of 128 tokens:
-//   warps 0-7   softmax, a thread to a row: scores from TMEM, probabilities back
-//               into the same TMEM columns as f16 (the A operand of P V)
-//   warps 8-11  codes and scales from global memory, decoded to f16 in shared
+// One block to an SM, two tiles of 128 query rows, tiles of 128 tokens:
+//   warps 0-15  softmax, two threads to a row, 64 columns each: scores from TMEM,
+//               probabilities back into the same TMEM columns as f16 (the A operand
+//               of P V). One thread to a row left the exponentials, the packing and
+//               the TMEM loads of its one warp per scheduler to run one after another
+//   warps 16-23 codes and scales from global memory, decoded to f16 in shared
 //               memory (128-byte swizzled rows; keys are K-major, values the same
 //               bytes read as MN-major); loads run one tile ahead in registers
-//   warp 12     issues tcgen05.mma: S = Q K^T and O += P V of each row tile in turn,
+//   warp 24     issues tcgen05.mma: S = Q K^T and O += P V of each row tile in turn,
 //               so that one row tile's products run under the other's softmax
 // TMEM: two score tiles and two output tiles of 128 columns. The codes are decoded
 // once for 256 rows, where the register path decodes them for every 32.
 //
-// A row's shift follows its maximum only when it is 2^8 behind (as in the register
-// path); then the softmax threads rescale their row of O in TMEM.
+// A row's shift follows its maximum only when 32 probabilities sum to 2^kRise above it
+// (the register path's rule, with less room above for more bits below in f16); then the
+// softmax threads rescale their row of O in TMEM. The two threads of a row may use
+// different shifts within a tile; at its end the lower half's probabilities are scaled.
 #pragma once
 
 #include "kv_attention.cuh"
@@ -33,12 +37,13 @@ using namespace kvatt;
 using namespace sm100;
 
 constexpr int kTok = 128;
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
+constexpr int kRise = 6;  // log2 of how far a sum of 32 probabilities may pass 1
+constexpr int kSoftWarps = 16, kLoadWarps = 8;
 constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgroups: three warps idle
-// Registers of a thread after setmaxnreg, by warpgroup; 2 x softmax + loads +
-// products are no more than the 4 x 128 that the block was launched with.
-constexpr uint32_t kSoftRegs = 152, kLoadRegs = 136, kMmaRegs = 72;
-static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs <= 4 * 128, "registers of the launch");
+// Registers of a thread after setmaxnreg, by warpgroup; 4 x softmax + 2 x loads +
+// products are no more than the 7 x 72 that the block was launched with.
+constexpr uint32_t kSoftRegs = 80, kLoadRegs = 72, kMmaRegs = 40;
+static_assert(4 * kSoftRegs + 2 * kLoadRegs + kMmaRegs <= 7 * 72, "registers of the launch");
 constexpr int kBlockBytes = 128 * 128;  // 128 rows of 64 f16, swizzled
 constexpr int kMeta = 4;                // a tile's scales outlive its key stage
 
@@ -59,7 +64,10 @@ struct alignas(128) Smem {
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
   Place place;
   uint32_t tmem, abort;
-  uint32_t odd[4];  // (the loads are at most two items ahead) number of the item whose drafted values are not all finite
+  float pair[2][2][2][128];  // [tile parity][row tile][half][row]: shifts, then sums
+  // Numbers of items whose drafted values are not all finite: one slot to an item, as
+  // the loads are at most two items ahead.
+  uint32_t odd[4];
 };
 
 __device__ __forceinline__ void fence_proxy_smem() {
@@ -125,21 +133,22 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------ loading
-// A warp decodes 32 of a tile's tokens: lane (t, c) reads token 8 g + t, piece 4 i
-// + c, for g < 4 and i < kHalves.
+// A warp decodes 16 of a tile's tokens: lane (t, c) reads token 8 g + t, piece 4 i
+// + c, for g < 2 and i < kHalves.
 template <int KIND, int FMT, int D>
 struct Loader {
   using S = Shape<KIND, D>;
   static constexpr int kHalves = S::kRowBytes / 64;
   static_assert(kHalves >= 1, "rows of at least 64 bytes");
-  uint4 w[4][kHalves];
-  uint32_t s[4][kHalves];  // scale byte(s) of the piece
+  static constexpr int kG = kTok / kLoadWarps / 8;
+  uint4 w[kG][kHalves];
+  uint32_t s[kG][kHalves];  // scale byte(s) of the piece
   uint4 e;                 // MXFP8: the scale bytes of tokens 4 lane .. + 3 (top of the tile)
 
   __device__ __forceinline__ void fetch(const uint8_t* data, const void* scale,
-                                        const int64_t (&row)[4], int64_t row4, int lane) {
+                                        const int64_t (&row)[kG], int64_t row4, int lane) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < kG; ++g)
 #pragma unroll
       for (int i = 0; i < kHalves; ++i) {
         w[g][i] = make_uint4(0u, 0u, 0u, 0u);
@@ -186,7 +195,7 @@ struct Loader {
                                          int dead, int drafted) {
     bool any = false;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < kG; ++g) {
       const int t = first + 8 * g + (lane >> 2);
 #pragma unroll
       for (int i = 0; i < kHalves; ++i) {
@@ -266,9 +275,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         mbar_init(&sm.v_full[i], kLoadWarps);
         mbar_init(&sm.k_empty[i], 1);
         mbar_init(&sm.v_empty[i], 1);
-        mbar_init(&sm.q_full[i], 128);
+        mbar_init(&sm.q_full[i], 256);
         mbar_init(&sm.s_full[i], 1);
-        mbar_init(&sm.p_full[i], 128);
+        mbar_init(&sm.p_full[i], 256);
         mbar_init(&sm.o_full[i], 1);
       }
       mbar_init(&sm.drain, 1);
@@ -285,10 +294,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
   if (warp < kSoftWarps) {
     // ================================================================ softmax
     regs_inc<kSoftRegs>();
-    const int r = warp >> 2;  // row tile
-    const int mine = tid & 127;
+    const int r = warp >> 3, half = (warp >> 2) & 1;  // row tile; half of its columns
+    const int mine = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes, in bits 16 ..
-    const uint32_t sc = (r ? s_col[1] : s_col[0]) + lanes, oc = (r ? o_col[1] : o_col[0]) + lanes;
+    const uint32_t sc = (r ? s_col[1] : s_col[0]) + lanes + 64 * half;
+    const uint32_t oc = (r ? o_col[1] : o_col[0]) + lanes + (D / 2) * half;
+    // The two warps of 32 rows meet once a tile. A warp that leaves early arrives
+    // in its place, and the other one finds the abort flag at its next wait.
+    const uint32_t pair_id = 1 + r * 4 + (warp & 3);
+    auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair_id) : "memory"); };
+    auto leave = [&]() { asm volatile("barrier.cta.arrive %0, 64;" ::"r"(pair_id) : "memory"); };
     uint32_t tile = 0, number = 0;  // tiles and items so far
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
@@ -325,7 +340,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         const float up = copysignf(__uint_as_float((uint32_t)(127 + 7 - k) << 23), a.scale_log2);
         rowf = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + k - 7) << 23);
 #pragma unroll 4
-        for (int i = 0; i < D / 8; ++i) {
+        for (int i = half * (D / 16); i < (half + 1) * (D / 16); ++i) {
           uint4 y = make_uint4(0u, 0u, 0u, 0u);
           if (valid) {
             float f[8];
@@ -343,20 +358,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       float m = -INFINITY, l = 0.f;
       int ev = -1000;
       for (int j = walk.s_begin; j < walk.s_end; ++j) {
-        if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.s_full[r], s_phase, abort, status, 1u)))) break;
+        if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.s_full[r], s_phase, abort, status, 1u)))) {
+          leave();
+          break;
+        }
         s_phase ^= 1u;
         tc_fence_after();
         const Meta& meta = sm.meta[(tile0 + (j - walk.s_begin)) % kMeta];
         const int64_t t0 = (int64_t)j * kTok;
         const float f = KIND == BRC_STE_MXFP8 ? rowf * e8m0_value(meta.ek) : rowf;
         const bool masked = t0 + kTok > seq.context || !meta.all;
-        uint32_t vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+        uint32_t vis[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             vis[c] = 0;
             for (int i = 0; i < 32; ++i) {
-              const int t = 32 * c + i;
+              const int t = 64 * half + 32 * c + i;
               const int64_t n = t0 + t - seq.context;
               bool see = valid && ((meta.live[t & 3] >> (t >> 2)) & 1u);
               if (see && n >= 0)
@@ -376,13 +394,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           if constexpr (KIND == BRC_STE_BLOCK_FP8) {
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-              const float4 g = *reinterpret_cast<const float4*>(&meta.sk[32 * c + 2 * i]);
+              const float4 g = *reinterpret_cast<const float4*>(&meta.sk[64 * half + 32 * c + 2 * i]);
               u[i] = __fmul2_rn(u[i], make_float2(g.x, g.y));
               u[i + 1] = __fmul2_rn(u[i + 1], make_float2(g.z, g.w));
             }
           }
           if (masked) {
-            const uint32_t bits = vis[c];
+            const uint32_t bits = c ? vis[1] : vis[0];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               if (!((bits >> (2 * i)) & 1u)) u[i].x = -INFINITY;
@@ -394,7 +412,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         auto scale_o = [&](float g) {
           if (j == walk.s_begin) return;
 #pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
+          for (int c = 0; c < D / 32; ++c) {  // this thread's half of the columns
             uint32_t x[16];
             tmem_ld16(oc + 16 * c, x);
             tmem_ld_wait16(x);
@@ -409,10 +427,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             ev = meta.ev;
           }
         }
-        if (j == walk.s_begin) {  // the first shift: the first tile's maximum
+        // This half's shift: the row's, until a score is far above it (and at first the
+        // half's maximum). Shifts are whole numbers: less the lift they are exact, so
+        // that the row's log-sum-exp does not get their rounding.
+        float own = m;
+        if (j == walk.s_begin) {
           float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
             uint32_t x[32];
             float2 u[16];
             tmem_ld32(sc + 32 * c, x);
@@ -422,15 +444,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(u[i].x, u[i].y));
           }
-          if (top != -INFINITY) m = top * f;
+          if (top != -INFINITY) own = ceilf(top * f);
         }
-        // Probabilities carry the factor 2^lift that the value scales ask for.
-        float lift = 6.f;
-        if constexpr (KIND == BRC_STE_BLOCK_FP8) lift = (float)(2 - ev);
-        else if constexpr (KIND == BRC_STE_MXFP8) lift = (float)(2 + meta.ev - ev);
-        float base = lift - (m == -INFINITY ? 0.f : m);
-        const float most = ex2(lift + kGrow);
+        // Probabilities carry the factor 2^lift that the value scales ask for. Their sum
+        // over 32 tokens may pass it by 2^kRise (32 scores at the shift reach 2^5), so
+        // that none leaves the range of f16, and the small ones keep the bits that are left.
+        float lift = 9.f;
+        if constexpr (KIND == BRC_STE_BLOCK_FP8) lift = (float)(4 - ev);
+        else if constexpr (KIND == BRC_STE_MXFP8) lift = (float)(4 + meta.ev - ev);
+        float base = lift - (own == -INFINITY ? 0.f : own);
+        const float most = ex2(lift + kRise);
         float2 l2 = make_float2(0.f, 0.f);
+        // this tile's probabilities so far (`upto` groups of 32 columns) times g
+        auto scale_p = [&](int upto, float g) {
+          // (g as f16 would be zero below 2^-25, where large ones are still needed)
+          tmem_st_wait();
+#pragma unroll 1
+          for (int b = 0; b < upto; ++b) {
+            uint32_t z[16];
+            tmem_ld16(sc + 16 * b, z);
+            tmem_ld_wait16(z);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&z[i]));
+              z[i] = half2_of(y.x * g, y.y * g);
+            }
+            tmem_st16(sc + 16 * b, z);
+          }
+        };
         auto exps = [&](float2 (&u)[16]) {
           float2 t = make_float2(0.f, 0.f);
 #pragma unroll
@@ -442,48 +483,39 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           return t;
         };
         // 32 scores to probabilities, into columns that their scores have left
-        auto work = [&](const uint32_t (&x)[32], int c) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t x[32];
           float2 u[16];
+          tmem_ld32(sc + 32 * c, x);
+          tmem_ld_wait();
+          reg_bind32(x);
           take(x, c, u);
           float2 t = exps(u);
-          // a score far above the shift shows in the sum (which has no lower bound
-          // on a row that has seen nothing: its shift is 0)
+          // a score far above the shift shows in the sum (a row that has seen
+          // nothing has the shift 0)
           const float all = t.x + t.y;
-          if (__any_sync(0xFFFFFFFFu, all > most || (m == -INFINITY && all > 0.f))) {
-            // the shift follows; sums, outputs and this tile's earlier columns with it
-            uint32_t y[32];
-            tmem_ld32(sc + 32 * c, y);
+          if (__any_sync(0xFFFFFFFFu, all > most || (own == -INFINITY && all > 0.f))) {
+            tmem_ld32(sc + 32 * c, x);
             tmem_ld_wait();
-            reg_bind32(y);
-            take(y, c, u);
+            reg_bind32(x);
+            take(x, c, u);
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(u[i].x, u[i].y));
-            top = top == -INFINITY ? top : top * f;
-            const float nm = fmaxf(m, top), g = nm == m || m == -INFINITY ? 1.f : ex2(m - nm);
-            m = nm;
-            base = lift - (m == -INFINITY ? 0.f : m);
-            l *= g;
+            top = top == -INFINITY ? top : ceilf(top * f);
+            const float nm = fmaxf(own, top), g = nm == own || own == -INFINITY ? 1.f : ex2(own - nm);
+            own = nm;
+            base = lift - (own == -INFINITY ? 0.f : own);
             l2 = __fmul2_rn(l2, make_float2(g, g));
-            scale_o(g);
-            tmem_st_wait();
-            const uint32_t gh = half2_of(g, g);
-#pragma unroll 1
-            for (int b = 0; b < c; ++b) {
-              uint32_t z[16];
-              tmem_ld16(sc + 16 * b, z);
-              tmem_ld_wait16(z);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) z[i] = hmul2(z[i], gh);
-              tmem_st16(sc + 16 * b, z);
-            }
+            scale_p(c, g);
             t = exps(u);
           }
           l2 = __fadd2_rn(l2, t);
           if constexpr (KIND == BRC_STE_BLOCK_FP8) {
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-              const float4 g = *reinterpret_cast<const float4*>(&meta.sv[32 * c + 2 * i]);
+              const float4 g = *reinterpret_cast<const float4*>(&meta.sv[64 * half + 32 * c + 2 * i]);
               u[i] = __fmul2_rn(u[i], make_float2(g.x, g.y));
               u[i + 1] = __fmul2_rn(u[i + 1], make_float2(g.z, g.w));
             }
@@ -492,46 +524,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
 #pragma unroll
           for (int i = 0; i < 16; ++i) p[i] = half2_of(u[i].x, u[i].y);
           tmem_st16(sc + 16 * c, p);
-        };
-        {
-          uint32_t x0[32], x1[32];
-          tmem_ld32(sc, x0);
-          tmem_ld_wait();
-          reg_bind32(x0);
-          tmem_ld32(sc + 32, x1);
-          work(x0, 0);
-          tmem_ld_wait();
-          reg_bind32(x1);
-          tmem_ld32(sc + 64, x0);
-          work(x1, 1);
-          tmem_ld_wait();
-          reg_bind32(x0);
-          tmem_ld32(sc + 96, x1);
-          work(x0, 2);
-          tmem_ld_wait();
-          reg_bind32(x1);
-          work(x1, 3);
         }
-        l += (l2.x + l2.y) * ex2(-lift);
+        // ---- the halves agree on the row's shift
+        const uint32_t parity = (tile0 + (j - walk.s_begin)) & 1u;
+        sm.pair[parity][r][half][mine] = own;
+        meet();
+        const float nm = fmaxf(own, sm.pair[parity][r][half ^ 1][mine]);
+        float part = (l2.x + l2.y) * ex2(-lift);
+        if (__any_sync(0xFFFFFFFFu, nm != own || nm != m)) {
+          const float gp = nm == own || nm == -INFINITY ? 1.f : ex2(own - nm);
+          const float go = nm == m || nm == -INFINITY ? 1.f : ex2(m - nm);
+          if (__any_sync(0xFFFFFFFFu, gp != 1.f)) scale_p(2, gp);
+          if (__any_sync(0xFFFFFFFFu, go != 1.f)) scale_o(go);
+          part *= gp;
+          l *= go;
+          m = nm;
+        }
+        l += part;
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&sm.p_full[r]);
       }
       if (!ok) break;
       // ---- the item's output
-      if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.o_full[r], o_phase, abort, status, 1u)))) break;
+      if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.o_full[r], o_phase, abort, status, 1u)))) {
+        leave();
+        break;
+      }
+      // the row's sum, of both halves (the slots of the next tile's parity are free:
+      // the other half has read them before it met this one at the last tile)
+      sm.pair[tile & 1u][r][half][mine] = l;
+      meet();
+      l = half ? sm.pair[tile & 1u][r][0][mine] + l : l + sm.pair[tile & 1u][r][1][mine];
       o_phase ^= 1u;
       tc_fence_after();
       const bool whole = walk.s_begin == 0 && walk.s_end == seq.steps;
-      const float so = KIND == BRC_STE_NVFP4 ? 0x1p-6f : ev < -900 ? 1.f : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : 0) - 2));
+      const float so = KIND == BRC_STE_NVFP4 ? 0x1p-9f : ev < -900 ? 1.f : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : 0) - 4));
       const bool none = !valid || l == 0.f;
       const float mul = whole ? (none ? 0.f : so / l) : so;
       const bool odd = sm.odd[number & 3u] == number && !none;
       const int64_t slot = 2 * (int64_t)blockIdx.x + (walk.s_begin > 0 ? 0 : 1);
       const int rr = r * 128 + mine;
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
+      for (int c = 0; c < D / 32; ++c) {
         uint32_t x[16];
+        const int col = (D / 2) * half + 16 * c;
         __syncwarp();
         tmem_ld16(oc + 16 * c, x);
         tmem_ld_wait16(x);
@@ -550,7 +587,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             const int64_t src = page * a.page_rows + (int64_t)walk.head * a.c.page_size +
                                 (t & (a.c.page_size - 1));
             for (int i = 0; i < 16; ++i) {
-              const float v = value_at<KIND, FMT, D>(a.c, src, 16 * c + i);
+              const float v = value_at<KIND, FMT, D>(a.c, src, col + i);
               if (!isfinite(v)) o[i] += v;
             }
           }
@@ -567,18 +604,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
                 y[i] = *reinterpret_cast<const uint32_t*>(&h);
               }
             }
-            uint16_t* const dst = static_cast<uint16_t*>(a.out) + at_row * D + 16 * c;
+            uint16_t* const dst = static_cast<uint16_t*>(a.out) + at_row * D + col;
             stg16(dst, make_uint4(y[0], y[1], y[2], y[3]));
             stg16(dst + 8, make_uint4(y[4], y[5], y[6], y[7]));
           } else {
-            float* const dst = a.part_o + (slot * a.rows_per_block + rr) * D + 16 * c;
+            float* const dst = a.part_o + (slot * a.rows_per_block + rr) * D + col;
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
               *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
       }
-      if (row < a.rows) {
+      if (row < a.rows && half == 0) {
         if (whole) {
           if (a.lse) a.lse[at_row] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         } else {
@@ -591,8 +628,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     }
   } else if (warp < kSoftWarps + kLoadWarps) {
     // ================================================================ codes
-    regs_inc<kLoadRegs>();
-    const int lw = warp - kSoftWarps, first = 32 * lw;
+    const int lw = warp - kSoftWarps, first = kTok / kLoadWarps * lw;
     uint32_t tile = 0, number = 0;
     bool ok = true;
     for (; ok && walk.take(a); walk.next()) {
@@ -600,22 +636,50 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       const Seq seq = walk.seq;
       const int32_t* const table = a.table + walk.b * a.table_stride;
       const int64_t head_row = (int64_t)walk.head * a.c.page_size;
-      auto row_at = [&](int64_t t) -> int64_t {
-        if (t >= seq.total) return -1;
-        const int64_t page = __ldg(table + (t >> a.page_shift));
-        if (page < 0 || page >= a.c.num_pages) return -1;
-        return page * a.page_rows + head_row + (t & (a.c.page_size - 1));
-      };
+      constexpr int kG = Loader<KIND, FMT, D>::kG;
       Loader<KIND, FMT, D> k, v;
-      int64_t row[4], row4;
-      auto rows_of_tile = [&](int j) {
-        const int64_t t0 = (int64_t)j * kTok;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) row[g] = row_at(t0 + first + 8 * g + (lane >> 2));
-        row4 = row_at(t0 + 4 * lane);
+      // A tile's pages, fetched a tile before they are needed: of this lane's
+      // tokens, and of tokens 4 lane .. + 3 (whose scales it looks at).
+      int pages[kG + 1];
+      int64_t row[kG], row4;
+      auto token = [&](int j, int g) {
+        return j * kTok + (g < kG ? first + 8 * g + (lane >> 2) : 4 * lane);
       };
-      rows_of_tile(walk.s_begin);
+      auto pages_of = [&](int j) {
+#pragma unroll
+        for (int g = 0; g <= kG; ++g) {
+          const int t = token(j, g);
+          pages[g] = j < walk.s_end && t < seq.total ? __ldg(table + (t >> a.page_shift)) : -1;
+        }
+      };
+      auto rows_of = [&](int j) {
+#pragma unroll
+        for (int g = 0; g <= kG; ++g) {
+          const int page = pages[g];
+          const int64_t at =
+              page < 0 || page >= a.c.num_pages
+                  ? -1
+                  : (int64_t)((uint64_t)(uint32_t)page * a.page_rows) +
+                        (head_row + (token(j, g) & (a.c.page_size - 1)));
+          if (g < kG) row[g] = at;
+          else row4 = at;
+        }
+      };
+      float4 sk4, sv4;  // block FP8, the first warp: the tokens' scales
+      auto scales = [&]() {
+        sk4 = sv4 = make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+          if (lw == 0 && row4 >= 0) {
+            sk4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.k_scale) + row4));
+            sv4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.v_scale) + row4));
+          }
+        }
+      };
+      pages_of(walk.s_begin);
+      rows_of(walk.s_begin);
       k.fetch(a.c.k_data, a.c.k_scale, row, row4, lane);
+      scales();
+      pages_of(walk.s_begin + 1);
       for (int j = walk.s_begin; j < walk.s_end; ++j, ++tile) {
         const uint32_t st = tile & 1u, use = (tile >> 1) & 1u;
         const int64_t t0 = (int64_t)j * kTok;
@@ -625,16 +689,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         const int live4 = row4 < 0 ? 0 : min(max(dead - 4 * lane, 0), 4);
         v.fetch(a.c.v_data, a.c.v_scale, row, row4, lane);
         int ek = 0, ev = 0;
-        float4 sk4 = make_float4(0.f, 0.f, 0.f, 0.f), sv4 = sk4;
         if constexpr (KIND == BRC_STE_MXFP8) {
           ek = k.top(live4);
           ev = v.top(live4);
-        }
-        if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-          if (lw == 0 && row4 >= 0) {
-            sk4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.k_scale) + row4));
-            sv4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.v_scale) + row4));
-          }
         }
         if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.k_empty[st], use ^ 1u, abort, status, 1u)))) break;
         if (lw == 0) {
@@ -674,8 +731,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.k_full[st]);
         if (j + 1 < walk.s_end) {
-          rows_of_tile(j + 1);
+          rows_of(j + 1);
           k.fetch(a.c.k_data, a.c.k_scale, row, row4, lane);
+          scales();
+          pages_of(j + 2);
         }
         if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.v_empty[st], use ^ 1u, abort, status, 1u)))) break;
         const int vref = max(ev, 27);  // no lower than 2^-100
@@ -735,8 +794,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           if (!ok) break;
           if (elect_lane()) {
 #pragma unroll
-            for (int i = 0; i < kTok / 16; ++i)  // 16 tokens: 8 columns of P, 16 rows of V
-              mma_f16_ts(o_col[r], s_col[r] + 8 * i,
+            for (int i = 0; i < kTok / 16; ++i)  // 16 tokens: 8 columns of P (each half's at its own start), 16 rows of V
+              mma_f16_ts(o_col[r], s_col[r] + 64 * (i / 4) + 8 * (i % 4),
                          smem_desc(smem_u32(sm.v[st][0]) + 2048 * i, kBlockBytes, 1024, 2), kIdO,
                          j > 0 || i > 0);
             if (j + 1 == n) tc_commit(&sm.o_full[r]);
