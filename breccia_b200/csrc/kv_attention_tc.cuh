@@ -44,12 +44,14 @@ constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgro
 // products are no more than the 7 x 72 that the block was launched with.
 constexpr uint32_t kSoftRegs = 80, kLoadRegs = 72, kMmaRegs = 40;
 static_assert(4 * kSoftRegs + 2 * kLoadRegs + kMmaRegs <= 7 * 72, "registers of the launch");
+// A tile's Meta is written when the scores of the tile two before are done, so that the
+// softmax three before is over: a ring of four.
+constexpr int kMeta = 4;
 constexpr int kBlockBytes = 128 * 128;  // 128 rows of 64 f16, swizzled
-constexpr int kMeta = 4;                // a tile's scales outlive its key stage
 
 struct alignas(16) Meta {
-  float sk[kTok], sv[kTok];  // block FP8
-  int ek, ev;                // MXFP8: E8M0 bytes that the tile is relative to; block FP8: ev
+  float sk[kTok];  // block FP8
+  int ek, ev;      // exponents that the tile is relative to: MXFP8 (as E8M0), values of block FP8
   uint32_t live[4];          // token 4 i + k: bit i of word k
   uint32_t all;              // every token is live
 };
@@ -60,7 +62,7 @@ struct alignas(128) Smem {
   uint8_t k[2][D / 64][kBlockBytes];
   uint8_t v[2][D / 64][kBlockBytes];
   Meta meta[kMeta];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t meta_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
   Place place;
   uint32_t tmem, abort;
@@ -133,6 +135,11 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------ loading
+// A scale below 2 times the largest code (448 of E4M3, 57344 of E5M2) times 2^this is
+// within f16.
+template <int FMT>
+constexpr int kValueLift = FMT == BRC_FP8_E4M3 ? 6 : -1;
+
 // A warp decodes 16 of a tile's tokens: lane (t, c) reads token 8 g + t, piece 4 i
 // + c, for g < 2 and i < kHalves.
 template <int KIND, int FMT, int D>
@@ -142,11 +149,12 @@ struct Loader {
   static_assert(kHalves >= 1, "rows of at least 64 bytes");
   static constexpr int kG = kTok / kLoadWarps / 8;
   uint4 w[kG][kHalves];
-  uint32_t s[kG][kHalves];  // scale byte(s) of the piece
-  uint4 e;                 // MXFP8: the scale bytes of tokens 4 lane .. + 3 (top of the tile)
+  uint32_t s[kG][kHalves];  // scale byte(s) of the piece; values of block FP8: the row's scale
 
+  // VALUES: block FP8 needs the row's scale too
+  template <bool VALUES>
   __device__ __forceinline__ void fetch(const uint8_t* data, const void* scale,
-                                        const int64_t (&row)[kG], int64_t row4, int lane) {
+                                        const int64_t (&row)[kG], int lane) {
 #pragma unroll
     for (int g = 0; g < kG; ++g)
 #pragma unroll
@@ -157,40 +165,26 @@ struct Loader {
           const int piece = 4 * i + (lane & 3);
           w[g][i] = ldg16(data + row[g] * S::kRowBytes + piece * 16);
           const uint8_t* sp = static_cast<const uint8_t*>(scale) + row[g] * S::kScales;
-          if constexpr (KIND == BRC_STE_MXFP8) s[g][i] = __ldg(sp + piece / 2);
-          else if constexpr (KIND == BRC_STE_NVFP4)
+          if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+            if (VALUES)
+              s[g][i] = __float_as_uint(__ldg(static_cast<const float*>(scale) + row[g]));
+          } else if constexpr (KIND == BRC_STE_MXFP8 && D == 128) {  // one load for both pieces
+            s[g][i] = (__ldg(reinterpret_cast<const uint32_t*>(sp)) >> (8 * (piece / 2))) & 0xFFu;
+          } else if constexpr (KIND == BRC_STE_MXFP8) {
+            s[g][i] = __ldg(sp + piece / 2);
+          } else if constexpr (KIND == BRC_STE_NVFP4)
             s[g][i] = __ldg(reinterpret_cast<const uint16_t*>(sp + 2 * piece));
         }
       }
-    if constexpr (KIND == BRC_STE_MXFP8) {
-      e = make_uint4(0u, 0u, 0u, 0u);
-      if (row4 >= 0) {
-        const uint8_t* sp = static_cast<const uint8_t*>(scale) + row4 * S::kScales;
-        if constexpr (D == 128) {
-          e = ldg16(sp);
-        } else {
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp));
-          e.x = v.x;
-          e.y = v.y;
-        }
-      }
-    }
-  }
-  // Largest E8M0 byte of the tile's live tokens, below 255; every lane gets it.
-  __device__ __forceinline__ int top(int live4) const {
-    uint32_t m = 0;
-    const uint32_t v[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-    for (int i = 0; i < 4 * S::kScales; ++i) {
-      const uint32_t x = (v[i / 4] >> (8 * (i % 4))) & 0xFFu;
-      if (x != 255u && i / S::kScales < live4) m = max(m, x);
-    }
-    return (int)__reduce_max_sync(0xFFFFFFFFu, m);
   }
   // Decode into a stage. `first`: token of the warp's first row; rows from `dead`
   // on hold anything and become zero. ODD: drafted tokens (from `drafted` on) that
-  // hold something not finite become zero too; returns whether there was one.
-  template <bool ODD>
+  // hold something not finite become zero too; returns whether there was one. VALUES:
+  // of block FP8 times scale * 2^(kValueLift - ref), which rounds them to f16 once (as
+  // the probabilities are). That factor on the probabilities instead, as on the scores,
+  // has every softmax thread read every token's from shared memory, 16 bytes to each
+  // lane (8 trees of 64 nodes over 16384 tokens: 498 us).
+  template <bool ODD, bool VALUES>
   __device__ __forceinline__ bool decode(uint8_t* stage, int first, int lane, int ref,
                                          int dead, int drafted) {
     bool any = false;
@@ -208,6 +202,7 @@ struct Loader {
 #pragma unroll
             for (int y = 0; y < 4; ++y) odd |= odd_codes<KIND, FMT>(x[y]);
             if constexpr (KIND == BRC_STE_MXFP8) odd |= s[g][i] == 255u;
+            if constexpr (KIND == BRC_STE_BLOCK_FP8) odd |= !isfinite(__uint_as_float(s[g][i]));
             if constexpr (KIND == BRC_STE_NVFP4)
               odd |= (s[g][i] & 0x7Fu) == 0x7Fu || (s[g][i] & 0x7F00u) == 0x7F00u;
             any |= odd;
@@ -233,6 +228,15 @@ struct Loader {
             const uint32_t f = half2_pow2<true>((int)s[g][i], (int)s[g][i], ref);
 #pragma unroll
             for (int y = 0; y < 8; ++y) h[y] = hmul2(h[y], f);
+          } else if constexpr (VALUES) {
+            constexpr int kDown = kValueLift<FMT> < 0 ? 2 : 0;  // (ref may be 127)
+            const float f = __uint_as_float(s[g][i]) * (kDown ? 0.25f : 1.f) *
+                            __uint_as_float((uint32_t)(127 + kValueLift<FMT> + kDown - ref) << 23);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&h[y]));
+              h[y] = half2_of(u.x * f, u.y * f);
+            }
           }
         }
         // a piece is kUnits 16-byte units of a 64-element block's row
@@ -248,6 +252,73 @@ struct Loader {
     return any;
   }
 };
+
+// The scales of a tile's tokens 4 lane .. + 3: what the tile is relative to.
+template <int KIND, int D>
+struct Scales {
+  using S = Shape<KIND, D>;
+  uint4 e;
+
+  __device__ __forceinline__ void fetch(const void* scale, int64_t row4) {
+    e = make_uint4(0u, 0u, 0u, 0u);
+    if (row4 >= 0) {
+      if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+        e = ldg16(static_cast<const float*>(scale) + row4);
+      } else if constexpr (KIND == BRC_STE_MXFP8) {
+        const uint8_t* sp = static_cast<const uint8_t*>(scale) + row4 * S::kScales;
+        if constexpr (D == 128) {
+          e = ldg16(sp);
+        } else {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp));
+          e.x = v.x;
+          e.y = v.y;
+        }
+      }
+    }
+  }
+  // Largest exponent of the tile's live tokens that is finite: an E8M0 byte below 255,
+  // or a float32 scale's; every lane gets it.
+  __device__ __forceinline__ int top(int live4) const {
+    uint32_t m = 0;
+    uint32_t v[4] = {e.x, e.y, e.z, e.w};
+    if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t x = v[y] & 0x7FFFFFFFu;
+        if (y < live4 && x < 0x7F800000u) m = max(m, x);
+      }
+      return max((int)(__reduce_max_sync(0xFFFFFFFFu, m) >> 23) - 127, -100);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (D == 128) {
+          if (i >= live4) v[i] = 0u;
+        } else {  // two bytes to a token
+          v[i] &= (2 * i < live4 ? 0xFFFFu : 0u) | (2 * i + 1 < live4 ? 0xFFFF0000u : 0u);
+        }
+        // a byte of 255 shows as a zero byte of ~v
+        if ((~v[i] - 0x01010101u) & v[i] & 0x80808080u) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (((v[i] >> (8 * y)) & 0xFFu) == 0xFFu) v[i] &= ~(0xFFu << (8 * y));
+        }
+      }
+      m = __vmaxu2(__vmaxu2(v[0] & 0x00FF00FFu, v[1] & 0x00FF00FFu),
+                   __vmaxu2((v[0] >> 8) & 0x00FF00FFu, (v[1] >> 8) & 0x00FF00FFu));
+      m = __vmaxu2(m, __vmaxu2(__vmaxu2(v[2] & 0x00FF00FFu, v[3] & 0x00FF00FFu),
+                               __vmaxu2((v[2] >> 8) & 0x00FF00FFu, (v[3] >> 8) & 0x00FF00FFu)));
+      return (int)__reduce_max_sync(0xFFFFFFFFu, max(m & 0xFFFFu, m >> 16));
+    }
+  }
+};
+
+// Row of a token in the cache's arrays; -1: no such page.
+__device__ __forceinline__ int64_t slot_of(const Args& a, int page, int64_t head_row, int token) {
+  return page < 0 || page >= a.c.num_pages
+             ? -1
+             : (int64_t)((uint64_t)(uint32_t)page * a.page_rows) +
+                   (head_row + (token & (a.c.page_size - 1)));
+}
 
 template <int KIND, int FMT, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* status) {
@@ -271,6 +342,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       sm.odd[0] = sm.odd[1] = sm.odd[2] = sm.odd[3] = 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.meta_full[i], 1);
         mbar_init(&sm.k_full[i], kLoadWarps);
         mbar_init(&sm.v_full[i], kLoadWarps);
         mbar_init(&sm.k_empty[i], 1);
@@ -446,12 +518,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           }
           if (top != -INFINITY) own = ceilf(top * f);
         }
-        // Probabilities carry the factor 2^lift that the value scales ask for. Their sum
+        // Probabilities carry the factor 2^lift: values are relative to their tile's
+        // largest scale, O to the row tile's (at most 2^4 less). Their sum
         // over 32 tokens may pass it by 2^kRise (32 scores at the shift reach 2^5), so
         // that none leaves the range of f16, and the small ones keep the bits that are left.
-        float lift = 9.f;
-        if constexpr (KIND == BRC_STE_BLOCK_FP8) lift = (float)(4 - ev);
-        else if constexpr (KIND == BRC_STE_MXFP8) lift = (float)(4 + meta.ev - ev);
+        const float lift = KIND == BRC_STE_NVFP4 ? 9.f : (float)(5 + meta.ev - ev);
         float base = lift - (own == -INFINITY ? 0.f : own);
         const float most = ex2(lift + kRise);
         float2 l2 = make_float2(0.f, 0.f);
@@ -512,14 +583,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             t = exps(u);
           }
           l2 = __fadd2_rn(l2, t);
-          if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float4 g = *reinterpret_cast<const float4*>(&meta.sv[64 * half + 32 * c + 2 * i]);
-              u[i] = __fmul2_rn(u[i], make_float2(g.x, g.y));
-              u[i + 1] = __fmul2_rn(u[i + 1], make_float2(g.z, g.w));
-            }
-          }
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) p[i] = half2_of(u[i].x, u[i].y);
@@ -559,7 +622,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       o_phase ^= 1u;
       tc_fence_after();
       const bool whole = walk.s_begin == 0 && walk.s_end == seq.steps;
-      const float so = KIND == BRC_STE_NVFP4 ? 0x1p-9f : ev < -900 ? 1.f : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : 0) - 4));
+      const float so = KIND == BRC_STE_NVFP4 ? 0x1p-9f
+                       : ev < -900 ? 1.f
+                                   : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : kValueLift<FMT>) - 5));
       const bool none = !valid || l == 0.f;
       const float mul = whole ? (none ? 0.f : so / l) : so;
       const bool odd = sm.odd[number & 3u] == number && !none;
@@ -638,47 +703,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       const int64_t head_row = (int64_t)walk.head * a.c.page_size;
       constexpr int kG = Loader<KIND, FMT, D>::kG;
       Loader<KIND, FMT, D> k, v;
-      // A tile's pages, fetched a tile before they are needed: of this lane's
-      // tokens, and of tokens 4 lane .. + 3 (whose scales it looks at).
-      int pages[kG + 1];
-      int64_t row[kG], row4;
-      auto token = [&](int j, int g) {
-        return j * kTok + (g < kG ? first + 8 * g + (lane >> 2) : 4 * lane);
-      };
+      // a tile's pages, fetched a tile before they are needed
+      int pages[kG];
+      int64_t row[kG];
+      auto token = [&](int j, int g) { return j * kTok + first + 8 * g + (lane >> 2); };
       auto pages_of = [&](int j) {
 #pragma unroll
-        for (int g = 0; g <= kG; ++g) {
+        for (int g = 0; g < kG; ++g) {
           const int t = token(j, g);
           pages[g] = j < walk.s_end && t < seq.total ? __ldg(table + (t >> a.page_shift)) : -1;
         }
       };
       auto rows_of = [&](int j) {
 #pragma unroll
-        for (int g = 0; g <= kG; ++g) {
-          const int page = pages[g];
-          const int64_t at =
-              page < 0 || page >= a.c.num_pages
-                  ? -1
-                  : (int64_t)((uint64_t)(uint32_t)page * a.page_rows) +
-                        (head_row + (token(j, g) & (a.c.page_size - 1)));
-          if (g < kG) row[g] = at;
-          else row4 = at;
-        }
-      };
-      float4 sk4, sv4;  // block FP8, the first warp: the tokens' scales
-      auto scales = [&]() {
-        sk4 = sv4 = make_float4(0.f, 0.f, 0.f, 0.f);
-        if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-          if (lw == 0 && row4 >= 0) {
-            sk4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.k_scale) + row4));
-            sv4 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.c.v_scale) + row4));
-          }
-        }
+        for (int g = 0; g < kG; ++g) row[g] = slot_of(a, pages[g], head_row, token(j, g));
       };
       pages_of(walk.s_begin);
       rows_of(walk.s_begin);
-      k.fetch(a.c.k_data, a.c.k_scale, row, row4, lane);
-      scales();
+      k.template fetch<false>(a.c.k_data, a.c.k_scale, row, lane);
       pages_of(walk.s_begin + 1);
       for (int j = walk.s_begin; j < walk.s_end; ++j, ++tile) {
         const uint32_t st = tile & 1u, use = (tile >> 1) & 1u;
@@ -686,62 +728,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         const int dead = (int)min((int64_t)kTok, seq.total - t0);
         const bool drafted = t0 + kTok > seq.context;
         const int from = (int)max((int64_t)0, seq.context - t0);
-        const int live4 = row4 < 0 ? 0 : min(max(dead - 4 * lane, 0), 4);
-        v.fetch(a.c.v_data, a.c.v_scale, row, row4, lane);
-        int ek = 0, ev = 0;
-        if constexpr (KIND == BRC_STE_MXFP8) {
-          ek = k.top(live4);
-          ev = v.top(live4);
-        }
-        if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.k_empty[st], use ^ 1u, abort, status, 1u)))) break;
-        if (lw == 0) {
-          Meta& meta = sm.meta[tile % kMeta];
-          if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-            float s4[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
-            uint32_t top = 0;
-            bool odd = false;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              if (y >= live4) s4[y] = 0.f;
-              const bool fine = isfinite(s4[y]);
-              if (!fine && 4 * lane + y >= from) {  // a drafted token
-                odd = true;
-                s4[y] = 0.f;
-              }
-              if (fine) top = max(top, __float_as_uint(s4[y]) & 0x7FFFFFFFu);
-            }
-            ev = max((int)(__reduce_max_sync(0xFFFFFFFFu, top) >> 23) - 127, -100);
-            if (__any_sync(0xFFFFFFFFu, odd) && lane == 0) sm.odd[number & 3u] = number;
-            *reinterpret_cast<float4*>(&meta.sk[4 * lane]) = sk4;
-            *reinterpret_cast<float4*>(&meta.sv[4 * lane]) = make_float4(s4[0], s4[1], s4[2], s4[3]);
-          }
-          uint32_t bal[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) bal[y] = __ballot_sync(0xFFFFFFFFu, y < live4);
-          if (lane == 0) {
-            meta.ek = ek;
-            meta.ev = KIND == BRC_STE_MXFP8 ? max(ev, 27) : ev;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) meta.live[y] = bal[y];
-            meta.all = (bal[0] & bal[1] & bal[2] & bal[3]) == 0xFFFFFFFFu;
-          }
-        }
-        k.template decode<false>(sm.k[st][0], first, lane, ek, dead, kTok);
+        v.template fetch<true>(a.c.v_data, a.c.v_scale, row, lane);
+        // (the scales' warp has waited for the key stage)
+        if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.meta_full[st], use, abort, status, 1u)))) break;
+        const int ek = sm.meta[tile % kMeta].ek, ev = sm.meta[tile % kMeta].ev;
+        k.template decode<false, false>(sm.k[st][0], first, lane, ek, dead, kTok);
         fence_proxy_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.k_full[st]);
         if (j + 1 < walk.s_end) {
           rows_of(j + 1);
-          k.fetch(a.c.k_data, a.c.k_scale, row, row4, lane);
-          scales();
+          k.template fetch<false>(a.c.k_data, a.c.k_scale, row, lane);
           pages_of(j + 2);
         }
         if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.v_empty[st], use ^ 1u, abort, status, 1u)))) break;
-        const int vref = max(ev, 27);  // no lower than 2^-100
         if (drafted) {
-          if (v.template decode<true>(sm.v[st][0], first, lane, vref, dead, from)) sm.odd[number & 3u] = number;
+          if (v.template decode<true, true>(sm.v[st][0], first, lane, ev, dead, from)) sm.odd[number & 3u] = number;
         } else {
-          v.template decode<false>(sm.v[st][0], first, lane, vref, dead, kTok);
+          v.template decode<false, true>(sm.v[st][0], first, lane, ev, dead, kTok);
         }
         fence_proxy_smem();
         __syncwarp();
@@ -820,6 +824,57 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     __syncwarp();
     uint32_t none = 0;
     mbar_wait(&sm.drain, 0u, &none, status, 1u);
+    } else if (warp == kSoftWarps + kLoadWarps + 1) {
+      // ============================================================== scales
+      uint32_t tile = 0;
+      bool ok = true;
+      for (; ok && walk.take(a); walk.next()) {
+        const Seq seq = walk.seq;
+        const int32_t* const table = a.table + walk.b * a.table_stride;
+        const int64_t head_row = (int64_t)walk.head * a.c.page_size;
+        Scales<KIND, D> k, v;
+        // pages a tile before the scales, scales a tile before they are needed
+        auto page_of = [&](int j) {
+          const int t = j * kTok + 4 * lane;
+          return j < walk.s_end && t < seq.total ? __ldg(table + (t >> a.page_shift)) : -1;
+        };
+        int page = page_of(walk.s_begin);
+        int64_t row = slot_of(a, page, head_row, walk.s_begin * kTok + 4 * lane);
+        k.fetch(a.c.k_scale, row);
+        v.fetch(a.c.v_scale, row);
+        page = page_of(walk.s_begin + 1);
+        for (int j = walk.s_begin; j < walk.s_end; ++j, ++tile) {
+          const uint32_t st = tile & 1u, use = (tile >> 1) & 1u;
+          const int left = (int)min((int64_t)kTok, seq.total - (int64_t)j * kTok) - 4 * lane;
+          const int live4 = row < 0 ? 0 : min(max(left, 0), 4);
+          int ek = 0, ev = 0;
+          if constexpr (KIND == BRC_STE_MXFP8) ek = k.top(live4);
+          if constexpr (KIND == BRC_STE_BLOCK_FP8) ev = v.top(live4);
+          if constexpr (KIND == BRC_STE_MXFP8) ev = max(v.top(live4), 27);  // no lower than 2^-100
+          if (!(ok = __all_sync(0xFFFFFFFFu,
+                                mbar_wait(&sm.k_empty[st], use ^ 1u, abort, status, 1u))))
+            break;
+          Meta& meta = sm.meta[tile % kMeta];
+          if constexpr (KIND == BRC_STE_BLOCK_FP8)
+            *reinterpret_cast<uint4*>(&meta.sk[4 * lane]) = k.e;
+          uint32_t bal[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) bal[y] = __ballot_sync(0xFFFFFFFFu, y < live4);
+          if (lane == 0) {
+            meta.ek = ek;
+            meta.ev = ev;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) meta.live[y] = bal[y];
+            meta.all = (bal[0] & bal[1] & bal[2] & bal[3]) == 0xFFFFFFFFu;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.meta_full[st]);
+          row = slot_of(a, page, head_row, (j + 1) * kTok + 4 * lane);
+          k.fetch(a.c.k_scale, row);
+          v.fetch(a.c.v_scale, row);
+          page = page_of(j + 2);
+        }
+      }
     }
   }
   tc_fence_before();
@@ -831,7 +886,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-static_assert(sizeof(Meta) % 16 == 0 && offsetof(Meta, sv) % 16 == 0, "16-byte accesses");
+static_assert(sizeof(Meta) % 16 == 0 && offsetof(Meta, sk) == 0, "16-byte accesses");
 static_assert(offsetof(Smem<128>, meta) % 16 == 0 && offsetof(Smem<128>, k) % 1024 == 0 &&
                   offsetof(Smem<128>, v) % 1024 == 0 && offsetof(Smem<64>, v) % 1024 == 0,
               "swizzled tiles");
