@@ -11,16 +11,23 @@ namespace {
 // four tiles to a warp (their accumulators take d / 4 registers each: two at d =
 // 256), then up to four row warps to a block.
 //
-// More rows than kTcRows go to the tensor-core kernel: 256 to a block.
+// More rows than tc_rows go to the tensor-core kernel: 256 to a block, its time nearly
+// the same up to that many. Both sides, 8 sequences of 16384 tokens, 8 cache heads (us,
+// register path / tensor cores), at the rows of a cache head:
+//                        32         48         64         72        128        256
+//   block FP8 d 128   115 / 227  184 / 227  188 / 229  320 / 231  338 / 239  597 / 283
+//   MXFP8 d 128       131 / 254  211 / 254  217 / 256  375 / 256  395 / 262  711 / 297
+//   NVFP4 d 128       119 / 168  193 / 170  199 / 172  340 / 174  359 / 180  637 / 219
+//   block FP8 d 64                          159 / 182  268 / 180  281 / 184
 struct Split {
   bool tc;
   int nt, row_warps, row_blocks, rows_per_block;
 };
-constexpr int kTcRows = 64;
+int tc_rows(const brc_kv_cache* c) { return c->kind == BRC_STE_BLOCK_FP8 ? 64 : 32; }
 Split split_rows(int rows, const brc_kv_cache* c) {
   const int d = c->head_dim;
   Split s{};
-  s.tc = rows > kTcRows && (d == 128 || (d == 64 && c->kind != BRC_STE_NVFP4));
+  s.tc = rows > tc_rows(c) && (d == 128 || (d == 64 && c->kind != BRC_STE_NVFP4));
   if (s.tc) {
     s.rows_per_block = 256;
     s.row_blocks = (rows + 255) / 256;

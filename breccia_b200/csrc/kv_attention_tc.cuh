@@ -2,18 +2,21 @@
 // quantised paged cache, on the 5th-generation tensor cores.
 //
 // The mathematics, the numbers and the split of the work are kv_attention.cuh's;
-// with more than kTcRows rows to a cache head the products bound it, not HBM.
+// with many rows to a cache head the products and the softmax bound it, not HBM.
 //
 // One block to an SM, two tiles of 128 query rows, tiles of 128 tokens:
 //   warps 0-15  softmax, two threads to a row, 64 columns each: scores from TMEM,
 //               probabilities back into the same TMEM columns as f16 (the A operand
 //               of P V). One thread to a row left the exponentials, the packing and
 //               the TMEM loads of its one warp per scheduler to run one after another
-//   warps 16-23 codes and scales from global memory, decoded to f16 in shared
+//   warps 16-23 codes and their scales from global memory, decoded to f16 in shared
 //               memory (128-byte swizzled rows; keys are K-major, values the same
 //               bytes read as MN-major); loads run one tile ahead in registers
 //   warp 24     issues tcgen05.mma: S = Q K^T and O += P V of each row tile in turn,
 //               so that one row tile's products run under the other's softmax
+//   warp 25     what a tile is relative to, which tokens are live and block FP8's key
+//               scales. Each of the warps that decode did this for itself before, and
+//               had no registers left for the loads ahead (MXFP8 525 -> 420 us)
 // TMEM: two score tiles and two output tiles of 128 columns. The codes are decoded
 // once for 256 rows, where the register path decodes them for every 32.
 //
@@ -40,10 +43,17 @@ constexpr int kTok = 128;
 constexpr int kRise = 6;  // log2 of how far a sum of 32 probabilities may pass 1
 constexpr int kSoftWarps = 16, kLoadWarps = 8;
 constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgroups: three warps idle
-// Registers of a thread after setmaxnreg, by warpgroup; 4 x softmax + 2 x loads +
-// products are no more than the 7 x 72 that the block was launched with.
-constexpr uint32_t kSoftRegs = 80, kLoadRegs = 72, kMmaRegs = 40;
-static_assert(4 * kSoftRegs + 2 * kLoadRegs + kMmaRegs <= 7 * 72, "registers of the launch");
+// Registers of a thread after setmaxnreg, by warpgroup; 4 x softmax + 2 x codes +
+// products are no more than the 7 x 72 that the block was launched with. Block FP8's
+// softmax, which holds the keys' scales too, takes them from the other warps (8 trees
+// of 64 nodes over 16384 tokens: 480 -> 452 us; MXFP8, whose codes need theirs, 410 ->
+// 426).
+template <int KIND>
+struct Regs {
+  static constexpr bool kBlock = KIND == BRC_STE_BLOCK_FP8;
+  static constexpr uint32_t kSoft = kBlock ? 88 : 80, kLoad = kBlock ? 56 : 64, kMma = kBlock ? 40 : 56;
+  static_assert(4 * kSoft + 2 * kLoad + kMma <= 7 * 72, "registers of the launch");
+};
 // A tile's Meta is written when the scores of the tile two before are done, so that the
 // softmax three before is over: a ring of four.
 constexpr int kMeta = 4;
@@ -365,7 +375,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
 
   if (warp < kSoftWarps) {
     // ================================================================ softmax
-    regs_inc<kSoftRegs>();
+    regs_inc<Regs<KIND>::kSoft>();
     const int r = warp >> 3, half = (warp >> 2) & 1;  // row tile; half of its columns
     const int mine = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes, in bits 16 ..
@@ -693,6 +703,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     }
   } else if (warp < kSoftWarps + kLoadWarps) {
     // ================================================================ codes
+    regs_dec<Regs<KIND>::kLoad>();
     const int lw = warp - kSoftWarps, first = kTok / kLoadWarps * lw;
     uint32_t tile = 0, number = 0;
     bool ok = true;
@@ -754,7 +765,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     }
   } else {
     // ================================================================ products
-    regs_dec<kMmaRegs>();
+    regs_dec<Regs<KIND>::kMma>();
     if (warp == kSoftWarps + kLoadWarps) {
     uint32_t tile = 0, q_phase = 0, p_phase[2] = {0, 0}, q_phase1 = 0;
     bool ok = true;
