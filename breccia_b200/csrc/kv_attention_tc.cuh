@@ -357,9 +357,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         mbar_init(&sm.v_full[i], kLoadWarps);
         mbar_init(&sm.k_empty[i], 1);
         mbar_init(&sm.v_empty[i], 1);
-        mbar_init(&sm.q_full[i], 256);
+        mbar_init(&sm.q_full[i], kSoftWarps / 2);
         mbar_init(&sm.s_full[i], 1);
-        mbar_init(&sm.p_full[i], 256);
+        mbar_init(&sm.p_full[i], kSoftWarps / 2);
         mbar_init(&sm.o_full[i], 1);
       }
       mbar_init(&sm.drain, 1);
@@ -435,7 +435,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           *reinterpret_cast<uint4*>(sm.q[r][i / 8] + mine * 128 + (((i & 7) ^ (mine & 7)) << 4)) = y;
         }
         fence_proxy_smem();
-        mbar_arrive(&sm.q_full[r]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[r]);
       }
       float m = -INFINITY, l = 0.f;
       int ev = -1000;
@@ -616,7 +617,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         l += part;
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&sm.p_full[r]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[r]);
       }
       if (!ok) break;
       // ---- the item's output
