@@ -1091,18 +1091,26 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
 
 // Join the parts of items that several blocks share: one warp to a query row,
 // the parts in the order of their tokens.
+// Warps that share a block's rows. Finding the parts of an item takes more
+// instructions than adding up a row of them, so a warp does it for 8 rows where a
+// block has 256 (the tensor-core kernel).
+__host__ __device__ __forceinline__ int join_units(const Args& a) {
+  return a.rows_per_block < 32 ? a.rows_per_block : 32;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
   const int lane = threadIdx.x & 31;
   const int64_t id = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int per_head = a.row_blocks * a.rows_per_block;
+  const int units = join_units(a), per_head = a.row_blocks * units;
   const int64_t per_b = (int64_t)a.c.heads * per_head;
   if (id >= per_b * a.batch) return;
   const int b = (int)(id / per_b);
   const int rest = (int)(id - b * per_b);
-  const int head = rest / per_head, row = rest - head * per_head;
-  if (row >= a.rows) return;
-  const int rb = row / a.rows_per_block, rr = row - rb * a.rows_per_block;
+  const int head = rest / per_head, unit = rest - head * per_head;
+  const int rb = unit / units, n_rows = a.rows_per_block / units;
+  const int first = (unit - rb * units) * n_rows;
+  if (rb * a.rows_per_block + first >= a.rows) return;
   const int per_seq = a.c.heads * a.row_blocks;
   Place p;
   locate(a, per_seq, blocks, 0, b, p);
@@ -1111,62 +1119,66 @@ __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
   const int64_t start = p.before * per_seq + (int64_t)(head * a.row_blocks + rb) * seq.steps;
   const int64_t c0 = start / p.share, c1 = (start + seq.steps - 1) / p.share;
   if (c0 == c1) return;
-  float m = -INFINITY;
-  for (int64_t c = c0 + lane; c <= c1; c += 32) {
-    const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
-    m = fmaxf(m, a.part_ml[(slot * a.rows_per_block + rr) * 2]);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  constexpr int N = D / 32;
-  float l = 0.f, o[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = 0.f;
-  for (int64_t base = c0; base <= c1; base += 32) {
-    const int64_t c = base + lane;
-    float f = 0.f, lp = 0.f;
-    if (c <= c1) {
+  for (int rr = first; rr < first + n_rows; ++rr) {
+    const int row = rb * a.rows_per_block + rr;
+    if (row >= a.rows) return;
+    float m = -INFINITY;
+    for (int64_t c = c0 + lane; c <= c1; c += 32) {
       const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot * a.rows_per_block + rr) * 2);
-      f = m == -INFINITY ? 1.f : ex2(ml.x - m);
-      lp = ml.y * f;
+      m = fmaxf(m, a.part_ml[(slot * a.rows_per_block + rr) * 2]);
     }
-    const int n = (int)min((int64_t)32, c1 - base + 1);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    constexpr int N = D / 32;
+    float l = 0.f, o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = 0.f;
+    for (int64_t base = c0; base <= c1; base += 32) {
+      const int64_t c = base + lane;
+      float f = 0.f, lp = 0.f;
+      if (c <= c1) {
+        const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot * a.rows_per_block + rr) * 2);
+        f = m == -INFINITY ? 1.f : ex2(ml.x - m);
+        lp = ml.y * f;
+      }
+      const int n = (int)min((int64_t)32, c1 - base + 1);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float fi = __shfl_sync(0xFFFFFFFFu, f, i);
-      l += __shfl_sync(0xFFFFFFFFu, lp, i);
-      const int64_t ci = base + i, slot = 2 * ci + (ci == c0 ? 1 : 0);
-      const float* y = a.part_o + (slot * a.rows_per_block + rr) * D + lane * N;
+      for (int i = 0; i < n; ++i) {
+        const float fi = __shfl_sync(0xFFFFFFFFu, f, i);
+        l += __shfl_sync(0xFFFFFFFFu, lp, i);
+        const int64_t ci = base + i, slot = 2 * ci + (ci == c0 ? 1 : 0);
+        const float* y = a.part_o + (slot * a.rows_per_block + rr) * D + lane * N;
 #pragma unroll
-      for (int j = 0; j < N; ++j) o[j] += fi * y[j];
-    }
-  }
-  const int nd = row / a.group;
-  const int64_t at = ((int64_t)b * a.draft + nd) * a.hq + head * a.group + (row - nd * a.group);
-  const bool none = nd >= seq.drafts || l == 0.f;
-  const float inv = none ? 0.f : 1.f / l;
-#pragma unroll
-  for (int j = 0; j < N; j += 2) {
-    uint32_t y = 0;
-    if (!none) {
-      if (a.q_f16) {
-        y = half2_of(o[j] * inv, o[j + 1] * inv);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(o[j] * inv, o[j + 1] * inv);
-        y = *reinterpret_cast<const uint32_t*>(&h);
+        for (int j = 0; j < N; ++j) o[j] += fi * y[j];
       }
     }
-    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + lane * N + j) = y;
+    const int nd = row / a.group;
+    const int64_t at = ((int64_t)b * a.draft + nd) * a.hq + head * a.group + (row - nd * a.group);
+    const bool none = nd >= seq.drafts || l == 0.f;
+    const float inv = none ? 0.f : 1.f / l;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      uint32_t y = 0;
+      if (!none) {
+        if (a.q_f16) {
+          y = half2_of(o[j] * inv, o[j + 1] * inv);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(o[j] * inv, o[j + 1] * inv);
+          y = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + lane * N + j) = y;
+    }
+    if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
-  if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ host
 // The join's blocks start, and find their places, while the last parts are written.
 template <int D>
 int launch_join(const Args& a, int blocks, cudaStream_t st) {
-  const int64_t warps = (int64_t)a.batch * a.c.heads * a.row_blocks * a.rows_per_block;
+  const int64_t warps = (int64_t)a.batch * a.c.heads * a.row_blocks * join_units(a);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((warps + kWarps - 1) / kWarps));
   cfg.blockDim = dim3(kThreads);
