@@ -1089,28 +1089,28 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
   }
 }
 
-// Join the parts of items that several blocks share: one warp to a query row,
-// the parts in the order of their tokens.
-// Warps that share a block's rows. Finding the parts of an item takes more
-// instructions than adding up a row of them, so a warp does it for 8 rows where a
-// block has 256 (the tensor-core kernel).
-__host__ __device__ __forceinline__ int join_units(const Args& a) {
-  return a.rows_per_block < 32 ? a.rows_per_block : 32;
+// Join the parts of items that several blocks share, in the order of their tokens. A
+// warp takes the R rows of one block: finding an item's parts takes more instructions
+// than adding up a row of them, and the rows' loads are in flight together (8 trees of
+// 64 nodes over 16384 tokens, caches cold: one row to a warp 36 us, eight one by one
+// 29, eight together 20).
+__host__ __device__ __forceinline__ int join_rows(int rows_per_block) {
+  return rows_per_block <= 32 ? 1 : rows_per_block / 32;
 }
 
-template <int D>
+template <int D, int R>
 __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
   const int lane = threadIdx.x & 31;
   const int64_t id = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int units = join_units(a), per_head = a.row_blocks * units;
+  const int units = a.rows_per_block / R, per_head = a.row_blocks * units;
   const int64_t per_b = (int64_t)a.c.heads * per_head;
   if (id >= per_b * a.batch) return;
   const int b = (int)(id / per_b);
   const int rest = (int)(id - b * per_b);
   const int head = rest / per_head, unit = rest - head * per_head;
-  const int rb = unit / units, n_rows = a.rows_per_block / units;
-  const int first = (unit - rb * units) * n_rows;
-  if (rb * a.rows_per_block + first >= a.rows) return;
+  const int rb = unit / units, first = (unit - rb * units) * R;
+  const int row0 = rb * a.rows_per_block + first;
+  if (row0 >= a.rows) return;
   const int per_seq = a.c.heads * a.row_blocks;
   Place p;
   locate(a, per_seq, blocks, 0, b, p);
@@ -1119,66 +1119,91 @@ __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
   const int64_t start = p.before * per_seq + (int64_t)(head * a.row_blocks + rb) * seq.steps;
   const int64_t c0 = start / p.share, c1 = (start + seq.steps - 1) / p.share;
   if (c0 == c1) return;
-  for (int rr = first; rr < first + n_rows; ++rr) {
-    const int row = rb * a.rows_per_block + rr;
-    if (row >= a.rows) return;
-    float m = -INFINITY;
-    for (int64_t c = c0 + lane; c <= c1; c += 32) {
-      const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
-      m = fmaxf(m, a.part_ml[(slot * a.rows_per_block + rr) * 2]);
-    }
+  // (rows past a.rows are read, as there is room for them, and not written)
+  auto part = [&](int64_t c) {
+    return (2 * c + (c == c0 ? 1 : 0)) * a.rows_per_block + first;
+  };
+  float m[R];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    constexpr int N = D / 32;
-    float l = 0.f, o[N];
+  for (int y = 0; y < R; ++y) m[y] = -INFINITY;
+  for (int64_t c = c0 + lane; c <= c1; c += 32) {
+    const float* const ml = a.part_ml + part(c) * 2;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = 0.f;
-    for (int64_t base = c0; base <= c1; base += 32) {
-      const int64_t c = base + lane;
-      float f = 0.f, lp = 0.f;
+    for (int y = 0; y < R; ++y) m[y] = fmaxf(m[y], ml[2 * y]);
+  }
+#pragma unroll
+  for (int y = 0; y < R; ++y)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m[y] = fmaxf(m[y], __shfl_xor_sync(0xFFFFFFFFu, m[y], o));
+  constexpr int N = D / 32;
+  float l[R], o[R][N];
+#pragma unroll
+  for (int y = 0; y < R; ++y) {
+    l[y] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[y][i] = 0.f;
+  }
+  for (int64_t base = c0; base <= c1; base += 32) {
+    const int64_t c = base + lane;
+    float f[R], lp[R];
+#pragma unroll
+    for (int y = 0; y < R; ++y) {
+      f[y] = lp[y] = 0.f;
       if (c <= c1) {
-        const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot * a.rows_per_block + rr) * 2);
-        f = m == -INFINITY ? 1.f : ex2(ml.x - m);
-        lp = ml.y * f;
-      }
-      const int n = (int)min((int64_t)32, c1 - base + 1);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float fi = __shfl_sync(0xFFFFFFFFu, f, i);
-        l += __shfl_sync(0xFFFFFFFFu, lp, i);
-        const int64_t ci = base + i, slot = 2 * ci + (ci == c0 ? 1 : 0);
-        const float* y = a.part_o + (slot * a.rows_per_block + rr) * D + lane * N;
-#pragma unroll
-        for (int j = 0; j < N; ++j) o[j] += fi * y[j];
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (part(c) + y) * 2);
+        f[y] = m[y] == -INFINITY ? 1.f : ex2(ml.x - m[y]);
+        lp[y] = ml.y * f[y];
       }
     }
+    const int n = (int)min((int64_t)32, c1 - base + 1);
+#pragma unroll(R > 2 ? 1 : 4)
+    for (int i = 0; i < n; ++i) {
+      const float* const x = a.part_o + part(base + i) * D + lane * N;
+      float v[R][N];
+#pragma unroll
+      for (int y = 0; y < R; ++y)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[y][j] = x[y * D + j];
+#pragma unroll
+      for (int y = 0; y < R; ++y) {
+        const float fi = __shfl_sync(0xFFFFFFFFu, f[y], i);
+        l[y] += __shfl_sync(0xFFFFFFFFu, lp[y], i);
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[y][j] += fi * v[y][j];
+      }
+    }
+  }
+#pragma unroll
+  for (int y = 0; y < R; ++y) {
+    const int row = row0 + y;
+    if (row >= a.rows) return;
     const int nd = row / a.group;
     const int64_t at = ((int64_t)b * a.draft + nd) * a.hq + head * a.group + (row - nd * a.group);
-    const bool none = nd >= seq.drafts || l == 0.f;
-    const float inv = none ? 0.f : 1.f / l;
+    const bool none = nd >= seq.drafts || l[y] == 0.f;
+    const float inv = none ? 0.f : 1.f / l[y];
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
-      uint32_t y = 0;
+      uint32_t w = 0;
       if (!none) {
         if (a.q_f16) {
-          y = half2_of(o[j] * inv, o[j + 1] * inv);
+          w = half2_of(o[y][j] * inv, o[y][j + 1] * inv);
         } else {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(o[j] * inv, o[j + 1] * inv);
-          y = *reinterpret_cast<const uint32_t*>(&h);
+          const __nv_bfloat162 h = __floats2bfloat162_rn(o[y][j] * inv, o[y][j + 1] * inv);
+          w = *reinterpret_cast<const uint32_t*>(&h);
         }
       }
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + lane * N + j) = y;
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + lane * N + j) = w;
     }
-    if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    if (a.lse && lane == 0)
+      a.lse[at] = none ? -INFINITY : (m[y] + log2f(l[y])) * 0.6931471805599453f;
   }
 }
 
 // ------------------------------------------------------------------ host
 // The join's blocks start, and find their places, while the last parts are written.
-template <int D>
-int launch_join(const Args& a, int blocks, cudaStream_t st) {
-  const int64_t warps = (int64_t)a.batch * a.c.heads * a.row_blocks * join_units(a);
+template <int D, int R>
+int launch_join_rows(const Args& a, int blocks, cudaStream_t st) {
+  const int64_t warps = (int64_t)a.batch * a.c.heads * a.row_blocks * (a.rows_per_block / R);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((warps + kWarps - 1) / kWarps));
   cfg.blockDim = dim3(kThreads);
@@ -1188,7 +1213,16 @@ int launch_join(const Args& a, int blocks, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, k_join<D>, a, blocks));
+  return check_cuda(cudaLaunchKernelEx(&cfg, k_join<D, R>, a, blocks));
+}
+template <int D>
+int launch_join(const Args& a, int blocks, cudaStream_t st) {
+  switch (join_rows(a.rows_per_block)) {
+    case 1: return launch_join_rows<D, 1>(a, blocks, st);
+    case 2: return launch_join_rows<D, 2>(a, blocks, st);
+    case 4: return launch_join_rows<D, 4>(a, blocks, st);
+    default: return launch_join_rows<D, 8>(a, blocks, st);
+  }
 }
 
 template <int KIND, int FMT, int D, int NT>
