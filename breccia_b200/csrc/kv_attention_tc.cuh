@@ -42,7 +42,7 @@ using namespace sm100;
 constexpr int kTok = 128;
 constexpr int kRise = 6;  // log2 of how far a sum of 32 probabilities may pass 1
 constexpr int kSoftWarps = 16, kLoadWarps = 8;
-constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgroups: three warps idle
+constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgroups: two warps idle
 // Registers of a thread after setmaxnreg, by warpgroup; 4 x softmax + 2 x codes +
 // products are no more than the 7 x 72 that the block was launched with. Block FP8's
 // softmax, which holds the keys' scales too, takes them from the other warps (8 trees
