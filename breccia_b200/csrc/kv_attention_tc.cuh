@@ -449,7 +449,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         tc_fence_after();
         const Meta& meta = sm.meta[(tile0 + (j - walk.s_begin)) % kMeta];
         const int64_t t0 = (int64_t)j * kTok;
-        const float f = KIND == BRC_STE_MXFP8 ? rowf * e8m0_value(meta.ek) : rowf;
+        // (a factor of zero, of a scale of zero or by underflow, would make NaN of the
+        // hidden places' minus infinity; a score, below 2^40, times 2^-126 is nothing)
+        float f = KIND == BRC_STE_MXFP8 ? rowf * e8m0_value(meta.ek) : rowf;
+        if (f < 0x1p-126f) f = 0x1p-126f;
         const bool masked = t0 + kTok > seq.context || !meta.all;
         uint32_t vis[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
         if (masked) {

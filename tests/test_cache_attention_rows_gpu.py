@@ -1,0 +1,160 @@
+"""cache_attention with row counts of a cache head on both sides of every choice
+that the entry point makes from them: the special cases of
+test_cache_attention_gpu.py with 24 rows, with 72 (more than any recipe keeps on
+the register path) and with 300 (two blocks of rows).
+
+The reference is 64 bits on the values that the cache holds; a mask says place by
+place what a row sees. Tolerances, from the kernels' own roundings. A score is a
+float32 sum of d products, off by at most d 2^-24 of the sum of magnitudes (S: the
+largest among the places that the row sees). A probability is off by that much
+relatively, by the exponential's 2^-21, and by one rounding to f16: 2^-11 of it or,
+below f16's normal numbers, 2^-31 of the row's largest (2^-24 on the register path of
+block FP8, where it carries a scale that may lie 2^7 below the reference). Values on
+tcgen05 in block FP8 are rounded to f16 once more: 2^-11 of them or, for E5M2's
+smallest codes, 2^-24 of the token's largest. Sums are float32. So an output is within
+
+    (2^-10 + 2 d 2^-24 S) sum p |v| + 2^-24 sum p max |v| + f max p sum |v|
+
+of the formula (f: 2^-31 or 2^-24), and half an ulp of its type; log-sum-exp is within
+d 2^-24 S + 2^-20 (1 + |lse|).
+"""
+
+import math
+
+import pytest
+import torch
+
+from test_cache_attention_gpu import HALF_ULP, RECIPES, Case, bb
+
+pytestmark = pytest.mark.gpu
+
+ROWS = [(6, 4), (18, 4), (75, 4)]  # draft, group: 24, 72, 300 rows
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _needs_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def causal(c):
+    """What every row sees, (draft, context + draft) for each sequence."""
+    t = c.draft
+    tri = torch.ones(t, t, dtype=torch.bool, device="cuda").tril()
+    return [torch.cat([tri.new_ones(t, n), tri], 1) for n in c.ctx]
+
+
+def with_tree(c, tree):
+    return [torch.cat([tree.new_ones(c.draft, n), tree[b] if tree.ndim == 3 else tree], 1)
+            for b, n in enumerate(c.ctx)]
+
+
+def rewrite(c, b, first, k=None, v=None):
+    """Put other keys or values at the places from `first` on of sequence b."""
+    page = c.cache.page_size
+    n = (k if k is not None else v).shape[0]
+    t = torch.arange(first, first + n, device="cuda")
+    at = c.table[b].long()[t // page], t % page
+    kk, vv = (x[b, first:first + n] for x in held(c))
+    old = [buf[at[0], :, at[1]].clone() for buf in c.cache._buffers]
+    c.cache.write(kk if k is None else k, vv if v is None else v, at[0] * page + at[1])
+    for side, given in ((0, k), (2, v)):  # the side that stays keeps its codes and scales
+        if given is None:
+            for i in (side, side + 1):
+                c.cache._buffers[i][at[0], :, at[1]] = old[i]
+
+
+def held(c, dtype=torch.float32):
+    return c.cache.read(c.table, c.context + c.draft, max(c.ctx) + c.draft, dtype)
+
+
+def verify(c, got, see, scale=None, columns=None, rows=None):
+    """Rows (all, or those of the mask (batch, draft)) and columns against the formula."""
+    out, lse = got
+    scale = c.d ** -0.5 if scale is None else scale
+    block = c.cache.recipe.name == "block"
+    floor = 2.0 ** (-24 if block and (c.draft * c.group <= 64 or c.d == 256) else -31)
+    k, v = held(c)
+    for b, m in enumerate(see):
+        n = m.shape[1]
+        kk, vv = (x[b, :n].double().repeat_interleave(c.group, 1).transpose(0, 1) for x in (k, v))
+        q = c.q[b].double().transpose(0, 1)
+        s = (q @ kk.transpose(1, 2) * scale).masked_fill(~m, -math.inf)
+        big = (q.abs() @ kk.abs().transpose(1, 2) * abs(scale)).masked_fill(~m, 0).amax(-1)
+        want_lse = torch.logsumexp(s, -1)
+        p = torch.exp(s - want_lse[..., None].nan_to_num(neginf=0.0))
+        # values that nobody sees may be anything
+        whole = torch.where(m.any(0)[None, :, None], vv, torch.zeros_like(vv))
+        vv = whole if columns is None else whole[..., columns]
+        want, mass = p @ vv, p @ vv.abs()
+        largest = p @ whole.abs().amax(-1, keepdim=True)
+        low = p.amax(-1, keepdim=True) * (m.double() @ vv.abs())
+        o, l = out[b].double().transpose(0, 1), lse[b].double().transpose(0, 1)
+        if columns is not None:
+            o = o[..., columns]
+        keep = torch.ones_like(m[:, 0]) if rows is None else rows[b]
+        none = ~m.any(1)
+        assert not o[:, none].any() and bool((l[:, none] == -math.inf).all())
+        keep = keep & ~none
+        tol = (2.0 ** -10 + 2 * c.d * 2.0 ** -24 * big[..., None]) * mass + \
+            HALF_ULP[out.dtype] * want.abs() + 2.0 ** -24 + 2.0 ** -24 * largest + floor * low
+        err = (o - want).abs()
+        assert bool((err <= tol)[:, keep].all()), (b, float((err / tol)[:, keep].nan_to_num(nan=math.inf).max()))
+        ltol = d_tol(c.d, big, want_lse)
+        lerr = (l - want_lse).abs()
+        assert bool((lerr <= ltol)[:, keep].all()), (b, float((lerr - ltol)[:, keep].nan_to_num(nan=math.inf).max()))
+
+
+def d_tol(d, big, lse):
+    return d * 2.0 ** -24 * big + 2.0 ** -20 * (1 + lse.abs())
+
+
+# ------------------------------------------------------------------ factors
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("draft,group", ROWS)
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+def test_scales(name, d, draft, group, scale):
+    c = Case(name, d, 1, group, [300, 2], draft, seed=21)
+    verify(c, c.run(scale=scale), causal(c), scale)
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_zero_and_tiny_queries_over_tiny_keys(name, draft, group):
+    c = Case(name, 128, 1, group, [200, 3], draft, seed=22)
+    g = torch.Generator().manual_seed(22)
+    for b, n in enumerate(c.ctx):
+        rewrite(c, b, 0, k=(1e-9 * torch.randn(n + draft, 1, 128, generator=g)).cuda())
+    c.q[:, 0] = 0
+    c.q[:, 1] *= 2.0 ** -40
+    verify(c, c.run(), causal(c))
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_cache_as_the_constructor_leaves_it(name, draft, group):
+    cache = Case(name, 128, 2, group, [1], draft, seed=23).cache
+    for buf in cache._buffers:
+        buf.zero_()
+    g = torch.Generator().manual_seed(23)
+    q = torch.randn(1, draft, 2 * group, 128, generator=g).to(torch.bfloat16).cuda()
+    q[:, 1] *= 2.0 ** -30
+    table = torch.zeros(1, 20, dtype=torch.int32, device="cuda")
+    n = torch.tensor([200], dtype=torch.int32, device="cuda")
+    out, lse = bb().cache_attention(q, cache, table, n, return_lse=True)
+    want = torch.log(201.0 + torch.arange(draft, device="cuda"))[:, None].expand(draft, 2 * group)
+    assert not out.any()
+    assert float((lse[0] - want).abs().max()) <= 2.0 ** -20 * (1 + math.log(300))
+
+
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_large_queries(draft, group):
+    c = Case("mx4", 128, 1, group, [150, 2], draft, seed=24)
+    c.q[0] *= 2.0 ** 60
+    got = c.run(scale=2.0 ** -60)
+    ref = Case("mx4", 128, 1, group, [150, 2], draft, seed=24)
+    want = ref.run(scale=1.0)
+    assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[1][0], want[1][0])
