@@ -577,10 +577,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           reg_bind32(x);
           take(x, c, u);
           float2 t = exps(u);
-          // a score far above the shift shows in the sum (a row that has seen
-          // nothing has the shift 0)
+          // a score far above the shift shows in the sum; a row that has seen nothing so
+          // far has the shift 0, below which its scores may vanish: it always looks
           const float all = t.x + t.y;
-          if (__any_sync(0xFFFFFFFFu, all > most || (own == -INFINITY && all > 0.f))) {
+          const bool sees = !masked || (c ? vis[1] : vis[0]) != 0u;
+          if (__any_sync(0xFFFFFFFFu, all > most || (own == -INFINITY && sees))) {
             tmem_ld32(sc + 32 * c, x);
             tmem_ld_wait();
             reg_bind32(x);

@@ -158,3 +158,43 @@ def test_large_queries(draft, group):
     ref = Case("mx4", 128, 1, group, [150, 2], draft, seed=24)
     want = ref.run(scale=1.0)
     assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[1][0], want[1][0])
+
+
+# ------------------------------------------------------------------ masks
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", ROWS)
+@pytest.mark.parametrize("low", [-200.0, -90.0, 3.0])
+def test_first_pages_outside_the_cache_and_low_scores(name, draft, group, low):
+    """A share that begins in pages that nobody sees, over scores far below zero."""
+    c = Case(name, 128, 1, group, [330, 200], draft, page=64, seed=31)
+    g = torch.Generator().manual_seed(32)
+    for b, n in enumerate(c.ctx):
+        k = 1 + 0.05 * torch.randn(n + draft, 1, 128, generator=g)
+        rewrite(c, b, 0, k=k.cuda())
+    c.q.copy_((1 + 0.05 * torch.randn(c.q.shape, generator=g)) * (low / 128))
+    see = causal(c)
+    for b, pages in enumerate(([0, 1], [0, 1, 2])):
+        for page in pages:
+            c.table[b, page] = [-1, c.cache.num_pages][page % 2]
+            see[b][:, page * 64:page * 64 + 64] = False
+    verify(c, c.run(scale=1.0), see, 1.0)
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", [(300, 1), (140, 2)])
+@pytest.mark.parametrize("ctx", [0, 5])
+def test_trees_of_separate_blocks(name, draft, group, ctx):
+    """Drafted tokens over several tiles, of which a row sees those of its own block."""
+    c = Case(name, 128, 1, group, [ctx], draft, seed=33)
+    g = torch.Generator().manual_seed(34)
+    k = 1 + 0.05 * torch.randn(ctx + draft, 1, 128, generator=g)
+    rewrite(c, 0, 0, k=k.cuda())
+    c.q.copy_((1 + 0.05 * torch.randn(c.q.shape, generator=g)) * (-200 / 128))
+    block = torch.arange(draft, device="cuda") // 70
+    tree = (block[:, None] == block[None]).tril()
+    tree[3] = False
+    see = with_tree(c, tree)
+    see[0][draft // 2:, :ctx] = True
+    verify(c, c.run(scale=1.0, tree_mask=tree), see, 1.0)
