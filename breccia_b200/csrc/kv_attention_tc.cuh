@@ -150,6 +150,15 @@ struct Walk {
 template <int FMT>
 constexpr int kValueLift = FMT == BRC_FP8_E4M3 ? 6 : -1;
 
+// Zero the codes of a word that stand for something not finite; true if there was one.
+template <int FMT>
+__device__ __forceinline__ bool clear_odd(uint32_t& w) {
+  const uint32_t odd = FMT == BRC_FP8_E4M3 ? ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u
+                                           : ((w & 0x7C7C7C7Cu) + 0x04040404u) & 0x80808080u;
+  w &= ~((odd >> 7) * 0xFFu);
+  return odd != 0u;
+}
+
 // A warp decodes 16 of a tile's tokens: lane (t, c) reads token 8 g + t, piece 4 i
 // + c, for g < 2 and i < kHalves.
 template <int KIND, int FMT, int D>
@@ -188,8 +197,9 @@ struct Loader {
       }
   }
   // Decode into a stage. `first`: token of the warp's first row; rows from `dead`
-  // on hold anything and become zero. ODD: drafted tokens (from `drafted` on) that
-  // hold something not finite become zero too; returns whether there was one. VALUES:
+  // on hold anything and become zero. ODD: of drafted tokens (from `drafted` on), what
+  // is not finite becomes zero too, code by code or scale by scale; returns whether
+  // there was any (the epilogue adds it to the rows that see it). VALUES:
   // of block FP8 times scale * 2^(kValueLift - ref), which rounds them to f16 once (as
   // the probabilities are). That factor on the probabilities instead, as on the scores,
   // has every softmax thread read every token's from shared memory, 16 bytes to each
@@ -208,15 +218,20 @@ struct Loader {
         bool zero = t >= dead;
         if constexpr (ODD) {
           if (t >= drafted && !zero) {
-            bool odd = false;
+            if constexpr (KIND == BRC_STE_NVFP4) {  // a scale of 16 elements each
 #pragma unroll
-            for (int y = 0; y < 4; ++y) odd |= odd_codes<KIND, FMT>(x[y]);
-            if constexpr (KIND == BRC_STE_MXFP8) odd |= s[g][i] == 255u;
-            if constexpr (KIND == BRC_STE_BLOCK_FP8) odd |= !isfinite(__uint_as_float(s[g][i]));
-            if constexpr (KIND == BRC_STE_NVFP4)
-              odd |= (s[g][i] & 0x7Fu) == 0x7Fu || (s[g][i] & 0x7F00u) == 0x7F00u;
-            any |= odd;
-            zero |= odd;
+              for (int y = 0; y < 16; y += 8)
+                if (((s[g][i] >> y) & 0x7Fu) == 0x7Fu) {
+                  s[g][i] &= 0xFF00u >> y;
+                  any = true;
+                }
+            } else {
+              if constexpr (KIND == BRC_STE_MXFP8) zero = s[g][i] == 255u;
+              else zero = !isfinite(__uint_as_float(s[g][i]));
+              any |= zero;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) any |= clear_odd<FMT>(x[y]);
+            }
           }
         }
         if (zero) x[0] = x[1] = x[2] = x[3] = s[g][i] = 0u;

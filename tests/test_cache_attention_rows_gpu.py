@@ -198,3 +198,81 @@ def test_trees_of_separate_blocks(name, draft, group, ctx):
     see = with_tree(c, tree)
     see[0][draft // 2:, :ctx] = True
     verify(c, c.run(scale=1.0, tree_mask=tree), see, 1.0)
+
+
+# ------------------------------------------------------------------ what is not finite
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", ROWS)
+@pytest.mark.parametrize("ctx", [21, 250])
+def test_unseen_nan(name, draft, group, ctx):
+    """NaN behind the end of a page, in other pages and in drafted tokens that a row
+    does not see; rows that see a drafted NaN get it, and where values are NaN only
+    in those columns."""
+    d = 128
+    c = Case(name, d, 2, group, [ctx, 40], draft, seed=37)
+    tree = torch.eye(draft, dtype=torch.bool, device="cuda").repeat(2, 1, 1)
+    tree[:, :, 0] = True
+    tree[:, 0, :] = False
+    tree[:, 4:, 3] = (torch.arange(4, draft, device="cuda") % 2 == 0)
+    see = with_tree(c, tree)
+    want = c.run(tree_mask=tree)
+    verify(c, want, see)
+    live = torch.zeros(c.cache.num_pages, c.cache.page_size, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(c.ctx):
+        t = torch.arange(n + draft, device="cuda")
+        live[c.table[b].long()[t // 16], t % 16] = True
+    for buf in c.cache._buffers:
+        buf[(~live)[:, None, :, None].expand_as(buf)] = float("nan") if buf.dtype == torch.float32 else 255
+    got = c.run(tree_mask=tree)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    seeing = tree[0, :, 3]
+    rows = torch.stack([~seeing, torch.ones_like(seeing)])
+    page, at = int(c.table[0, (ctx + 3) // 16]), (ctx + 3) % 16
+    for side in ("k", "v"):
+        data, scale = getattr(c.cache, side + "_data"), getattr(c.cache, side + "_scale")
+        keep = data[page, :, at].clone(), scale[page, :, at].clone()
+        data[page, :, at] = 255
+        scale[page, :, at] = float("nan") if scale.dtype == torch.float32 else 255
+        out, lse = c.run(tree_mask=tree)
+        assert torch.isnan(out[0, seeing]).all()
+        data[page, :, at], scale[page, :, at] = keep
+        verify(c, (out, lse), see, rows=rows)
+    # some of a token's values only
+    if name == "nvfp4":
+        c.cache.v_scale[page, 1, at, 3] = 0x7F
+        bad = torch.arange(48, 64, device="cuda")
+    elif name.startswith("mx"):
+        c.cache.v_data[page, 1, at, 77] = 255
+        c.cache.v_data[page, 1, at, 78] = 127
+        bad = torch.tensor([77, 78], device="cuda")
+    else:
+        c.cache.v_data[page, 1, at, 3] = 255
+        bad = torch.tensor([3], device="cuda")
+    out, lse = c.run(tree_mask=tree)
+    odd = torch.zeros_like(out, dtype=torch.bool)
+    odd[0, :, group:] = seeing[:, None, None] & torch.isin(torch.arange(d, device="cuda"), bad)
+    assert torch.equal(torch.isnan(out), odd)
+    fine = torch.tensor([i for i in range(d) if i not in bad.tolist()], device="cuda")
+    if name == "nvfp4":
+        c.cache.v_scale[page, 1, at, 3] = 0
+    else:
+        c.cache.v_data[page, 1, at, bad] = 0
+    verify(c, (out, lse), see, columns=fine)
+
+
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_infinite_values(draft, group):
+    """E5M2 holds infinities: a row that sees one gets it in that column."""
+    c = Case("mx5", 128, 1, group, [140], draft, seed=38)
+    at = 140 + 2
+    page, place = int(c.table[0, at // 16]), at % 16
+    c.cache.v_data[page, 0, place, 5] = 0x7C
+    c.cache.v_data[page, 0, place, 6] = 0xFC
+    out, lse = c.run()
+    c.cache.v_data[page, 0, place, 5:7] = 0
+    assert bool((out[0, 2:, :, 5] == math.inf).all()) and bool((out[0, 2:, :, 6] == -math.inf).all())
+    assert torch.isfinite(out[0, :2]).all()
+    fine = torch.tensor([i for i in range(128) if i not in (5, 6)], device="cuda")
+    verify(c, (out, lse), causal(c), columns=fine)
