@@ -50,6 +50,10 @@ namespace kvatt {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr float kGrow = 8.f;  // a row's shift follows its maximum when it is this far (log2) behind
+// Sums of p v carry the factor 2^-kSumDown until they are divided by the sum of p, which
+// may be as large as 2^kGrow for each token: values up to the largest float do not overflow.
+constexpr int kSumDown = 30;
+constexpr float kSumUp = 1 << kSumDown;
 
 struct Args {
   brc_kv_cache c;
@@ -66,7 +70,7 @@ struct Args {
   float scale_log2;
   void* out;
   float* lse;
-  float* part_o;   // (2 * blocks, rows per block, d)
+  float* part_o;   // (2 * blocks, rows per block, d): sums of p v
   float* part_ml;  // (2 * blocks, rows per block, 2)
   int row_warps, row_blocks, rows_per_block, min_share;
 };
@@ -1016,7 +1020,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
         }
       }
     __syncthreads();  // the stages are no longer read
-    const float scale_o = w.e < -900 ? 1.f : exp2f((float)(w.e - 6));
+    const float scale_o = w.e < -900 ? 1.f : exp2f((float)(w.e - 6 - kSumDown));
     constexpr int kPitch = D + 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -1055,7 +1059,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
         const int64_t at_row =
             ((int64_t)b * a.draft + nd) * a.hq + head * a.group + (row - nd * a.group);
         const bool none = nd >= seq.drafts || l == 0.f;
-        const float inv = none ? 0.f : 1.f / l;
+        const float inv = none ? 0.f : kSumUp / l;
         uint2 y;
         if (none) {
           y = make_uint2(0u, 0u);
@@ -1180,7 +1184,7 @@ __global__ void __launch_bounds__(kThreads) k_join(Args a, int blocks) {
     const int nd = row / a.group;
     const int64_t at = ((int64_t)b * a.draft + nd) * a.hq + head * a.group + (row - nd * a.group);
     const bool none = nd >= seq.drafts || l[y] == 0.f;
-    const float inv = none ? 0.f : 1.f / l[y];
+    const float inv = none ? 0.f : kSumUp / l[y];
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       uint32_t w = 0;

@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
                        : ev < -900 ? 1.f
                                    : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : kValueLift<FMT>) - 5));
       const bool none = !valid || l == 0.f;
-      const float mul = whole ? (none ? 0.f : so / l) : so;
+      const float mul = whole ? (none ? 0.f : so / l) : so * (1.f / kSumUp);
       const bool odd = sm.odd[number & 3u] == number && !none;
       const int64_t slot = 2 * (int64_t)blockIdx.x + (walk.s_begin > 0 ? 0 : 1);
       const int rr = r * 128 + mine;

@@ -276,3 +276,17 @@ def test_infinite_values(draft, group):
     assert torch.isfinite(out[0, :2]).all()
     fine = torch.tensor([i for i in range(128) if i not in (5, 6)], device="cuda")
     verify(c, (out, lse), causal(c), columns=fine)
+
+
+# ------------------------------------------------------------------ magnitudes
+
+
+@pytest.mark.parametrize("name", ["block4", "block5", "mx4", "mx5"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_values_near_the_largest_float(name, d, draft, group):
+    c = Case(name, d, 1, group, [1500, 20], draft, seed=42)
+    for b, n in enumerate(c.ctx):
+        v = torch.randn(n + draft, 1, d, generator=torch.Generator().manual_seed(43)).clamp(-3, 3) * 1e38
+        rewrite(c, b, 0, v=v.cuda())
+    verify(c, c.run(), causal(c))
