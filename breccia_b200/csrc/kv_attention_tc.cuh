@@ -40,7 +40,11 @@ using namespace kvatt;
 using namespace sm100;
 
 constexpr int kTok = 128;
-constexpr int kRise = 6;  // log2 of how far a sum of 32 probabilities may pass 1
+constexpr int kLift = 9;  // log2 of the factor that probabilities carry in f16
+constexpr int kRise = 6;  // log2 of how far a sum of 32 of them may pass it
+// Values are relative to the largest scale of their item's tiles so far, and this much
+// (log2) above it, so that it seldom rises.
+constexpr int kSlack = 2;
 constexpr int kSoftWarps = 16, kLoadWarps = 8;
 constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgroups: two warps idle
 // Registers of a thread after setmaxnreg, by warpgroup; 4 x softmax + 2 x codes +
@@ -61,7 +65,9 @@ constexpr int kBlockBytes = 128 * 128;  // 128 rows of 64 f16, swizzled
 
 struct alignas(16) Meta {
   float sk[kTok];  // block FP8
-  int ek, ev;      // exponents that the tile is relative to: MXFP8 (as E8M0), values of block FP8
+  // Exponents (MXFP8: as E8M0) that keys are relative to in this tile, values in this
+  // and all later ones until it rises
+  int ek, ev;
   uint32_t live[4];          // token 4 i + k: bit i of word k
   uint32_t all;              // every token is live
 };
@@ -523,7 +529,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           }
         };
         if constexpr (KIND != BRC_STE_NVFP4) {
-          if (meta.ev > ev + 4) {  // (the same for every row)
+          if (meta.ev > ev) {  // (the same for every row)
             if (ev > -900) scale_o(__uint_as_float((uint32_t)max(127 + ev - meta.ev, 0) << 23));
             ev = meta.ev;
           }
@@ -547,13 +553,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           }
           if (top != -INFINITY) own = ceilf(top * f);
         }
-        // Probabilities carry the factor 2^lift: values are relative to their tile's
-        // largest scale, O to the row tile's (at most 2^4 less). Their sum
-        // over 32 tokens may pass it by 2^kRise (32 scores at the shift reach 2^5), so
-        // that none leaves the range of f16, and the small ones keep the bits that are left.
-        const float lift = KIND == BRC_STE_NVFP4 ? 9.f : (float)(5 + meta.ev - ev);
-        float base = lift - (own == -INFINITY ? 0.f : own);
-        const float most = ex2(lift + kRise);
+        // Probabilities carry the factor 2^kLift. Their sum over 32 tokens may pass it by
+        // 2^kRise (32 scores at the shift reach 2^5), so that none leaves the range of f16,
+        // and the small ones keep the bits that are left. (The values' scales are no part of
+        // it: a row's sum does not depend on them.)
+        float base = kLift - (own == -INFINITY ? 0.f : own);
+        constexpr float most = (float)(1 << (kLift + kRise));
         float2 l2 = make_float2(0.f, 0.f);
         // this tile's probabilities so far (`upto` groups of 32 columns) times g
         auto scale_p = [&](int upto, float g) {
@@ -607,7 +612,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             top = top == -INFINITY ? top : ceilf(top * f);
             const float nm = fmaxf(own, top), g = nm == own || own == -INFINITY ? 1.f : ex2(own - nm);
             own = nm;
-            base = lift - (own == -INFINITY ? 0.f : own);
+            base = kLift - (own == -INFINITY ? 0.f : own);
             l2 = __fmul2_rn(l2, make_float2(g, g));
             scale_p(c, g);
             t = exps(u);
@@ -623,7 +628,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         sm.pair[parity][r][half][mine] = own;
         meet();
         const float nm = fmaxf(own, sm.pair[parity][r][half ^ 1][mine]);
-        float part = (l2.x + l2.y) * ex2(-lift);
+        float part = (l2.x + l2.y) * (1.f / (1 << kLift));
         if (__any_sync(0xFFFFFFFFu, nm != own || nm != m)) {
           const float gp = nm == own || nm == -INFINITY ? 1.f : ex2(own - nm);
           const float go = nm == m || nm == -INFINITY ? 1.f : ex2(m - nm);
@@ -653,9 +658,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       o_phase ^= 1u;
       tc_fence_after();
       const bool whole = walk.s_begin == 0 && walk.s_end == seq.steps;
-      const float so = KIND == BRC_STE_NVFP4 ? 0x1p-9f
+      const float so = KIND == BRC_STE_NVFP4 ? 1.f / (1 << kLift)
                        : ev < -900 ? 1.f
-                                   : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : kValueLift<FMT>) - 5));
+                                   : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : kValueLift<FMT>) - kLift));
       const bool none = !valid || l == 0.f;
       const float mul = whole ? (none ? 0.f : so / l) : so * (1.f / kSumUp);
       const bool odd = sm.odd[number & 3u] == number && !none;
@@ -875,14 +880,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         k.fetch(a.c.k_scale, row);
         v.fetch(a.c.v_scale, row);
         page = page_of(walk.s_begin + 1);
+        int run = -1000;
         for (int j = walk.s_begin; j < walk.s_end; ++j, ++tile) {
           const uint32_t st = tile & 1u, use = (tile >> 1) & 1u;
           const int left = (int)min((int64_t)kTok, seq.total - (int64_t)j * kTok) - 4 * lane;
           const int live4 = row < 0 ? 0 : min(max(left, 0), 4);
-          int ek = 0, ev = 0;
+          int ek = 0;
           if constexpr (KIND == BRC_STE_MXFP8) ek = k.top(live4);
-          if constexpr (KIND == BRC_STE_BLOCK_FP8) ev = v.top(live4);
-          if constexpr (KIND == BRC_STE_MXFP8) ev = max(v.top(live4), 27);  // no lower than 2^-100
+          if constexpr (KIND != BRC_STE_NVFP4) {
+            constexpr int k100 = KIND == BRC_STE_MXFP8 ? 27 : -100;  // 2^-100
+            const int top = max(v.top(live4), k100);
+            if (top > run) run = min(top + kSlack, k100 + 227);
+          }
           if (!(ok = __all_sync(0xFFFFFFFFu,
                                 mbar_wait(&sm.k_empty[st], use ^ 1u, abort, status, 1u))))
             break;
@@ -894,7 +903,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           for (int y = 0; y < 4; ++y) bal[y] = __ballot_sync(0xFFFFFFFFu, y < live4);
           if (lane == 0) {
             meta.ek = ek;
-            meta.ev = ev;
+            meta.ev = run;
 #pragma unroll
             for (int y = 0; y < 4; ++y) meta.live[y] = bal[y];
             meta.all = (bal[0] & bal[1] & bal[2] & bal[3]) == 0xFFFFFFFFu;

@@ -290,3 +290,16 @@ def test_values_near_the_largest_float(name, d, draft, group):
         v = torch.randn(n + draft, 1, d, generator=torch.Generator().manual_seed(43)).clamp(-3, 3) * 1e38
         rewrite(c, b, 0, v=v.cuda())
     verify(c, c.run(), causal(c))
+
+
+@pytest.mark.parametrize("name", ["block4", "block5", "mx4", "mx5"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_sum_does_not_depend_on_values(name, d, draft, group):
+    """Values near the largest float beside tiny ones, tiles apart."""
+    c = Case(name, d, 1, group, [400], draft, seed=42)
+    v = torch.randn(400 + draft, 1, d, generator=torch.Generator().manual_seed(43)).clamp(-3, 3)
+    v[:128] *= 1e38
+    v[128:] *= 1e-12
+    rewrite(c, 0, 0, v=v.cuda())
+    verify(c, c.run(), causal(c))
