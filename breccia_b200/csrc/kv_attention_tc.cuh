@@ -551,7 +551,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(u[i].x, u[i].y));
           }
-          if (top != -INFINITY) own = ceilf(top * f);
+          // A shift beyond 2^18 is a rounded score, and the unrounded product of that score
+          // and its factor may be far off it: left to the chunk, which rounds the product
+          top = ceilf(top * f);
+          if (fabsf(top) < 0x1p18f) own = top;
         }
         // Probabilities carry the factor 2^kLift. Their sum over 32 tokens may pass it by
         // 2^kRise (32 scores at the shift reach 2^5), so that none leaves the range of f16,
@@ -615,7 +618,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             base = kLift - (own == -INFINITY ? 0.f : own);
             l2 = __fmul2_rn(l2, make_float2(g, g));
             scale_p(c, g);
-            t = exps(u);
+            // as exps, with the rounded product (the compiler may join packed operations)
+            const float down = own == -INFINITY ? 0.f : -own;
+            t = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              u[i].x = ex2(__fadd_rn(__fadd_rn(__fmul_rn(u[i].x, f), down), kLift));
+              u[i].y = ex2(__fadd_rn(__fadd_rn(__fmul_rn(u[i].y, f), down), kLift));
+              t = __fadd2_rn(t, u[i]);
+            }
           }
           l2 = __fadd2_rn(l2, t);
           uint32_t p[16];

@@ -160,6 +160,30 @@ def test_large_queries(draft, group):
     assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[1][0], want[1][0])
 
 
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("draft,group", ROWS)
+@pytest.mark.parametrize("scale", [2.0 ** 12, -2.0 ** 30, 2.0 ** 80])
+def test_large_scores(name, d, draft, group, scale):
+    """Every row's weight lies on one place, and its score is beyond 2^18, 2^36, 2^86."""
+    c = Case(name, d, 1, group, [300, 1], draft, seed=25)
+    out, lse = c.run(scale=scale)
+    k, v = held(c)
+    for b, m in enumerate(causal(c)):
+        n = m.shape[1]
+        kk, vv = (x[b, :n].double().repeat_interleave(group, 1).transpose(0, 1) for x in (k, v))
+        s = (c.q[b].double().transpose(0, 1) @ kk.transpose(1, 2) * scale).masked_fill(~m, -math.inf)
+        top, at = s.topk(2, -1) if n > 1 else (s, torch.zeros_like(s, dtype=torch.int64))
+        big = (c.q[b].double().abs().transpose(0, 1) @ kk.abs().transpose(1, 2) * abs(scale)).amax(-1)
+        # rows whose second score is below the first by more than the scores' error and 64
+        clear = top[..., 0] - top[..., 1] > 2 * d * 2.0 ** -24 * big + 64
+        assert float(clear.double().mean()) > 0.5
+        want = vv.gather(1, at[..., :1].expand(-1, -1, d))
+        o, l = out[b].double().transpose(0, 1), lse[b].double().transpose(0, 1)
+        assert bool(((o - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10)[clear].all())
+        assert bool(((l - top[..., 0]).abs() <= d_tol(d, big, top[..., 0]))[clear].all())
+
+
 # ------------------------------------------------------------------ masks
 
 
