@@ -23,11 +23,14 @@
 // Numbers. FP8 and FP4 codes are exact in f16. Queries are scaled per row by a
 // power of two into f16 (elements below 2^-21 of the row's largest lose bits).
 // Key scales: block FP8 multiplies the score; MXFP8's per-block powers of two
-// go onto the codes relative to the token's largest, which multiplies the
-// score; NVFP4's E4M3 scales times E2M1 codes are exact in f16. Value scales
-// likewise, with the largest seen so far by the warp (a power of two) taken
-// out, so that f16 holds probability x scale: 11 bits each, against the 8 of a
-// bf16 output. Scores, sums, the running maximum and the output are float32.
+// go onto the codes relative to one that the warp's tokens share; NVFP4's E4M3
+// scales times E2M1 codes are exact in f16. Value scales likewise, relative to a
+// power of two for each channel block (block FP8's go onto the probabilities, so
+// that f16 holds probability x scale: 11 bits each, against the 8 of a bf16
+// output). These references move with the scales; tokens of a step that do not
+// go with one of them are taken in passes of their own ("references" below), so
+// that no token's scale touches another one's bits. Scores, sums, the running
+// maximum and the output are float32.
 //
 // Work split. The steps of 16 tokens of all (sequence, cache head, row block)
 // items are cut into equal shares, one per block, whatever the lengths: the
@@ -188,6 +191,102 @@ __device__ __forceinline__ uint32_t half2_pow2(int e0, int e1, int ref) {
   return half2_of(f(e0), f(e1));
 }
 
+// ------------------------------------------------------------------ references
+// What codes are relative to in f16. Scales are taken as biased exponents, a byte to a
+// channel block (MXFP8: E8M0 bytes; block FP8: the float32 scale's); 255 is not finite
+// and goes with any reference.
+//
+// Codes whose scale is up to kSpan (log2) below its reference keep their bits: E4M3 codes
+// are multiples of 2^-9 and E5M2 codes of 2^-16, f16 holds multiples of 2^-24. Block
+// FP8's scales are multiplied in before the rounding to f16, onto the probabilities (here:
+// they then keep what is above 2^-20 of the row's largest, as 2^-31 without) or the values
+// (tcgen05: E4M3's smallest codes then just are normal numbers). Tokens further apart do
+// not go together. A reference is set kSlack above the scale that asks for it, so that it
+// seldom moves.
+template <int KIND, int FMT>
+constexpr int kSpan = KIND == BRC_STE_BLOCK_FP8 ? 11 : FMT == BRC_FP8_E4M3 ? 15 : 7;
+constexpr int kSlack = 2;
+constexpr uint32_t kLowest = 27;  // references are not below 2^-100
+
+template <int KIND, int D>
+constexpr int kScaleBlocks = KIND == BRC_STE_MXFP8 ? D / 32 : 1;
+
+// Whether up to four bytes lie within SPAN below their references: both as 16-bit
+// fields, offset so that the difference does not borrow. Bytes without a block are zero
+// on both sides.
+template <int SPAN>
+struct Near {
+  static_assert((SPAN & (SPAN + 1)) == 0, "a mask");
+  uint32_t even, odd;
+  __device__ __forceinline__ Near() {}
+  __device__ __forceinline__ explicit Near(uint32_t refs)
+      : even(0x01000100u + SPAN * 0x00010001u - (refs & 0x00FF00FFu)),
+        odd(0x01000100u + SPAN * 0x00010001u - ((refs >> 8) & 0x00FF00FFu)) {}
+  __device__ __forceinline__ uint32_t refs() const {
+    return (0x01000100u + SPAN * 0x00010001u - even) |
+           ((0x01000100u + SPAN * 0x00010001u - odd) << 8);
+  }
+  __device__ __forceinline__ bool operator()(uint32_t x) const {
+    const uint32_t a = ((x & 0x00FF00FFu) + even) ^ 0x01000100u;
+    const uint32_t b = (((x >> 8) & 0x00FF00FFu) + odd) ^ 0x01000100u;
+    return ((a | b) & ~(SPAN * 0x00010001u)) == 0u;
+  }
+};
+
+// The largest finite byte of up to four.
+__device__ __forceinline__ uint32_t top_byte(uint32_t x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const uint32_t y = (x >> i) & 0xFFu;
+    if (y != 255u) m = max(m, y);
+  }
+  return m;
+}
+
+// Of the tokens in `left` (bit y of each lane: its token y of N), those that go together,
+// at least one: block by block, the ones near the largest scale of those that are left.
+// W words of four blocks' bytes to a token's values; km: the largest byte of its keys
+// (MXFP8). `refs` moves for them where it has to; returns what their keys are relative to.
+template <int SPAN, int BLOCKS, int N, int W>
+__device__ __forceinline__ uint32_t choose(const uint32_t (&v)[N][W], const uint32_t (&km)[N],
+                                           uint32_t left, uint32_t& take, uint32_t (&refs)[W]) {
+  constexpr uint32_t kTake = SPAN - kSlack;
+  take = left;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+#pragma unroll 1
+    for (int i = 0; i < 8 * (BLOCKS < 4 ? BLOCKS : 4); i += 8) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int y = 0; y < N; ++y) {
+        const uint32_t x = (v[y][w] >> i) & 0xFFu;
+        if (((take >> y) & 1u) && x != 255u) top = max(top, x);
+      }
+      top = __reduce_max_sync(0xFFFFFFFFu, top);
+      const uint32_t ref = (refs[w] >> i) & 0xFFu;
+      bool off = top > ref;
+#pragma unroll
+      for (int y = 0; y < N; ++y) {
+        const uint32_t x = (v[y][w] >> i) & 0xFFu;
+        if (x + kTake < top) take &= ~(1u << y);
+        else off |= ((take >> y) & 1u) && x + SPAN < ref;
+      }
+      if (__any_sync(0xFFFFFFFFu, off))
+        refs[w] += (min(max(top + kSlack, kLowest), 254u) - ref) << i;
+    }
+  }
+  uint32_t k = 0;
+#pragma unroll
+  for (int y = 0; y < N; ++y)
+    if ((take >> y) & 1u) k = max(k, km[y]);
+  k = __reduce_max_sync(0xFFFFFFFFu, k);
+#pragma unroll
+  for (int y = 0; y < N; ++y)
+    if (km[y] + kTake < k) take &= ~(1u << y);
+  return k;
+}
+
 // A step is two 16-token tiles: two independent chains of products, one set of
 // votes and waits for both. Heads of 256 take one, or a ring would not fit.
 constexpr __host__ __device__ int subtiles(int d) { return d == 256 ? 1 : 2; }
@@ -297,15 +396,35 @@ __device__ __forceinline__ bool odd_codes(uint32_t w) {
   else return (((w & 0x7C7C7C7Cu) + 0x04040404u) & 0x80808080u) != 0;
 }
 
+// A warp's notes on an item's steps (in shared memory: they are rare, and registers are not).
+struct Later {
+  static constexpr int kMost = 13;
+  int count, climb, fall;  // steps put off; how far references climbed and fell, in all
+  int step[kMost];
+};
+
 template <int KIND, int FMT, int D, int NT>
 struct Warp {
   using S = Shape<KIND, D>;
+  static constexpr int kSpans = kSpan<KIND, FMT>;
+  static constexpr int kMask = KIND == BRC_STE_MXFP8 ? kSpans : 15;
+  static constexpr int kBlocks = kScaleBlocks<KIND, D>;
+  static constexpr int kWords = (kBlocks + 3) / 4;
+  static constexpr int kOwn = kBlocks == 8 ? 2 : 1;  // channel blocks of a lane's outputs
   float o[NT][S::kTiles][4];  // [elements 2j, 2j + 1][rows 2c, 2c + 1]
   float m[NT][2], l[NT][2];   // shift and (the lane's part of the) sum of rows 2c, 2c + 1
-  int e;                      // value scales are relative to 2^e
-  int ke;                     // MXFP8: key scales are relative to this E8M0 byte
+  // What values are relative to: this lane's own (biased exponents), and in MXFP8 all of
+  // the warp's as the check wants them, and what keys are relative to
+  int e[kOwn];
+  Near<kMask> near[kWords];
+  uint32_t ke;
 
-  __device__ __forceinline__ void clear() {
+  // A lane's outputs are of one block (heads of 256: of two, one in each word of bytes):
+  // elements 16 (lane / 4) .. or, in heads of 64, 8 (lane / 4) ..
+  __device__ static __forceinline__ int byte_of(int lane) {
+    return kBlocks == 1 ? 0 : kBlocks == 2 ? lane >> 4 : lane >> 3;
+  }
+  __device__ __forceinline__ Warp() {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -313,21 +432,52 @@ struct Warp {
       m[i][0] = m[i][1] = -INFINITY;
       l[i][0] = l[i][1] = 0.f;
     }
-    e = -1000;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w)
+      near[w] = Near<kMask>(kLowest * (kBlocks == 1 ? 1u : kBlocks == 2 ? 0x0101u : 0x01010101u));
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) e[i] = KIND == BRC_STE_NVFP4 ? 127 : (int)kLowest;
     ke = 0;
   }
-  // Raise the reference of the value scales (a power of two) to 2^to, at least 2^-100.
-  __device__ __forceinline__ void raise(int to) {
-    to = max(to, -100);
-    if (to <= e) return;
-    const float f = e < -900 ? 1.f : __uint_as_float((uint32_t)max(127 + e - to, 0) << 23);
+  // What the values are relative to becomes `refs`; o is still zero.
+  __device__ __forceinline__ void start(const uint32_t (&refs)[kWords], int lane) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < kWords; ++i) {
+      near[i] = Near<kMask>(refs[i]);
+      e[i] = (int)((refs[i] >> (8 * byte_of(lane))) & 0xFFu);
+    }
+  }
+  // The same where o is not; not so low that its largest element passes 2^100.
+  __device__ __forceinline__ void move(const uint32_t (&refs)[kWords], int lane) {
+    uint32_t to[kWords];
 #pragma unroll
-      for (int j = 0; j < S::kTiles; ++j)
+    for (int i = 0; i < kWords; ++i) {
+      float most = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[i][j][x] *= f;
-    e = to;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = i * (S::kTiles / kOwn); j < (i + 1) * (S::kTiles / kOwn); ++j)
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (isfinite(o[n][j][y])) most = fmaxf(most, fabsf(o[n][j][y]));
+      const int room = 227 - (int)(__float_as_uint(most) >> 23);
+      // a lane's bound for its block, then the block's: the largest of its lanes'
+      const int own = max((int)((refs[i] >> (8 * byte_of(lane))) & 0xFFu),
+                          most == 0.f ? 0 : e[i] - room);
+      to[i] = 0;
+#pragma unroll
+      for (int y = 0; y < (kBlocks < 4 ? kBlocks : 4); ++y)
+        to[i] |= __reduce_max_sync(0xFFFFFFFFu, byte_of(lane) == y ? (uint32_t)own : 0u) << (8 * y);
+      const int by = max(e[i] - (int)((to[i] >> (8 * byte_of(lane))) & 0xFFu), -127);
+      const float f = kv::pow2i(by - by / 2), f2 = kv::pow2i(by / 2);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = i * (S::kTiles / kOwn); j < (i + 1) * (S::kTiles / kOwn); ++j)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) o[n][j][y] = o[n][j][y] * f * f2;
+    }
+    start(to, lane);
   }
 };
 
@@ -352,11 +502,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return d;
 }
 
-template <bool B>
-struct Bool {
-  static constexpr bool value = B;
-};
-
 template <int KIND, int FMT, int D, int NT>
 struct Step {
   using S = Shape<KIND, D>;
@@ -364,10 +509,11 @@ struct Step {
   static constexpr int kSub = S::kSub;
 
   // s[u][nt][2 h + x]: score of token 16 u + r + 8 h and row 2c + x, in units of
-  // the rows' factors. `live`: the rows of the stage that hold a token (the
-  // others' scales are not to be looked at).
-  __device__ static __forceinline__ void scores(W& w, const uint8_t* st, const uint4* q, int lane,
-                                                uint32_t live, float (&s)[kSub][NT][4]) {
+  // the rows' factors. `live`: the tokens of this pass (the others' scales are not to
+  // be looked at). ANY: MXFP8, their scales are not all near the reference.
+  template <bool ANY>
+  __device__ static __forceinline__ void scores(const W& w, const uint8_t* st, const uint4* q,
+                                                int lane, uint32_t live, float (&s)[kSub][NT][4]) {
     const int r = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
@@ -376,7 +522,7 @@ struct Step {
     constexpr int kReads = S::kKeyWords / S::kKeyRead;
     uint32_t f[kSub][2][kReads];  // scales of a read's codes
     if constexpr (KIND == BRC_STE_MXFP8) {
-      int e[kSub][2][kReads], top = 0;
+      int e[kSub][2][kReads];
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -387,31 +533,14 @@ struct Step {
             const int t = 16 * u + 8 * n + r;
             e[u][n][i] = st[S::kKeyScales + t * S::kScales + 2 * i + (c >> 1)];
             if (live != S::kAll && !((live >> t) & 1u)) e[u][n][i] = 0;
-            top = max(top, e[u][n][i]);
           }
-      auto factors = [&](auto inf) {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int i = 0; i < kReads; ++i)
-              f[u][n][i] = half2_pow2<decltype(inf)::value>(e[u][n][i], e[u][n][i], w.ke);
-      };
-      if (__any_sync(0xFFFFFFFFu, top > w.ke)) {  // a larger scale, or 255
-        int t = 0;
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < kReads; ++i)
-              if (e[u][n][i] != 255) t = max(t, e[u][n][i]);
-        w.ke = max(w.ke, (int)__reduce_max_sync(0xFFFFFFFFu, t));
-        factors(Bool<true>{});
-      } else {
-        factors(Bool<false>{});
-      }
+          for (int i = 0; i < kReads; ++i)
+            f[u][n][i] = half2_pow2<ANY>(e[u][n][i], e[u][n][i], (int)w.ke);
     }
 #pragma unroll
     for (int i = 0; i < kReads; ++i) {
@@ -541,7 +670,7 @@ struct Step {
   // f16 keeps those down to 2^-30 of the largest. TWO: a second product with
   // what the rounding to f16 left (f16 outputs of few rows: its 2^-11 would
   // show beside the output's own).
-  template <bool TWO>
+  template <bool TWO, bool ANY>
   __device__ static __forceinline__ void values(W& w, const uint8_t* st, int lane, uint32_t live,
                                                 const float (&p)[kSub][NT][4]) {
     const int r = lane >> 2, c = lane & 3;
@@ -551,26 +680,17 @@ struct Step {
     float f[kSub][2];        // factor of tokens r, r + 8
     uint32_t h[kSub][2][2];  // [token pair][half of the lane's elements]: f16 pair of value factors
     if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-      const uint32_t* sp = reinterpret_cast<const uint32_t*>(st + S::kValScales);
-      uint32_t sv[kSub][2], top = 0;
+      const float* sp = reinterpret_cast<const float*>(st + S::kValScales);
+      const float g = __uint_as_float((uint32_t)(254 + 6 - w.e[0]) << 23);
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int t = 16 * u + 8 * n + r;
-          sv[u][n] = sp[t];
-          if (!all && !((live >> t) & 1u)) sv[u][n] = 0;
-          if (sv[u][n] < 0x7F800000u) top = max(top, sv[u][n]);
+          f[u][n] = !all && !((live >> t) & 1u) ? 0.f : sp[t] * g;
         }
-      if (__any_sync(0xFFFFFFFFu, (int)(top >> 23) - 127 > w.e))
-        w.raise((int)(__reduce_max_sync(0xFFFFFFFFu, top) >> 23) - 127);
-      const float g = __uint_as_float((uint32_t)(127 - w.e + 6) << 23);
-#pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) f[u][n] = __uint_as_float(sv[u][n]) * g;
     } else if constexpr (KIND == BRC_STE_MXFP8) {
-      int e[kSub][4][2], top = 0;
+      int e[kSub][4][2];
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -580,36 +700,17 @@ struct Step {
             const int blk = D == 64 ? r >> 2 : 4 * i + (r >> 1);
             e[u][t][i] = st[S::kValScales + token(u, t) * S::kScales + blk];
             if (!all && !((live >> token(u, t)) & 1u)) e[u][t][i] = 0;
-            top = max(top, e[u][t][i]);
           }
-      auto factors = [&](auto inf) {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            f[u][t] = 64.f;
+        for (int t = 0; t < 2; ++t) {
+          f[u][t] = 64.f;
 #pragma unroll
-            for (int i = 0; i < kReads; ++i)
-              h[u][t][i] = half2_pow2<decltype(inf)::value>(e[u][2 * t][i], e[u][2 * t + 1][i],
-                                                            w.e + 127);
-          }
-      };
-      if (__any_sync(0xFFFFFFFFu, top - 127 > w.e)) {  // a larger scale, or 255
-        int m = 0;
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < kReads; ++i)
-              if (e[u][t][i] != 255) m = max(m, e[u][t][i]);
-        w.raise((int)__reduce_max_sync(0xFFFFFFFFu, m) - 127);
-        factors(Bool<true>{});
-      } else {
-        factors(Bool<false>{});
-      }
+          for (int i = 0; i < kReads; ++i)
+            h[u][t][i] = half2_pow2<ANY>(e[u][2 * t][i], e[u][2 * t + 1][i], w.e[i]);
+        }
     } else {
-      if (w.e < -900) w.e = 0;
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -706,6 +807,134 @@ struct Step {
     }
   }
 
+  // One token to a lane: its scales' bytes.
+  struct Token {
+    uint32_t k[1][W::kWords], v[1][W::kWords];  // (keys: MXFP8)
+    __device__ __forceinline__ Token(const uint8_t* st, int t) {
+      if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+        v[0][0] = (reinterpret_cast<const uint32_t*>(st + S::kValScales)[t] >> 23) & 0xFFu;
+      } else if constexpr (KIND == BRC_STE_MXFP8) {
+        const uint8_t* const pk = st + S::kKeyScales + t * S::kScales;
+        const uint8_t* const pv = st + S::kValScales + t * S::kScales;
+        if constexpr (D == 64) {
+          k[0][0] = *reinterpret_cast<const uint16_t*>(pk);
+          v[0][0] = *reinterpret_cast<const uint16_t*>(pv);
+        } else {
+          lds_words<W::kWords>(pk, k[0]);
+          lds_words<W::kWords>(pv, v[0]);
+        }
+      }
+    }
+    // Whether the references hold it.
+    __device__ __forceinline__ bool fits(const W& w) const {
+      if constexpr (KIND == BRC_STE_BLOCK_FP8) return w.e[0] - v[0][0] <= (uint32_t)W::kSpans;
+      bool in = w.ke - top_key() <= (uint32_t)W::kSpans;
+#pragma unroll
+      for (int i = 0; i < W::kWords; ++i) in &= w.near[i](v[0][i]);
+      return in;
+    }
+    __device__ __forceinline__ uint32_t top_key() const {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < W::kWords; ++i)
+        m = __vmaxu2(m, __vmaxu2(k[0][i] & 0x00FF00FFu, (k[0][i] >> 8) & 0x00FF00FFu));
+      return max(m & 0xFFFFu, m >> 16);
+    }
+  };
+  // References that hold the tokens of lanes with `on`, if they go together.
+  __device__ static __forceinline__ void around(const Token& mine, bool on,
+                                                uint32_t (&refs)[W::kWords], uint32_t& ke) {
+#pragma unroll
+    for (int i = 0; i < W::kWords; ++i) {
+      refs[i] = 0;
+#pragma unroll
+      for (int y = 0; y < 8 * (W::kBlocks < 4 ? W::kBlocks : 4); y += 8) {
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, on ? (mine.v[0][i] >> y) & 0xFFu : 0u);
+        refs[i] |= min(max(top + kSlack, kLowest), 254u) << y;
+      }
+    }
+    ke = 0;
+    if constexpr (KIND == BRC_STE_MXFP8)
+      ke = min(__reduce_max_sync(0xFFFFFFFFu, on ? mine.top_key() : 0u) + kSlack, 254u);
+  }
+  __device__ static __forceinline__ void first(W& w, const Token& mine, int lane, uint32_t live) {
+    uint32_t refs[W::kWords];
+    around(mine, (live >> (lane % S::kRows)) & 1u, refs, w.ke);
+    w.start(refs, lane);
+  }
+  // Moves the references to a step that they do not hold. False (and nothing moves) if its
+  // tokens do not go together, or if o might leave float32: o falls with references that
+  // climb, which only what a row sees may cause, so drafted tokens climb little, and it
+  // grows with references that fall.
+  __device__ static __forceinline__ bool follow(W& w, const Token& mine, int lane, bool on,
+                                                bool drafted, Later& later) {
+    uint32_t refs[W::kWords], ke;
+    around(mine, on, refs, ke);
+    int climb = 0, fall = 0;
+    bool in = KIND != BRC_STE_MXFP8 || ke - mine.top_key() <= (uint32_t)W::kSpans;
+    int own[W::kOwn];
+#pragma unroll
+    for (int i = 0; i < W::kWords; ++i) {
+      if constexpr (KIND == BRC_STE_BLOCK_FP8) in &= refs[0] - mine.v[0][0] <= (uint32_t)W::kSpans;
+      else in &= Near<W::kMask>(refs[i])(mine.v[0][i]);
+      own[i] = (int)((refs[i] >> (8 * W::byte_of(lane))) & 0xFFu);
+      climb = max(climb, own[i] - w.e[i]);
+      fall = max(fall, w.e[i] - own[i]);
+    }
+    climb = drafted ? (int)__reduce_max_sync(0xFFFFFFFFu, climb) + later.climb : later.climb;
+    fall = (int)__reduce_max_sync(0xFFFFFFFFu, fall) + later.fall;
+    if (!__all_sync(0xFFFFFFFFu, !on || in) || climb > 60 || fall > 60) return false;
+    __syncwarp();
+    if (lane == 0) {
+      later.climb = climb;
+      later.fall = fall;
+    }
+#pragma unroll
+    for (int i = 0; i < W::kOwn; ++i) {
+      const float f = kv::pow2i(max(w.e[i] - own[i], -126));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = i * (S::kTiles / W::kOwn); j < (i + 1) * (S::kTiles / W::kOwn); ++j)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) w.o[n][j][y] *= f;
+    }
+    w.start(refs, lane);
+    w.ke = ke;
+    return true;
+  }
+  // Takes tokens that go together out of `left`, moves the references to them and
+  // returns them; tokens that no row sees (`seen` says) are dropped, whatever they hold.
+  template <class Seen>
+  __device__ static __forceinline__ uint32_t pick(W& w, const uint8_t* st, int lane, uint32_t& left,
+                                                  const Seen& seen) {
+    const Token mine(st, lane % S::kRows);
+    uint32_t taken = 0;
+#pragma unroll 1
+    while (left) {  // (choose takes one token at least)
+      uint32_t km[1] = {0u}, take, refs[W::kWords];
+#pragma unroll
+      for (int i = 0; i < W::kWords; ++i) {
+        refs[i] = KIND == BRC_STE_BLOCK_FP8 ? (uint32_t)w.e[0] : w.near[i].refs();
+        if constexpr (KIND == BRC_STE_MXFP8) km[0] = max(km[0], top_byte(mine.k[0][i]));
+      }
+      const uint32_t k = choose<W::kSpans, W::kBlocks>(
+          mine.v, km, (left >> (lane % S::kRows)) & 1u, take, refs);
+      const uint32_t group = __ballot_sync(0xFFFFFFFFu, take != 0u) & S::kAll;
+      left &= ~group;
+      if (seen(group)) {
+        taken = group;
+        if constexpr (KIND == BRC_STE_MXFP8) {
+          if (__any_sync(0xFFFFFFFFu, k > w.ke || (take && km[0] + W::kSpans < w.ke)))
+            w.ke = min(k + kSlack, 254u);
+        }
+        w.move(refs, lane);
+        break;
+      }
+    }
+    return taken;
+  }
+
   // Does any value of the step's live rows stand for something not finite?
   __device__ static __forceinline__ bool odd_values(const uint8_t* st, int lane, uint32_t live) {
     bool odd = false;
@@ -734,8 +963,9 @@ struct Step {
                                                         const int64_t (&row)[kSub], int lane,
                                                         const float (&p)[kSub][NT][4],
                                                         uint32_t live, uint32_t seen) {
-    if (w.e < -900) w.e = 0;
-    const float f = 64.f * exp2f((float)-w.e);
+    float f[W::kOwn];
+#pragma unroll
+    for (int i = 0; i < W::kOwn; ++i) f[i] = 64.f * exp2f((float)(127 - w.e[i]));
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
       for (int t = 0; t < 16; ++t) {
@@ -746,13 +976,14 @@ struct Step {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
-            pr[n][x] = __shfl_sync(0xFFFFFFFFu, half ? p[u][n][2 + x] : p[u][n][x], src) * f;
+            pr[n][x] = __shfl_sync(0xFFFFFFFFu, half ? p[u][n][2 + x] : p[u][n][x], src);
         const uint32_t sees = __shfl_sync(0xFFFFFFFFu, seen, src) >> (4 * NT * u + 2 * half);
 #pragma unroll
         for (int j = 0; j < S::kTiles; ++j)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const float v = value_at<KIND, FMT, D>(c, row[u] + t, S::elem(2 * j + y, lane >> 2));
+            const float v = value_at<KIND, FMT, D>(c, row[u] + t, S::elem(2 * j + y, lane >> 2)) *
+                            f[j / (S::kTiles / W::kOwn)];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -762,6 +993,160 @@ struct Step {
       }
   }
 };
+
+// An item, as the warps of a block walk it.
+struct Item {
+  Seq seq;
+  int b, page_mask;
+  uint32_t head_row;
+  const int32_t* table;
+  // First cache row of the 16-token tile at token t, or -1.
+  __device__ __forceinline__ int64_t row_at(const Args& a, int t) const {
+    if (t >= seq.total) return -1;
+    const int page = __ldg(table + (t >> a.page_shift));
+    if (page < 0 || page >= a.c.num_pages) return -1;
+    return (int64_t)((uint64_t)(uint32_t)page * a.page_rows) + (head_row + (t & page_mask));
+  }
+  // The tokens of the step of ROWS at t0, of whose 16-token tiles `bits` are there.
+  template <int ROWS>
+  __device__ __forceinline__ uint32_t live_of(int t0, uint32_t bits) const {
+    uint32_t live = ROWS == 32 ? 0xFFFFFFFFu : 0xFFFFu;
+    if (t0 > seq.total - ROWS) live >>= ROWS - (seq.total - t0);
+    if (ROWS == 32 && bits != 3) live &= bits == 1 ? 0xFFFFu : 0xFFFF0000u;
+    return live;
+  }
+  // Whether query `node` sees drafted token j (j < 0: a token of the context).
+  __device__ __forceinline__ bool sees(const Args& a, int node, int j) const {
+    if (j < 0) return true;
+    return a.tree ? a.tree[b * a.tree_stride + (int64_t)node * a.draft + j] != 0 : j <= node;
+  }
+};
+template <int NT>
+struct Rows {  // rows 2c, 2c + 1 of a lane's tiles: what a score is times, and their nodes
+  float factor[NT][2];
+  int node[NT][2];
+};
+
+// Adds the tokens `live` of the step at t0 in stage st.
+template <int KIND, int FMT, int D, int NT, bool ANY>
+__device__ __forceinline__ void add_step(Warp<KIND, FMT, D, NT>& w, const Args& a, const Item& it,
+                                         const Rows<NT>& rows, const uint8_t* st, const uint4* q,
+                                         int lane, int t0, uint32_t live) {
+  using S = Shape<KIND, D>;
+  using St = Step<KIND, FMT, D, NT>;
+  constexpr int kSub = S::kSub;
+  constexpr bool kTwo = NT <= 2;
+  float p[kSub][NT][4];
+  St::template scores<ANY>(w, st, q, lane, live, p);
+  const float kf = KIND == BRC_STE_MXFP8 ? e8m0_value(w.ke) : 1.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float f = KIND == BRC_STE_MXFP8 ? rows.factor[n][x] * kf : rows.factor[n][x];
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        p[u][n][x] *= f;
+        p[u][n][2 + x] *= f;
+      }
+    }
+  uint32_t seen = 0;
+  bool checked = false;
+  if (t0 > it.seq.context - S::kRows || live != S::kAll) {  // drafted tokens, or none
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int at = 16 * u + 8 * h + (lane >> 2);
+            if (((live >> at) & 1u) && rows.node[n][x] < it.seq.drafts &&
+                it.sees(a, rows.node[n][x], t0 - it.seq.context + at))
+              seen |= 1u << (4 * (NT * u + n) + 2 * h + x);
+            else p[u][n][2 * h + x] = -INFINITY;
+          }
+    // a drafted value that is not finite must not meet a probability of
+    // zero in the product
+    checked = St::odd_values(st, lane, live);
+  }
+  St::softmax(w, p);
+  if (checked) {
+    int64_t at[kSub];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) at[u] = it.row_at(a, t0 + 16 * u);
+    St::values_checked(w, a.c, at, lane, p, live, seen);
+  } else if constexpr (kTwo) {
+    if (a.q_f16) St::template values<true, ANY>(w, st, lane, live, p);
+    else St::template values<false, ANY>(w, st, lane, live, p);
+  } else {
+    St::template values<false, ANY>(w, st, lane, live, p);
+  }
+}
+
+// The same for the steps that were put off, and those from `s` on, in passes, each with
+// tokens that go together. A function of its own, called after the usual steps with the
+// warp's state handed over in memory: it is rare, and inlined, or called between them, it
+// costs them registers (32 rows of MXFP8: 118 -> 134 us). `ring`: the warp's, free now.
+template <int KIND, int FMT, int D, int NT>
+struct Passes {
+  Warp<KIND, FMT, D, NT> w;
+  Item it;
+  Rows<NT> rows;
+};
+template <int KIND, int FMT, int D, int NT>
+__device__ __noinline__ void add_in_passes(Passes<KIND, FMT, D, NT>& x, const Args& a,
+                                           uint8_t* ring, const uint4* q, int lane,
+                                           const Later& later, int s, int s_end, int stride) {
+  using S = Shape<KIND, D>;
+  using St = Step<KIND, FMT, D, NT>;
+  Warp<KIND, FMT, D, NT> w = x.w;
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring);
+  int put_off = 0;
+#pragma unroll 1
+  while (true) {
+    int t0;
+    if (put_off < later.count) {
+      t0 = later.step[put_off++] * S::kRows;
+    } else if (s < s_end) {
+      t0 = s * S::kRows;
+      s += stride;
+    } else {
+      break;
+    }
+    uint32_t bits = 0;
+    for (int u = 0; u < S::kSub; ++u) {
+      const int64_t row = x.it.row_at(a, t0 + 16 * u);
+      if (row < 0) continue;
+      copy_tile<KIND, D>(a.c, row, lane, to, u);
+      bits |= 1u << u;
+    }
+    cp_commit();
+    cp_wait<0>();
+    __syncwarp();
+    uint32_t live = bits ? x.it.template live_of<S::kRows>(t0, bits) : 0u;
+    auto seen = [&](uint32_t tokens) {
+      if (t0 <= x.it.seq.context - S::kRows) return true;
+      bool see = false;
+      for (int at = 0; at < S::kRows; ++at) {
+        if (!((tokens >> at) & 1u)) continue;
+        for (int n = 0; n < NT; ++n)
+          for (int i = 0; i < 2; ++i)
+            see |= x.rows.node[n][i] < x.it.seq.drafts &&
+                   x.it.sees(a, x.rows.node[n][i], t0 - x.it.seq.context + at);
+      }
+      return __any_sync(0xFFFFFFFFu, see) != 0;
+    };
+#pragma unroll 1
+    for (int pass = 0; pass < S::kRows && live; ++pass) {
+      const uint32_t take = St::pick(w, ring, lane, live, seen);
+      if (take) add_step<KIND, FMT, D, NT, true>(w, a, x.it, x.rows, ring, q, lane, t0, take);
+    }
+    __syncwarp();  // the stage is read
+  }
+  x.w = w;
+}
 
 // Blocks that an SM is to hold, as many as the accumulators' registers allow.
 constexpr __host__ __device__ int blocks_per_sm(int kind, int d, int nt) {
@@ -791,11 +1176,11 @@ constexpr __host__ __device__ int ring_bytes(int kind, int d, int nt) {
 }
 
 template <int KIND, int FMT, int D, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend(Args a) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT))
+    k_attend(const __grid_constant__ Args a) {
   using S = Shape<KIND, D>;
   using St = Step<KIND, FMT, D, NT>;
   constexpr int kStages = stages(KIND, D, NT);
-  constexpr bool kTwo = NT <= 2;
   constexpr int kSub = S::kSub;
   extern __shared__ __align__(16) uint8_t smem[];
   // the warps' stages (later: their outputs), then the queries as operand fragments
@@ -804,6 +1189,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
   uint4* const sq = reinterpret_cast<uint4*>(smem + ring_bytes(KIND, D, NT));
   __shared__ float s_m[kWarps][8 * NT], s_l[kWarps][8 * NT], s_rowf[kWarps * 8 * NT];
   __shared__ Place s_place;
+  __shared__ Later s_later[kWarps];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row_warps = a.row_warps, token_warps = kWarps / row_warps;
@@ -833,16 +1219,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
     const int row0 = rb * rows_per_block;
 
     // ---- the first stages are on their way while the queries are laid out
-    const int32_t* const table = a.table + b * a.table_stride;
-    const int page_mask = a.c.page_size - 1;
-    const uint32_t head_row = (uint32_t)head * a.c.page_size;
-    // First cache row of the 16-token tile at token t, or -1.
-    auto row_at = [&](int t) -> int64_t {
-      if (t >= seq.total) return -1;
-      const int page = __ldg(table + (t >> a.page_shift));
-      if (page < 0 || page >= a.c.num_pages) return -1;
-      return (int64_t)((uint64_t)(uint32_t)page * a.page_rows) + (head_row + (t & page_mask));
-    };
+    const Item it{seq, b, a.c.page_size - 1, (uint32_t)head * a.c.page_size,
+                  a.table + b * a.table_stride};
     // the warp's own ring of stages
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rings) + warp * (kStages * S::kStageBytes);
     const uint8_t* const ring_p = rings + warp * (kStages * S::kStageBytes);
@@ -853,7 +1231,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
       if (ahead < s_end) {
         const int t = ahead * S::kRows;  // (positions fit in 31 bits)
         const uint32_t to = ring + slot_in * S::kStageBytes;
-        const int64_t row = row_at(t);
+        const int64_t row = it.row_at(a, t);
         if (row >= 0) {
           copy_tile<KIND, D>(a.c, row, lane, to, 0);
           bits = 1;
@@ -861,7 +1239,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
         if constexpr (kSub == 2) {
           // pages of 32 tokens and more hold the step whole
           const int64_t row1 = a.page_shift > 4 ? (row >= 0 && t + 16 < seq.total ? row + 16 : -1)
-                                                : row_at(t + 16);
+                                                : it.row_at(a, t + 16);
           if (row1 >= 0) {
             copy_tile<KIND, D>(a.c, row1, lane, to, 1);
             bits |= 2;
@@ -925,83 +1303,68 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
     __syncthreads();
 
     Warp<KIND, FMT, D, NT> w;
-    w.clear();
     const uint4* const q = sq + rw * NT * (S::kSteps / 2) * 32;
-    float rowf[NT][2];
-    int node[NT][2];
+    Rows<NT> rows;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int rr = (rw * NT + n) * 8 + 2 * (lane & 3) + x;
-        rowf[n][x] = s_rowf[rr];
+        rows.factor[n][x] = s_rowf[rr];
         const int row = row0 + rr;
-        node[n][x] = row < a.rows ? row / a.group : a.draft;
+        rows.node[n][x] = row < a.rows ? row / a.group : a.draft;
       }
 
+    auto live_of = [&](int t0, uint32_t bits) { return it.template live_of<S::kRows>(t0, bits); };
+    if constexpr (KIND != BRC_STE_NVFP4) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      const uint32_t bits = there >> ((kStages - 2) * kSub) & ((1u << kSub) - 1);
+      if (s < s_end && bits)
+        St::first(w, typename St::Token(ring_p, lane % S::kRows), lane, live_of(s * S::kRows, bits));
+    }
+    Later& later = s_later[warp];
+    if (lane == 0) later.count = later.climb = later.fall = 0;
+    __syncwarp();
     for (; s < s_end; s += token_warps) {
       cp_wait<kStages - 2>();
       __syncwarp();  // every lane's pieces are there, and the oldest stage is read
       fetch();
       const uint32_t bits = there >> ((kStages - 1) * kSub) & ((1u << kSub) - 1);
-      if (bits) {
+      bool now = bits != 0;
+      if (now) {
         const uint8_t* const st = ring_p + slot_out * S::kStageBytes;
-        const int t0 = s * S::kRows;
-        uint32_t live = S::kAll;
-        if (t0 > seq.total - S::kRows) live >>= S::kRows - (seq.total - t0);
-        if (kSub == 2 && bits != 3) live &= bits == 1 ? 0xFFFFu : 0xFFFF0000u;
-        float p[kSub][NT][4];
-        St::scores(w, st, q, lane, live, p);
-        const float kf = KIND == BRC_STE_MXFP8 ? e8m0_value(w.ke) : 1.f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float f = KIND == BRC_STE_MXFP8 ? rowf[n][x] * kf : rowf[n][x];
-#pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-              p[u][n][x] *= f;
-              p[u][n][2 + x] *= f;
+        const uint32_t live = live_of(s * S::kRows, bits);
+        if constexpr (KIND != BRC_STE_NVFP4) {
+          const typename St::Token mine(st, lane % S::kRows);
+          const bool on = (live >> (lane % S::kRows)) & 1u;
+          if (!__all_sync(0xFFFFFFFFu, !on || mine.fits(w))) {
+            now = St::follow(w, mine, lane, on, s * S::kRows > seq.context - S::kRows, later);
+            if (!now) {
+              const int n = later.count;
+              if (n == Later::kMost) break;  // the rest of the share, then
+              __syncwarp();
+              if (lane == 0) {
+                later.step[n] = s;
+                later.count = n + 1;
+              }
+              __syncwarp();
             }
           }
-        uint32_t seen = 0;
-        bool checked = false;
-        if (t0 > seq.context - S::kRows || live != S::kAll) {  // drafted tokens, or none
-#pragma unroll
-          for (int u = 0; u < kSub; ++u)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                  const int at = 16 * u + 8 * h + (lane >> 2);
-                  const int j = t0 - seq.context + at;
-                  bool see = ((live >> at) & 1u) && node[n][x] < seq.drafts;
-                  if (see && j >= 0)
-                    see = a.tree ? a.tree[b * a.tree_stride + (int64_t)node[n][x] * a.draft + j] != 0
-                                 : j <= node[n][x];
-                  if (see) seen |= 1u << (4 * (NT * u + n) + 2 * h + x);
-                  else p[u][n][2 * h + x] = -INFINITY;
-                }
-          // a drafted value that is not finite must not meet a probability of
-          // zero in the product
-          checked = St::odd_values(st, lane, live);
         }
-        St::softmax(w, p);
-        if (checked) {
-          int64_t rows[kSub];
-#pragma unroll
-          for (int u = 0; u < kSub; ++u) rows[u] = row_at(t0 + 16 * u);
-          St::values_checked(w, a.c, rows, lane, p, live, seen);
-        } else if constexpr (kTwo) {
-          if (a.q_f16) St::template values<true>(w, st, lane, live, p);
-          else St::template values<false>(w, st, lane, live, p);
-        } else {
-          St::template values<false>(w, st, lane, live, p);
-        }
+        if (now) add_step<KIND, FMT, D, NT, false>(w, a, it, rows, st, q, lane, s * S::kRows, live);
       }
       slot_out = slot_out + 1 == kStages ? 0 : slot_out + 1;
+    }
+    if constexpr (KIND != BRC_STE_NVFP4) {
+      if (later.count || s < s_end) {
+        cp_wait<0>();
+        __syncwarp();
+        Passes<KIND, FMT, D, NT> x{w, it, rows};
+        add_in_passes<KIND, FMT, D, NT>(x, a, rings + warp * (kStages * S::kStageBytes), q, lane,
+                                        later, s, s_end, token_warps);
+        w = x.w;
+      }
     }
     cp_wait<0>();
 
@@ -1020,7 +1383,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
         }
       }
     __syncthreads();  // the stages are no longer read
-    const float scale_o = w.e < -900 ? 1.f : exp2f((float)(w.e - 6 - kSumDown));
     constexpr int kPitch = D + 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -1028,6 +1390,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND, D, NT)) k_attend
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int j = 0; j < S::kTiles; j += 2) {
+          const float scale_o = exp2f((float)(w.e[j / (S::kTiles / w.kOwn)] - 133 - kSumDown));
           const int rr = 8 * n + 2 * (lane & 3) + x;
           *reinterpret_cast<float4*>(so + (warp * 8 * NT + rr) * kPitch + S::elem(2 * j, lane >> 2)) =
               make_float4(w.o[n][j][x] * scale_o, w.o[n][j][2 + x] * scale_o,

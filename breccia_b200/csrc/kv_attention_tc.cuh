@@ -20,6 +20,12 @@
 // TMEM: two score tiles and two output tiles of 128 columns. The codes are decoded
 // once for 256 rows, where the register path decodes them for every 32.
 //
+// Values are relative to one power of two for each of their scales' channel blocks. A tile
+// whose scales lie too far apart for that (keys: for one power of two) is walked in several
+// passes, each with the tokens that go together and the others hidden; the scales' warp
+// says so, and every role walks passes. So the scale of a token does not touch another
+// one's bits, whether a row sees it or not.
+//
 // A row's shift follows its maximum only when 32 probabilities sum to 2^kRise above it
 // (the register path's rule, with less room above for more bits below in f16); then the
 // softmax threads rescale their row of O in TMEM. The two threads of a row may use
@@ -42,34 +48,31 @@ using namespace sm100;
 constexpr int kTok = 128;
 constexpr int kLift = 9;  // log2 of the factor that probabilities carry in f16
 constexpr int kRise = 6;  // log2 of how far a sum of 32 of them may pass it
-// Values are relative to the largest scale of their item's tiles so far, and this much
-// (log2) above it, so that it seldom rises.
-constexpr int kSlack = 2;
 constexpr int kSoftWarps = 16, kLoadWarps = 8;
 constexpr int kTcThreads = (kSoftWarps + kLoadWarps + 4) * 32;  // whole warpgroups: two warps idle
 // Registers of a thread after setmaxnreg, by warpgroup; 4 x softmax + 2 x codes +
 // products are no more than the 7 x 72 that the block was launched with. Block FP8's
 // softmax, which holds the keys' scales too, takes them from the other warps (8 trees
-// of 64 nodes over 16384 tokens: 480 -> 452 us; MXFP8, whose codes need theirs, 410 ->
-// 426).
+// of 64 nodes over 16384 tokens: 480 -> 452 us), and so does NVFP4's (366 -> 355); MXFP8,
+// whose codes need theirs, takes longer so (412 -> 427).
 template <int KIND>
 struct Regs {
-  static constexpr bool kBlock = KIND == BRC_STE_BLOCK_FP8;
-  static constexpr uint32_t kSoft = kBlock ? 88 : 80, kLoad = kBlock ? 56 : 64, kMma = kBlock ? 40 : 56;
+  static constexpr bool kMx = KIND == BRC_STE_MXFP8;
+  static constexpr uint32_t kSoft = kMx ? 80 : 88, kLoad = kMx ? 64 : 56, kMma = kMx ? 56 : 40;
   static_assert(4 * kSoft + 2 * kLoad + kMma <= 7 * 72, "registers of the launch");
 };
-// A tile's Meta is written when the scores of the tile two before are done, so that the
+// A pass's Meta is written when the scores of the pass two before are done, so that the
 // softmax three before is over: a ring of four.
 constexpr int kMeta = 4;
 constexpr int kBlockBytes = 128 * 128;  // 128 rows of 64 f16, swizzled
 
 struct alignas(16) Meta {
   float sk[kTok];  // block FP8
-  // Exponents (MXFP8: as E8M0) that keys are relative to in this tile, values in this
-  // and all later ones until it rises
-  int ek, ev;
-  uint32_t live[4];          // token 4 i + k: bit i of word k
-  uint32_t all;              // every token is live
+  int ek;            // MXFP8: what keys are relative to, as E8M0
+  uint32_t ev;       // what values are relative to: a biased exponent to each channel block
+  uint32_t all;      // every token of the tile is in this pass
+  uint32_t more;     // another pass of the tile follows
+  uint32_t live[4];  // which are: token 4 i + k, bit i of word k
 };
 
 template <int D>
@@ -82,7 +85,13 @@ struct alignas(128) Smem {
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
   Place place;
   uint32_t tmem, abort;
-  float pair[2][2][2][128];  // [tile parity][row tile][half][row]: shifts, then sums
+  float pair[2][2][2][128];    // [turn][row tile][half][row]: shifts, then sums
+  uint8_t sees[2][2][2][128];  // whether the row sees any of the half's places
+  // What a thread's part of a row of O is relative to (a byte to a channel block), and the
+  // most that it was while the row saw something. It follows the values, but not below
+  // 2^-60 of that, and only where the row sees them.
+  uint2 refs[2][2][128];
+  uint32_t start[4];           // first pass of an item, one slot to an item as of odd
   // Numbers of items whose drafted values are not all finite: one slot to an item, as
   // the loads are at most two items ahead.
   uint32_t odd[4];
@@ -202,17 +211,18 @@ struct Loader {
         }
       }
   }
-  // Decode into a stage. `first`: token of the warp's first row; rows from `dead`
-  // on hold anything and become zero. ODD: of drafted tokens (from `drafted` on), what
+  // Decode into a stage. `first`: token of the warp's first row; `refs`: what each
+  // channel block is relative to (a byte); tokens 8 g + lane / 4 of the warp without
+  // bit g of `on` become zero. ODD: of drafted tokens (from `drafted` on), what
   // is not finite becomes zero too, code by code or scale by scale; returns whether
   // there was any (the epilogue adds it to the rows that see it). VALUES:
-  // of block FP8 times scale * 2^(kValueLift - ref), which rounds them to f16 once (as
+  // of block FP8 times scale * 2^(kValueLift + 127 - ref), which rounds them to f16 once (as
   // the probabilities are). That factor on the probabilities instead, as on the scores,
   // has every softmax thread read every token's from shared memory, 16 bytes to each
   // lane (8 trees of 64 nodes over 16384 tokens: 498 us).
   template <bool ODD, bool VALUES>
-  __device__ __forceinline__ bool decode(uint8_t* stage, int first, int lane, int ref,
-                                         int dead, int drafted) {
+  __device__ __forceinline__ bool decode(uint8_t* stage, int first, int lane, uint32_t refs,
+                                         uint32_t on, int drafted) {
     bool any = false;
 #pragma unroll
     for (int g = 0; g < kG; ++g) {
@@ -221,7 +231,8 @@ struct Loader {
       for (int i = 0; i < kHalves; ++i) {
         const int piece = 4 * i + (lane & 3);
         uint32_t x[4] = {w[g][i].x, w[g][i].y, w[g][i].z, w[g][i].w};
-        bool zero = t >= dead;
+        bool zero = !((on >> g) & 1u);
+        const int ref = (int)((refs >> (8 * (piece / 2))) & 0xFFu);
         if constexpr (ODD) {
           if (t >= drafted && !zero) {
             if constexpr (KIND == BRC_STE_NVFP4) {  // a scale of 16 elements each
@@ -260,9 +271,9 @@ struct Loader {
 #pragma unroll
             for (int y = 0; y < 8; ++y) h[y] = hmul2(h[y], f);
           } else if constexpr (VALUES) {
-            constexpr int kDown = kValueLift<FMT> < 0 ? 2 : 0;  // (ref may be 127)
+            constexpr int kDown = kValueLift<FMT> < 0 ? 2 : 0;  // (the reference may be 254)
             const float f = __uint_as_float(s[g][i]) * (kDown ? 0.25f : 1.f) *
-                            __uint_as_float((uint32_t)(127 + kValueLift<FMT> + kDown - ref) << 23);
+                            __uint_as_float((uint32_t)(254 + kValueLift<FMT> + kDown - (int)(refs & 0xFFu)) << 23);
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
               const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&h[y]));
@@ -284,7 +295,7 @@ struct Loader {
   }
 };
 
-// The scales of a tile's tokens 4 lane .. + 3: what the tile is relative to.
+// The scales of a tile's tokens 4 lane .. + 3.
 template <int KIND, int D>
 struct Scales {
   using S = Shape<KIND, D>;
@@ -307,39 +318,12 @@ struct Scales {
       }
     }
   }
-  // Largest exponent of the tile's live tokens that is finite: an E8M0 byte below 255,
-  // or a float32 scale's; every lane gets it.
-  __device__ __forceinline__ int top(int live4) const {
-    uint32_t m = 0;
-    uint32_t v[4] = {e.x, e.y, e.z, e.w};
-    if constexpr (KIND == BRC_STE_BLOCK_FP8) {
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const uint32_t x = v[y] & 0x7FFFFFFFu;
-        if (y < live4 && x < 0x7F800000u) m = max(m, x);
-      }
-      return max((int)(__reduce_max_sync(0xFFFFFFFFu, m) >> 23) - 127, -100);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (D == 128) {
-          if (i >= live4) v[i] = 0u;
-        } else {  // two bytes to a token
-          v[i] &= (2 * i < live4 ? 0xFFFFu : 0u) | (2 * i + 1 < live4 ? 0xFFFF0000u : 0u);
-        }
-        // a byte of 255 shows as a zero byte of ~v
-        if ((~v[i] - 0x01010101u) & v[i] & 0x80808080u) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (((v[i] >> (8 * y)) & 0xFFu) == 0xFFu) v[i] &= ~(0xFFu << (8 * y));
-        }
-      }
-      m = __vmaxu2(__vmaxu2(v[0] & 0x00FF00FFu, v[1] & 0x00FF00FFu),
-                   __vmaxu2((v[0] >> 8) & 0x00FF00FFu, (v[1] >> 8) & 0x00FF00FFu));
-      m = __vmaxu2(m, __vmaxu2(__vmaxu2(v[2] & 0x00FF00FFu, v[3] & 0x00FF00FFu),
-                               __vmaxu2((v[2] >> 8) & 0x00FF00FFu, (v[3] >> 8) & 0x00FF00FFu)));
-      return (int)__reduce_max_sync(0xFFFFFFFFu, max(m & 0xFFFFu, m >> 16));
-    }
+  // Token y's biased exponents, a byte to each channel block.
+  __device__ __forceinline__ uint32_t bytes(int y) const {
+    const uint32_t w[4] = {e.x, e.y, e.z, e.w};
+    if constexpr (KIND == BRC_STE_BLOCK_FP8) return (w[y] >> 23) & 0xFFu;
+    else if constexpr (D == 128) return w[y];
+    else return (w[y / 2] >> (16 * (y & 1))) & 0xFFFFu;
   }
 };
 
@@ -402,22 +386,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes, in bits 16 ..
     const uint32_t sc = (r ? s_col[1] : s_col[0]) + lanes + 64 * half;
     const uint32_t oc = (r ? o_col[1] : o_col[0]) + lanes + (D / 2) * half;
-    // The two warps of 32 rows meet once a tile. A warp that leaves early arrives
+    // channel block of this half's 16 columns c (block FP8: the only one)
+    auto channel_block = [&](int c) { return KIND == BRC_STE_MXFP8 ? (D / 2 * half + 16 * c) / 32 : 0; };
+    // The two warps of 32 rows meet once a pass. A warp that leaves early arrives
     // in its place, and the other one finds the abort flag at its next wait.
     const uint32_t pair_id = 1 + r * 4 + (warp & 3);
     auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair_id) : "memory"); };
     auto leave = [&]() { asm volatile("barrier.cta.arrive %0, 64;" ::"r"(pair_id) : "memory"); };
-    uint32_t tile = 0, number = 0;  // tiles and items so far
+    uint32_t pass = 0, number = 0, turn = 0;  // passes and items so far; times met
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
     for (; ok && walk.take(a); walk.next()) {
       ++number;
       const Seq seq = walk.seq;
       const int rows_left = a.rows - walk.row0;
-      const bool active = r == 0 || rows_left > 128;
-      const uint32_t tile0 = tile;
-      tile += walk.s_end - walk.s_begin;
-      if (!active) continue;
+      if (r != 0 && rows_left <= 128) continue;
       const int row = walk.row0 + r * 128 + mine, node = row / a.group;
       const bool valid = row < a.rows && node < seq.drafts;
       const int64_t at_row = ((int64_t)walk.b * a.draft + node) * a.hq + walk.head * a.group +
@@ -460,15 +443,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         if (lane == 0) mbar_arrive(&sm.q_full[r]);
       }
       float m = -INFINITY, l = 0.f;
-      int ev = -1000;
-      for (int j = walk.s_begin; j < walk.s_end; ++j) {
+      bool fresh = true;
+      uint2& refs = sm.refs[r][half][mine];
+      for (int j = walk.s_begin; j < walk.s_end;) {
         if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.s_full[r], s_phase, abort, status, 1u)))) {
           leave();
           break;
         }
         s_phase ^= 1u;
         tc_fence_after();
-        const Meta& meta = sm.meta[(tile0 + (j - walk.s_begin)) % kMeta];
+        if (fresh) pass = sm.start[number & 3u];
+        const Meta& meta = sm.meta[pass++ % kMeta];
+        const bool more = meta.more;
         const int64_t t0 = (int64_t)j * kTok;
         // (a factor of zero, of a scale of zero or by underflow, would make NaN of the
         // hidden places' minus infinity; a score, below 2^40, times 2^-126 is nothing)
@@ -492,7 +478,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           }
         }
         __syncwarp();
-        const float2 f2 = make_float2(f, f);
         // 32 scores in units of the row's factor; masked ones -inf
         auto take = [&](const uint32_t (&x)[32], int c, float2 (&u)[16]) {
 #pragma unroll
@@ -515,30 +500,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             }
           }
         };
-        // O times g; the products up to here are done: S came after them
-        auto scale_o = [&](float g) {
-          if (j == walk.s_begin) return;
+        // O times g, and relative to `to`; the products up to here are done: S came after
+        auto scale_o = [&](float g, uint32_t from, uint32_t to) {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {  // this thread's half of the columns
             uint32_t x[16];
             tmem_ld16(oc + 16 * c, x);
             tmem_ld_wait16(x);
+            const int shift = 8 * channel_block(c);
+            const int by = (int)((from >> shift) & 0xFFu) - (int)((to >> shift) & 0xFFu);
+            // (the two may be further apart than one float32 exponent)
+            const int near = max(by, -127);
+            const float h = g * kv::pow2i(near - near / 2), h2 = kv::pow2i(near / 2);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * g);
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * h * h2);
             tmem_st16(oc + 16 * c, x);
           }
         };
-        if constexpr (KIND != BRC_STE_NVFP4) {
-          if (meta.ev > ev) {  // (the same for every row)
-            if (ev > -900) scale_o(__uint_as_float((uint32_t)max(127 + ev - meta.ev, 0) << 23));
-            ev = meta.ev;
-          }
-        }
         // This half's shift: the row's, until a score is far above it (and at first the
         // half's maximum). Shifts are whole numbers: less the lift they are exact, so
         // that the row's log-sum-exp does not get their rounding.
         float own = m;
-        if (j == walk.s_begin) {
+        if (fresh) {
           float top = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
@@ -580,11 +563,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             tmem_st16(sc + 16 * b, z);
           }
         };
-        auto exps = [&](float2 (&u)[16]) {
+        auto exps = [&](float2 (&u)[16], float by, float add) {
           float2 t = make_float2(0.f, 0.f);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            u[i] = __ffma2_rn(u[i], f2, make_float2(base, base));
+            u[i] = __ffma2_rn(u[i], make_float2(by, by), make_float2(add, add));
             u[i] = make_float2(ex2(u[i].x), ex2(u[i].y));
             t = __fadd2_rn(t, u[i]);
           }
@@ -599,12 +582,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           tmem_ld_wait();
           reg_bind32(x);
           take(x, c, u);
-          float2 t = exps(u);
-          // a score far above the shift shows in the sum; a row that has seen nothing so
-          // far has the shift 0, below which its scores may vanish: it always looks
-          const float all = t.x + t.y;
-          const bool sees = !masked || (c ? vis[1] : vis[0]) != 0u;
-          if (__any_sync(0xFFFFFFFFu, all > most || (own == -INFINITY && sees))) {
+          float2 t;
+          float by = f, add = base;
+#pragma unroll 1
+          for (bool looked = false;; looked = true) {
+            t = exps(u, by, add);
+            // a score far above the shift shows in the sum; a row that has seen nothing so
+            // far has the shift 0, below which its scores may vanish: it always looks
+            if (looked || !__any_sync(0xFFFFFFFFu, t.x + t.y > most || own == -INFINITY)) break;
             tmem_ld32(sc + 32 * c, x);
             tmem_ld_wait();
             reg_bind32(x);
@@ -618,15 +603,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             base = kLift - (own == -INFINITY ? 0.f : own);
             l2 = __fmul2_rn(l2, make_float2(g, g));
             scale_p(c, g);
-            // as exps, with the rounded product (the compiler may join packed operations)
+            // the rounded product (the compiler may join packed operations)
             const float down = own == -INFINITY ? 0.f : -own;
-            t = make_float2(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              u[i].x = ex2(__fadd_rn(__fadd_rn(__fmul_rn(u[i].x, f), down), kLift));
-              u[i].y = ex2(__fadd_rn(__fadd_rn(__fmul_rn(u[i].y, f), down), kLift));
-              t = __fadd2_rn(t, u[i]);
+              u[i].x = __fadd_rn(__fmul_rn(u[i].x, f), down);
+              u[i].y = __fadd_rn(__fmul_rn(u[i].y, f), down);
             }
+            by = 1.f;
+            add = kLift;
           }
           l2 = __fadd2_rn(l2, t);
           uint32_t p[16];
@@ -635,25 +620,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           tmem_st16(sc + 16 * c, p);
         }
         // ---- the halves agree on the row's shift
-        const uint32_t parity = (tile0 + (j - walk.s_begin)) & 1u;
-        sm.pair[parity][r][half][mine] = own;
+        sm.pair[turn][r][half][mine] = own;
+        bool sees = !masked || (vis[0] | vis[1]) != 0u;
+        if (masked && KIND != BRC_STE_NVFP4) sm.sees[turn][r][half][mine] = sees;
         meet();
-        const float nm = fmaxf(own, sm.pair[parity][r][half ^ 1][mine]);
+        const float nm = fmaxf(own, sm.pair[turn][r][half ^ 1][mine]);
+        const bool moved = KIND != BRC_STE_NVFP4 && (fresh || meta.ev != refs.x);
         float part = (l2.x + l2.y) * (1.f / (1 << kLift));
-        if (__any_sync(0xFFFFFFFFu, nm != own || nm != m)) {
+        if (__any_sync(0xFFFFFFFFu, nm != own || nm != m || moved)) {
           const float gp = nm == own || nm == -INFINITY ? 1.f : ex2(own - nm);
           const float go = nm == m || nm == -INFINITY ? 1.f : ex2(m - nm);
           if (__any_sync(0xFFFFFFFFu, gp != 1.f)) scale_p(2, gp);
-          if (__any_sync(0xFFFFFFFFu, go != 1.f)) scale_o(go);
+          uint32_t from = 0, to = 0;
+          if (moved) {
+            from = to = refs.x;
+            uint32_t most_seen = fresh ? 0u : refs.y;
+            if (masked) sees |= sm.sees[turn][r][half ^ 1][mine] != 0;
+            if (sees) {
+              to = __vmaxu4(meta.ev, __vsubus4(most_seen, 0x3C3C3C3Cu));
+              most_seen = __vmaxu4(most_seen, to);
+            }
+            if (fresh) to = meta.ev;
+            refs = make_uint2(to, most_seen);
+          }
+          if (!fresh && __any_sync(0xFFFFFFFFu, go != 1.f || to != from)) scale_o(go, from, to);
           part *= gp;
           l *= go;
           m = nm;
         }
+        turn ^= 1u;
         l += part;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[r]);
+        fresh = false;
+        if (!more) ++j;
       }
       if (!ok) break;
       // ---- the item's output
@@ -661,19 +663,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         leave();
         break;
       }
-      // the row's sum, of both halves (the slots of the next tile's parity are free:
-      // the other half has read them before it met this one at the last tile)
-      sm.pair[tile & 1u][r][half][mine] = l;
+      // the row's sum, of both halves (this turn's slots are free: the other half has
+      // read them before it met this one last)
+      sm.pair[turn][r][half][mine] = l;
       meet();
-      l = half ? sm.pair[tile & 1u][r][0][mine] + l : l + sm.pair[tile & 1u][r][1][mine];
+      l = half ? sm.pair[turn][r][0][mine] + l : l + sm.pair[turn][r][1][mine];
+      turn ^= 1u;
       o_phase ^= 1u;
       tc_fence_after();
       const bool whole = walk.s_begin == 0 && walk.s_end == seq.steps;
-      const float so = KIND == BRC_STE_NVFP4 ? 1.f / (1 << kLift)
-                       : ev < -900 ? 1.f
-                                   : exp2f((float)(ev - (KIND == BRC_STE_MXFP8 ? 127 : kValueLift<FMT>) - kLift));
       const bool none = !valid || l == 0.f;
-      const float mul = whole ? (none ? 0.f : so / l) : so * (1.f / kSumUp);
+      const float so = whole ? (none ? 0.f : 1.f / l) : 1.f / kSumUp;
       const bool odd = sm.odd[number & 3u] == number && !none;
       const int64_t slot = 2 * (int64_t)blockIdx.x + (walk.s_begin > 0 ? 0 : 1);
       const int rr = r * 128 + mine;
@@ -684,6 +684,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         __syncwarp();
         tmem_ld16(oc + 16 * c, x);
         tmem_ld_wait16(x);
+        float mul = so * (1.f / (1 << kLift));
+        if constexpr (KIND != BRC_STE_NVFP4) {
+          constexpr int kOff = KIND == BRC_STE_MXFP8 ? 0 : kValueLift<FMT>;
+          mul *= exp2f((float)((int)((refs.x >> (8 * channel_block(c))) & 0xFFu) - 127 - kOff));
+        }
         float o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = none ? 0.f : __uint_as_float(x[i]) * mul;
@@ -742,7 +747,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     // ================================================================ codes
     regs_dec<Regs<KIND>::kLoad>();
     const int lw = warp - kSoftWarps, first = kTok / kLoadWarps * lw;
-    uint32_t tile = 0, number = 0;
+    uint32_t pass = 0, number = 0;
     bool ok = true;
     for (; ok && walk.take(a); walk.next()) {
       ++number;
@@ -770,41 +775,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       rows_of(walk.s_begin);
       k.template fetch<false>(a.c.k_data, a.c.k_scale, row, lane);
       pages_of(walk.s_begin + 1);
-      for (int j = walk.s_begin; j < walk.s_end; ++j, ++tile) {
-        const uint32_t st = tile & 1u, use = (tile >> 1) & 1u;
+      for (int j = walk.s_begin; j < walk.s_end; ++pass) {
+        const uint32_t st = pass & 1u, use = (pass >> 1) & 1u;
         const int64_t t0 = (int64_t)j * kTok;
-        const int dead = (int)min((int64_t)kTok, seq.total - t0);
         const bool drafted = t0 + kTok > seq.context;
         const int from = (int)max((int64_t)0, seq.context - t0);
         v.template fetch<true>(a.c.v_data, a.c.v_scale, row, lane);
         // (the scales' warp has waited for the key stage)
         if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.meta_full[st], use, abort, status, 1u)))) break;
-        const int ek = sm.meta[tile % kMeta].ek, ev = sm.meta[tile % kMeta].ev;
-        k.template decode<false, false>(sm.k[st][0], first, lane, ek, dead, kTok);
+        const Meta& meta = sm.meta[pass % kMeta];
+        const uint32_t ek = (uint32_t)meta.ek * 0x01010101u, ev = meta.ev;
+        const bool more = meta.more;
+        uint32_t on = 0;
+#pragma unroll
+        for (int g = 0; g < kG; ++g) {
+          const int t = first + 8 * g + (lane >> 2);
+          on |= ((meta.live[t & 3] >> (t >> 2)) & 1u) << g;
+        }
+        k.template decode<false, false>(sm.k[st][0], first, lane, ek, on, kTok);
         fence_proxy_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.k_full[st]);
-        if (j + 1 < walk.s_end) {
+        if (more) {
+          k.template fetch<false>(a.c.k_data, a.c.k_scale, row, lane);
+        } else if (j + 1 < walk.s_end) {
           rows_of(j + 1);
           k.template fetch<false>(a.c.k_data, a.c.k_scale, row, lane);
           pages_of(j + 2);
         }
         if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.v_empty[st], use ^ 1u, abort, status, 1u)))) break;
         if (drafted) {
-          if (v.template decode<true, true>(sm.v[st][0], first, lane, ev, dead, from)) sm.odd[number & 3u] = number;
+          if (v.template decode<true, true>(sm.v[st][0], first, lane, ev, on, from)) sm.odd[number & 3u] = number;
         } else {
-          v.template decode<false, true>(sm.v[st][0], first, lane, ev, dead, kTok);
+          v.template decode<false, true>(sm.v[st][0], first, lane, ev, on, kTok);
         }
         fence_proxy_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.v_full[st]);
+        if (!more) ++j;
       }
     }
   } else {
     // ================================================================ products
     regs_dec<Regs<KIND>::kMma>();
     if (warp == kSoftWarps + kLoadWarps) {
-    uint32_t tile = 0, q_phase = 0, p_phase[2] = {0, 0}, q_phase1 = 0;
+    uint32_t pass = 0, q_phase = 0, p_phase[2] = {0, 0}, q_phase1 = 0;
     bool ok = true;
     constexpr uint32_t kIdS = idesc_f16(128, kTok, false), kIdO = idesc_f16(128, D, true);
     const uint64_t hi_k = desc_sw128_hi();
@@ -825,23 +840,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     };
     for (; ok && walk.take(a); walk.next()) {
       const int tiles = a.rows - walk.row0 > 128 ? 2 : 1;
-      const int n = walk.s_end - walk.s_begin;
       for (int r = 0; ok && r < tiles; ++r) {
         ok = wait(&sm.q_full[r], r ? q_phase1 : q_phase);
         if (r) q_phase1 ^= 1u;
         else q_phase ^= 1u;
-        if (ok && r == 0) ok = wait(&sm.k_full[tile & 1u], (tile >> 1) & 1u);
+        if (ok && r == 0) ok = wait(&sm.k_full[pass & 1u], (pass >> 1) & 1u);
         tc_fence_after();
-        if (ok) scores(r, tile & 1u);
+        if (ok) scores(r, pass & 1u);
       }
-      if (ok && elect_lane()) tc_commit(&sm.k_empty[tile & 1u]);
+      if (ok && elect_lane()) tc_commit(&sm.k_empty[pass & 1u]);
       __syncwarp();
-      for (int j = 0; ok && j < n; ++j, ++tile) {
-        const uint32_t st = tile & 1u, nx = (tile + 1) & 1u;
+      bool fresh = true;
+      for (int j = walk.s_begin; ok && j < walk.s_end; ++pass, fresh = false) {
+        const uint32_t st = pass & 1u, nx = (pass + 1) & 1u;
+        if (!sm.meta[pass % kMeta].more) ++j;  // (written before this pass's keys)
+        const bool last = j == walk.s_end;
         for (int r = 0; ok && r < tiles; ++r) {
           ok = wait(&sm.p_full[r], p_phase[r]);
           p_phase[r] ^= 1u;
-          if (ok && r == 0) ok = wait(&sm.v_full[st], (tile >> 1) & 1u);
+          if (ok && r == 0) ok = wait(&sm.v_full[st], (pass >> 1) & 1u);
           tc_fence_after();
           if (!ok) break;
           if (elect_lane()) {
@@ -849,13 +866,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             for (int i = 0; i < kTok / 16; ++i)  // 16 tokens: 8 columns of P (each half's at its own start), 16 rows of V
               mma_f16_ts(o_col[r], s_col[r] + 64 * (i / 4) + 8 * (i % 4),
                          smem_desc(smem_u32(sm.v[st][0]) + 2048 * i, kBlockBytes, 1024, 2), kIdO,
-                         j > 0 || i > 0);
-            if (j + 1 == n) tc_commit(&sm.o_full[r]);
+                         !fresh || i > 0);
+            if (last) tc_commit(&sm.o_full[r]);
             if (r + 1 == tiles) tc_commit(&sm.v_empty[st]);
           }
           __syncwarp();
-          if (j + 1 < n) {
-            if (r == 0) ok = wait(&sm.k_full[nx], ((tile + 1) >> 1) & 1u);
+          if (!last) {
+            if (r == 0) ok = wait(&sm.k_full[nx], ((pass + 1) >> 1) & 1u);
             tc_fence_after();
             if (!ok) break;
             scores(r, nx);
@@ -874,9 +891,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
     mbar_wait(&sm.drain, 0u, &none, status, 1u);
     } else if (warp == kSoftWarps + kLoadWarps + 1) {
       // ============================================================== scales
-      uint32_t tile = 0;
+      uint32_t pass = 0, number = 0;
       bool ok = true;
       for (; ok && walk.take(a); walk.next()) {
+        ++number;
         const Seq seq = walk.seq;
         const int32_t* const table = a.table + walk.b * a.table_stride;
         const int64_t head_row = (int64_t)walk.head * a.c.page_size;
@@ -891,36 +909,67 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         k.fetch(a.c.k_scale, row);
         v.fetch(a.c.v_scale, row);
         page = page_of(walk.s_begin + 1);
-        int run = -1000;
-        for (int j = walk.s_begin; j < walk.s_end; ++j, ++tile) {
-          const uint32_t st = tile & 1u, use = (tile >> 1) & 1u;
-          const int left = (int)min((int64_t)kTok, seq.total - (int64_t)j * kTok) - 4 * lane;
-          const int live4 = row < 0 ? 0 : min(max(left, 0), 4);
-          int ek = 0;
-          if constexpr (KIND == BRC_STE_MXFP8) ek = k.top(live4);
-          if constexpr (KIND != BRC_STE_NVFP4) {
-            constexpr int k100 = KIND == BRC_STE_MXFP8 ? 27 : -100;  // 2^-100
-            const int top = max(v.top(live4), k100);
-            if (top > run) run = min(top + kSlack, k100 + 227);
-          }
-          if (!(ok = __all_sync(0xFFFFFFFFu,
-                                mbar_wait(&sm.k_empty[st], use ^ 1u, abort, status, 1u))))
-            break;
-          Meta& meta = sm.meta[tile % kMeta];
-          if constexpr (KIND == BRC_STE_BLOCK_FP8)
-            *reinterpret_cast<uint4*>(&meta.sk[4 * lane]) = k.e;
-          uint32_t bal[4];
+        constexpr int kBlocks = kScaleBlocks<KIND, D>;
+        // what values are relative to, at first: the lowest
+        uint32_t refs[1] = {kLowest * (kBlocks == 1 ? 1u : kBlocks == 2 ? 0x0101u : 0x01010101u)};
+        bool fresh = true;
+        for (int j = walk.s_begin; ok && j < walk.s_end; ++j) {
+          const int there = (int)min((int64_t)kTok, seq.total - (int64_t)j * kTok) - 4 * lane;
+          const int live4 = row < 0 ? 0 : min(max(there, 0), 4);
+          uint32_t left = (1u << live4) - 1u, take, more;
+          do {
+            take = left;
+            int ek = 0;
+            if constexpr (KIND != BRC_STE_NVFP4) {
+              uint32_t vb[4][1], km[4] = {0u, 0u, 0u, 0u}, hi = 0, lo = 255;
+              constexpr uint32_t kFar = kSpan<KIND, FMT>;
+              const Near<KIND == BRC_STE_MXFP8 ? kFar : 15> near(refs[0]);
+              bool off = false;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) bal[y] = __ballot_sync(0xFFFFFFFFu, y < live4);
-          if (lane == 0) {
-            meta.ek = ek;
-            meta.ev = run;
+              for (int y = 0; y < 4; ++y) {
+                vb[y][0] = v.bytes(y);
+                if constexpr (KIND == BRC_STE_MXFP8) km[y] = top_byte(k.bytes(y));
+                if ((left >> y) & 1u) {
+                  off |= KIND == BRC_STE_MXFP8 ? !near(vb[y][0]) : refs[0] - vb[y][0] > kFar;
+                  hi = max(hi, km[y]);
+                  lo = min(lo, km[y]);
+                }
+              }
+              if constexpr (KIND == BRC_STE_MXFP8) {
+                hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+                off |= lo + kFar < hi;
+              }
+              ek = (int)hi;
+              if (__any_sync(0xFFFFFFFFu, off))
+                ek = (int)choose<kFar, kBlocks>(vb, km, left, take, refs);
+            }
+            more = __any_sync(0xFFFFFFFFu, (left & ~take) != 0u);
+            left &= ~take;
+            const uint32_t st = pass & 1u, use = (pass >> 1) & 1u;
+            if (!(ok = __all_sync(0xFFFFFFFFu,
+                                  mbar_wait(&sm.k_empty[st], use ^ 1u, abort, status, 1u))))
+              break;
+            Meta& meta = sm.meta[pass % kMeta];
+            if constexpr (KIND == BRC_STE_BLOCK_FP8)
+              *reinterpret_cast<uint4*>(&meta.sk[4 * lane]) = k.e;
+            uint32_t bal[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) meta.live[y] = bal[y];
-            meta.all = (bal[0] & bal[1] & bal[2] & bal[3]) == 0xFFFFFFFFu;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.meta_full[st]);
+            for (int y = 0; y < 4; ++y) bal[y] = __ballot_sync(0xFFFFFFFFu, (take >> y) & 1u);
+            if (lane == 0) {
+              meta.ek = ek;
+              meta.ev = refs[0];
+              meta.more = more;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) meta.live[y] = bal[y];
+              meta.all = (bal[0] & bal[1] & bal[2] & bal[3]) == 0xFFFFFFFFu;
+              if (fresh) sm.start[number & 3u] = pass;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.meta_full[st]);
+            ++pass;
+            fresh = false;
+          } while (more);
+          if (!ok) break;
           row = slot_of(a, page, head_row, (j + 1) * kTok + 4 * lane);
           k.fetch(a.c.k_scale, row);
           v.fetch(a.c.v_scale, row);
