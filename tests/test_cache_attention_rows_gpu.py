@@ -9,11 +9,12 @@ float32 sum of d products, off by at most d 2^-24 of the sum of magnitudes (S: t
 largest among the places that the row sees). A probability is off by that much
 relatively, by the exponential's 2^-21, and by one rounding to f16: 2^-11 of it or,
 below f16's normal numbers, 2^-31 of the row's largest (2^-20 on the register path of
-block FP8, where it carries a scale that may lie 2^11 below the reference). Values on
+block FP8, where it carries a scale that may lie 2^11 below the reference), or all of it
+where that is less. Values on
 tcgen05 in block FP8 are rounded to f16 once more: 2^-11 of them or, for E5M2's
 smallest codes, 2^-24 of the token's largest. Sums are float32. So an output is within
 
-    (2^-10 + 2 d 2^-24 S) sum p |v| + 2^-24 sum p max |v| + f max p sum |v|
+    (2^-10 + 2 d 2^-24 S) sum p |v| + 2^-24 sum p max |v| + sum min(p, f max p) |v|
 
 of the formula (f: 2^-31 or 2^-20), and half an ulp of its type; log-sum-exp is within
 d 2^-24 S + 2^-20 (1 + |lse|).
@@ -88,7 +89,7 @@ def verify(c, got, see, scale=None, columns=None, rows=None):
         vv = whole if columns is None else whole[..., columns]
         want, mass = p @ vv, p @ vv.abs()
         largest = p @ whole.abs().amax(-1, keepdim=True)
-        low = p.amax(-1, keepdim=True) * (m.double() @ vv.abs())
+        low = torch.minimum(p, floor * p.amax(-1, keepdim=True)) @ vv.abs()
         o, l = out[b].double().transpose(0, 1), lse[b].double().transpose(0, 1)
         if columns is not None:
             o = o[..., columns]
@@ -97,7 +98,7 @@ def verify(c, got, see, scale=None, columns=None, rows=None):
         assert not o[:, none].any() and bool((l[:, none] == -math.inf).all())
         keep = keep & ~none
         tol = (2.0 ** -10 + 2 * c.d * 2.0 ** -24 * big[..., None]) * mass + \
-            HALF_ULP[out.dtype] * want.abs() + 2.0 ** -24 + 2.0 ** -24 * largest + floor * low
+            HALF_ULP[out.dtype] * want.abs() + 2.0 ** -24 + 2.0 ** -24 * largest + low
         err = (o - want).abs()
         assert bool((err <= tol)[:, keep].all()), (b, float((err / tol)[:, keep].nan_to_num(nan=math.inf).max()))
         ltol = d_tol(c.d, big, want_lse)
@@ -222,6 +223,22 @@ def test_trees_of_separate_blocks(name, draft, group, ctx):
     see = with_tree(c, tree)
     see[0][draft // 2:, :ctx] = True
     verify(c, c.run(scale=1.0, tree_mask=tree), see, 1.0)
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_random_trees_and_missing_drafts(name, draft, group):
+    c = Case(name, 64, 2, group, [0, 77, 128], draft, page=32, seed=35)
+    tree = torch.rand(3, draft, draft, generator=torch.Generator().manual_seed(36)) < 0.3
+    tree[:, 1] = False
+    tree = tree.cuda()
+    drafts = [draft, draft - 2, 1]
+    see = with_tree(c, tree)
+    for b, n in enumerate(drafts):
+        see[b][n:] = False
+        see[b][:, c.ctx[b] + n:] = False
+    lens = torch.tensor(drafts, dtype=torch.int32, device="cuda")
+    verify(c, c.run(tree_mask=tree, draft_lens=lens), see)
 
 
 # ------------------------------------------------------------------ what is not finite
@@ -413,18 +430,80 @@ def test_large_values_with_little_weight(name, d, draft, group):
 @pytest.mark.parametrize("name", ["mx4", "block4"])
 def test_many_steps_of_sizes_apart(name):
     """Hardly any step's tokens go together, and a warp has more steps than it notes."""
-    heads, d, ctx, page = 32, 64, 16400, 64
+    heads, d, ctx, page, n = 32, 64, 16400, 64, 3
     pages = -(-(ctx + 1) // page)
-    cache = bb().QuantizedKVCache(2 * pages, page, heads, d, recipe(name, d))
+    cache = bb().QuantizedKVCache(n * pages, page, heads, d, recipe(name, d))
     g = torch.Generator("cuda").manual_seed(49)
-    for b in range(2):
+    for b in range(n):
         x = torch.randn(2, ctx + 1, heads, d, generator=g, device="cuda")
         v = x[1] * torch.exp(6 * torch.randn(ctx + 1, heads, 1, generator=g, device="cuda"))
         t = torch.arange(ctx + 1, device="cuda")
         cache.write(x[0], v, b * pages * page + t)
     c = Case.__new__(Case)
-    c.cache, c.ctx, c.draft, c.group, c.d, c.heads = cache, [ctx, ctx // 3], 1, 1, d, heads
-    c.table = torch.arange(2 * pages, dtype=torch.int32, device="cuda").view(2, pages)
+    c.cache, c.ctx, c.draft, c.group, c.d, c.heads = cache, [ctx] * n, 1, 1, d, heads
+    c.table = torch.arange(n * pages, dtype=torch.int32, device="cuda").view(n, pages)
     c.context = torch.tensor(c.ctx, dtype=torch.int32, device="cuda")
-    c.q = (0.3 * torch.randn(2, 1, heads, d, generator=g, device="cuda")).bfloat16()
+    c.q = (0.3 * torch.randn(n, 1, heads, d, generator=g, device="cuda")).bfloat16()
     verify(c, c.run(), causal(c))
+
+
+# ------------------------------------------------------------------ lengths, pages, order
+
+
+@pytest.mark.parametrize("name", ["block4", "mx4", "nvfp4"])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("draft,group", [(18, 4), (75, 4)])
+def test_long_contexts_split_over_blocks(name, page, draft, group):
+    c = Case(name, 128, 2, group, [9001, 40, 20011], draft, page=page, seed=51, spare_columns=3)
+    verify(c, c.run(), causal(c))
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257])
+def test_row_counts_around_the_choices(name, d, rows):
+    c = Case(name, d, 1, 1, [270, 0], rows, page=32, seed=52)
+    verify(c, c.run(), causal(c))
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_many_sequences_to_a_block(name, draft, group):
+    """More items than blocks, so that a block goes from one to the next."""
+    c = Case(name, 128, 4, group, [(61 * i) % 397 for i in range(90)], draft, page=32, seed=53)
+    verify(c, c.run(), causal(c))
+
+
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_pages_outside_the_cache(name, draft, group):
+    c = Case(name, 128, 2, group, [400, 50], draft, page=32, seed=54)
+    see = causal(c)
+    for b, page, to in ((0, 1, -1), (0, 2, c.cache.num_pages), (0, 9, -7), (1, 0, -1)):
+        c.table[b, page] = to
+        see[b][:, page * 32:page * 32 + 32] = False
+    verify(c, c.run(), see)
+    out, lse = bb().cache_attention(c.q, c.cache, c.table[:, :0], c.context, return_lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("name", ["mx4", "block4", "nvfp4"])
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_repeatable_other_stream_and_graph(name, draft, group):
+    c = Case(name, 128, 2, group, [5000, 300], draft, page=64, seed=55)
+    want = c.run()
+    for _ in range(3):
+        got = c.run()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = bb().cache_attention(c.q * 1, c.cache, c.table, c.context)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = bb().cache_attention(c.q, c.cache, c.table, c.context)
+    c.context.copy_(torch.tensor([4000, 77], dtype=torch.int32))  # lengths are read by the replay
+    graph.replay()
+    assert torch.equal(out, c.run()[0])
