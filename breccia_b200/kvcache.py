@@ -21,6 +21,7 @@ import math
 from typing import Any, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .api import _IN_DT, _require_cuda
@@ -73,11 +74,21 @@ def _like(x: torch.Tensor) -> torch.Tensor:
 
 
 def _no_grad(what: str, *tensors) -> None:
-    """A serving call has no backward pass: it refuses rather than cut a graph silently."""
+    """A serving call has no derivatives: it refuses rather than cut a graph, or drop a
+    forward-mode tangent, silently."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
                 raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    if _in_dual_level():
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
+def _in_dual_level() -> bool:
+    """Whether forward-mode tangents are carried here (under torch.no_grad() they are)."""
+    return forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
 
 
 def _on(t: torch.Tensor, what: str, dev) -> None:

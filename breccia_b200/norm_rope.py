@@ -17,7 +17,8 @@ import torch
 
 from . import _lib
 from .api import _IN_DT
-from .kvcache import QuantizedKVCache, _Entry, _heads, _index, _like, _no_grad, _on
+from .kvcache import (QuantizedKVCache, _Entry, _heads, _in_dual_level, _index, _like, _no_grad,
+                      _on)
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_write"]
 
@@ -156,9 +157,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     float32 ``(table, rotated / 2)`` with ``rotated`` at most ``d``.
     ``positions``: one int32 or int64 per token; a position outside the table
     gives a row of NaN. ``d`` and ``rotated`` are multiples of 16, ``d`` at
-    most 256. Returns new ``q`` and ``k`` of the inputs' dtype and shape."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or
-                                    k_weight.requires_grad):
+    most 256. Returns new ``q`` and ``k`` of the inputs' dtype and shape. Forward-mode
+    derivatives are refused."""
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or
+                                     k_weight.requires_grad)) or _in_dual_level():
+        # (with a forward-mode tangent autograd refuses: there is no such derivative here)
         return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     a, q3, k3, _rest = _arguments(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     q_out, k_out = _forward(a, q3, k3)
