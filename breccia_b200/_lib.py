@@ -144,7 +144,11 @@ def lib() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Call ``name`` and raise on a non-zero status."""
-    rc = getattr(lib(), name)(*args)
+    check(name, getattr(lib(), name)(*args))
+
+
+def check(name: str, rc: int) -> None:
+    """Raise for a non-zero status that ``name`` returned."""
     if rc != BRC_OK:
         detail = lib().brc_status_string(rc).decode()
         if rc == BRC_ERR_CUDA:

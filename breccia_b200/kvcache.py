@@ -53,14 +53,12 @@ class _Entry:
         if fn is None:
             fn = self.fn = getattr(_lib.lib(), self.name)
         if index == _current_device():
-            if fn(*args, _current_stream(index)) == 0:
-                return
+            rc = fn(*args, _current_stream(index))
         else:
             with torch.cuda.device(index):
-                if fn(*args, _current_stream(index)) == 0:
-                    return
-        with torch.cuda.device(index):  # refused: once more, for its exception
-            _lib.call(self.name, *args, _current_stream(index))
+                rc = fn(*args, _current_stream(index))
+        if rc:
+            _lib.check(self.name, rc)
 
 
 _kv_write, _kv_read, _kv_attention = (_Entry(n) for n in
