@@ -232,9 +232,12 @@ __device__ __forceinline__ float squares(const float2* x) {
 }
 
 // ------------------------------------------------------------------ forward
-// R heads of a token in place; every lane of the warp calls it. Rows whose
-// squares pass float32's range are taken 2^-64 times (x r does not change when
-// eps goes with 2^-128).
+// Rows whose squares pass float32's range are taken kDown times (x r does not change
+// when eps goes with its square): elements up to 2^128 then have squares up to 2^56, and
+// of 256 that did pass it the largest is 2^60 or more, so that its square does not vanish.
+constexpr float kDown = 0x1p-100f;
+
+// R heads of a token in place; every lane of the warp calls it.
 template <int L, int NP, int R, bool INTER>
 __device__ __forceinline__ void norm_turn(float2 (&x)[R][NP], const float2* w, const float2* c,
                                           const float2* s, float inv_d, float eps) {
@@ -243,8 +246,8 @@ __device__ __forceinline__ void norm_turn(float2 (&x)[R][NP], const float2* w, c
   for (int i = 0; i < R; ++i) v[i] = squares<NP>(x[i]);
   float ss = sum_rows<L, R>(v);
   if (__any_sync(0xFFFFFFFFu, isinf(ss))) {
-    const float by = isinf(ss) ? 0x1p-64f : 1.f;
-    eps *= by * by;
+    const float by = isinf(ss) ? kDown : 1.f;
+    eps = eps * by * by;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const float f = of_row<L, R>(by, i);
@@ -551,8 +554,8 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdPerSm) k_bwd(BwdArgs g) {
       float t = sums();
       const bool sq = part < L / 2;  // this lane holds a sum of squares
       if (__any_sync(0xFFFFFFFFu, sq && isinf(t))) {
-        by = sq && isinf(t) ? 0x1p-64f : 1.f;
-        eps *= by * by;
+        by = sq && isinf(t) ? kDown : 1.f;
+        eps = eps * by * by;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           const float f = of_row<L, 2 * R>(by, i);
