@@ -67,3 +67,28 @@ def test_gradients_of_large_rows(d, rot, dtype):
         tol = tol + 2.0 ** -133  # half a step of its numbers below 2^-126
     assert bool(((gx.double() - wx).abs() <= tol).all())
     assert bool(((gw.double() - ww).abs() <= 64 * F32 * (2 * gmax * size).sum((0, 1))).all())
+
+
+@pytest.mark.parametrize("d,rot", [(64, 32), (96, 48), (128, 64), (256, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_infinity_stays_in_its_pair(d, rot, dtype, interleaved):
+    """An infinite element makes itself NaN and, where it is rotated, its partner; the rest
+    of its head is 0. A head of infinite gradients makes no other weight's gradient NaN."""
+    x = torch.randn(d, 1, d, generator=torch.Generator().manual_seed(6)).to(dtype).cuda()
+    at = torch.arange(d, device="cuda")
+    x[at, 0, at] = float("inf")
+    w = torch.rand(d, device="cuda") + 0.5
+    cos, sin = tables(d + 1, rot)
+    pos = at + 1
+    y, _ = bb().qk_norm_rope(x, x[:, :0], w, w, cos, sin, pos, interleaved=interleaved)
+    want = reference(x, w, cos, sin, pos, 1e-6, interleaved)
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    assert not torch.nan_to_num(y, nan=0.0).any()
+    leaf = w.clone().requires_grad_(True)
+    ones = torch.ones(1, 1, d, dtype=dtype, device="cuda")
+    z, _ = bb().qk_norm_rope(ones, ones[:, :0], leaf, w, cos, sin, pos[:1], interleaved=interleaved)
+    g = torch.zeros_like(z)
+    g[..., d - 3] = float("inf")
+    (gw,) = torch.autograd.grad(z, leaf, g)
+    assert not bool(torch.isfinite(gw[d - 3])) and int((~torch.isfinite(gw)).sum()) == 1
