@@ -1151,6 +1151,9 @@ __device__ __noinline__ void add_in_passes(Passes<KIND, FMT, D, NT>& x, const Ar
 // Blocks that an SM is to hold, as many as the accumulators' registers allow.
 constexpr __host__ __device__ int blocks_per_sm(int kind, int d, int nt) {
   if (kind == BRC_STE_NVFP4 && d * nt == 128) return 4;
+  // (with the check of the references a third block spills: 16 rows, 8 sequences of 16384
+  // tokens, block FP8 76 us with three blocks and 73 with two, MXFP8 83 and 81)
+  if (kind != BRC_STE_NVFP4 && d == 128 && nt == 2) return 2;
   return d * nt <= 64 ? 4 : d * nt <= 256 ? 3 : 2;
 }
 // Stages of a warp's ring: what fits beside the queries in the block's part of
