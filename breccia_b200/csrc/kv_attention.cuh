@@ -197,16 +197,20 @@ __device__ __forceinline__ uint32_t half2_pow2(int e0, int e1, int ref) {
 // and goes with any reference.
 //
 // Codes whose scale is up to kSpan (log2) below its reference keep their bits: E4M3 codes
-// are multiples of 2^-9 and E5M2 codes of 2^-16, f16 holds multiples of 2^-24. Block
-// FP8's scales are multiplied in before the rounding to f16, onto the probabilities (here:
-// they then keep what is above 2^-20 of the row's largest, as 2^-31 without) or the values
-// (tcgen05: E4M3's smallest codes then just are normal numbers). Tokens further apart do
-// not go together. A reference is set kSlack above the scale that asks for it, so that it
-// seldom moves.
+// are multiples of 2^-9 and f16 holds multiples of 2^-24 (E5M2's smallest lose what is
+// below 2^-25 of their block's largest). Block FP8's scales are multiplied in before the
+// rounding to f16, onto the probabilities (here: they then keep what is above 2^-20 of the
+// row's largest, as 2^-31 without) or the values (tcgen05: E4M3's smallest codes then just
+// are normal numbers). Tokens further apart do not go together, but for scales as the
+// casts give them to zeros (kFloor: values below 6e-8, in block FP8 1e-10), which count as
+// zero beside larger ones: rows of zeros are common. A reference is set kSlack above the
+// scale that asks for it, so that it seldom moves, and not below kSpan, so that scales of
+// zero, as a new cache holds them, go together.
+template <int KIND>
+constexpr int kSpan = KIND == BRC_STE_BLOCK_FP8 ? 11 : 15;
 template <int KIND, int FMT>
-constexpr int kSpan = KIND == BRC_STE_BLOCK_FP8 ? 11 : FMT == BRC_FP8_E4M3 ? 15 : 7;
+constexpr uint32_t kFloor = KIND == BRC_STE_MXFP8 ? 94 : FMT == BRC_FP8_E4M3 ? 84 : 77;
 constexpr int kSlack = 2;
-constexpr uint32_t kLowest = 27;  // references are not below 2^-100
 
 template <int KIND, int D>
 constexpr int kScaleBlocks = KIND == BRC_STE_MXFP8 ? D / 32 : 1;
@@ -248,7 +252,7 @@ __device__ __forceinline__ uint32_t top_byte(uint32_t x) {
 // at least one: block by block, the ones near the largest scale of those that are left.
 // W words of four blocks' bytes to a token's values; km: the largest byte of its keys
 // (MXFP8). `refs` moves for them where it has to; returns what their keys are relative to.
-template <int SPAN, int BLOCKS, int N, int W>
+template <int SPAN, uint32_t FLOOR, int BLOCKS, int N, int W>
 __device__ __forceinline__ uint32_t choose(const uint32_t (&v)[N][W], const uint32_t (&km)[N],
                                            uint32_t left, uint32_t& take, uint32_t (&refs)[W]) {
   constexpr uint32_t kTake = SPAN - kSlack;
@@ -269,11 +273,12 @@ __device__ __forceinline__ uint32_t choose(const uint32_t (&v)[N][W], const uint
 #pragma unroll
       for (int y = 0; y < N; ++y) {
         const uint32_t x = (v[y][w] >> i) & 0xFFu;
+        if (x <= FLOOR) continue;  // (its reference is no lower: the largest is not)
         if (x + kTake < top) take &= ~(1u << y);
         else off |= ((take >> y) & 1u) && x + SPAN < ref;
       }
       if (__any_sync(0xFFFFFFFFu, off))
-        refs[w] += (min(max(top + kSlack, kLowest), 254u) - ref) << i;
+        refs[w] += (min(max(top + kSlack, (uint32_t)SPAN), 254u) - ref) << i;
     }
   }
   uint32_t k = 0;
@@ -283,7 +288,7 @@ __device__ __forceinline__ uint32_t choose(const uint32_t (&v)[N][W], const uint
   k = __reduce_max_sync(0xFFFFFFFFu, k);
 #pragma unroll
   for (int y = 0; y < N; ++y)
-    if (km[y] + kTake < k) take &= ~(1u << y);
+    if (km[y] > FLOOR && km[y] + kTake < k) take &= ~(1u << y);
   return k;
 }
 
@@ -406,7 +411,8 @@ struct Later {
 template <int KIND, int FMT, int D, int NT>
 struct Warp {
   using S = Shape<KIND, D>;
-  static constexpr int kSpans = kSpan<KIND, FMT>;
+  static constexpr int kSpans = kSpan<KIND>;
+  static constexpr uint32_t kZero = kFloor<KIND, FMT>;
   static constexpr int kMask = KIND == BRC_STE_MXFP8 ? kSpans : 15;
   static constexpr int kBlocks = kScaleBlocks<KIND, D>;
   static constexpr int kWords = (kBlocks + 3) / 4;
@@ -434,9 +440,9 @@ struct Warp {
     }
 #pragma unroll
     for (int w = 0; w < kWords; ++w)
-      near[w] = Near<kMask>(kLowest * (kBlocks == 1 ? 1u : kBlocks == 2 ? 0x0101u : 0x01010101u));
+      near[w] = Near<kMask>(kSpans * (kBlocks == 1 ? 1u : kBlocks == 2 ? 0x0101u : 0x01010101u));
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) e[i] = KIND == BRC_STE_NVFP4 ? 127 : (int)kLowest;
+    for (int i = 0; i < kOwn; ++i) e[i] = KIND == BRC_STE_NVFP4 ? 127 : kSpans;
     ke = 0;
   }
   // What the values are relative to becomes `refs`; o is still zero.
@@ -833,6 +839,23 @@ struct Step {
       for (int i = 0; i < W::kWords; ++i) in &= w.near[i](v[0][i]);
       return in;
     }
+    // The same, scales as of zeros left out.
+    __device__ __forceinline__ bool fits_but_zeros(const uint32_t (&refs)[W::kWords],
+                                                   uint32_t ke) const {
+      bool in = true;
+      if constexpr (KIND == BRC_STE_BLOCK_FP8) {
+        in = refs[0] - v[0][0] <= (uint32_t)W::kSpans || (v[0][0] <= W::kZero && v[0][0] <= refs[0]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W::kWords; ++i) {
+          const uint32_t zero = __vcmpleu4(v[0][i], __vminu4(refs[i], W::kZero * 0x01010101u));
+          in &= Near<W::kMask>(refs[i])((v[0][i] & ~zero) | (refs[i] & zero));
+        }
+        const uint32_t k = top_key();
+        in &= ke - k <= (uint32_t)W::kSpans || (k <= W::kZero && k <= ke);
+      }
+      return in;
+    }
     __device__ __forceinline__ uint32_t top_key() const {
       uint32_t m = 0;
 #pragma unroll
@@ -850,7 +873,7 @@ struct Step {
 #pragma unroll
       for (int y = 0; y < 8 * (W::kBlocks < 4 ? W::kBlocks : 4); y += 8) {
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, on ? (mine.v[0][i] >> y) & 0xFFu : 0u);
-        refs[i] |= min(max(top + kSlack, kLowest), 254u) << y;
+        refs[i] |= min(max(top + kSlack, (uint32_t)W::kSpans), 254u) << y;
       }
     }
     ke = 0;
@@ -868,15 +891,16 @@ struct Step {
   // grows with references that fall.
   __device__ static __forceinline__ bool follow(W& w, const Token& mine, int lane, bool on,
                                                 bool drafted, Later& later) {
-    uint32_t refs[W::kWords], ke;
+    uint32_t refs[W::kWords], ke = w.ke;
+#pragma unroll
+    for (int i = 0; i < W::kWords; ++i)
+      refs[i] = KIND == BRC_STE_BLOCK_FP8 ? (uint32_t)w.e[0] : w.near[i].refs();
+    if (__all_sync(0xFFFFFFFFu, !on || mine.fits_but_zeros(refs, ke))) return true;
     around(mine, on, refs, ke);
-    int climb = 0, fall = 0;
-    bool in = KIND != BRC_STE_MXFP8 || ke - mine.top_key() <= (uint32_t)W::kSpans;
-    int own[W::kOwn];
+    const bool in = mine.fits_but_zeros(refs, ke);
+    int climb = 0, fall = 0, own[W::kOwn];
 #pragma unroll
     for (int i = 0; i < W::kWords; ++i) {
-      if constexpr (KIND == BRC_STE_BLOCK_FP8) in &= refs[0] - mine.v[0][0] <= (uint32_t)W::kSpans;
-      else in &= Near<W::kMask>(refs[i])(mine.v[0][i]);
       own[i] = (int)((refs[i] >> (8 * W::byte_of(lane))) & 0xFFu);
       climb = max(climb, own[i] - w.e[i]);
       fall = max(fall, w.e[i] - own[i]);
@@ -918,14 +942,14 @@ struct Step {
         refs[i] = KIND == BRC_STE_BLOCK_FP8 ? (uint32_t)w.e[0] : w.near[i].refs();
         if constexpr (KIND == BRC_STE_MXFP8) km[0] = max(km[0], top_byte(mine.k[0][i]));
       }
-      const uint32_t k = choose<W::kSpans, W::kBlocks>(
+      const uint32_t k = choose<W::kSpans, W::kZero, W::kBlocks>(
           mine.v, km, (left >> (lane % S::kRows)) & 1u, take, refs);
       const uint32_t group = __ballot_sync(0xFFFFFFFFu, take != 0u) & S::kAll;
       left &= ~group;
       if (seen(group)) {
         taken = group;
         if constexpr (KIND == BRC_STE_MXFP8) {
-          if (__any_sync(0xFFFFFFFFu, k > w.ke || (take && km[0] + W::kSpans < w.ke)))
+          if (__any_sync(0xFFFFFFFFu, k > w.ke || (take && km[0] > W::kZero && km[0] + W::kSpans < w.ke)))
             w.ke = min(k + kSlack, 254u);
         }
         w.move(refs, lane);

@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         page = page_of(walk.s_begin + 1);
         constexpr int kBlocks = kScaleBlocks<KIND, D>;
         // what values are relative to, at first: the lowest
-        uint32_t refs[1] = {kLowest * (kBlocks == 1 ? 1u : kBlocks == 2 ? 0x0101u : 0x01010101u)};
+        uint32_t refs[1] = {kSpan<KIND> * (kBlocks == 1 ? 1u : kBlocks == 2 ? 0x0101u : 0x01010101u)};
         bool fresh = true;
         for (int j = walk.s_begin; ok && j < walk.s_end; ++j) {
           const int there = (int)min((int64_t)kTok, seq.total - (int64_t)j * kTok) - 4 * lane;
@@ -922,7 +922,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
             int ek = 0;
             if constexpr (KIND != BRC_STE_NVFP4) {
               uint32_t vb[4][1], km[4] = {0u, 0u, 0u, 0u}, hi = 0, lo = 255;
-              constexpr uint32_t kFar = kSpan<KIND, FMT>;
+              constexpr uint32_t kFar = kSpan<KIND>;
               const Near<KIND == BRC_STE_MXFP8 ? kFar : 15> near(refs[0]);
               bool off = false;
 #pragma unroll
@@ -941,7 +941,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
               }
               ek = (int)hi;
               if (__any_sync(0xFFFFFFFFu, off))
-                ek = (int)choose<kFar, kBlocks>(vb, km, left, take, refs);
+                ek = (int)choose<kFar, kFloor<KIND, FMT>, kBlocks>(vb, km, left, take, refs);
             }
             more = __any_sync(0xFFFFFFFFu, (left & ~take) != 0u);
             left &= ~take;

@@ -447,6 +447,24 @@ def test_many_steps_of_sizes_apart(name):
     verify(c, c.run(), causal(c))
 
 
+@pytest.mark.parametrize("name", RECIPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("draft,group", ROWS)
+def test_zeros_among_ordinary_values(name, d, draft, group):
+    """Rows and channel blocks of zeros, keys and values, drafted ones too."""
+    c = Case(name, d, 1, group, [600, 0], draft, seed=50)
+    g = torch.Generator().manual_seed(51)
+    for b, n in enumerate(c.ctx):
+        n += draft
+        k, v = torch.randn(n, 1, d, generator=g), torch.randn(n, 1, d, generator=g)
+        v[torch.rand(n, generator=g) < 0.1] = 0
+        k[torch.rand(n, generator=g) < 0.1] = 0
+        v[torch.rand(n, generator=g) < 0.1, :, :32] = 0
+        v[torch.rand(n, generator=g) < 0.05] *= 0.02
+        rewrite(c, b, 0, k=k.cuda(), v=v.cuda())
+    verify(c, c.run(), causal(c))
+
+
 # ------------------------------------------------------------------ lengths, pages, order
 
 
