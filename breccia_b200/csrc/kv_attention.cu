@@ -12,14 +12,22 @@ namespace {
 // 256), then up to four row warps to a block.
 //
 // More rows than tc_rows go to the tensor-core kernel: 256 to a block, its time nearly
-// the same up to that many. Both sides, 8 sequences of 16384 tokens, 8 cache heads (us,
-// register path / tensor cores), at the rows of a cache head:
+// the same up to that many. Both sides, 8 cache heads (us, register path / tensor cores,
+// caches cold), at the rows of a cache head; 8 sequences of 16384 tokens:
 //                        32         48         64         72        128        256
-//   block FP8 d 128   115 / 197  182 / 199  188 / 201  320 / 201  338 / 209  597 / 266
-//   MXFP8 d 128       131 / 182  211 / 184  217 / 184  375 / 186  395 / 195  711 / 244
-//   NVFP4 d 128       119 / 164  193 / 166  199 / 166  340 / 168  359 / 176  637 / 225
-//   block FP8 d 64     96 / 160  155 / 162  158 / 162  268 / 164  281 / 168
-//   MXFP8 d 64        106 / 145  170 / 147  172 / 148  297 / 148  309 / 154
+//   block FP8 d 128   114 / 204  181 / 204  187 / 208  321 / 208  337 / 214  599 / 263
+//   MXFP8 d 128       122 / 191  200 / 194  206 / 193  353 / 196  370 / 200  663 / 241
+//   NVFP4 d 128       112 / 171  183 / 173  189 / 173  325 / 175  343 / 179  611 / 210
+//   block FP8 d 64    103 / 165  159 / 165  163 / 167  273 / 167  282 / 169  513 / 206
+//   MXFP8 d 64        110 / 155  177 / 155  179 / 157  308 / 157  316 / 159  589 / 193
+// one sequence of 16384 tokens, 8 of 1024 and one of 1024, where the two lie closer
+// together:
+//   block FP8 d 128    52 / 71    67 / 71    71 / 73    93 / 73   107 / 79   134 / 101
+//                      42 / 54    54 / 54    58 / 56    71 / 56    85 / 62   107 / 83
+//                      36 / 46    44 / 46    46 / 48    54 / 48    65 / 54    69 / 71
+//   MXFP8 d 128        56 / 71    71 / 71    75 / 73    99 / 73   112 / 77   144 / 97
+//                      44 / 54    56 / 56    60 / 56    75 / 56    87 / 62   112 / 81
+//                      38 / 48    44 / 48    50 / 48    56 / 50    67 / 54    71 / 71
 // Block FP8 decodes in fewer instructions than the others, so that its register path
 // holds out longer.
 struct Split {

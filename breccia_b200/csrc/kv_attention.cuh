@@ -39,7 +39,7 @@
 // joins the parts in a fixed order.
 //
 // Measured on B200, 8 cache heads of 128: 64 tokens of 32 query heads over 8192 tokens
-// each (join included) block FP8 190 us (5.8 TB/s), MXFP8 202, NVFP4 174; HBM bounds
+// each (join included) block FP8 191 us (5.8 TB/s), MXFP8 192, NVFP4 158; HBM bounds
 // the first, the decoding of codes and scales the other two. Two sequences of 131072
 // tokens in NVFP4, 64 query heads: 96 us (3.1 TB/s).
 #pragma once

@@ -334,7 +334,14 @@ def cache_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.
     Returns ``softmax(scale q k^T) v`` in ``q``'s dtype and shape (``scale``
     defaults to ``head_dim ** -0.5``), and with ``return_lse`` also the
     float32 log-sum-exp of every row. A row that sees nothing gives 0 and
-    ``-inf``; what it does not see, NaN included, does not reach it."""
+    ``-inf``; what it does not see, NaN included, does not reach it. Values more
+    than ``2**60`` below the largest that a row sees (MXFP8: in the same 32
+    elements) may vanish beside it, and values as small as the casts hold zeros
+    (below 6e-8, in block FP8 1e-10) count as zero beside larger ones.
+
+    Many rows of a cache head run with bounded waits: if one runs out (2 s), rows
+    stay unwritten and ``brc_gemm_status`` tells, as for the GEMMs. Scratch is
+    allocated per call on the current stream, up to 40 MB."""
     if not isinstance(cache, QuantizedKVCache):
         raise TypeError(f"cache must be a QuantizedKVCache, got {type(cache).__name__}")
     dev = cache.device

@@ -448,8 +448,9 @@ typedef struct {
 } brc_kv_cache;
 /* Quantise keys and values (tokens, heads, head_dim; strides in elements) into
  * the rows slots[token] = page * page_size + place in page (int32, or int64
- * with slots64). A slot outside the cache is not written (-1: padding). Two
- * tokens of one call with the same slot leave either's row. */
+ * with slots64). A slot outside the cache is not written (-1: padding). The
+ * slots of one call are distinct: of two tokens with the same slot, codes and
+ * scales of either may be left. */
 int brc_kv_write(const brc_kv_cache* c, const void* k, const void* v, int dtype, int64_t tokens,
                  int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
                  const void* slots, int slots64, void* stream);
@@ -479,7 +480,18 @@ int brc_kv_read(const brc_kv_cache* c, const int32_t* table, int64_t table_strid
  * A row that sees nothing gives out 0 and lse -inf. What lies in places that
  * a row does not see (NaN included) does not reach it. Tokens past the
  * table's columns or in a page outside the cache are not seen.
- * workspace: brc_kv_attention_workspace(...) bytes, 16-byte aligned. */
+ * Scores, sums and the output are float32 until they are stored. Queries enter
+ * as f16 times a power of two to a row, probabilities as f16: what is below
+ * 2^-30 of a row's largest counts in lse only (block FP8 below 2^-19, where its
+ * values are 2^9 smaller than others around). Values more than 2^60 below the
+ * largest that a row sees (MXFP8: in the same 32 elements) may vanish beside it,
+ * and values as small as the casts hold zeros (below 6e-8, in block FP8 1e-10)
+ * count as zero beside tokens' that are 2^9 times as large.
+ * More than 64 query rows of a cache head (MXFP8 and NVFP4: 32) run on tcgen05
+ * at head_dim 128, and at 64 with FP8 codes. Its waits are bounded as the
+ * GEMMs' are: if one runs out, rows stay unwritten and brc_gemm_status() tells.
+ * workspace: brc_kv_attention_workspace(...) bytes, 16-byte aligned; at most 40
+ * MB, by the rows of a cache head and the number of multiprocessors. */
 int64_t brc_kv_attention_workspace(const brc_kv_cache* c, int batch, int draft, int hq);
 int brc_kv_attention(const brc_kv_cache* c, const void* q, int q_dtype, int batch, int draft,
                      int hq, const int32_t* table, int64_t table_stride, int table_pages,
