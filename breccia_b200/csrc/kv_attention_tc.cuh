@@ -87,10 +87,9 @@ struct alignas(128) Smem {
   uint32_t tmem, abort;
   float pair[2][2][2][128];    // [turn][row tile][half][row]: shifts, then sums
   uint8_t sees[2][2][2][128];  // whether the row sees any of the half's places
-  // What a thread's part of a row of O is relative to (a byte to a channel block), and the
-  // most that it was while the row saw something. It follows the values, but not below
-  // 2^-60 of that, and only where the row sees them.
-  uint2 refs[2][2][128];
+  // What a thread's part of a row of O is relative to (a byte to a channel block). It
+  // follows the values, where the row sees them, but not so low that O passes 2^100.
+  uint32_t refs[2][2][128];
   uint32_t start[4];           // first pass of an item, one slot to an item as of odd
   // Numbers of items whose drafted values are not all finite: one slot to an item, as
   // the loads are at most two items ahead.
@@ -444,7 +443,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
       }
       float m = -INFINITY, l = 0.f;
       bool fresh = true;
-      uint2& refs = sm.refs[r][half][mine];
+      uint32_t& refs = sm.refs[r][half][mine];
       for (int j = walk.s_begin; j < walk.s_end;) {
         if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.s_full[r], s_phase, abort, status, 1u)))) {
           leave();
@@ -515,6 +514,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * h * h2);
             tmem_st16(oc + 16 * c, x);
+          }
+        };
+        // `to` no lower than what keeps O times g, relative to `from`, within 2^100. (What a row
+        // adds relative to less than its O is then too large by the difference, but O is 2^100,
+        // and that at most 2^18 a token.)
+        auto low = [&](float g, uint32_t from, uint32_t& to) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[16];
+            tmem_ld16(oc + 16 * c, x);
+            tmem_ld_wait16(x);
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float y = fabsf(__uint_as_float(x[i]) * g);
+              if (y < INFINITY) most = fmaxf(most, y);
+            }
+            const int shift = 8 * channel_block(c);
+            const int is = (int)((to >> shift) & 0xFFu);
+            const int least = (int)((from >> shift) & 0xFFu) + (int)(__float_as_uint(most) >> 23) - 227;
+            if (most > 0.f && least > is) to += (uint32_t)(least - is) << shift;
           }
         };
         // This half's shift: the row's, until a score is far above it (and at first the
@@ -625,7 +645,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         if (masked && KIND != BRC_STE_NVFP4) sm.sees[turn][r][half][mine] = sees;
         meet();
         const float nm = fmaxf(own, sm.pair[turn][r][half ^ 1][mine]);
-        const bool moved = KIND != BRC_STE_NVFP4 && (fresh || meta.ev != refs.x);
+        const bool moved = KIND != BRC_STE_NVFP4 && (fresh || meta.ev != refs);
         float part = (l2.x + l2.y) * (1.f / (1 << kLift));
         if (__any_sync(0xFFFFFFFFu, nm != own || nm != m || moved)) {
           const float gp = nm == own || nm == -INFINITY ? 1.f : ex2(own - nm);
@@ -633,16 +653,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
           if (__any_sync(0xFFFFFFFFu, gp != 1.f)) scale_p(2, gp);
           uint32_t from = 0, to = 0;
           if (moved) {
-            from = to = refs.x;
-            uint32_t most_seen = fresh ? 0u : refs.y;
+            from = to = refs;
             if (masked) sees |= sm.sees[turn][r][half ^ 1][mine] != 0;
-            if (sees) {
-              to = __vmaxu4(meta.ev, __vsubus4(most_seen, 0x3C3C3C3Cu));
-              most_seen = __vmaxu4(most_seen, to);
-            }
-            if (fresh) to = meta.ev;
-            refs = make_uint2(to, most_seen);
+            if (sees || fresh) to = meta.ev;
           }
+          if (!fresh && __any_sync(0xFFFFFFFFu, __vsubus4(from, to) & 0xE0E0E0E0u)) low(go, from, to);
+          if (moved) refs = to;
           if (!fresh && __any_sync(0xFFFFFFFFu, go != 1.f || to != from)) scale_o(go, from, to);
           part *= gp;
           l *= go;
@@ -687,7 +703,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attend_tc(Args a, uint32_t* s
         float mul = so * (1.f / (1 << kLift));
         if constexpr (KIND != BRC_STE_NVFP4) {
           constexpr int kOff = KIND == BRC_STE_MXFP8 ? 0 : kValueLift<FMT>;
-          mul *= exp2f((float)((int)((refs.x >> (8 * channel_block(c))) & 0xFFu) - 127 - kOff));
+          mul *= exp2f((float)((int)((refs >> (8 * channel_block(c))) & 0xFFu) - 127 - kOff));
         }
         float o[16];
 #pragma unroll

@@ -408,8 +408,9 @@ def test_garbage_in_unseen_places(name, draft, group):
 @pytest.mark.parametrize("name", ["mx4", "mx5", "block4", "block5"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("draft,group", ROWS)
-def test_large_values_with_little_weight(name, d, draft, group):
-    """Tokens of the context whose values are 2^30 times the others' and whose scores are
+@pytest.mark.parametrize("power", [30, 90])
+def test_large_values_with_little_weight(name, d, draft, group, power):
+    """Tokens of the context whose values are 2^power times the others' and whose scores are
     so low that they do not count; and channel blocks 2^30 apart."""
     c = Case(name, d, 1, group, [500], draft, seed=47)
     g = torch.Generator().manual_seed(48)
@@ -417,9 +418,9 @@ def test_large_values_with_little_weight(name, d, draft, group):
     k = torch.randn(n, 1, d, generator=g)
     v = torch.randn(n, 1, d, generator=g)
     far = torch.rand(n, generator=g) < 0.1
-    far[0] = True
+    far[0], far[128:256] = True, power > 60  # a tile of them, too
     k[far] = -1.0
-    v[far] *= 2.0 ** 30
+    v[far] *= 2.0 ** power
     if name.startswith("mx"):
         v[..., :32] *= 2.0 ** 30
     c.q.copy_(1 + 0.02 * torch.randn(c.q.shape, generator=g))
