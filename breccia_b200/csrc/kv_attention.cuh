@@ -203,13 +203,15 @@ __device__ __forceinline__ uint32_t half2_pow2(int e0, int e1, int ref) {
 // row's largest, as 2^-31 without) or the values (tcgen05: E4M3's smallest codes then just
 // are normal numbers). Tokens further apart do not go together, but for scales as the
 // casts give them to zeros (kFloor: values below 6e-8, in block FP8 1e-10), which count as
-// zero beside larger ones: rows of zeros are common. A reference is set kSlack above the
+// zero beside larger ones: rows of zeros are common. (MXFP8's E5M2 gives zeros the scale
+// of values up to 7e-6, so there only what no cast writes counts.) A reference is set kSlack above the
 // scale that asks for it, so that it seldom moves, and not below kSpan, so that scales of
 // zero, as a new cache holds them, go together.
 template <int KIND>
 constexpr int kSpan = KIND == BRC_STE_BLOCK_FP8 ? 11 : 15;
 template <int KIND, int FMT>
-constexpr uint32_t kFloor = KIND == BRC_STE_MXFP8 ? 94 : FMT == BRC_FP8_E4M3 ? 84 : 77;
+constexpr uint32_t kFloor = KIND == BRC_STE_MXFP8 ? (FMT == BRC_FP8_E4M3 ? 94 : 93)
+                                                  : (FMT == BRC_FP8_E4M3 ? 84 : 77);
 constexpr int kSlack = 2;
 
 template <int KIND, int D>

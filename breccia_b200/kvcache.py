@@ -337,7 +337,7 @@ def cache_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.
     ``-inf``; what it does not see, NaN included, does not reach it. Values more
     than ``2**60`` below the largest that a row sees (MXFP8: in the same 32
     elements) may vanish beside it, and values as small as the casts hold zeros
-    (below 6e-8, in block FP8 1e-10) count as zero beside larger ones.
+    (E4M3: below 6e-8; block FP8: 1e-10) count as zero beside larger ones.
 
     Many rows of a cache head run with bounded waits: if one runs out (2 s), rows
     stay unwritten and ``brc_gemm_status`` tells, as for the GEMMs. Scratch is

@@ -485,8 +485,8 @@ int brc_kv_read(const brc_kv_cache* c, const int32_t* table, int64_t table_strid
  * 2^-30 of a row's largest counts in lse only (block FP8 below 2^-19, where its
  * values are 2^9 smaller than others around). Values more than 2^60 below the
  * largest that a row sees (MXFP8: in the same 32 elements) may vanish beside it,
- * and values as small as the casts hold zeros (below 6e-8, in block FP8 1e-10)
- * count as zero beside tokens' that are 2^9 times as large.
+ * and values as small as the casts hold zeros (E4M3: below 6e-8; block FP8:
+ * 1e-10) count as zero beside tokens' that are 2^9 times as large.
  * More than 64 query rows of a cache head (MXFP8 and NVFP4: 32) run on tcgen05
  * at head_dim 128, and at 64 with FP8 codes. Its waits are bounded as the
  * GEMMs' are: if one runs out, rows stay unwritten and brc_gemm_status() tells.

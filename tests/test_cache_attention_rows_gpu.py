@@ -325,8 +325,9 @@ def test_infinite_values(draft, group):
 @pytest.mark.parametrize("name", RECIPES)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("draft,group", ROWS)
-def test_values_and_keys_of_very_different_size(name, d, draft, group):
-    c = Case(name, d, 2, group, [700, 31], draft, seed=41, spread=4.0)
+@pytest.mark.parametrize("spread", [4.0, 6.0])
+def test_values_and_keys_of_very_different_size(name, d, draft, group, spread):
+    c = Case(name, d, 2, group, [700, 31], draft, seed=41, spread=spread)
     verify(c, c.run(scale=0.02), causal(c), 0.02)
 
 
